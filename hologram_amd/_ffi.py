@@ -126,6 +126,46 @@ class AttentionI8RowsCallC(ctypes.Structure):
     _fields_ = [("attn", DecodeAttentionI8CallC), ("q_rows", ctypes.c_uint32)]
 
 
+class AttentionPackedCallC(ctypes.Structure):
+    _fields_ = [("q", BufferRefC), ("k", BufferRefC), ("v", BufferRefC), ("starts", BufferRefC),
+                ("output", BufferRefC), ("tokens", ctypes.c_uint32), ("batch",
+                ctypes.c_uint32), ("heads", ctypes.c_uint32), ("kv_heads",
+                ctypes.c_uint32), ("head_dim", ctypes.c_uint32), ("q_stride",
+                ctypes.c_uint32), ("k_stride", ctypes.c_uint32), ("v_stride",
+                ctypes.c_uint32), ("scale_bits", ctypes.c_uint32), ("dtype",
+                ctypes.c_uint8)]
+
+
+class KvBlockAppendCallC(ctypes.Structure):
+    _fields_ = [("new_rows_buf", BufferRefC), ("starts", BufferRefC), ("pos", BufferRefC), ("cache",
+                BufferRefC), ("cache_scales", BufferRefC), ("output", BufferRefC),
+                ("output_scales", BufferRefC), ("tokens", ctypes.c_uint32),
+                ("batch", ctypes.c_uint32), ("kv_heads", ctypes.c_uint32),
+                ("bucket_rows", ctypes.c_uint32), ("block_rows", ctypes.c_uint32),
+                ("head_dim", ctypes.c_uint32), ("new_stride", ctypes.c_uint32),
+                ("dtype", ctypes.c_uint8)]
+
+
+class AttentionI8BlocksCallC(ctypes.Structure):
+    _fields_ = [("q", BufferRefC), ("k_cache", BufferRefC), ("v_cache", BufferRefC), ("k_scales",
+                BufferRefC), ("v_scales", BufferRefC), ("starts", BufferRefC),
+                ("lens", BufferRefC), ("output", BufferRefC), ("tokens",
+                ctypes.c_uint32), ("batch", ctypes.c_uint32), ("heads",
+                ctypes.c_uint32), ("kv_heads", ctypes.c_uint32), ("bucket_rows",
+                ctypes.c_uint32), ("block_rows", ctypes.c_uint32), ("head_dim",
+                ctypes.c_uint32), ("q_stride", ctypes.c_uint32), ("scale_bits",
+                ctypes.c_uint32), ("dtype", ctypes.c_uint8)]
+
+
+class LogitsProcessCallC(ctypes.Structure):
+    _fields_ = [("logits", BufferRefC), ("history", BufferRefC), ("spans", BufferRefC), ("params",
+                BufferRefC), ("bias_ids", BufferRefC), ("bias_values", BufferRefC),
+                ("mask", BufferRefC), ("output", BufferRefC), ("rows",
+                ctypes.c_uint32), ("cols", ctypes.c_uint32), ("history_len",
+                ctypes.c_uint32), ("biases", ctypes.c_uint32), ("dtype",
+                ctypes.c_uint8)]
+
+
 class TransposeCallC(ctypes.Structure):
     _fields_ = [("input", BufferRefC), ("output", BufferRefC), ("rank", ctypes.c_uint8),
                 ("dims", ctypes.c_uint32 * 8), ("perm", ctypes.c_uint8 * 8),
@@ -175,7 +215,10 @@ class CallUnion(ctypes.Union):
                 ("dequantize", DequantizeCallC), ("matmul_dequant", MatMulDequantCallC),
                 ("dequant_act", DequantActivationCallC), ("attn_i8", DecodeAttentionI8CallC),
                 ("attn_i8_rows", AttentionI8RowsCallC), ("transpose", TransposeCallC),
-                ("layout", LayoutCallC)]
+                ("layout", LayoutCallC), ("attn_packed", AttentionPackedCallC),
+                ("kv_block_append", KvBlockAppendCallC),
+                ("attn_i8_blocks", AttentionI8BlocksCallC),
+                ("logits_process", LogitsProcessCallC)]
 
 
 class KernelCallC(ctypes.Structure):

@@ -1488,6 +1488,256 @@ int do_argmax(holo_backend *be, const SlotTable &st, const holo_argmax_call &c) 
                     op);
 }
 
+// The backend's device made current for a call's launches and allocations, the
+// caller's own restored after it.
+struct OnDevice {
+    int before = -1;
+    explicit OnDevice(int device) {
+        int d;
+        if (hipGetDevice(&d) == hipSuccess && d != device && hipSetDevice(device) == hipSuccess) before = d;
+    }
+    ~OnDevice() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+
+// The score divisor of the attention calls (float_kernels.rs:4256-4266).
+float score_divisor(uint32_t head_dim, uint32_t scale_bits) {
+    float s = std::sqrt(static_cast<float>(head_dim));
+    if (s < 1.0f) s = 1.0f;
+    if (scale_bits != 0) {
+        float sm;
+        memcpy(&sm, &scale_bits, 4);
+        if (sm > 0.0f) s = 1.0f / sm;
+    }
+    return s;
+}
+
+// `tokens` rows of `width` elements, `stride` (0: width) from one to the next:
+// *stride made explicit, and the elements they span.
+int strided(uint32_t tokens, uint64_t width, uint32_t *stride, uint64_t *span, const char *op,
+            const char *what) {
+    if (width > 0xffffffffull)
+        return fail(HOLO_ERR_UNSUPPORTED_OP, std::string(op) + ": a row of " + what + " above 2^32 elements");
+    if (*stride == 0) *stride = uint32_t(width);
+    if (*stride < width)
+        return fail(HOLO_ERR_SHAPE_MISMATCH, std::string(op) + ": the stride of " + what +
+                                                 " is below its row of " + std::to_string(width));
+    *span = uint64_t(tokens - 1) * *stride + width;
+    return HOLO_OK;
+}
+
+// What the packed-batch calls ask of their sizes alike.
+int packed_shape(const char *op, uint32_t tokens, uint32_t batch, uint32_t heads, uint32_t hkv,
+                 uint32_t head_dim, uint8_t dtype) {
+    if (heads % hkv != 0)
+        return fail(HOLO_ERR_UNSUPPORTED_OP,
+                    std::string(op) + ": heads must be a multiple of kv_heads (grouped-query)");
+    if (dtype != HOLO_DTYPE_BF16 && dtype != HOLO_DTYPE_F16 && dtype != HOLO_DTYPE_F32)
+        return fail(HOLO_ERR_UNSUPPORTED_OP, std::string(op) + ": rows must be bf16, f16 or f32");
+    if (head_dim > holo::kPackedMaxDim)
+        return fail(HOLO_ERR_UNSUPPORTED_OP, std::string(op) + ": head_dim above 1024");
+    // a launch holds at most a workgroup for each row and head, and two for each
+    // sequence and head
+    if ((uint64_t(tokens) + 2 * uint64_t(batch)) * heads > 0x3fffffffull)
+        return fail(HOLO_ERR_UNSUPPORTED_OP, std::string(op) + ": (tokens + 2 batch) * heads above 2^30");
+    return HOLO_OK;
+}
+
+// ---------------------------------------------------- AttentionPacked ----
+int do_attn_packed(holo_backend *be, const SlotTable &st, const holo_attention_packed_call &c) {
+    const char *op = "attention_packed";
+    if (c.tokens == 0 || c.batch == 0 || c.heads == 0 || c.head_dim == 0) return HOLO_OK;
+    const uint32_t hkv = c.kv_heads == 0 ? c.heads : c.kv_heads;
+    HOLO_TRY(packed_shape(op, c.tokens, c.batch, c.heads, hkv, c.head_dim, c.dtype));
+    const uint64_t es = dtype_size(c.dtype), D = c.head_dim;
+    holo::AttnPackedArgs a;
+    a.q_stride = c.q_stride, a.k_stride = c.k_stride, a.v_stride = c.v_stride;
+    uint64_t qn, kn, vn;
+    HOLO_TRY(strided(c.tokens, c.heads * D, &a.q_stride, &qn, op, "q"));
+    HOLO_TRY(strided(c.tokens, hkv * D, &a.k_stride, &kn, op, "k"));
+    HOLO_TRY(strided(c.tokens, hkv * D, &a.v_stride, &vn, op, "v"));
+    holo_buffer_ref reads[4] = {c.q, c.k, c.v, c.starts};
+    View rv[4], out;
+    HOLO_TRY(split_borrow(st, reads, rv, 4, c.output, &out, op));
+    HOLO_TRY(need(rv[0], qn * es, c.q.slot, op, "q"));
+    HOLO_TRY(need(rv[1], kn * es, c.k.slot, op, "k"));
+    HOLO_TRY(need(rv[2], vn * es, c.v.slot, op, "v"));
+    HOLO_TRY(need(rv[3], (uint64_t(c.batch) + 1) * 4, c.starts.slot, op, "starts"));
+    HOLO_TRY(need(out, uint64_t(c.tokens) * c.heads * D * es, c.output.slot, op, "output"));
+    if (!aligned(rv[0], es) || !aligned(rv[1], es) || !aligned(rv[2], es) || !aligned(out, es) ||
+        !aligned(rv[3], 4))
+        return fail(HOLO_ERR_UNSUPPORTED_OP, std::string(op) + ": operands must be element-aligned");
+    if (!be) return HOLO_OK;
+    OnDevice on(be->device);
+    a.pb = {reinterpret_cast<const uint32_t *>(rv[3].base), c.tokens, c.batch, be->dev_err};
+    a.q = rv[0].base, a.k = rv[1].base, a.v = rv[2].base, a.out = out.base;
+    a.H = c.heads, a.Hkv = hkv, a.D = c.head_dim;
+    a.score_scale = score_divisor(c.head_dim, c.scale_bits);
+    a.dtype = c.dtype;
+    return launched(holo::launch_attn_packed(a, be->stream), op);
+}
+
+// ------------------------------------------------------ KvBlockAppend ----
+int do_kv_block_append(holo_backend *be, const SlotTable &st, const holo_kv_block_append_call &c) {
+    const char *op = "kv_block_append";
+    if (c.bucket_rows == 0 || c.block_rows == 0 || c.head_dim == 0 || c.kv_heads == 0)
+        return fail(HOLO_ERR_UNSUPPORTED_OP,
+                    "kv_block_append: kv_heads, bucket_rows, block_rows and head_dim must be >= 1");
+    HOLO_TRY(packed_shape(op, c.tokens, c.batch, c.kv_heads, c.kv_heads, c.head_dim, c.dtype));
+    const uint64_t es = dtype_size(c.dtype), D = c.head_dim;
+    const uint64_t planes = uint64_t(c.batch) * c.kv_heads;
+    const uint64_t nb = (uint64_t(c.bucket_rows) + c.block_rows - 1) / c.block_rows;
+    if (uint64_t(c.bucket_rows) * D > (uint64_t(1) << 40))
+        return fail(HOLO_ERR_UNSUPPORTED_OP, "kv_block_append: bucket_rows * head_dim above 2^40");
+    const uint64_t qbytes = planes * c.bucket_rows * D, sbytes = planes * nb * 4;
+    const bool in_place = c.output.slot == c.cache.slot && c.output.offset == c.cache.offset &&
+                          c.output_scales.slot == c.cache_scales.slot &&
+                          c.output_scales.offset == c.cache_scales.offset;
+    holo::KvBlockArgs a;
+    a.stride = c.new_stride;
+    uint64_t nn = 0;
+    if (c.tokens) HOLO_TRY(strided(c.tokens, c.kv_heads * D, &a.stride, &nn, op, "new"));
+    holo_buffer_ref reads[5] = {c.new_rows_buf, c.starts, c.pos, c.cache, c.cache_scales};
+    View rv[5], oq, os;
+    // in place, the cache and its scales are the outputs themselves
+    HOLO_TRY(split_borrow(st, reads, rv, in_place ? 3 : 5, c.output, &oq, op));
+    HOLO_TRY(split_borrow(st, reads, rv, in_place ? 3 : 5, c.output_scales, &os, op));
+    if (overlaps(oq, os))
+        return fail(HOLO_ERR_SLOT_OUT_OF_RANGE, "kv_block_append: the cache overlaps its scales");
+    HOLO_TRY(need(rv[0], nn * es, c.new_rows_buf.slot, op, "new rows"));
+    HOLO_TRY(need(rv[1], (uint64_t(c.batch) + 1) * 4, c.starts.slot, op, "starts"));
+    HOLO_TRY(need(rv[2], uint64_t(c.batch) * 4, c.pos.slot, op, "pos"));
+    if (!in_place) {
+        HOLO_TRY(need(rv[3], qbytes, c.cache.slot, op, "cache"));
+        HOLO_TRY(need(rv[4], sbytes, c.cache_scales.slot, op, "cache_scales"));
+    }
+    HOLO_TRY(need(oq, qbytes, c.output.slot, op, "output"));
+    HOLO_TRY(need(os, sbytes, c.output_scales.slot, op, "output_scales"));
+    if (!aligned(rv[0], es) || !aligned(rv[1], 4) || !aligned(rv[2], 4) || !aligned(os, 4) ||
+        (!in_place && !aligned(rv[4], 4)))
+        return fail(HOLO_ERR_UNSUPPORTED_OP, std::string(op) + ": operands must be element-aligned");
+    if (!be) return HOLO_OK;
+    OnDevice on(be->device);
+    if (!in_place && qbytes) {
+        HOLO_TRY(launched(holo::launch_copy_bytes(rv[3].base, oq.base, qbytes, be->stream), op));
+        HOLO_TRY(launched(holo::launch_copy_bytes(rv[4].base, os.base, sbytes, be->stream), op));
+    }
+    if (c.tokens == 0 || c.batch == 0) return HOLO_OK;
+    a.pb = {reinterpret_cast<const uint32_t *>(rv[1].base), c.tokens, c.batch, be->dev_err};
+    a.nw = rv[0].base;
+    a.pos = reinterpret_cast<const uint32_t *>(rv[2].base);
+    a.cache = reinterpret_cast<int8_t *>(oq.base);
+    a.scales = reinterpret_cast<float *>(os.base);
+    a.Hkv = c.kv_heads, a.bucket = c.bucket_rows, a.block = c.block_rows, a.D = c.head_dim;
+    a.dtype = c.dtype;
+    return launched(holo::launch_kv_block_append(a, be->stream), op);
+}
+
+// -------------------------------------------------- AttentionI8Blocks ----
+int do_attn_i8_blocks(holo_backend *be, const SlotTable &st, const holo_attention_i8_blocks_call &c) {
+    const char *op = "attention_i8_blocks";
+    if (c.tokens == 0 || c.batch == 0 || c.heads == 0 || c.head_dim == 0) return HOLO_OK;
+    const uint32_t hkv = c.kv_heads == 0 ? c.heads : c.kv_heads;
+    HOLO_TRY(packed_shape(op, c.tokens, c.batch, c.heads, hkv, c.head_dim, c.dtype));
+    if (c.block_rows == 0 || c.bucket_rows == 0)
+        return fail(HOLO_ERR_UNSUPPORTED_OP, "attention_i8_blocks: bucket_rows and block_rows must be >= 1");
+    const uint64_t es = dtype_size(c.dtype), D = c.head_dim;
+    if (c.bucket_rows * D > (uint64_t(1) << 30))
+        return fail(HOLO_ERR_UNSUPPORTED_OP, "attention_i8_blocks: bucket_rows * head_dim above 2^30");
+    const uint64_t planes = uint64_t(c.batch) * hkv;
+    const uint64_t nb = (uint64_t(c.bucket_rows) + c.block_rows - 1) / c.block_rows;
+    holo::AttnBlocksArgs a;
+    a.q_stride = c.q_stride;
+    uint64_t qn;
+    HOLO_TRY(strided(c.tokens, c.heads * D, &a.q_stride, &qn, op, "q"));
+    holo_buffer_ref reads[7] = {c.q, c.k_cache, c.v_cache, c.k_scales, c.v_scales, c.starts, c.lens};
+    View rv[7], out;
+    HOLO_TRY(split_borrow(st, reads, rv, 7, c.output, &out, op));
+    HOLO_TRY(need(rv[0], qn * es, c.q.slot, op, "q"));
+    HOLO_TRY(need(rv[1], planes * c.bucket_rows * D, c.k_cache.slot, op, "k_cache"));
+    HOLO_TRY(need(rv[2], planes * c.bucket_rows * D, c.v_cache.slot, op, "v_cache"));
+    HOLO_TRY(need(rv[3], planes * nb * 4, c.k_scales.slot, op, "k_scales"));
+    HOLO_TRY(need(rv[4], planes * nb * 4, c.v_scales.slot, op, "v_scales"));
+    HOLO_TRY(need(rv[5], (uint64_t(c.batch) + 1) * 4, c.starts.slot, op, "starts"));
+    HOLO_TRY(need(rv[6], uint64_t(c.batch) * 4, c.lens.slot, op, "lens"));
+    HOLO_TRY(need(out, uint64_t(c.tokens) * c.heads * D * es, c.output.slot, op, "output"));
+    if (!aligned(rv[0], es) || !aligned(out, es) || !aligned(rv[3], 4) || !aligned(rv[4], 4) ||
+        !aligned(rv[5], 4) || !aligned(rv[6], 4))
+        return fail(HOLO_ERR_UNSUPPORTED_OP, std::string(op) + ": operands must be element-aligned");
+    if (!be) return HOLO_OK;
+    OnDevice on(be->device);
+    a.pb = {reinterpret_cast<const uint32_t *>(rv[5].base), c.tokens, c.batch, be->dev_err};
+    a.q = rv[0].base, a.out = out.base;
+    a.kq = reinterpret_cast<const int8_t *>(rv[1].base);
+    a.vq = reinterpret_cast<const int8_t *>(rv[2].base);
+    a.ks = reinterpret_cast<const float *>(rv[3].base);
+    a.vs = reinterpret_cast<const float *>(rv[4].base);
+    a.lens = reinterpret_cast<const uint32_t *>(rv[6].base);
+    a.H = c.heads, a.Hkv = hkv, a.bucket = c.bucket_rows, a.block = c.block_rows, a.D = c.head_dim;
+    a.score_scale = score_divisor(c.head_dim, c.scale_bits);
+    a.dtype = c.dtype;
+    HOLO_TRY(ensure_scratch(be, holo::attn_blocks_scratch_bytes(a), op));
+    return launched(holo::launch_attn_blocks(a, be->scratch, be->stream), op);
+}
+
+// ------------------------------------------------------ LogitsProcess ----
+int do_logits(holo_backend *be, const SlotTable &st, const holo_logits_process_call &c) {
+    const char *op = "logits_process";
+    if (c.dtype != HOLO_DTYPE_BF16 && c.dtype != HOLO_DTYPE_F16 && c.dtype != HOLO_DTYPE_F32)
+        return fail(HOLO_ERR_UNSUPPORTED_OP, "logits_process: logits must be bf16, f16 or f32");
+    if (c.rows == 0 || c.cols == 0) return HOLO_OK;
+    if (c.history_len > holo::kLogitsMaxHistory || c.biases > holo::kLogitsMaxBiases)
+        return fail(HOLO_ERR_UNSUPPORTED_OP, "logits_process: history_len above 524287 or biases above 4095");
+    if (c.cols > 0x7fffffffu || uint64_t(c.rows) * ((uint64_t(c.cols) + 4095) / 4096) > 0x7fffffffull)
+        return fail(HOLO_ERR_UNSUPPORTED_OP, "logits_process: too many rows and columns for one launch");
+    const uint64_t es = dtype_size(c.dtype), n = uint64_t(c.rows) * c.cols * es;
+    const bool hist = c.history_len != 0, bias = c.biases != 0;
+    const bool mask = c.mask.slot != HOLO_SLOT_ABSENT;
+    // absent operands stand as the logits in the list of reads
+    holo_buffer_ref reads[7] = {c.logits,
+                                hist ? c.history : c.logits,
+                                hist ? c.spans : c.logits,
+                                hist ? c.params : c.logits,
+                                bias ? c.bias_ids : c.logits,
+                                bias ? c.bias_values : c.logits,
+                                mask ? c.mask : c.logits};
+    View rv[7], out;
+    HOLO_TRY(split_borrow(st, reads, rv, 7, c.output, &out, op));
+    const uint64_t rows = c.rows;
+    HOLO_TRY(need(rv[0], n, c.logits.slot, op, "logits"));
+    HOLO_TRY(need(out, n, c.output.slot, op, "output"));
+    if (hist) {
+        HOLO_TRY(need(rv[1], rows * c.history_len * 4, c.history.slot, op, "history"));
+        HOLO_TRY(need(rv[2], rows * 8, c.spans.slot, op, "spans"));
+        HOLO_TRY(need(rv[3], rows * 12, c.params.slot, op, "params"));
+    }
+    if (bias) {
+        HOLO_TRY(need(rv[4], rows * c.biases * 4, c.bias_ids.slot, op, "bias_ids"));
+        HOLO_TRY(need(rv[5], rows * c.biases * 4, c.bias_values.slot, op, "bias_values"));
+    }
+    if (mask) HOLO_TRY(need(rv[6], rows * ((uint64_t(c.cols) + 31) / 32) * 4, c.mask.slot, op, "mask"));
+    if (!aligned(rv[0], es) || !aligned(out, es))
+        return fail(HOLO_ERR_UNSUPPORTED_OP, std::string(op) + ": operands must be element-aligned");
+    const bool used[7] = {false, hist, hist, hist, bias, bias, mask};
+    for (int i = 1; i < 7; ++i)
+        if (used[i] && !aligned(rv[i], 4))
+            return fail(HOLO_ERR_UNSUPPORTED_OP, std::string(op) + ": operands must be element-aligned");
+    if (!be) return HOLO_OK;
+    OnDevice on(be->device);
+    holo::LogitsArgs a;
+    a.logits = rv[0].base, a.out = out.base;
+    a.history = hist ? reinterpret_cast<const int32_t *>(rv[1].base) : nullptr;
+    a.spans = reinterpret_cast<const uint32_t *>(rv[2].base);
+    a.params = reinterpret_cast<const float *>(rv[3].base);
+    a.bias_ids = bias ? reinterpret_cast<const int32_t *>(rv[4].base) : nullptr;
+    a.bias_values = reinterpret_cast<const float *>(rv[5].base);
+    a.mask = mask ? reinterpret_cast<const uint32_t *>(rv[6].base) : nullptr;
+    a.rows = c.rows, a.cols = c.cols, a.history_len = c.history_len, a.biases = c.biases;
+    a.dtype = c.dtype;
+    return launched(holo::launch_logits(a, be->stream), op);
+}
+
 int dispatch_impl(holo_backend *be, const SlotTable &st, const holo_kernel_call *call) {
     if (!call) return fail(HOLO_ERR_DISPATCH, "dispatch: null call");
     switch (call->tag) {
@@ -1527,6 +1777,10 @@ int dispatch_impl(holo_backend *be, const SlotTable &st, const holo_kernel_call 
         case HOLO_OP_DECODE_ATTN_I8: return do_attn_i8(be, st, call->u.attn_i8);
         case HOLO_OP_ATTN_I8_ROWS:
             return do_attn_i8(be, st, call->u.attn_i8_rows.attn, call->u.attn_i8_rows.q_rows);
+        case HOLO_OP_ATTN_PACKED: return do_attn_packed(be, st, call->u.attn_packed);
+        case HOLO_OP_KV_BLOCK_APPEND: return do_kv_block_append(be, st, call->u.kv_block_append);
+        case HOLO_OP_ATTN_I8_BLOCKS: return do_attn_i8_blocks(be, st, call->u.attn_i8_blocks);
+        case HOLO_OP_LOGITS_PROCESS: return do_logits(be, st, call->u.logits_process);
         case HOLO_OP_TRANSPOSE: return do_transpose(be, st, call->u.transpose);
         case HOLO_OP_RESHAPE:
         case HOLO_OP_SLICE: return do_layout(be, st, call->tag, call->u.layout);
@@ -1836,6 +2090,83 @@ int decode_impl(const uint8_t *wire, size_t len, holo_kernel_call *out, size_t *
             if (out->tag == HOLO_OP_ATTN_I8_ROWS) out->u.attn_i8_rows.q_rows = r.get<uint32_t>();
             break;
         }
+        case HOLO_OP_ATTN_PACKED: {  // field order of holo_attention_packed_call
+            auto &c = out->u.attn_packed;
+            c.q = r.buf();
+            c.k = r.buf();
+            c.v = r.buf();
+            c.starts = r.buf();
+            c.output = r.buf();
+            c.tokens = r.get<uint32_t>();
+            c.batch = r.get<uint32_t>();
+            c.heads = r.get<uint32_t>();
+            c.kv_heads = r.get<uint32_t>();
+            c.head_dim = r.get<uint32_t>();
+            c.q_stride = r.get<uint32_t>();
+            c.k_stride = r.get<uint32_t>();
+            c.v_stride = r.get<uint32_t>();
+            c.scale_bits = r.get<uint32_t>();
+            c.dtype = r.get<uint8_t>();
+            break;
+        }
+        case HOLO_OP_KV_BLOCK_APPEND: {  // field order of holo_kv_block_append_call
+            auto &c = out->u.kv_block_append;
+            c.new_rows_buf = r.buf();
+            c.starts = r.buf();
+            c.pos = r.buf();
+            c.cache = r.buf();
+            c.cache_scales = r.buf();
+            c.output = r.buf();
+            c.output_scales = r.buf();
+            c.tokens = r.get<uint32_t>();
+            c.batch = r.get<uint32_t>();
+            c.kv_heads = r.get<uint32_t>();
+            c.bucket_rows = r.get<uint32_t>();
+            c.block_rows = r.get<uint32_t>();
+            c.head_dim = r.get<uint32_t>();
+            c.new_stride = r.get<uint32_t>();
+            c.dtype = r.get<uint8_t>();
+            break;
+        }
+        case HOLO_OP_ATTN_I8_BLOCKS: {  // field order of holo_attention_i8_blocks_call
+            auto &c = out->u.attn_i8_blocks;
+            c.q = r.buf();
+            c.k_cache = r.buf();
+            c.v_cache = r.buf();
+            c.k_scales = r.buf();
+            c.v_scales = r.buf();
+            c.starts = r.buf();
+            c.lens = r.buf();
+            c.output = r.buf();
+            c.tokens = r.get<uint32_t>();
+            c.batch = r.get<uint32_t>();
+            c.heads = r.get<uint32_t>();
+            c.kv_heads = r.get<uint32_t>();
+            c.bucket_rows = r.get<uint32_t>();
+            c.block_rows = r.get<uint32_t>();
+            c.head_dim = r.get<uint32_t>();
+            c.q_stride = r.get<uint32_t>();
+            c.scale_bits = r.get<uint32_t>();
+            c.dtype = r.get<uint8_t>();
+            break;
+        }
+        case HOLO_OP_LOGITS_PROCESS: {  // field order of holo_logits_process_call
+            auto &c = out->u.logits_process;
+            c.logits = r.buf();
+            c.history = r.buf();
+            c.spans = r.buf();
+            c.params = r.buf();
+            c.bias_ids = r.buf();
+            c.bias_values = r.buf();
+            c.mask = r.buf();
+            c.output = r.buf();
+            c.rows = r.get<uint32_t>();
+            c.cols = r.get<uint32_t>();
+            c.history_len = r.get<uint32_t>();
+            c.biases = r.get<uint32_t>();
+            c.dtype = r.get<uint8_t>();
+            break;
+        }
         case HOLO_OP_RESHAPE:
         case HOLO_OP_SLICE: {  // put_layout :681-686
             auto &c = out->u.layout;
@@ -2048,7 +2379,8 @@ int holo_hip_synchronize(holo_backend *be) {
     if (e != hipSuccess) return fail(HOLO_ERR_DISPATCH, std::string("synchronize: ") + hipGetErrorString(e));
     // refusals the kernels could only see on the device: bit 1 a Gather index out
     // of range, bit 2 a multi-row attention length past the ring, bit 4 a nonzero
-    // W8A8 zero point
+    // W8A8 zero point, bit 8 a packed batch's offsets, bit 16 an append past its
+    // bucket
     int flag = 0;
     e = hipMemcpy(&flag, be->dev_err, sizeof(int), hipMemcpyDeviceToHost);
     if (e != hipSuccess) return fail(HOLO_ERR_DISPATCH, std::string("synchronize: ") + hipGetErrorString(e));
@@ -2058,6 +2390,14 @@ int holo_hip_synchronize(holo_backend *be) {
             return fail(HOLO_ERR_SLOT_OUT_OF_RANGE,
                         "gather: an index is outside [-axis_dim, axis_dim) (reported by the device; "
                         "its output row was zeroed)");
+        if (flag & 8)
+            return fail(HOLO_ERR_SLOT_OUT_OF_RANGE,
+                        "packed batch: starts decreases or passes tokens (reported by the device; the "
+                        "call's outputs must be discarded)");
+        if (flag & 16)
+            return fail(HOLO_ERR_UNSUPPORTED_OP,
+                        "kv_block_append: rows at or past bucket_rows (reported by the device; they "
+                        "were dropped)");
         if (flag & 4)
             return fail(HOLO_ERR_UNSUPPORTED_OP,
                         "matmul_dequant: W8A8 requires symmetric per-channel i8/i4/e8cb within the k "

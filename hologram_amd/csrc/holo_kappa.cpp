@@ -239,6 +239,38 @@ bool op_signature(const holo_kernel_call &c, uint16_t *opcode, uint8_t params[64
         case HOLO_OP_ATTN_I8_ROWS:
             s = p_attn_i8(c.u.attn_i8_rows.attn), s.u32(c.u.attn_i8_rows.q_rows), op = 125;
             break;
+        // (q, k, v and the new rows may be views of one value: where a view starts is
+        // a parameter, so that calls over different views derive different labels)
+        case HOLO_OP_ATTN_PACKED: {
+            const auto &a = c.u.attn_packed;
+            s.u32(a.tokens).u32(a.batch).u32(a.heads).u32(a.kv_heads).u32(a.head_dim)
+                .u32(a.q_stride).u32(a.k_stride).u32(a.v_stride).u32(a.scale_bits).u8(a.dtype)
+                .u64(a.q.offset).u64(a.k.offset).u64(a.v.offset);
+            op = 126;
+            break;
+        }
+        case HOLO_OP_KV_BLOCK_APPEND: {
+            const auto &a = c.u.kv_block_append;
+            s.u32(a.tokens).u32(a.batch).u32(a.kv_heads).u32(a.bucket_rows).u32(a.block_rows)
+                .u32(a.head_dim).u32(a.new_stride).u8(a.dtype).u64(a.new_rows_buf.offset);
+            op = 127;
+            break;
+        }
+        case HOLO_OP_ATTN_I8_BLOCKS: {
+            const auto &a = c.u.attn_i8_blocks;
+            s.u32(a.tokens).u32(a.batch).u32(a.heads).u32(a.kv_heads).u32(a.bucket_rows)
+                .u32(a.block_rows).u32(a.head_dim).u32(a.q_stride).u32(a.scale_bits)
+                .u8(a.dtype)
+                .u64(a.q.offset);
+            op = 128;
+            break;
+        }
+        case HOLO_OP_LOGITS_PROCESS: {
+            const auto &a = c.u.logits_process;
+            s.u32(a.rows).u32(a.cols).u32(a.history_len).u32(a.biases).u8(a.dtype);
+            op = 129;
+            break;
+        }
         default: return false;
     }
     if (s.n > 64) return false;
@@ -319,6 +351,29 @@ bool label_operands(const holo_kernel_call &c, std::vector<uint32_t> *ins,
         case HOLO_OP_DECODE_ATTN_I8: case HOLO_OP_ATTN_I8_ROWS: {
             const auto &a = c.tag == HOLO_OP_ATTN_I8_ROWS ? c.u.attn_i8_rows.attn : c.u.attn_i8;
             r(a.q), r(a.k_cache), r(a.v_cache), r(a.k_scales), r(a.v_scales), r(a.lens), w(a.output);
+            break;
+        }
+        case HOLO_OP_ATTN_PACKED: {
+            const auto &a = c.u.attn_packed;
+            r(a.q), r(a.k), r(a.v), r(a.starts), w(a.output);
+            break;
+        }
+        case HOLO_OP_KV_BLOCK_APPEND: {
+            const auto &a = c.u.kv_block_append;
+            r(a.new_rows_buf), r(a.starts), r(a.pos), r(a.cache), r(a.cache_scales), w(a.output),
+            w(a.output_scales);
+            break;
+        }
+        case HOLO_OP_ATTN_I8_BLOCKS: {
+            const auto &a = c.u.attn_i8_blocks;
+            r(a.q), r(a.k_cache), r(a.v_cache), r(a.k_scales), r(a.v_scales), r(a.starts),
+            r(a.lens), w(a.output);
+            break;
+        }
+        case HOLO_OP_LOGITS_PROCESS: {
+            const auto &a = c.u.logits_process;
+            r(a.logits), r(a.history), r(a.spans), r(a.params), r(a.bias_ids), r(a.bias_values),
+            r(a.mask), w(a.output);
             break;
         }
         case HOLO_OP_ARGMAX: r(c.u.argmax.input), w(c.u.argmax.output); break;

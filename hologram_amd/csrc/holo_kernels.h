@@ -102,6 +102,70 @@ hipError_t launch_attn_valid(const AttnValidArgs &a, void *scratch, hipStream_t 
 bool attn_valid_mfma_applies(const AttnValidArgs &a);
 hipError_t launch_attn_valid_mfma(const AttnValidArgs &a, void *scratch, hipStream_t stream);
 
+// A packed batch: sequence b's rows are [starts[b], starts[b + 1]) of `tokens`.
+// Offsets that decrease or pass `tokens` raise bit 8 of *err; every kernel clamps
+// what it reads of them.
+constexpr uint32_t kPackedMaxDim = 1024;
+struct PackedBatch {
+    const uint32_t *starts;   // [batch + 1]
+    uint32_t tokens, batch;
+    int *err;
+};
+// attn_packed.hip — causal attention of a packed batch over its own K and V.
+struct AttnPackedArgs {
+    PackedBatch pb;
+    const void *q, *k, *v;            // [tokens, H, D], [tokens, Hkv, D]
+    void *out;                        // [tokens, H, D]
+    uint32_t H, Hkv, D;
+    uint32_t q_stride, k_stride, v_stride;   // elements a token
+    float score_scale;                // the divisor
+    uint8_t dtype;
+};
+hipError_t launch_attn_packed(const AttnPackedArgs &a, hipStream_t stream);
+// kv_blocks.hip — int8 append with one power-of-two scale a block of rows, in
+// place; bit 16 of *err for rows past the bucket.
+struct KvBlockArgs {
+    PackedBatch pb;
+    const void *nw;                   // [tokens, Hkv, D]
+    const uint32_t *pos;              // [batch]
+    int8_t *cache;                    // [batch * Hkv, bucket, D]
+    float *scales;                    // [batch * Hkv, ceil(bucket / block)]
+    uint32_t Hkv, bucket, block, D, stride;
+    uint8_t dtype;
+};
+hipError_t launch_kv_block_append(const KvBlockArgs &a, hipStream_t stream);
+// attn_blocks.hip — attention of a packed batch over that cache. `scratch`
+// holds the split keys' partials, attn_blocks_scratch_bytes() of them.
+struct AttnBlocksArgs {
+    PackedBatch pb;
+    const void *q;                    // [tokens, H, D]
+    const int8_t *kq, *vq;            // [batch * Hkv, bucket, D]
+    const float *ks, *vs;             // [batch * Hkv, ceil(bucket / block)]
+    const uint32_t *lens;             // [batch]
+    void *out;                        // [tokens, H, D]
+    uint32_t H, Hkv, bucket, block, D, q_stride;
+    float score_scale;
+    uint8_t dtype;
+};
+size_t attn_blocks_scratch_bytes(const AttnBlocksArgs &a);
+hipError_t launch_attn_blocks(const AttnBlocksArgs &a, void *scratch, hipStream_t stream);
+// logits.hip — penalties, biases and a mask on logits. Null history, bias_ids
+// and mask: none.
+constexpr uint32_t kLogitsMaxHistory = 524287, kLogitsMaxBiases = 4095;
+struct LogitsArgs {
+    const void *logits;
+    const int32_t *history;
+    const uint32_t *spans;
+    const float *params;
+    const int32_t *bias_ids;
+    const float *bias_values;
+    const uint32_t *mask;
+    void *out;
+    uint32_t rows, cols, history_len, biases;
+    uint8_t dtype;
+};
+hipError_t launch_logits(const LogitsArgs &a, hipStream_t stream);
+
 // quant.hip — MatMulDequant's output-major W8A8 GEMM (f32 A quantized per
 // row on the device, exact int32 dots, (acc as f32) * (scale_a * scales[j]),
 // then + residual and the fused activation), Dequantize and

@@ -192,6 +192,29 @@ void call_operands(const holo_kernel_call &c, std::vector<holo_buffer_ref> *read
             r(a.q); r(a.k_cache); r(a.v_cache); r(a.k_scales); r(a.v_scales); r(a.lens);
             w(a.output); break;
         }
+        case HOLO_OP_ATTN_PACKED: {
+            const auto &a = c.u.attn_packed;
+            r(a.q); r(a.k); r(a.v); r(a.starts); w(a.output);
+            break;
+        }
+        case HOLO_OP_KV_BLOCK_APPEND: {
+            const auto &a = c.u.kv_block_append;
+            r(a.new_rows_buf); r(a.starts); r(a.pos); r(a.cache); r(a.cache_scales); w(a.output);
+            w(a.output_scales);
+            break;
+        }
+        case HOLO_OP_ATTN_I8_BLOCKS: {
+            const auto &a = c.u.attn_i8_blocks;
+            r(a.q); r(a.k_cache); r(a.v_cache); r(a.k_scales); r(a.v_scales); r(a.starts);
+            r(a.lens); w(a.output);
+            break;
+        }
+        case HOLO_OP_LOGITS_PROCESS: {
+            const auto &a = c.u.logits_process;
+            r(a.logits); r(a.history); r(a.spans); r(a.params); r(a.bias_ids); r(a.bias_values);
+            r(a.mask); w(a.output);
+            break;
+        }
         default: break;
     }
 }
@@ -1271,13 +1294,18 @@ void elide_steps(holo_session *s, const std::vector<uint8_t> &is_output,
             const auto &k = c.u.kv_quant_append;
             mark(k.cache), mark(k.cache_scales), mark(k.output), mark(k.output_scales);
         }
+        if (c.tag == HOLO_OP_KV_BLOCK_APPEND) {
+            const auto &k = c.u.kv_block_append;
+            mark(k.cache), mark(k.cache_scales), mark(k.output), mark(k.output_scales);
+        }
     }
     for (const auto &a : s->aliases) {
         if (a.first < nslots) kv[a.first] = 1;
         if (a.second < nslots) kv[a.second] = 1;
     }
     auto is_kv_op = [](uint32_t tag) {
-        return tag == HOLO_OP_KV_CACHE_WRITE || tag == HOLO_OP_KV_QUANT_APPEND;
+        return tag == HOLO_OP_KV_CACHE_WRITE || tag == HOLO_OP_KV_QUANT_APPEND ||
+               tag == HOLO_OP_KV_BLOCK_APPEND;
     };
     // a slot only this step writes, that no port, constant or KV op touches
     auto plain = [&](uint32_t sl) {
@@ -1869,6 +1897,23 @@ plan_moves:
                 continue;
             if (k.new_rows_buf.slot == cq || k.new_rows_buf.slot == cs || k.pos.slot == cq || k.pos.slot == cs)
                 continue;
+            s->aliases.push_back({oq, cq});
+            s->aliases.push_back({os, cs});
+            k.output = k.cache;
+            k.output_scales = k.cache_scales;
+        } else if (call.tag == HOLO_OP_KV_BLOCK_APPEND) {
+            auto &k = call.u.kv_block_append;
+            const uint32_t cq = k.cache.slot, cs = k.cache_scales.slot;
+            const uint32_t oq = k.output.slot, os = k.output_scales.slot;
+            if (cq == HOLO_SLOT_ABSENT || cs == HOLO_SLOT_ABSENT || cq == oq || cs == os || cq == cs || readers[cq] != 1 || readers[cs] != 1 ||
+                is_output[cq] || is_output[cs] || is_const[cq] || is_const[cs] ||
+                k.cache.offset != 0 || k.cache_scales.offset != 0 || k.output.offset != 0 ||
+                k.output_scales.offset != 0)
+                continue;
+            bool apart = true;
+            for (const uint32_t r : {k.new_rows_buf.slot, k.starts.slot, k.pos.slot})
+                apart = apart && r != cq && r != cs;
+            if (!apart) continue;
             s->aliases.push_back({oq, cq});
             s->aliases.push_back({os, cs});
             k.output = k.cache;

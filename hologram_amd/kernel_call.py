@@ -70,6 +70,10 @@ D_KVQA = 122   # new: int8 quantize + append
 D_DAI8 = 123   # new: decode attention over an int8 cache
 D_ARGMAX = 124  # new: per-row argmax (the greedy pick of a decode step)
 D_AI8R = 125    # new: multi-row (prefill) form of D_DAI8
+D_APK = 126     # new: causal attention of a packed batch of prompts
+D_KVBA = 127    # new: int8 append, one scale a block of rows
+D_AI8B = 128    # new: attention over the cache D_KVBA fills
+D_LOGITS = 129  # new: penalties, biases and a mask on logits
 D_TRANSPOSE = 61
 D_RESHAPE = 60
 D_SLICE = 63
@@ -512,6 +516,120 @@ class AttentionI8RowsCall:
 
 
 @dataclass(frozen=True)
+class AttentionPackedCall:
+    """New (discriminant 126): causal attention of a packed batch of prompts over
+    their own K and V (include/holo_hip.h)."""
+    q: BufferRef
+    k: BufferRef
+    v: BufferRef
+    starts: BufferRef
+    output: BufferRef
+    tokens: int
+    batch: int
+    heads: int
+    kv_heads: int
+    head_dim: int
+    q_stride: int = 0
+    k_stride: int = 0
+    v_stride: int = 0
+    scale_bits: int = 0
+    dtype: int = DTYPE_BF16
+
+    def wire(self) -> bytes:
+        return (self.q.wire() + self.k.wire() + self.v.wire() + self.starts.wire()
+                + self.output.wire()
+                + struct.pack("<IIIIIIIIIB", self.tokens, self.batch, self.heads, self.kv_heads,
+                              self.head_dim, self.q_stride, self.k_stride, self.v_stride,
+                              self.scale_bits, self.dtype))
+
+
+@dataclass(frozen=True)
+class KvBlockAppendCall:
+    """New (discriminant 127): int8 append of a packed batch's rows, one
+    power-of-two scale for each block of rows (include/holo_hip.h)."""
+    new: BufferRef
+    starts: BufferRef
+    pos: BufferRef
+    cache: BufferRef
+    cache_scales: BufferRef
+    output: BufferRef
+    output_scales: BufferRef
+    tokens: int
+    batch: int
+    kv_heads: int
+    bucket_rows: int
+    block_rows: int
+    head_dim: int
+    new_stride: int = 0
+    dtype: int = DTYPE_BF16
+
+    def wire(self) -> bytes:
+        return (self.new.wire() + self.starts.wire() + self.pos.wire() + self.cache.wire()
+                + self.cache_scales.wire() + self.output.wire() + self.output_scales.wire()
+                + struct.pack("<IIIIIIIB", self.tokens, self.batch, self.kv_heads,
+                              self.bucket_rows, self.block_rows, self.head_dim, self.new_stride,
+                              self.dtype))
+
+
+@dataclass(frozen=True)
+class AttentionI8BlocksCall:
+    """New (discriminant 128): attention of a packed batch's rows over the cache
+    that KvBlockAppend fills (include/holo_hip.h)."""
+    q: BufferRef
+    k_cache: BufferRef
+    v_cache: BufferRef
+    k_scales: BufferRef
+    v_scales: BufferRef
+    starts: BufferRef
+    lens: BufferRef
+    output: BufferRef
+    tokens: int
+    batch: int
+    heads: int
+    kv_heads: int
+    bucket_rows: int
+    block_rows: int
+    head_dim: int
+    q_stride: int = 0
+    scale_bits: int = 0
+    dtype: int = DTYPE_BF16
+
+    def wire(self) -> bytes:
+        return (self.q.wire() + self.k_cache.wire() + self.v_cache.wire() + self.k_scales.wire()
+                + self.v_scales.wire() + self.starts.wire() + self.lens.wire()
+                + self.output.wire()
+                + struct.pack("<IIIIIIIIIB", self.tokens, self.batch, self.heads, self.kv_heads,
+                              self.bucket_rows, self.block_rows, self.head_dim, self.q_stride,
+                              self.scale_bits, self.dtype))
+
+
+@dataclass(frozen=True)
+class LogitsProcessCall:
+    """New (discriminant 129): penalties, biases and a mask on logits, before the
+    pick (include/holo_hip.h); NO_BUFFER for what a batch does not use."""
+    logits: BufferRef
+    history: BufferRef
+    spans: BufferRef
+    params: BufferRef
+    bias_ids: BufferRef
+    bias_values: BufferRef
+    mask: BufferRef
+    output: BufferRef
+    rows: int
+    cols: int
+    history_len: int
+    biases: int
+    dtype: int = DTYPE_BF16
+
+    def wire(self) -> bytes:
+        return (self.logits.wire() + self.history.wire() + self.spans.wire()
+                + self.params.wire() + self.bias_ids.wire() + self.bias_values.wire()
+                + self.mask.wire() + self.output.wire()
+                + struct.pack("<IIIIB", self.rows, self.cols, self.history_len, self.biases,
+                              self.dtype))
+
+
+@dataclass(frozen=True)
 class TransposeCall:
     """kernel_call.rs:487-499: output axis i is input axis perm[i]."""
     input: BufferRef
@@ -550,7 +668,8 @@ _NAMES = {D_RESHAPE: "Reshape", D_SLICE: "Slice", D_ADD: "Add", D_MUL: "Mul", D_
           D_GATHER: "Gather", D_ARGMAX: "ArgMax", D_SIGMOID: "Sigmoid", D_TANH: "Tanh", D_GELU: "Gelu", D_SILU: "Silu", D_EXP: "Exp",
           D_MATMUL: "MatMul", D_MMA: "MatMulActivation", D_MMADD: "MatMulAdd",
           D_MMAA: "MatMulAddActivation", D_KVWR: "KvCacheWrite", D_KVQA: "KvQuantAppend",
-          D_DECATTN: "DecodeAttention", D_DAVL: "DecodeAttentionValid", D_DAI8: "DecodeAttentionI8", D_AI8R: "AttentionI8Rows", D_TRANSPOSE: "Transpose"}
+          D_DECATTN: "DecodeAttention", D_DAVL: "DecodeAttentionValid", D_DAI8: "DecodeAttentionI8", D_AI8R: "AttentionI8Rows", D_TRANSPOSE: "Transpose",
+          D_APK: "AttentionPacked", D_KVBA: "KvBlockAppend", D_AI8B: "AttentionI8Blocks", D_LOGITS: "LogitsProcess"}
 
 
 @dataclass(frozen=True)
@@ -677,6 +796,22 @@ class KernelCall:
         return cls(D_AI8R, c)
 
     @classmethod
+    def AttentionPacked(cls, c: AttentionPackedCall) -> "KernelCall":  # noqa: N802
+        return cls(D_APK, c)
+
+    @classmethod
+    def KvBlockAppend(cls, c: KvBlockAppendCall) -> "KernelCall":  # noqa: N802
+        return cls(D_KVBA, c)
+
+    @classmethod
+    def AttentionI8Blocks(cls, c: AttentionI8BlocksCall) -> "KernelCall":  # noqa: N802
+        return cls(D_AI8B, c)
+
+    @classmethod
+    def LogitsProcess(cls, c: LogitsProcessCall) -> "KernelCall":  # noqa: N802
+        return cls(D_LOGITS, c)
+
+    @classmethod
     def Transpose(cls, c: TransposeCall) -> "KernelCall":  # noqa: N802
         return cls(D_TRANSPOSE, c)
 
@@ -741,6 +876,26 @@ class KernelCall:
                 p.output_scales.c(), p.planes, p.bucket_rows, p.new_rows, p.head_dim, p.dtype)
         elif isinstance(p, AttentionI8RowsCall):
             kc.u.attn_i8_rows = _ffi.AttentionI8RowsCallC(_attn_c(p.attn), p.q_rows)
+        elif isinstance(p, AttentionPackedCall):
+            kc.u.attn_packed = _ffi.AttentionPackedCallC(
+                p.q.c(), p.k.c(), p.v.c(), p.starts.c(), p.output.c(), p.tokens, p.batch,
+                p.heads, p.kv_heads, p.head_dim, p.q_stride, p.k_stride, p.v_stride,
+                p.scale_bits, p.dtype)
+        elif isinstance(p, KvBlockAppendCall):
+            kc.u.kv_block_append = _ffi.KvBlockAppendCallC(
+                p.new.c(), p.starts.c(), p.pos.c(), p.cache.c(), p.cache_scales.c(),
+                p.output.c(), p.output_scales.c(), p.tokens, p.batch, p.kv_heads, p.bucket_rows,
+                p.block_rows, p.head_dim, p.new_stride, p.dtype)
+        elif isinstance(p, AttentionI8BlocksCall):
+            kc.u.attn_i8_blocks = _ffi.AttentionI8BlocksCallC(
+                p.q.c(), p.k_cache.c(), p.v_cache.c(), p.k_scales.c(), p.v_scales.c(),
+                p.starts.c(), p.lens.c(), p.output.c(), p.tokens, p.batch, p.heads, p.kv_heads,
+                p.bucket_rows, p.block_rows, p.head_dim, p.q_stride, p.scale_bits, p.dtype)
+        elif isinstance(p, LogitsProcessCall):
+            kc.u.logits_process = _ffi.LogitsProcessCallC(
+                p.logits.c(), p.history.c(), p.spans.c(), p.params.c(), p.bias_ids.c(),
+                p.bias_values.c(), p.mask.c(), p.output.c(), p.rows, p.cols, p.history_len,
+                p.biases, p.dtype)
         elif isinstance(p, TransposeCall):
             rank = len(p.dims)
             kc.u.transpose = _ffi.TransposeCallC(
@@ -838,6 +993,10 @@ _FLAT = {cls: _flat_form(ctype) for cls, ctype in (
     (DecodeAttentionCall, _ffi.DecodeAttentionCallC),
     (DecodeAttentionValidCall, _ffi.DecodeAttentionValidCallC),
     (DecodeAttentionI8Call, _ffi.DecodeAttentionI8CallC),
+    (AttentionPackedCall, _ffi.AttentionPackedCallC),
+    (KvBlockAppendCall, _ffi.KvBlockAppendCallC),
+    (AttentionI8BlocksCall, _ffi.AttentionI8BlocksCallC),
+    (LogitsProcessCall, _ffi.LogitsProcessCallC),
     (MatMulDequantCall, _ffi.MatMulDequantCallC))}
 
 

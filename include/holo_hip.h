@@ -98,6 +98,10 @@ typedef enum holo_status {
 #define HOLO_OP_DECODE_ATTN_I8 123u       /* new: GQA decode over an int8 cache */
 #define HOLO_OP_ARGMAX 124u               /* new: per-row argmax (greedy pick)  */
 #define HOLO_OP_ATTN_I8_ROWS 125u         /* new: multi-row (prefill) form of 123 */
+#define HOLO_OP_ATTN_PACKED 126u          /* new: causal attention of a packed batch of prompts */
+#define HOLO_OP_KV_BLOCK_APPEND 127u      /* new: int8 append, one scale a block of rows */
+#define HOLO_OP_ATTN_I8_BLOCKS 128u       /* new: attention over the cache 127 fills */
+#define HOLO_OP_LOGITS_PROCESS 129u       /* new: penalties, biases and a mask on logits */
 #define HOLO_OP_TRANSPOSE 61u             /* Transpose (kernel_codec.rs:80)     */
 #define HOLO_OP_RESHAPE 60u               /* Reshape (kernel_codec.rs:79, D_RESHAPE) */
 #define HOLO_OP_SLICE 63u                 /* Slice (kernel_codec.rs:82, D_SLICE)     */
@@ -415,6 +419,124 @@ typedef struct holo_attention_i8_rows_call {
     uint32_t q_rows;
 } holo_attention_i8_rows_call;
 
+/* The packed batch of the next three calls: the rows of `batch` sequences lie
+ * end to end, sequence b's at rows [starts[b], starts[b + 1]) of `tokens`.
+ * starts is u32 [batch + 1], device-resident and non-decreasing, with
+ * starts[batch] <= tokens; a sequence may be empty. Rows outside every
+ * sequence (before starts[0], from starts[batch] on) take no part and their
+ * output rows stay as they were. Offsets that decrease or pass `tokens` are
+ * reported (SlotOutOfRange) by the next holo_hip_synchronize; no access leaves
+ * the operands, and the call's outputs are to be discarded. */
+
+/* New (tag 126): causal grouped-query attention of a packed batch of prompts
+ * over their own K and V, all of `dtype` (bf16, f16 or f32). q is [tokens,
+ * heads, head_dim], k and v [tokens, kv_heads, head_dim], output [tokens, heads,
+ * head_dim]. Row t of a sequence sees its rows 0..t, head h reads kv head h /
+ * (heads / kv_heads): scores dot(q, k) / s with s as in DecodeAttentionValid,
+ * f32 softmax, the result rounded to nearest. q_stride, k_stride and v_stride
+ * are the elements from one token to the next (0: tight), so that q, k and v
+ * may be views of one projection's output. What an invisible row holds, NaN and
+ * infinity too, does not reach a result. kv_heads 0 means heads;
+ * head_dim <= 1024. */
+typedef struct holo_attention_packed_call {
+    holo_buffer_ref q;
+    holo_buffer_ref k;
+    holo_buffer_ref v;
+    holo_buffer_ref starts;
+    holo_buffer_ref output;
+    uint32_t tokens, batch, heads, kv_heads, head_dim;
+    uint32_t q_stride, k_stride, v_stride;
+    uint32_t scale_bits;
+    uint8_t dtype;
+} holo_attention_packed_call;
+
+/* New (tag 127): int8 append of a packed batch's new K (or V) rows, [tokens,
+ * kv_heads, head_dim] of bf16, f16 or f32 (new_stride elements from one token
+ * to the next, 0: tight), to a cache int8 [batch * kv_heads, bucket_rows,
+ * head_dim] with one f32 scale for each block of block_rows rows, scales
+ * [batch * kv_heads, ceil(bucket_rows / block_rows)]. Row j of sequence b takes
+ * row pos[b] + j of its planes (pos u32 [batch], device-resident; no ring: rows
+ * at or past bucket_rows are dropped, and reported (UnsupportedOp) by the next
+ * holo_hip_synchronize).
+ * A block's scale is the least power of two 2^e, e >= -126, with
+ * max|x| <= 127 * 2^e over the rows written to it (0 if all are zero); where the
+ * block holds rows before pos[b], also at least the scale it has, and if that
+ * grows, those rows are rounded again, q = rne(q * (old / new)). A new value is
+ * q = rne(x / scale). Powers of two keep every quotient exact and let a scale
+ * grow only by doublings, so rows appended one at a time are rounded again
+ * rarely. A NaN or infinite value makes its block's scale NaN: the block reads
+ * as NaN until a row is appended at its first row again. Rows at and past
+ * pos[b] that this call does not write keep their bytes; a block's scale is no
+ * input where pos[b] is its first row.
+ *   output == cache and output_scales == cache_scales (same slot and offset):
+ *       in place; otherwise the caches are copied first. */
+typedef struct holo_kv_block_append_call {
+    holo_buffer_ref new_rows_buf;
+    holo_buffer_ref starts;
+    holo_buffer_ref pos;
+    holo_buffer_ref cache;
+    holo_buffer_ref cache_scales;
+    holo_buffer_ref output;
+    holo_buffer_ref output_scales;
+    uint32_t tokens, batch, kv_heads, bucket_rows, block_rows, head_dim;
+    uint32_t new_stride;
+    uint8_t dtype;
+} holo_kv_block_append_call;
+
+/* New (tag 128): attention of a packed batch's rows q [tokens, heads, head_dim]
+ * (q_stride elements from one token to the next, 0: tight) over int8 K and V
+ * caches laid out as 127 writes them; any f32 block scales. Row t of the n rows
+ * of sequence b sees the first lens[b] - (n - 1 - t) rows of its planes, at
+ * least 0 and at most bucket_rows (lens u32 [batch], device-resident: the
+ * visible length of the sequence's last row), so one row a sequence is a decode
+ * step and many are a prompt's next chunk, whose own rows were appended before.
+ * Scores, softmax and rounding as in 126; a row that sees no key is zeros. What
+ * an invisible row or block scale holds does not reach a result. dtype (q,
+ * output): bf16, f16 or f32; kv_heads 0 means heads; head_dim <= 1024. */
+typedef struct holo_attention_i8_blocks_call {
+    holo_buffer_ref q;
+    holo_buffer_ref k_cache;
+    holo_buffer_ref v_cache;
+    holo_buffer_ref k_scales;
+    holo_buffer_ref v_scales;
+    holo_buffer_ref starts;
+    holo_buffer_ref lens;
+    holo_buffer_ref output;
+    uint32_t tokens, batch, heads, kv_heads, bucket_rows, block_rows, head_dim;
+    uint32_t q_stride;
+    uint32_t scale_bits;
+    uint8_t dtype;
+} holo_attention_i8_blocks_call;
+
+/* New (tag 129): what a request's sampling rules do to its logits before the
+ * pick (124): out[r][c] from logits [rows, cols] of bf16, f16 or f32, in f32
+ * and rounded to nearest once:
+ *   x = logits[r][c]
+ *   c among the row's history:            x = x > 0 ? x / rep : x * rep
+ *   c generated n >= 1 times:             x = x - (freq * n + pres)
+ *   each of the row's biases for c:       x = x + bias, in the list's order
+ *   mask given and its bit of c clear:    x = -inf
+ * history is i32 [rows, history_len] token ids, of which the first
+ * min(spans[r][1], history_len) count, the first spans[r][0] of those as prompt
+ * (no generated tokens); spans u32 [rows, 2]; params f32 [rows, 3]: rep, freq,
+ * pres. bias_ids i32 and bias_values f32 are [rows, biases]. Ids outside
+ * [0, cols) are passed over. mask: u32 [rows, ceil(cols / 32)], bit c % 32 of
+ * word c / 32. history (with spans and params; history_len 0), the bias pair
+ * (biases 0) and the mask may be absent. An element that no rule names keeps
+ * its bits. history_len <= 524287, biases <= 4095. */
+typedef struct holo_logits_process_call {
+    holo_buffer_ref logits;
+    holo_buffer_ref history;
+    holo_buffer_ref spans;
+    holo_buffer_ref params;
+    holo_buffer_ref bias_ids;
+    holo_buffer_ref bias_values;
+    holo_buffer_ref mask;
+    holo_buffer_ref output;
+    uint32_t rows, cols, history_len, biases;
+    uint8_t dtype;
+} holo_logits_process_call;
+
 /* TransposeCall, kernel_call.rs:487-499 (transpose_float,
  * src/cpu/float_kernels.rs:2980-3028): output axis i is input axis perm[i] of
  * the row-major input of shape dims[0..rank). rank 1..8; f16/bf16/f32 elements;
@@ -467,6 +589,10 @@ typedef struct holo_kernel_call {
         holo_dequant_activation_call dequant_act;
         holo_decode_attention_i8_call attn_i8;
         holo_attention_i8_rows_call attn_i8_rows;
+        holo_attention_packed_call attn_packed;
+        holo_kv_block_append_call kv_block_append;
+        holo_attention_i8_blocks_call attn_i8_blocks;
+        holo_logits_process_call logits_process;
         holo_transpose_call transpose;
         holo_layout_call layout;
     } u;
