@@ -4,6 +4,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 #include "holo_kernels.h"
 #include "packed_batch.h"
 
@@ -11,6 +13,326 @@ namespace holo {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+
+// ------------------------------------------------------------ tiled form ----
+// bf16 and f16 rows. A sequence's n * G query rows of a kv head (G = H / Hkv; row
+// r = token r / G, head r % G) go 128 to a workgroup, 32 to a wavefront, over
+// 64-key tiles of the sequence, staged through registers a tile ahead into one of
+// two LDS buffers while the other is multiplied. Per tile and wavefront:
+//     S^T[64 keys x 32 rows] = K . Q^T    32x32x16, a row is a lane column
+//     causal limit, online softmax in f32 (a row's keys are in its lane and in
+//                                         the lane 32 apart)
+//     O^T[DP x 32 rows] += V^T . P^T      32x32x16, P rounded to the rows' type:
+//                                         the product the type can take, each
+//                                         weight off by half a step at most, as the
+//                                         result itself is; the sum l holds them
+//                                         unrounded in f32
+// f16 weights are held as 2^15 p (l too, so the quotient is the same), which keeps
+// all down to 2^-29 p clear of f16's subnormals.
+// Sequence s owns places [floor(starts[s] G / 128) + s, floor(starts[s + 1] G / 128)
+// + s + 1) of the grid: as many as its row tiles or more, so no prefix sum is
+// needed. Neighbouring workgroups take the kv heads of one place, so that with
+// eight of them an XCD's L2 holds one head's K and V; late places, which see the
+// most keys, go first.
+// A masked key's weight is 0, and 0 times a V that is not finite is NaN: in a tile
+// that some row does not see to its end such elements are staged as 0, and then
+// added by the rows that see their keys (add_odd); the other rows' bits are what
+// they are without them.
+constexpr uint32_t kRows = 128, kKeys = 64;
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef short i16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+typedef __attribute__((address_space(3))) uint8_t lds_u8;
+
+// A workgroup barrier over LDS only: the loads in flight are not waited for.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4));   // lgkmcnt(0)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+template <class E>
+__device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+    if constexpr (std::is_same_v<E, Bf16>)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// Two weights narrowed to nearest.
+template <class E>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if constexpr (std::is_same_v<E, Bf16>) {
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, bf16x2{__bf16(lo), __bf16(hi)});
+    } else {
+        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, f16x2{_Float16(lo), _Float16(hi)});
+    }
+}
+
+template <class E, int DP>
+__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void packed_tile_kernel(AttnPackedArgs a, float mul,
+                                                                           uint32_t places) {
+    constexpr int RB = 2 * DP, NK = DP / 16, DB = DP / 32, CT = DP / 32;   // CT: 16-byte chunks a thread stages
+    constexpr float kUp = std::is_same_v<E, F16> ? 15.0f : 0.0f;
+    struct Tile {
+        uint8_t k[kKeys * RB], v[kKeys * RB];
+    };
+    __shared__ __attribute__((aligned(1024))) Tile tl0, tl1;
+    __shared__ uint32_t odd_v[2][4];
+    auto swz_k = [](uint32_t row) { return DP >= 128 ? (row & 15u) : ((row >> 1) & 7u); };
+    auto swz_v = [](uint32_t row) { return DP >= 128 ? 4u * (row & 3u) : 4u * ((row >> 1) & 1u); };
+
+    if (blockIdx.x == 0) check_starts(a.pb);
+    const uint32_t G = a.H / a.Hkv, kh = blockIdx.x % a.Hkv, place = places - 1 - blockIdx.x / a.Hkv;
+    const uint32_t b = last_at_most(a.pb.batch, place, [&](uint32_t s) {
+        return uint64_t(start_of(a.pb, s)) * G / kRows + s;
+    });
+    const uint32_t t0 = pk_uni(start_of(a.pb, b)), t1 = pk_uni(start_of(a.pb, b + 1));
+    const uint64_t first = uint64_t(t0) * G / kRows + b;
+    if (t1 <= t0 || place < first) return;
+    const uint64_t R = uint64_t(t1 - t0) * G, r0 = (place - first) * kRows;
+    if (r0 >= R) return;
+    const int tid = threadIdx.x, lane = tid & 63, lr = lane & 31, lg = lane >> 5;
+    const uint32_t wave = pk_uni(uint32_t(tid) >> 6);
+    // token of a row, the last one's past the end
+    auto token = [&](uint64_t r) { return uint32_t((r < R ? r : R - 1) / G); };
+    const uint64_t wr0 = r0 + 32 * wave, row = wr0 + lr < R ? wr0 + lr : R - 1;
+    const uint32_t lim = uint32_t(row / G) + 1;
+    const uint32_t kmin = pk_uni(token(r0) + 1), kmax = pk_uni(token(r0 + kRows - 1) + 1);
+    const uint32_t wmin = pk_uni(token(wr0) + 1), wmax = pk_uni(token(wr0 + 31) + 1);
+    const bool live = pk_uni(wr0 < R);   // the wavefront has rows
+
+    // K and V: key tid / 4 of the tile, chunks tid % 4 + 4 i of its row. A resource a
+    // tile, so that offsets stay small and rows past the sequence read as zeros, as
+    // chunks past D do.
+    typedef typename E::T T;
+    const T *kp = static_cast<const T *>(a.k) + uint64_t(t0) * a.k_stride + uint64_t(kh) * a.D;
+    const T *vp = static_cast<const T *>(a.v) + uint64_t(t0) * a.v_stride + uint64_t(kh) * a.D;
+    const uint32_t key = uint32_t(tid) >> 2, part = uint32_t(tid) & 3u, n = t1 - t0;
+    u32x4 kr[CT], vr[CT];
+    uint32_t koff[CT], voff[CT];
+#pragma unroll
+    for (int i = 0; i < CT; ++i) {
+        const bool in = 8 * (part + 4 * i) < a.D;
+        koff[i] = in ? (key * a.k_stride + 8 * (part + 4 * i)) * 2u : 0xfffffff0u;
+        voff[i] = in ? (key * a.v_stride + 8 * (part + 4 * i)) * 2u : 0xfffffff0u;
+    }
+    auto fetch = [&](uint32_t j0) {
+        const uint32_t left = j0 < n ? (n - j0 < kKeys ? n - j0 : kKeys) : 0u;
+        const uint64_t at = j0 < n ? j0 : 0u;
+        const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(kp + at * a.k_stride), 0,
+                                                          left ? int(((left - 1) * a.k_stride + a.D) * 2u) : 0, 0x00020000);
+        const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(vp + at * a.v_stride), 0,
+                                                          left ? int(((left - 1) * a.v_stride + a.D) * 2u) : 0, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < CT; ++i) kr[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, koff[i], 0, 0));
+#pragma unroll
+        for (int i = 0; i < CT; ++i) vr[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, voff[i], 0, 0));
+    };
+    fetch(0);
+
+    u32x4 qf[NK];
+    {
+        const T *q = static_cast<const T *>(a.q) + (t0 + row / G) * a.q_stride + (uint64_t(kh) * G + row % G) * a.D;
+#pragma unroll
+        for (int k = 0; k < NK; ++k) {
+            const uint32_t d = 16 * k + 8 * lg;
+            qf[k] = u32x4{0, 0, 0, 0};
+            if (d < a.D) qf[k] = *reinterpret_cast<const u32x4 *>(q + d);
+        }
+    }
+
+    uint32_t kw[CT], vw[CT];
+#pragma unroll
+    for (int i = 0; i < CT; ++i) {
+        kw[i] = key * RB + (((part + 4u * i) ^ swz_k(key)) * 16u);
+        vw[i] = key * RB + (((part + 4u * i) ^ swz_v(key)) * 16u);
+    }
+    // (one of) a pair of f16 or bf16 with all exponent bits set
+    constexpr uint32_t kExp = std::is_same_v<E, Bf16> ? 0x7f80u : 0x7c00u;
+    auto odd = [](uint32_t w) { return (w & kExp) == kExp || ((w >> 16) & kExp) == kExp; };
+    auto put = [&](Tile &tl, uint32_t *flag, uint32_t j0) {
+        if (j0 + kKeys > kmin) {   // some row does not see all of it
+            bool any = false;
+#pragma unroll
+            for (int i = 0; i < CT; ++i)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) any |= odd(vr[i][w]);
+            if (__builtin_expect(any, 0)) {
+#pragma unroll
+                for (int i = 0; i < CT; ++i)
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        uint32_t x = vr[i][w];
+                        x = (x & kExp) == kExp ? x & 0xffff0000u : x;
+                        vr[i][w] = ((x >> 16) & kExp) == kExp ? x & 0xffffu : x;
+                    }
+            }
+            const bool found = __ballot(any) != 0;
+            if (lane == 0) flag[wave] = found;
+        }
+#pragma unroll
+        for (int i = 0; i < CT; ++i) {
+            *reinterpret_cast<u32x4 *>(tl.k + kw[i]) = kr[i];
+            *reinterpret_cast<u32x4 *>(tl.v + vw[i]) = vr[i];
+        }
+    };
+
+    f32x16 o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+    const uint32_t g16 = uint32_t(lane) >> 4, r16 = uint32_t(lane) & 15u;
+    const uint32_t vrow = 4u * (g16 >> 1) + (r16 >> 2);
+    const uint32_t vchunk = 2u * (g16 & 1u) + ((r16 & 3u) >> 1);
+
+    // The elements that `put` left out, for the rows that see their keys: an infinity
+    // or NaN with a weight above 0 is the sum it joins.
+    auto add_odd = [&](uint32_t j0) __attribute__((always_inline)) {
+#pragma unroll 1
+        for (uint32_t j = j0; j < j0 + kKeys && j < n; ++j)
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const uint32_t dim = 32u * d + 8u * c + 4u * lg;
+                    if (j >= lim || dim >= a.D) continue;
+                    const uint2 v = *reinterpret_cast<const uint2 *>(vp + uint64_t(j) * a.v_stride + dim);
+                    const uint16_t x[4] = {uint16_t(v.x), uint16_t(v.x >> 16), uint16_t(v.y), uint16_t(v.y >> 16)};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (odd(x[e])) o[d][4 * c + e] += E::widen(x[e]);
+                }
+    };
+
+    // one tile's products; `full`: every row of the wavefront sees all of it
+    auto tile_work = [&](const Tile &tl, const uint32_t *flag, uint32_t j0, bool full) {
+        const lds_u8 *kb0 = (const lds_u8 *)tl.k, *vb0 = (const lds_u8 *)tl.v;
+        f32x16 s[2];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[kb][r] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NK; ++k)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                const u32x4 kf = *reinterpret_cast<const lds_u32x4 *>(
+                    kb0 + (32u * kb + lr) * RB + ((uint32_t(2 * k + lg) ^ swz_k(lr)) * 16u));
+                s[kb] = mfma<E>(kf, qf[k], s[kb]);
+            }
+        float mt = -INFINITY;
+        if (!full) {
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    s[kb][r] = j0 + 32u * kb + 8u * (r >> 2) + 4u * lg + (r & 3) < lim ? s[kb][r] : -INFINITY;
+        }
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[kb][r]);
+        {
+            const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(mt), __float_as_uint(mt), false, false);
+            mt = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * mul;
+        }
+        const float mn = fmaxf(m, mt);
+        if (__any(mn > m)) {
+            const float al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            l *= al;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) o[d] *= al;
+            m = mn;
+        }
+        const float ref = (m == -INFINITY ? 0.0f : m) - kUp;
+        u32x4 pf[4];
+#pragma unroll
+        for (int st = 0; st < 4; ++st)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                float p[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int r = 8 * (st & 1) + 2 * c + e;
+                    p[e] = __builtin_amdgcn_exp2f(fmaf(s[st >> 1][r], mul, -ref));
+                    l += p[e];
+                }
+                pf[st][c] = pack2<E>(p[0], p[1]);
+            }
+#pragma unroll
+        for (int st = 0; st < 4; ++st)
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                const lds_u8 *p = vb0 + (16u * st + vrow) * RB + ((vchunk + 4u * d) ^ swz_v(vrow)) * 16u +
+                                  (r16 & 1u) * 8u;
+                const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    reinterpret_cast<lds_i16x4 *>(const_cast<lds_u8 *>(p)));
+                const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    reinterpret_cast<lds_i16x4 *>(const_cast<lds_u8 *>(p + 8u * RB)));
+                const u32x4 vf = __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+                o[d] = mfma<E>(vf, pf[st], o[d]);
+            }
+        if (!full && __builtin_expect(flag[0] | flag[1] | flag[2] | flag[3], 0)) add_odd(j0);
+    };
+    auto step = [&](const Tile &tl, const uint32_t *flag, Tile &next, uint32_t *next_flag, uint32_t j0) {
+        lds_barrier();     // this tile is in its buffer, the other buffer's readers are done
+        if (j0 + kKeys < kmax) {
+            put(next, next_flag, j0 + kKeys);
+            fetch(j0 + 2 * kKeys);
+        }
+        if (live && j0 < wmax) tile_work(tl, flag, j0, j0 + kKeys <= wmin);
+    };
+    put(tl0, odd_v[0], 0);
+    fetch(kKeys);
+    for (uint32_t j0 = 0; j0 < kmax; j0 += 2 * kKeys) {
+        step(tl0, odd_v[0], tl1, odd_v[1], j0);
+        if (j0 + kKeys < kmax) step(tl1, odd_v[1], tl0, odd_v[0], j0 + kKeys);
+    }
+    l += __shfl_xor(l, 32, 64);
+    if (wr0 + lr >= R) return;
+    // O^T: a lane holds dims 32 d + 8 c + 4 lg + i of its row
+    T *out = static_cast<T *>(a.out) + ((t0 + row / G) * a.H + uint64_t(kh) * G + row % G) * a.D;
+    const float inv = 1.0f / l;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const uint32_t dim = 32 * d + 8 * c + 4 * lg;
+            if (dim < a.D)
+                *reinterpret_cast<uint2 *>(out + dim) =
+                    make_uint2(pack2<E>(o[d][4 * c] * inv, o[d][4 * c + 1] * inv),
+                               pack2<E>(o[d][4 * c + 2] * inv, o[d][4 * c + 3] * inv));
+        }
+}
+
+// What the tiles take: 16-byte rows of q, k, v and out, offsets within a tile below
+// 2^31 bytes.
+bool tiles_apply(const AttnPackedArgs &a) {
+    auto at16 = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+    const uint32_t far = a.k_stride > a.v_stride ? a.k_stride : a.v_stride;
+    return a.dtype != 8 && a.D % 8 == 0 && a.D <= 256 && a.q_stride % 8 == 0 && a.k_stride % 8 == 0 &&
+           a.v_stride % 8 == 0 && at16(a.q) && at16(a.k) && at16(a.v) && at16(a.out) && far < (1u << 24);
+}
+
+template <class E>
+void launch_tiles(const AttnPackedArgs &a, float mul, hipStream_t stream) {
+    const uint32_t G = a.H / a.Hkv;
+    const uint32_t places = uint32_t(uint64_t(a.pb.tokens) * G / kRows) + a.pb.batch, grid = places * a.Hkv;
+    if (a.D <= 64) packed_tile_kernel<E, 64><<<grid, 256, 0, stream>>>(a, mul, places);
+    else if (a.D <= 128) packed_tile_kernel<E, 128><<<grid, 256, 0, stream>>>(a, mul, places);
+    else packed_tile_kernel<E, 256><<<grid, 256, 0, stream>>>(a, mul, places);
+}
 
 // ---------------------------------------------------------- general form ----
 // One wavefront a token and head, any head_dim, stride and alignment.
@@ -57,6 +379,11 @@ void launch_rows(const AttnPackedArgs &a, float mul, hipStream_t stream) {
 
 hipError_t launch_attn_packed(const AttnPackedArgs &a, hipStream_t stream) {
     const float mul = kLog2e / a.score_scale;
+    if (tiles_apply(a)) {
+        if (a.dtype == 7) launch_tiles<Bf16>(a, mul, stream);
+        else launch_tiles<F16>(a, mul, stream);
+        return hipGetLastError();
+    }
     if (a.dtype == 7) launch_rows<Bf16>(a, mul, stream);
     else if (a.dtype == 6) launch_rows<F16>(a, mul, stream);
     else launch_rows<F32>(a, mul, stream);
