@@ -27,8 +27,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 //                                         weight off by half a step at most, as the
 //                                         result itself is; the sum l holds them
 //                                         unrounded in f32
-// f16 weights are held as 2^15 p (l too, so the quotient is the same), which keeps
-// all down to 2^-29 p clear of f16's subnormals.
+// f16 weights are held as 2^7 p (l too, so the quotient is the same): p reaches 2^8
+// at most, and down to 2^-21 it stays clear of f16's subnormals.
 // Sequence s owns places [floor(starts[s] G / 128) + s, floor(starts[s + 1] G / 128)
 // + s + 1) of the grid: as many as its row tiles or more, so no prefix sum is
 // needed. Neighbouring workgroups take the kv heads of one place, so that with
@@ -57,6 +57,15 @@ __device__ __forceinline__ void lds_barrier() {
     asm volatile("" ::: "memory");
 }
 
+// The same, with the loads into LDS landed.
+__device__ __forceinline__ void all_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(7 << 4);   // vmcnt(0) lgkmcnt(0)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 template <class E>
 __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
     if constexpr (std::is_same_v<E, Bf16>)
@@ -78,15 +87,13 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 }
 
 template <class E, int DP>
-__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void packed_tile_kernel(AttnPackedArgs a, float mul,
-                                                                           uint32_t places) {
-    constexpr int RB = 2 * DP, NK = DP / 16, DB = DP / 32, CT = DP / 32;   // CT: 16-byte chunks a thread stages
-    constexpr float kUp = std::is_same_v<E, F16> ? 15.0f : 0.0f;
-    struct Tile {
-        uint8_t k[kKeys * RB], v[kKeys * RB];
-    };
-    __shared__ __attribute__((aligned(1024))) Tile tl0, tl1;
-    __shared__ uint32_t odd_v[2][4];
+__device__ __forceinline__ void packed_tile(const AttnPackedArgs &a, const float mul, const uint32_t places) {
+    constexpr int RB = 2 * DP, NK = DP / 16, DB = DP / 32, LPW = RB / 64;   // LPW: 1 KiB loads a wavefront
+    constexpr uint32_t CPR = RB / 16, RPL = 1024 / RB, kOob = 0x80000000u;   // chunks a row, rows a load
+    constexpr float kLag = 8.0f, kUp = std::is_same_v<E, F16> ? 7.0f : 0.0f;
+    typedef uint8_t Buf[kKeys * RB];
+    __shared__ __attribute__((aligned(1024))) Buf kb0, kb1, vb0, vb1;
+    __shared__ uint32_t odd0[4], odd1[4];   // found in vb0, vb1, by wavefront
     auto swz_k = [](uint32_t row) { return DP >= 128 ? (row & 15u) : ((row >> 1) & 7u); };
     auto swz_v = [](uint32_t row) { return DP >= 128 ? 4u * (row & 3u) : 4u * ((row >> 1) & 1u); };
 
@@ -110,34 +117,34 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void packed_tile_kernel(Attn
     const uint32_t wmin = pk_uni(token(wr0) + 1), wmax = pk_uni(token(wr0 + 31) + 1);
     const bool live = pk_uni(wr0 < R);   // the wavefront has rows
 
-    // K and V: key tid / 4 of the tile, chunks tid % 4 + 4 i of its row. A resource a
-    // tile, so that offsets stay small and rows past the sequence read as zeros, as
-    // chunks past D do.
+    // K and V straight into LDS: a load of a wavefront fills 1 KiB, RPL rows, and lane
+    // i's 16 bytes land at 16 i, so the swizzle picks the chunk that the lane reads. A
+    // resource a tile: rows past the sequence, like chunks past D, read as zeros.
     typedef typename E::T T;
     const T *kp = static_cast<const T *>(a.k) + uint64_t(t0) * a.k_stride + uint64_t(kh) * a.D;
     const T *vp = static_cast<const T *>(a.v) + uint64_t(t0) * a.v_stride + uint64_t(kh) * a.D;
-    const uint32_t key = uint32_t(tid) >> 2, part = uint32_t(tid) & 3u, n = t1 - t0;
-    u32x4 kr[CT], vr[CT];
-    uint32_t koff[CT], voff[CT];
+    const uint32_t n = t1 - t0;
+    uint32_t koff[LPW], voff[LPW];
 #pragma unroll
-    for (int i = 0; i < CT; ++i) {
-        const bool in = 8 * (part + 4 * i) < a.D;
-        koff[i] = in ? (key * a.k_stride + 8 * (part + 4 * i)) * 2u : 0xfffffff0u;
-        voff[i] = in ? (key * a.v_stride + 8 * (part + 4 * i)) * 2u : 0xfffffff0u;
+    for (int t = 0; t < LPW; ++t) {
+        const uint32_t r = (wave * LPW + t) * RPL + lane / CPR, c = lane % CPR;
+        const uint32_t ck = c ^ swz_k(r), cv = c ^ swz_v(r);
+        koff[t] = 8 * ck < a.D ? (r * a.k_stride + 8 * ck) * 2u : kOob;
+        voff[t] = 8 * cv < a.D ? (r * a.v_stride + 8 * cv) * 2u : kOob;
     }
-    auto fetch = [&](uint32_t j0) {
+    auto load_tile = [&](const T *base, uint32_t stride, uint32_t j0, const uint32_t (&off)[LPW], uint8_t *buf) {
         const uint32_t left = j0 < n ? (n - j0 < kKeys ? n - j0 : kKeys) : 0u;
-        const uint64_t at = j0 < n ? j0 : 0u;
-        const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(kp + at * a.k_stride), 0,
-                                                          left ? int(((left - 1) * a.k_stride + a.D) * 2u) : 0, 0x00020000);
-        const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(vp + at * a.v_stride), 0,
-                                                          left ? int(((left - 1) * a.v_stride + a.D) * 2u) : 0, 0x00020000);
+        const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(base + uint64_t(left ? j0 : 0u) * stride), 0,
+                                                         left ? int(((left - 1) * stride + a.D) * 2u) : 0, 0x00020000);
+        lds_u8 *to = (lds_u8 *)buf + wave * (LPW * 1024u);
 #pragma unroll
-        for (int i = 0; i < CT; ++i) kr[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, koff[i], 0, 0));
-#pragma unroll
-        for (int i = 0; i < CT; ++i) vr[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, voff[i], 0, 0));
+        for (int t = 0; t < LPW; ++t) __builtin_amdgcn_raw_ptr_buffer_load_lds(r, to + 1024 * t, 16, off[t], 0, 0, 0);
     };
-    fetch(0);
+    auto load_k = [&](uint32_t j0, uint8_t *buf) { load_tile(kp, a.k_stride, j0, koff, buf); };
+    auto load_v = [&](uint32_t j0, uint8_t *buf) { load_tile(vp, a.v_stride, j0, voff, buf); };
+    load_k(0, kb0);
+    load_v(0, vb0);
+    load_k(kKeys, kb1);
 
     u32x4 qf[NK];
     {
@@ -150,40 +157,28 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void packed_tile_kernel(Attn
         }
     }
 
-    uint32_t kw[CT], vw[CT];
-#pragma unroll
-    for (int i = 0; i < CT; ++i) {
-        kw[i] = key * RB + (((part + 4u * i) ^ swz_k(key)) * 16u);
-        vw[i] = key * RB + (((part + 4u * i) ^ swz_v(key)) * 16u);
-    }
     // (one of) a pair of f16 or bf16 with all exponent bits set
     constexpr uint32_t kExp = std::is_same_v<E, Bf16> ? 0x7f80u : 0x7c00u;
     auto odd = [](uint32_t w) { return (w & kExp) == kExp || ((w >> 16) & kExp) == kExp; };
-    auto put = [&](Tile &tl, uint32_t *flag, uint32_t j0) {
-        if (j0 + kKeys > kmin) {   // some row does not see all of it
-            bool any = false;
+    // V of a tile that some row does not see to its end: elements that are not finite
+    // become zeros; whether there were any is *flag's.
+    auto screen = [&](uint8_t *buf, uint32_t *flag) {
+        bool any = false;
+#pragma unroll 1
+        for (uint32_t at = uint32_t(tid) * 16u; at < kKeys * RB; at += 4096u) {
+            u32x4 x = *reinterpret_cast<u32x4 *>(buf + at);
+            const bool here = odd(x[0]) || odd(x[1]) || odd(x[2]) || odd(x[3]);
+            any |= here;
+            if (!here) continue;
 #pragma unroll
-            for (int i = 0; i < CT; ++i)
-#pragma unroll
-                for (int w = 0; w < 4; ++w) any |= odd(vr[i][w]);
-            if (__builtin_expect(any, 0)) {
-#pragma unroll
-                for (int i = 0; i < CT; ++i)
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        uint32_t x = vr[i][w];
-                        x = (x & kExp) == kExp ? x & 0xffff0000u : x;
-                        vr[i][w] = ((x >> 16) & kExp) == kExp ? x & 0xffffu : x;
-                    }
+            for (int w = 0; w < 4; ++w) {
+                x[w] = (x[w] & kExp) == kExp ? x[w] & 0xffff0000u : x[w];
+                x[w] = ((x[w] >> 16) & kExp) == kExp ? x[w] & 0xffffu : x[w];
             }
-            const bool found = __ballot(any) != 0;
-            if (lane == 0) flag[wave] = found;
+            *reinterpret_cast<u32x4 *>(buf + at) = x;
         }
-#pragma unroll
-        for (int i = 0; i < CT; ++i) {
-            *reinterpret_cast<u32x4 *>(tl.k + kw[i]) = kr[i];
-            *reinterpret_cast<u32x4 *>(tl.v + vw[i]) = vr[i];
-        }
+        const bool found = __ballot(any) != 0;
+        if (lane == 0) flag[wave] = found;
     };
 
     f32x16 o[DB];
@@ -195,6 +190,10 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void packed_tile_kernel(Attn
     const uint32_t g16 = uint32_t(lane) >> 4, r16 = uint32_t(lane) & 15u;
     const uint32_t vrow = 4u * (g16 >> 1) + (r16 >> 2);
     const uint32_t vchunk = 2u * (g16 & 1u) + ((r16 & 3u) >> 1);
+    // where a lane reads: chunk 2 k + lg of key row lr, swizzled, is the chunk of k = 0
+    // with 2 k toggled; V's 4 d likewise
+    const uint32_t kat = uint32_t(lr) * RB + ((uint32_t(lg) ^ swz_k(lr)) * 16u);
+    const uint32_t vat = vrow * RB + ((vchunk ^ swz_v(vrow)) * 16u) + (r16 & 1u) * 8u;
 
     // The elements that `put` left out, for the rows that see their keys: an infinity
     // or NaN with a weight above 0 is the sum it joins.
@@ -215,89 +214,150 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void packed_tile_kernel(Attn
                 }
     };
 
-    // one tile's products; `full`: every row of the wavefront sees all of it
-    auto tile_work = [&](const Tile &tl, const uint32_t *flag, uint32_t j0, bool full) {
-        const lds_u8 *kb0 = (const lds_u8 *)tl.k, *vb0 = (const lds_u8 *)tl.v;
-        f32x16 s[2];
+    f32x16 s[2];
+    // operand k (of NK) of the K tile in `buf`, key half h; of V's, 16-key step st and
+    // 32-dim block d
+    auto k_frag = [&](const uint8_t *buf, uint32_t at, int k, int h) __attribute__((always_inline)) {
+        return *reinterpret_cast<const lds_u32x4 *>((const lds_u8 *)buf + (at ^ (32u * k)) + 32u * RB * h);
+    };
+    auto v_frag = [&](const uint8_t *buf, uint32_t at, int st, int d) __attribute__((always_inline)) {
+        const lds_u8 *p = (const lds_u8 *)buf + (at ^ (64u * d)) + 16u * RB * st;
+        const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            reinterpret_cast<lds_i16x4 *>(const_cast<lds_u8 *>(p)));
+        const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            reinterpret_cast<lds_i16x4 *>(const_cast<lds_u8 *>(p + 8u * RB)));
+        return __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    auto limit = [&](uint32_t j0) __attribute__((always_inline)) {   // keys the row does not see
+        if (j0 + kKeys <= wmin) return;
+        int sees = int(lim) - int(j0) - 4 * lg;
+        asm volatile("" : "+v"(sees));   // a branch of its own: full tiles pass it by
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[kb][r] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < NK; ++k)
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
-                const u32x4 kf = *reinterpret_cast<const lds_u32x4 *>(
-                    kb0 + (32u * kb + lr) * RB + ((uint32_t(2 * k + lg) ^ swz_k(lr)) * 16u));
-                s[kb] = mfma<E>(kf, qf[k], s[kb]);
-            }
-        float mt = -INFINITY;
-        if (!full) {
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    s[kb][r] = j0 + 32u * kb + 8u * (r >> 2) + 4u * lg + (r & 3) < lim ? s[kb][r] : -INFINITY;
-        }
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[kb][r]);
-        {
-            const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(mt), __float_as_uint(mt), false, false);
-            mt = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * mul;
-        }
-        const float mn = fmaxf(m, mt);
-        if (__any(mn > m)) {
+            for (int r = 0; r < 16; ++r) s[h][r] = 32 * h + 8 * (r >> 2) + (r & 3) < sees ? s[h][r] : -INFINITY;
+    };
+    // m is a row's largest score up to kLag: a weight may reach 2^kLag, and the sums
+    // are rescaled only where a row passes that
+    auto rescale = [&](float mt) __attribute__((always_inline)) {
+        if (__any(mt > m + kLag)) {
+            const float mn = fmaxf(m, mt);
             const float al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
             l *= al;
 #pragma unroll
             for (int d = 0; d < DB; ++d) o[d] *= al;
             m = mn;
         }
+    };
+    auto add_found = [&](const uint32_t *flag, uint32_t j0) __attribute__((always_inline)) {
+        if (j0 + kKeys > kmin && __builtin_expect(flag[0] | flag[1] | flag[2] | flag[3], 0)) add_odd(j0);
+    };
+    // S = K . Q^T of a tile into `to`, beside the weights of the tile in s (kWeigh): a
+    // product takes the matrix cores 32 cycles, the weights' vector instructions run
+    // under it. The operands are read two steps ahead, and the barriers keep the
+    // compiler from gathering the products behind the rest.
+    u32x4 pf[4];
+    auto scores = [&](const uint8_t *buf, f32x16 (&to)[2], const bool weigh) __attribute__((always_inline)) {
+        constexpr int kPairs = 16 / NK;
+        uint32_t at = kat;
+        asm volatile("" : "+v"(at));   // one register, not one a step
+        u32x4 kf[2][2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) kf[k][h] = k_frag(buf, at, k, h);
         const float ref = (m == -INFINITY ? 0.0f : m) - kUp;
-        u32x4 pf[4];
 #pragma unroll
-        for (int st = 0; st < 4; ++st)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                float p[2];
+            for (int r = 0; r < 16; ++r) to[h][r] = 0.0f;
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int r = 8 * (st & 1) + 2 * c + e;
-                    p[e] = __builtin_amdgcn_exp2f(fmaf(s[st >> 1][r], mul, -ref));
-                    l += p[e];
+        for (int k = 0; k < NK; ++k) {
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) to[h] = mfma<E>(kf[k & 1][h], qf[k], to[h]);
+            if (k + 2 < NK)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) kf[k & 1][h] = k_frag(buf, at, k + 2, h);
+            if (weigh)
+#pragma unroll
+                for (int i = kPairs * k; i < kPairs * (k + 1); ++i) {
+                    float p[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        p[e] = __builtin_amdgcn_exp2f(fmaf(s[i >> 3][2 * (i & 7) + e], mul, -ref));
+                        l += p[e];
+                    }
+                    uint32_t w = pack2<E>(p[0], p[1]);
+                    asm volatile("" : "+v"(w), "+v"(l));   // here, not where they are used
+                    pf[i >> 2][i & 3] = w;
                 }
-                pf[st][c] = pack2<E>(p[0], p[1]);
-            }
-#pragma unroll
-        for (int st = 0; st < 4; ++st)
-#pragma unroll
-            for (int d = 0; d < DB; ++d) {
-                const lds_u8 *p = vb0 + (16u * st + vrow) * RB + ((vchunk + 4u * d) ^ swz_v(vrow)) * 16u +
-                                  (r16 & 1u) * 8u;
-                const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    reinterpret_cast<lds_i16x4 *>(const_cast<lds_u8 *>(p)));
-                const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    reinterpret_cast<lds_i16x4 *>(const_cast<lds_u8 *>(p + 8u * RB)));
-                const u32x4 vf = __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-                o[d] = mfma<E>(vf, pf[st], o[d]);
-            }
-        if (!full && __builtin_expect(flag[0] | flag[1] | flag[2] | flag[3], 0)) add_odd(j0);
-    };
-    auto step = [&](const Tile &tl, const uint32_t *flag, Tile &next, uint32_t *next_flag, uint32_t j0) {
-        lds_barrier();     // this tile is in its buffer, the other buffer's readers are done
-        if (j0 + kKeys < kmax) {
-            put(next, next_flag, j0 + kKeys);
-            fetch(j0 + 2 * kKeys);
         }
-        if (live && j0 < wmax) tile_work(tl, flag, j0, j0 + kKeys <= wmin);
+        __builtin_amdgcn_sched_barrier(0);
     };
-    put(tl0, odd_v[0], 0);
-    fetch(kKeys);
+    // O^T += V^T . P^T, beside the largest of the scores in s
+    auto products = [&](const uint8_t *buf) __attribute__((always_inline)) {
+        constexpr int kSteps = 2 * DB, kMax = 32 / kSteps;
+        uint32_t at = vat;
+        asm volatile("" : "+v"(at));
+        u32x4 vf[2][2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) vf[i][h] = v_frag(buf, at, i / (DB / 2), 2 * (i % (DB / 2)) + h);
+        float mt = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            __builtin_amdgcn_sched_barrier(0);
+            const int st = i / (DB / 2), d = 2 * (i % (DB / 2));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) o[d + h] = mfma<E>(vf[i & 1][h], pf[st], o[d + h]);
+            if (i + 2 < kSteps)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    vf[i & 1][h] = v_frag(buf, at, (i + 2) / (DB / 2), 2 * ((i + 2) % (DB / 2)) + h);
+#pragma unroll
+            for (int r = kMax * i; r < kMax * (i + 1); ++r) mt = fmaxf(mt, s[r >> 4][r & 15]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(mt), __float_as_uint(mt), false, false);
+        return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * mul;
+    };
+    // Tile j0, whose scores are in s, limited and no more than kLag above m: its weights
+    // beside the next tile's scores, then its products beside those scores' largest.
+    auto step = [&](uint8_t *k_this, uint8_t *k_next, uint8_t *v_this, uint8_t *v_next, uint32_t *flag,
+                    uint32_t j0) __attribute__((always_inline)) {
+        all_barrier();     // k_next and v_this are filled, k_this and v_next are done with
+        const bool more = j0 + kKeys < kmax;
+        if (more) {
+            load_k(j0 + 2 * kKeys, k_this);
+            load_v(j0 + kKeys, v_next);
+        }
+        if (j0 + kKeys > kmin) {
+            screen(v_this, flag);
+            lds_barrier();
+        }
+        if (!live) return;
+        f32x16 nx[2];
+        scores(k_next, nx, true);   // (past the last tile: what the buffer held, all limited)
+        s[0] = nx[0], s[1] = nx[1];
+        limit(j0 + kKeys);
+        const float mt = products(v_this);
+        add_found(flag, j0);
+        if (more) rescale(mt);
+    };
+    all_barrier();
+    scores(kb0, s, false);
+    limit(0);
+    {
+        float mt = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < 32; ++r) mt = fmaxf(mt, s[r >> 4][r & 15]);
+        rescale(fmaxf(mt, __shfl_xor(mt, 32, 64)) * mul);
+    }
     for (uint32_t j0 = 0; j0 < kmax; j0 += 2 * kKeys) {
-        step(tl0, odd_v[0], tl1, odd_v[1], j0);
-        if (j0 + kKeys < kmax) step(tl1, odd_v[1], tl0, odd_v[0], j0 + kKeys);
+        step(kb0, kb1, vb0, vb1, odd0, j0);
+        if (j0 + kKeys < kmax) step(kb1, kb0, vb1, vb0, odd1, j0 + kKeys);
     }
     l += __shfl_xor(l, 32, 64);
     if (wr0 + lr >= R) return;
@@ -314,6 +374,12 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void packed_tile_kernel(Attn
                     make_uint2(pack2<E>(o[d][4 * c] * inv, o[d][4 * c + 1] * inv),
                                pack2<E>(o[d][4 * c + 2] * inv, o[d][4 * c + 3] * inv));
         }
+}
+
+template <class E, int DP>
+__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void packed_tile_kernel(AttnPackedArgs a, float mul,
+                                                                           uint32_t places) {
+    packed_tile<E, DP>(a, mul, places);
 }
 
 // What the tiles take: 16-byte rows of q, k, v and out, offsets within a tile below
