@@ -37,6 +37,37 @@ __device__ __forceinline__ uint32_t last_at_most(uint32_t n, uint64_t t, F at) {
     return lo;
 }
 
+// The sequence of place `t` where sequence s owns places [floor(starts[s] m / unit) +
+// s, floor(starts[s + 1] m / unit) + s + 1): as many as its rows times m fill units of
+// `unit`, or one more, so that neither a prefix sum nor the lengths are needed on the
+// host. (tokens * m < 2^30.) Its first and one-past-last row and the place's number
+// in it; false for a place that no unit of the sequence takes. As last_at_most, with
+// the bounds taken from the probes of its last step.
+struct Place {
+    uint32_t b, lo, hi, unit;
+};
+__device__ __forceinline__ bool place_of(const PackedBatch &pb, uint32_t m, uint32_t unit, uint32_t t, Place *o) {
+    const uint32_t lane = threadIdx.x & 63u;
+    uint32_t lo = 0, n = pb.batch, v;
+    int at;
+    for (;;) {
+        const uint32_t step = (n + 63) / 64;
+        const uint64_t s = lo + uint64_t(lane) * step;
+        v = start_of(pb, s < pb.batch ? uint32_t(s) : pb.batch);
+        const uint64_t hit = __ballot(lane * uint64_t(step) < n && v * m / unit + s <= t);
+        at = hit ? 63 - __builtin_clzll(hit) : 0;
+        lo = pk_uni(lo + at * step);
+        if (step == 1) break;
+        n = pk_uni(pb.batch - lo < step ? pb.batch - lo : step);
+    }
+    o->b = lo;
+    o->lo = __builtin_amdgcn_readlane(v, at);
+    o->hi = at < 63 ? __builtin_amdgcn_readlane(v, at + 1) : pk_uni(start_of(pb, lo + 1));
+    const uint32_t first = o->lo * m / unit + lo;
+    o->unit = t - first;
+    return o->hi > o->lo && t >= first && o->unit * unit < (o->hi - o->lo) * m;
+}
+
 // Bit 8 of *err if the offsets decrease or pass `tokens`; the threads of one
 // workgroup call it.
 __device__ __forceinline__ void check_starts(const PackedBatch &pb) {

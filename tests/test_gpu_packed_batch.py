@@ -99,6 +99,16 @@ def test_packed_many_sequences(torch_cuda, backend, dtype):
 
 
 @pytest.mark.parametrize("dtype", ALL)
+def test_packed_longest_first(torch_cuda, backend, dtype):
+    """More workgroups than the GPU holds at once: the tiles that see most keys go first."""
+    rng = np.random.default_rng(5)
+    rows = [129, 1, 0, 90, 200, 128]
+    qkv, _, _ = packed_case(rng, rows, 64, 64, 32, dtype, gap=1, tail=1)
+    got = run_packed(torch_cuda, backend, qkv, rows, 64, 64, 32, dtype, 0, gap=1)
+    check_packed(got, qkv, rows, 64, 64, 32, dtype, 0, gap=1)
+
+
+@pytest.mark.parametrize("dtype", ALL)
 @pytest.mark.parametrize("D", [64, 128, 96])
 def test_what_a_row_does_not_see_stays_out(torch_cuda, backend, dtype, D):
     """NaN and infinities in later rows of the sequence (K, V and Q) and all over its neighbours:
