@@ -4,6 +4,7 @@
 
 #include <math.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "holo_kernels.h"
@@ -107,9 +108,9 @@ __device__ __forceinline__ void packed_tile(const AttnPackedArgs &a, const float
     // token of a row, the last one's past the end
     auto token = [&](uint32_t r) { return (r < R ? r : R - 1) / G; };
     const uint32_t wr0 = r0 + 32 * wave, row = wr0 + lr < R ? wr0 + lr : R - 1;
-    const uint32_t tok = row / G, head = row - tok * G, lim = tok + 1;
+    const uint32_t lim = row / G + 1;
     const uint32_t kmin = pk_uni(token(r0) + 1), kmax = pk_uni(token(r0 + kRows - 1) + 1);
-    const uint32_t wmin = pk_uni(token(wr0) + 1), wmax = pk_uni(token(wr0 + 31) + 1);
+    const uint32_t wmin = pk_uni(token(wr0) + 1);
     const bool live = pk_uni(wr0 < R);   // the wavefront has rows
 
     // K and V straight into LDS: a load of a wavefront fills 1 KiB, RPL rows, and lane
@@ -136,20 +137,26 @@ __device__ __forceinline__ void packed_tile(const AttnPackedArgs &a, const float
     };
     auto load_k = [&](uint32_t j0, uint8_t *buf) { load_tile(kp, a.k_stride, j0, koff, buf); };
     auto load_v = [&](uint32_t j0, uint8_t *buf) { load_tile(vp, a.v_stride, j0, voff, buf); };
-    load_k(0, kb0);
-    load_v(0, vb0);
-    load_k(kKeys, kb1);
-
-    u32x4 qf[NK];
+    // 16-byte chunk c of row r of a wavefront's 32 rows in LDS
+    auto chunk_at = [&](uint32_t r, uint32_t c) { return r * RB + (c ^ (r & (CPR - 1u) & 15u)) * 16u; };
+    // Q the same way, whole rows into the wavefront's part of the two buffers that are
+    // needed last; a row past R is a copy of the last
+    uint8_t *qbuf = (wave & 2 ? vb1 : kb1) + (wave & 1) * (32 * RB);
     {
-        const T *q = static_cast<const T *>(a.q) + uint64_t(t0 + tok) * a.q_stride + (uint64_t(kh) * G + head) * a.D;
+        const uint32_t tok0 = r0 / G;
+        const auto r = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<T *>(static_cast<const T *>(a.q) + uint64_t(t0 + tok0) * a.q_stride + kh * G * a.D), 0, int(kOob),
+            0x00020000);
 #pragma unroll
-        for (int k = 0; k < NK; ++k) {
-            const uint32_t d = 16 * k + 8 * lg;
-            qf[k] = u32x4{0, 0, 0, 0};
-            if (d < a.D) qf[k] = *reinterpret_cast<const u32x4 *>(q + d);
+        for (int t = 0; t < 2 * LPW; ++t) {
+            const uint32_t at = t * RPL + lane / CPR, rr = wr0 + at < R ? wr0 + at : R - 1, tq = rr / G;
+            const uint32_t c = (lane % CPR) ^ (at & (CPR - 1u) & 15u);
+            const uint32_t off = ((tq - tok0) * a.q_stride + (rr - tq * G) * a.D + 8 * c) * 2u;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_u8 *)qbuf + 1024 * t, 16, 8 * c < a.D ? off : kOob, 0, 0, 0);
         }
     }
+    load_k(0, kb0);
+    load_v(0, vb0);
 
     // (one of) a pair of f16 or bf16 with all exponent bits set
     constexpr uint32_t kExp = std::is_same_v<E, Bf16> ? 0x7f80u : 0x7c00u;
@@ -209,6 +216,7 @@ __device__ __forceinline__ void packed_tile(const AttnPackedArgs &a, const float
     };
 
     f32x16 s[2];
+    u32x4 qf[NK];
     // operand k (of NK) of the K tile in `buf`, key half h; of V's, 16-key step st and
     // 32-dim block d
     auto k_frag = [&](const uint8_t *buf, uint32_t at, int k, int h) __attribute__((always_inline)) {
@@ -349,6 +357,10 @@ __device__ __forceinline__ void packed_tile(const AttnPackedArgs &a, const float
         if (more) rescale(mt);
     };
     all_barrier();
+#pragma unroll
+    for (int k = 0; k < NK; ++k) qf[k] = *reinterpret_cast<const u32x4 *>(qbuf + chunk_at(lr, 2 * k + lg));
+    lds_barrier();   // the buffers that held Q are free
+    load_k(kKeys, kb1);
     scores(kb0, s, false);
     limit(0);
     {
@@ -367,7 +379,6 @@ __device__ __forceinline__ void packed_tile(const AttnPackedArgs &a, const float
     lds_barrier();
     uint8_t *turn = (wave & 2 ? kb1 : kb0) + (wave & 1) * (32 * RB);
     const float inv = 1.0f / l;
-    auto chunk_at = [&](uint32_t r, uint32_t c) { return r * RB + (c ^ (r & (CPR - 1u) & 15u)) * 16u; };
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -379,8 +390,8 @@ __device__ __forceinline__ void packed_tile(const AttnPackedArgs &a, const float
     T *out = static_cast<T *>(a.out) + (uint64_t(t0) * a.H + kh * G) * a.D;
     const uint32_t c = lane % CPR;
 #pragma unroll
-    for (uint32_t r = lane / CPR; r < 32; r += RPL) {
-        const uint32_t rr = wr0 + r, t = rr / G;
+    for (uint32_t i = 0; i < 32 / RPL; ++i) {
+        const uint32_t r = i * RPL + lane / CPR, rr = wr0 + r, t = rr / G;
         if (rr < R && 8 * c < a.D)
             *reinterpret_cast<u32x4 *>(out + (uint64_t(t) * a.H + (rr - t * G)) * a.D + 8 * c) =
                 *reinterpret_cast<const u32x4 *>(turn + chunk_at(r, c));
@@ -393,13 +404,13 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void packed_tile_kernel(Attn
     packed_tile<E, DP>(a, mul, places);
 }
 
-// What the tiles take: 16-byte rows of q, k, v and out, offsets within a tile below
-// 2^31 bytes.
+// What the tiles take: 16-byte rows of q, k, v and out, offsets within a tile's 64 keys
+// and a workgroup's 128 rows below 2^31 bytes.
 bool tiles_apply(const AttnPackedArgs &a) {
     auto at16 = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
-    const uint32_t far = a.k_stride > a.v_stride ? a.k_stride : a.v_stride;
+    const uint32_t far = std::max({a.q_stride, a.k_stride, a.v_stride});
     return a.dtype != 8 && a.D % 8 == 0 && a.D <= 256 && a.q_stride % 8 == 0 && a.k_stride % 8 == 0 &&
-           a.v_stride % 8 == 0 && at16(a.q) && at16(a.k) && at16(a.v) && at16(a.out) && far < (1u << 24);
+           a.v_stride % 8 == 0 && at16(a.q) && at16(a.k) && at16(a.v) && at16(a.out) && far < (1u << 23);
 }
 
 template <class E>
