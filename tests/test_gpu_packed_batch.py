@@ -218,6 +218,11 @@ BLOCK_SHAPES = [  # rows, lens, H, Hkv, D, bucket, block, pad
     ([5], [9], 1, 1, 320, 16, 7, 0),
     ([1, 4], [40, 50], 2, 1, 64, 50, 100, 0),                           # one block, longer than the bucket
     ([1], [4000000000], 2, 1, 64, 96, 32, 0),                           # a length past the bucket
+    ([1, 1, 4, 0, 1], [2500, 0, 2100, 9, 17], 4, 2, 128, 2500, 32, 0),  # shares that end inside a sequence
+    ([1, 2], [2500, 1], 34, 2, 256, 2560, 128, 0),                      # two units a row
+    ([1, 9], [5000, 4001], 3, 3, 96, 5000, 16, 0),                      # few: shares of two quads
+    ([300], [4000], 2, 1, 64, 4096, 64, 0),                             # a chunk whose keys are split
+    ([40, 1], [4000, 3000], 6, 2, 256, 4096, 32, 0),
 ]
 
 
@@ -231,11 +236,11 @@ def test_blocks_parity(torch_cuda, backend, rows, lens, H, Hkv, D, bucket, block
 
 
 @pytest.mark.parametrize("dtype", ALL)
-@pytest.mark.parametrize("rows", [1, 3, 60])
-def test_blocks_many_ragged_sequences(torch_cuda, backend, rows, dtype):
+@pytest.mark.parametrize("rows,bucket", [(1, 1500), (1, 2500), (3, 2500), (60, 1500), (60, 2500)])
+def test_blocks_many_ragged_sequences(torch_cuda, backend, rows, bucket, dtype):
     """Keys split among workgroups wherever a share ends, lengths from 0 to the bucket."""
     rng = np.random.default_rng(rows)
-    B, bucket = 70, 1500
+    B = 70
     lens = np.concatenate([[0, 1, 127, 128, 129, bucket], rng.integers(0, bucket + 1, B - 6)])
     c = blocks_case(rng, [rows] * B, lens, 8, 2, 64, bucket, 32, dtype)
     check_blocks(run_blocks(torch_cuda, backend, c), c, sequences=(0, 1, 2, 3, 4, 5, 20, 69))
