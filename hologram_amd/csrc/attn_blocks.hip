@@ -7,7 +7,7 @@
 #include <type_traits>
 
 #include "holo_kernels.h"
-#include "packed_batch.h"
+#include "packed_tile.h"
 
 namespace holo {
 namespace {
@@ -50,8 +50,6 @@ __device__ __forceinline__ uint32_t visible_keys(int64_t len, uint32_t n, uint32
 // launch of its own: partials pass between XCDs' L2s at its boundary).
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr uint32_t kUnit = 16, kStep = 32, kQuad = 128, kOob = 1u << 30;   // past every plane, twice it too
 constexpr uint32_t kDirect = 2048, kShares = 512, kMinQuads = 2;
 constexpr int kVeMin = -100;   // 2^ve's floor keeps 2^-ve finite
@@ -523,13 +521,463 @@ __global__ __launch_bounds__(256) void merge_kernel(Blocks k) {
     }
 }
 
+// -------------------------------------------------------------- tiled form ----
+// Many rows a sequence. As AttentionPacked's tiles: 128 packed rows a workgroup, 32 a
+// wavefront, over 64-key tiles, a tile's weights under the next one's scores; but the
+// tiles are the cache's bytes, loaded into registers a tile ahead and widened to f16
+// (exact) on their way into LDS. Q as f16, each row by a power of two so that its largest
+// is in [2^14, 2^15): exact for 16-bit rows but for elements 2^-38 of the largest, and in
+// two parts, 22 bits, for f32 rows; a row's power and log2(e) / divisor join K's scales.
+// The scale of a 16-key step is one number: K's |ks| times the row's factor is the
+// step's c, with s c - m one instruction; V's joins the exponent, w = 2^(s c - m +
+// log2|vs| + 7 - ve) (log2 rounded to 2^-21 at worst, where it is 8 or less: a weight off
+// by 2^-21), and the sum l takes a step's weights back by 1 / |vs|. 2^ve is above every
+// finite |vs| of the steps the row sees so far. A scale's sign is put on the bytes, and a
+// zero V scale makes them zeros, on the way into LDS.
+// In a tile that some row does not see to its end, s is scaled and limited first (c = 1),
+// and a step that a row does not see brings it no scale.
+// Where the rows give too few workgroups, a row tile's keys are cut into `splits` shares
+// of whole tiles, whose partials join_kernel joins.
+constexpr uint32_t kRows = 128, kKeys = 64, kResident = 512, kMaxSplits = 32;
+
+struct Chunk {
+    AttnBlocksArgs a;
+    float mul;
+    uint32_t shift, places, splits;
+    float *part;         // [places * Hkv * splits][kRows][DP + 2], as Blocks::part
+};
+
+// Four int8 (xor 0x80) as f16.
+__device__ __forceinline__ uint2 widen4(uint32_t w) {
+    typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+    const uint32_t b = w ^ 0x80808080u;
+    const uint2 m = {__builtin_amdgcn_perm(0x64646464u, b, 0x04010400u), __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u)};
+    return __builtin_bit_cast(uint2, __builtin_bit_cast(f16x4, m) - (f16x4)(_Float16)1152.0f);
+}
+
+__device__ __forceinline__ f32x16 mfma_f16(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// The largest of a row's 64 scores, a step's times its factor (not below 0).
+__device__ __forceinline__ float largest(const float (&mg)[4], const float (&c)[4]) {
+    const float mt = fmaxf(fmaxf(mg[0] * c[0], mg[1] * c[1]), fmaxf(mg[2] * c[2], mg[3] * c[3]));
+    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(mt), __float_as_uint(mt), false, false);
+    return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+}
+
+template <class E, int DP>
+__device__ __forceinline__ void chunk_tile(const Chunk &k) {
+    constexpr int RB = 2 * DP, NK = DP / 16, DB = DP / 32, CT = DP / 64;   // CT: 16-byte chunks a thread widens
+    constexpr bool kF32 = std::is_same_v<E, F32>;
+    constexpr int P = kF32 ? 2 : 1;
+    constexpr float kLag = 8.0f;
+    typedef typename E::T T;
+    typedef uint8_t Buf[kKeys * RB];
+    __shared__ __attribute__((aligned(1024))) Buf kb0, kb1, vb0, vb1;
+    const AttnBlocksArgs &a = k.a;
+    if (blockIdx.x == 0) check_starts(a.pb);
+    const uint32_t G = a.H / a.Hkv, kh = blockIdx.x % a.Hkv, rest = blockIdx.x / a.Hkv;
+    const uint32_t split = rest % k.splits, place = k.places - 1 - rest / k.splits;
+    Place at;
+    if (!place_of(a.pb, G, kRows, place, &at)) return;
+    const uint32_t t0 = at.lo, n = at.hi - at.lo, R = n * G, r0 = at.unit * kRows;
+    const int tid = threadIdx.x, lane = tid & 63, lr = lane & 31, lg = lane >> 5;
+    const uint32_t wave = pk_uni(uint32_t(tid) >> 6);
+    const int64_t len = a.lens[at.b];
+    auto sees = [&](uint32_t r) { return visible_keys(len, n, (r < R ? r : R - 1) / G, a.bucket); };
+    const uint32_t wr0 = r0 + 32 * wave, row = wr0 + lr < R ? wr0 + lr : R - 1, tok = row / G;
+    const uint32_t lim = sees(row), wmin = pk_uni(sees(wr0));
+    const uint32_t kall = pk_uni(sees(r0 + kRows - 1)), tiles = (kall + kKeys - 1) / kKeys;
+    const uint32_t per = (tiles + k.splits - 1) / k.splits * kKeys;
+    const uint32_t j1 = split * per < kall ? split * per : kall;                  // this share's keys
+    const uint32_t kmax = j1 + per < kall ? j1 + per : kall;
+    const bool live = pk_uni(wr0 < R);
+
+    // the tile's bytes: key tid / 4, chunks tid % 4 + 4 i of its row; its step's scales
+    const uint64_t plane = uint64_t(at.b) * a.Hkv + kh;
+    const auto rk = range(a.kq + plane * a.bucket * a.D, a.bucket * a.D);
+    const auto rv = range(a.vq + plane * a.bucket * a.D, a.bucket * a.D);
+    const uint32_t nb = (a.bucket + a.block - 1) >> k.shift;
+    const float *ks = a.ks + plane * nb, *vs = a.vs + plane * nb;
+    const uint32_t key = uint32_t(tid) >> 2, part = uint32_t(tid) & 3u;
+    auto scale_at = [&](const float *x, uint32_t j) {
+        const uint32_t i = j >> k.shift;
+        return x[i < nb ? i : nb - 1];
+    };
+    u32x4 kr[CT], vr[CT];
+    float ksk, vsk;
+    auto fetch = [&](const __amdgpu_buffer_rsrc_t r, uint32_t j, u32x4 (&x)[CT]) {
+#pragma unroll
+        for (int i = 0; i < CT; ++i) {
+            const uint32_t b = 16 * (part + 4 * i), off = j < kall && b < a.D ? (j + key) * a.D + b : kOob;
+            x[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+        }
+    };
+    auto fetch_k = [&](uint32_t j) { fetch(rk, j, kr), ksk = scale_at(ks, j + key); };
+    auto fetch_v = [&](uint32_t j) { fetch(rv, j, vr), vsk = scale_at(vs, j + key); };
+    auto put = [&](uint8_t *buf, const u32x4 (&x)[CT], float scale, bool zero, auto swz) {
+        const uint32_t flip = __float_as_uint(scale) >> 31 ? 0x80008000u : 0u;
+        const bool plain = !__any(flip != 0 || zero);
+#pragma unroll
+        for (int i = 0; i < CT; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint2 lo = widen4(x[i][2 * h]), hi = widen4(x[i][2 * h + 1]);
+                u32x4 v = {lo.x, lo.y, hi.x, hi.y};
+                if (!plain)
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) v[w] = zero ? 0u : v[w] ^ flip;
+                *reinterpret_cast<u32x4 *>(buf + key * RB + (((2u * (part + 4u * i) + h) ^ swz(key)) * 16u)) = v;
+            }
+    };
+    auto put_k = [&](uint8_t *buf) { put(buf, kr, ksk, false, [](uint32_t r) { return swz_k<DP>(r); }); };
+    auto put_v = [&](uint8_t *buf) { put(buf, vr, vsk, vsk == 0.0f, [](uint32_t r) { return swz_v<DP>(r); }); };
+    fetch_k(j1);
+    fetch_v(j1);
+
+    // Q's parts
+    u32x4 qf[P][NK];
+    float mul;
+    {
+        const T *q = static_cast<const T *>(a.q) + uint64_t(t0 + tok) * a.q_stride + (uint64_t(kh) * G + (row - tok * G)) * a.D;
+        float top = 0.0f;
+        bool bad = false;
+        // a chunk of 8 elements, dims 16 i + 8 lg on
+        auto chunk = [&](int i, float (&x)[8]) {
+#pragma unroll
+            for (int w = 0; w < int(sizeof(T)) / 2; ++w) {
+                u32x4 v = {0, 0, 0, 0};
+                if (uint32_t(16 * i + 8 * lg) < a.D) v = *reinterpret_cast<const u32x4 *>(q + 16 * i + 8 * lg + 4 * w);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (kF32) {
+                        x[4 * w + e] = __uint_as_float(v[e]);
+                    } else {
+                        x[2 * e] = E::widen(uint16_t(v[e]));
+                        x[2 * e + 1] = E::widen(uint16_t(v[e] >> 16));
+                    }
+                }
+            }
+        };
+#pragma unroll 2
+        for (int i = 0; i < NK; ++i) {
+            float x[8];
+            chunk(i, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                top = fmaxf(top, fabsf(x[e]));
+                bad |= !(fabsf(x[e]) <= 3.4028235e38f);
+            }
+        }
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        bad |= __shfl_xor(int(bad), 32, 64) != 0;
+        int qe = 0;
+        if (top > 0.0f && !bad) {
+            (void)frexpf(top, &qe);     // top < 2^qe
+            qe = 15 - qe;
+        }
+        mul = bad ? __uint_as_float(0x7fc00000u) : ldexpf(k.mul, -qe);
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+            float x[8];
+            chunk(i, x);
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float y[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float v = bad ? 0.0f : ldexpf(x[2 * e + h], qe);
+                        y[h] = p == 0 ? v : v - float(_Float16(v));
+                    }
+                    qf[p][i][e] = pack2<F16>(y[0], y[1]);
+                }
+        }
+    }
+
+    f32x16 o[DB], s[2];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+    int ve = kVeMin;
+    const uint32_t kat = k_place<DP>(lane), vat = v_place<DP>(lane);
+    // of the steps of the tile in s: K's factor; |vs| = fr 2^ex, log2(fr)
+    float c[4], fr[4], lf[4];
+    int ex[4];
+
+    // the scales of tile j, and s limited; the largest exponent of the steps the row sees
+    auto limit = [&](uint32_t j, int *top) __attribute__((always_inline)) {
+        *top = kVeMin;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            float v = fabsf(scale_at(vs, j + 16 * g));
+            c[g] = fabsf(scale_at(ks, j + 16 * g)) * mul;
+            v = v == 0.0f ? 1.0f : v;      // (its bytes are zeros)
+            const bool finite = v <= 3.4028235e38f;
+            ex[g] = 0;
+            fr[g] = finite ? frexpf(v, &ex[g]) : v;        // fr in [0.5, 1)
+            if (j + kKeys > wmin && j + 16 * g >= lim) fr[g] = 0.5f, ex[g] = kVeMin;
+            lf[g] = __builtin_amdgcn_logf(fr[g]);
+            *top = finite && ex[g] > *top ? ex[g] : *top;
+        }
+        if (j + kKeys <= wmin) return;
+        int see = int(lim < kmax ? lim : kmax) - int(j) - 4 * lg;
+        asm volatile("" : "+v"(see));
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                s[h][r] = 32 * h + 8 * (r >> 2) + (r & 3) < see ? s[h][r] * c[2 * h + (r >> 3)] : -INFINITY;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) c[g] = 1.0f;
+    };
+    auto rescale = [&](float mt, int top) __attribute__((always_inline)) {
+        if (__any(mt > m + kLag || top > ve)) {
+            const float mn = mt > m + kLag ? mt : m;
+            const int vn = top > ve ? top : ve;
+            const float al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            const float sh = ldexpf(al, ve - vn);
+            l *= al;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) o[d] *= sh;
+            m = mn, ve = vn;
+        }
+    };
+    u32x4 pf[P][4];
+    float up[4], back[4];         // per step: log2|vs| + 7 - ve - m, and 2^(ve - 7) / |vs|
+    auto prepare = [&]() __attribute__((always_inline)) {
+        const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            up[g] = (lf[g] + float(ex[g] + 7 - ve)) - ref;
+            back[g] = ldexpf(1.0f / fr[g], ve - 7 - ex[g]);
+        }
+    };
+    auto weight_pair = [&](int i) __attribute__((always_inline)) {
+        const int g = i >> 2;
+        float w[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const float x = s[i >> 3][2 * (i & 7) + e];
+            w[e] = __builtin_amdgcn_exp2f(fmaf(x, c[g], up[g]));
+        }
+        l = fmaf(w[0] + w[1], back[g], l);
+        uint32_t hi = pack2<F16>(w[0], w[1]);
+        if constexpr (kF32) {
+            typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+            const f16x2 f = __builtin_bit_cast(f16x2, hi);
+            uint32_t lo = pack2<F16>(w[0] - float(f[0]), w[1] - float(f[1]));
+            asm volatile("" : "+v"(lo));
+            pf[P - 1][i >> 2][i & 3] = lo;
+        }
+        asm volatile("" : "+v"(hi), "+v"(l));   // here, not where they are used
+        pf[0][i >> 2][i & 3] = hi;
+    };
+    auto scores = [&](const uint8_t *buf, f32x16 (&to)[2], const bool weigh) __attribute__((always_inline)) {
+        constexpr int kPairs = 16 / NK;
+        uint32_t x = kat;
+        asm volatile("" : "+v"(x));
+        u32x4 kf[2][2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) kf[i][h] = k_frag<DP>(buf, x, i, h);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) to[h][r] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) to[h] = mfma_f16(kf[i & 1][h], qf[p][i], to[h]);
+            if (i + 2 < NK)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) kf[i & 1][h] = k_frag<DP>(buf, x, i + 2, h);
+            if (weigh)
+#pragma unroll
+                for (int q = kPairs * i; q < kPairs * (i + 1); ++q) weight_pair(q);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // O^T += V^T . P^T of one tile, beside the largest of the next tile's scores
+    auto products = [&](const uint8_t *buf) __attribute__((always_inline)) {
+        constexpr int kSteps = 2 * DB, kMax = 32 / kSteps;
+        uint32_t x = vat;
+        asm volatile("" : "+v"(x));
+        u32x4 vf[2][2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) vf[i][h] = v_frag<DP>(buf, x, i / (DB / 2), 2 * (i % (DB / 2)) + h);
+        float mg[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            __builtin_amdgcn_sched_barrier(0);
+            const int st = i / (DB / 2), d = 2 * (i % (DB / 2));
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) o[d + h] = mfma_f16(vf[i & 1][h], pf[p][st], o[d + h]);
+            if (i + 2 < kSteps)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    vf[i & 1][h] = v_frag<DP>(buf, x, (i + 2) / (DB / 2), 2 * ((i + 2) % (DB / 2)) + h);
+#pragma unroll
+            for (int r = kMax * i; r < kMax * (i + 1); ++r) mg[r >> 3] = fmaxf(mg[r >> 3], s[r >> 4][r & 15]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        return largest(mg, c);
+    };
+    auto step = [&](uint8_t *k_this, uint8_t *k_next, uint8_t *v_this, uint8_t *v_next, uint32_t j)
+        __attribute__((always_inline)) {
+        lds_barrier();     // k_next and v_this are filled, k_this and v_next are done with
+        const bool more = j + kKeys < kmax;
+        if (more) {
+            put_k(k_this);
+            put_v(v_next);
+            fetch_k(j + 3 * kKeys);
+            fetch_v(j + 2 * kKeys);
+        }
+        if (!live) return;
+        prepare();
+        int top = kVeMin;
+        if (more) {
+            f32x16 nx[2];
+            scores(k_next, nx, true);
+            s[0] = nx[0], s[1] = nx[1];
+            limit(j + kKeys, &top);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) weight_pair(i);
+        }
+        const float mt = products(v_this);
+        if (more) rescale(mt, top);
+    };
+    if (j1 < kmax) {
+        put_k(kb0);
+        put_v(vb0);
+        fetch_k(j1 + kKeys);
+        fetch_v(j1 + kKeys);
+        put_k(kb1);
+        fetch_k(j1 + 2 * kKeys);
+        lds_barrier();
+        scores(kb0, s, false);
+        int top;
+        limit(j1, &top);
+        float mg[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int r = 0; r < 32; ++r) mg[r >> 3] = fmaxf(mg[r >> 3], s[r >> 4][r & 15]);
+        rescale(largest(mg, c), top);
+        for (uint32_t j = j1; j < kmax; j += 2 * kKeys) {
+            step(kb0, kb1, vb0, vb1, j);
+            if (j + kKeys < kmax) step(kb1, kb0, vb1, vb0, j + kKeys);
+        }
+    }
+    l += __shfl_xor(l, 32, 64);
+    const float unit = ldexpf(1.0f, ve - 7);
+    if (k.splits > 1) {
+        if (wr0 + lr >= R) return;
+        float *dst = k.part + (((uint64_t(place) * a.Hkv + kh) * k.splits + split) * kRows + 32 * wave + lr) * (DP + 2);
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) dst[32 * d + 8 * g + 4 * lg + e] = o[d][4 * g + e] * unit;
+        if (lg == 0) dst[DP] = m, dst[DP + 1] = l;
+        return;
+    }
+    // rows stored whole through LDS (16-bit), or as they are (f32)
+    const float inv = lim == 0 ? 0.0f : unit / l;
+    T *out = static_cast<T *>(a.out) + (uint64_t(t0) * a.H + kh * G) * a.D;
+    if constexpr (kF32) {
+        if (wr0 + lr >= R) return;
+        T *to = out + (uint64_t(tok) * a.H + (row - tok * G)) * a.D;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const uint32_t dim = 32 * d + 8 * g + 4 * lg;
+                if (dim < a.D)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) to[dim + e] = o[d][4 * g + e] * inv;
+            }
+    } else {
+        lds_barrier();
+        uint8_t *turn = (wave & 2 ? kb1 : kb0) + (wave & 1) * (32 * RB);
+        constexpr uint32_t CPR = RB / 16, RPL = 1024 / RB;
+        auto chunk_at = [&](uint32_t r, uint32_t q) { return r * RB + (q ^ (r & (CPR - 1u) & 15u)) * 16u; };
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<uint2 *>(turn + chunk_at(lr, 4 * d + g) + 8 * lg) =
+                    make_uint2(pack2<E>(o[d][4 * g] * inv, o[d][4 * g + 1] * inv),
+                               pack2<E>(o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv));
+        __builtin_amdgcn_wave_barrier();
+        const uint32_t q = lane % CPR;
+#pragma unroll
+        for (uint32_t i = 0; i < 32 / RPL; ++i) {
+            const uint32_t r = i * RPL + lane / CPR, rr = wr0 + r, t = rr / G;
+            if (rr < R && 8 * q < a.D)
+                *reinterpret_cast<u32x4 *>(out + (uint64_t(t) * a.H + (rr - t * G)) * a.D + 8 * q) =
+                    *reinterpret_cast<const u32x4 *>(turn + chunk_at(r, q));
+        }
+    }
+}
+
+template <class E, int DP>
+__global__ __launch_bounds__(256, (DP > 128 || sizeof(typename E::T) == 4 ? 1 : 2)) void chunk_tile_kernel(Chunk k) {
+    chunk_tile<E, DP>(k);
+}
+
+// Joins a row tile's shares: grid places * Hkv * (kRows / 4), a wavefront a row.
+template <class E, int DP>
+__global__ __launch_bounds__(256) void join_kernel(Chunk k) {
+    const AttnBlocksArgs &a = k.a;
+    const uint32_t G = a.H / a.Hkv, kh = blockIdx.x % a.Hkv, rest = blockIdx.x / a.Hkv;
+    const uint32_t place = rest / (kRows / 4), c = rest % (kRows / 4) * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63u;
+    Place at;
+    if (!place_of(a.pb, G, kRows, place, &at)) return;
+    const uint32_t n = at.hi - at.lo, rr = at.unit * kRows + c;
+    if (rr >= n * G) return;
+    const uint32_t t = rr / G;
+    const bool none = visible_keys(a.lens[at.b], n, t, a.bucket) == 0;
+    const float *p = k.part + ((uint64_t(place) * a.Hkv + kh) * k.splits * kRows + c) * (DP + 2);
+    constexpr uint32_t kStride = kRows * (DP + 2);
+    float M = -INFINITY;
+    for (uint32_t w = 0; w < k.splits; ++w) M = fmaxf(M, p[w * kStride + DP]);
+    const float ref = M == -INFINITY ? 0.0f : M;
+    float l = 0.0f, o[DP / 64];
+#pragma unroll
+    for (int i = 0; i < DP / 64; ++i) o[i] = 0.0f;
+    for (uint32_t w = 0; w < k.splits; ++w) {
+        const float *x = p + w * kStride;
+        const float e = __builtin_amdgcn_exp2f(x[DP] - ref);
+        l = fmaf(x[DP + 1], e, l);
+#pragma unroll
+        for (int i = 0; i < DP / 64; ++i) o[i] = fmaf(x[lane + 64 * i], e, o[i]);
+    }
+    auto *out = static_cast<typename E::T *>(a.out) + (uint64_t(at.lo + t) * a.H + kh * G + (rr - t * G)) * a.D;
+#pragma unroll
+    for (int i = 0; i < DP / 64; ++i)
+        if (lane + 64 * i < a.D) out[lane + 64 * i] = E::narrow(none ? 0.0f : o[i] / l);
+}
+
 // What the matrix forms take: 16-byte rows of q and the caches, whole 16-key steps in
 // a block.
 bool matrix_applies(const AttnBlocksArgs &a) {
     auto at16 = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
     const uint32_t es = a.dtype == 8 ? 4 : 2;
     return a.D % 16 == 0 && a.D <= 256 && a.block >= 16 && (a.block & (a.block - 1)) == 0 && at16(a.kq) &&
-           at16(a.vq) && at16(a.q) && uint64_t(a.q_stride) * es % 16 == 0;
+           at16(a.vq) && at16(a.q) && at16(a.out) && uint64_t(a.q_stride) * es % 16 == 0;
 }
 uint32_t few_places(const AttnBlocksArgs &a) {
     return uint32_t(uint64_t(a.pb.tokens) * (a.H / a.Hkv) / kUnit) + a.pb.batch;
@@ -550,6 +998,30 @@ void launch_few(const Blocks &k, hipStream_t stream) {
     }
     few_shares_kernel<E, DP><<<kShares, 256, 0, stream>>>(k);
     merge_kernel<E, DP><<<grid, 256, 0, stream>>>(k);
+}
+uint32_t chunk_places(const AttnBlocksArgs &a) {
+    return uint32_t(uint64_t(a.pb.tokens) * (a.H / a.Hkv) / kRows) + a.pb.batch;
+}
+// Shares of a row tile's keys: as many as let the grid fill the GPU, none shorter than
+// four tiles of a full bucket.
+uint32_t chunk_splits(const AttnBlocksArgs &a) {
+    const uint64_t grid = uint64_t(chunk_places(a)) * a.Hkv;
+    const uint64_t most = a.bucket / (4 * kKeys), want = kResident / (grid ? grid : 1);
+    const uint64_t s = want < most ? want : most;
+    return uint32_t(s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s);
+}
+
+template <class E, int DP>
+void launch_chunk(const Chunk &k, hipStream_t stream) {
+    const uint32_t grid = k.places * k.a.Hkv;
+    chunk_tile_kernel<E, DP><<<grid * k.splits, 256, 0, stream>>>(k);
+    if (k.splits > 1) join_kernel<E, DP><<<grid * (kRows / 4), 256, 0, stream>>>(k);
+}
+template <class E>
+void launch_chunk(const Chunk &k, hipStream_t stream) {
+    if (k.a.D <= 64) launch_chunk<E, 64>(k, stream);
+    else if (k.a.D <= 128) launch_chunk<E, 128>(k, stream);
+    else launch_chunk<E, 256>(k, stream);
 }
 template <class E>
 void launch_few(const Blocks &k, hipStream_t stream) {
@@ -604,12 +1076,25 @@ void launch_rows(const AttnBlocksArgs &a, float mul, hipStream_t stream) {
 
 size_t attn_blocks_scratch_bytes(const AttnBlocksArgs &a) {
     if (!matrix_applies(a)) return 0;
+    if (!few_rows(a)) {
+        const uint64_t s = chunk_splits(a);
+        return s == 1 ? 0 : uint64_t(chunk_places(a)) * a.Hkv * s * kRows * (padded(a.D) + 2) * 4;
+    }
     if (a.bucket <= kDirect) return 0;
     return (uint64_t(few_places(a)) * a.Hkv + kShares) * kUnit * (padded(a.D) + 2) * 4;
 }
 
 hipError_t launch_attn_blocks(const AttnBlocksArgs &a, void *scratch, hipStream_t stream) {
     const float mul = kLog2e / a.score_scale;
+    if (matrix_applies(a) && !few_rows(a)) {
+        Chunk k;
+        k.a = a, k.mul = mul, k.places = chunk_places(a), k.splits = chunk_splits(a);
+        k.part = static_cast<float *>(scratch), k.shift = uint32_t(__builtin_ctz(a.block));
+        if (a.dtype == 7) launch_chunk<Bf16>(k, stream);
+        else if (a.dtype == 6) launch_chunk<F16>(k, stream);
+        else launch_chunk<F32>(k, stream);
+        return hipGetLastError();
+    }
     if (matrix_applies(a)) {
         Blocks k;
         k.a = a, k.mul = mul, k.places = few_places(a), k.part = static_cast<float *>(scratch);

@@ -8,7 +8,7 @@
 #include <type_traits>
 
 #include "holo_kernels.h"
-#include "packed_batch.h"
+#include "packed_tile.h"
 
 namespace holo {
 namespace {
@@ -40,51 +40,12 @@ constexpr float kLog2e = 1.4426950408889634f;
 // added by the rows that see their keys (add_odd); the other rows' bits are what
 // they are without them.
 constexpr uint32_t kRows = 128, kKeys = 64;
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef short i16x4 __attribute__((ext_vector_type(4)));
-typedef short i16x8 __attribute__((ext_vector_type(8)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
-typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
-typedef __attribute__((address_space(3))) uint8_t lds_u8;
-
-// A workgroup barrier over LDS only: the loads in flight are not waited for.
-__device__ __forceinline__ void lds_barrier() {
-    __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4));   // lgkmcnt(0)
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-}
-
-// The same, with the loads into LDS landed.
-__device__ __forceinline__ void all_barrier() {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(7 << 4);   // vmcnt(0) lgkmcnt(0)
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-}
-
 template <class E>
 __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
     if constexpr (std::is_same_v<E, Bf16>)
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     else
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-
-// Two weights narrowed to nearest.
-template <class E>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-    if constexpr (std::is_same_v<E, Bf16>) {
-        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-        return __builtin_bit_cast(uint32_t, bf16x2{__bf16(lo), __bf16(hi)});
-    } else {
-        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-        return __builtin_bit_cast(uint32_t, f16x2{_Float16(lo), _Float16(hi)});
-    }
 }
 
 template <class E, int DP>
@@ -95,9 +56,6 @@ __device__ __forceinline__ void packed_tile(const AttnPackedArgs &a, const float
     typedef uint8_t Buf[kKeys * RB];
     __shared__ __attribute__((aligned(1024))) Buf kb0, kb1, vb0, vb1;
     __shared__ uint32_t odd0[4], odd1[4];   // found in vb0, vb1, by wavefront
-    auto swz_k = [](uint32_t row) { return DP >= 128 ? (row & 15u) : ((row >> 1) & 7u); };
-    auto swz_v = [](uint32_t row) { return DP >= 128 ? 4u * (row & 3u) : 4u * ((row >> 1) & 1u); };
-
     if (blockIdx.x == 0) check_starts(a.pb);
     const uint32_t G = a.H / a.Hkv, kh = blockIdx.x % a.Hkv;
     Place at;
@@ -123,7 +81,7 @@ __device__ __forceinline__ void packed_tile(const AttnPackedArgs &a, const float
 #pragma unroll
     for (int t = 0; t < LPW; ++t) {
         const uint32_t r = (wave * LPW + t) * RPL + lane / CPR, c = lane % CPR;
-        const uint32_t ck = c ^ swz_k(r), cv = c ^ swz_v(r);
+        const uint32_t ck = c ^ swz_k<DP>(r), cv = c ^ swz_v<DP>(r);
         koff[t] = 8 * ck < a.D ? (r * a.k_stride + 8 * ck) * 2u : kOob;
         voff[t] = 8 * cv < a.D ? (r * a.v_stride + 8 * cv) * 2u : kOob;
     }
@@ -188,15 +146,9 @@ __device__ __forceinline__ void packed_tile(const AttnPackedArgs &a, const float
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
     float m = -INFINITY, l = 0.0f;
-    const uint32_t g16 = uint32_t(lane) >> 4, r16 = uint32_t(lane) & 15u;
-    const uint32_t vrow = 4u * (g16 >> 1) + (r16 >> 2);
-    const uint32_t vchunk = 2u * (g16 & 1u) + ((r16 & 3u) >> 1);
-    // where a lane reads: chunk 2 k + lg of key row lr, swizzled, is the chunk of k = 0
-    // with 2 k toggled; V's 4 d likewise
-    const uint32_t kat = uint32_t(lr) * RB + ((uint32_t(lg) ^ swz_k(lr)) * 16u);
-    const uint32_t vat = vrow * RB + ((vchunk ^ swz_v(vrow)) * 16u) + (r16 & 1u) * 8u;
+    const uint32_t kat = k_place<DP>(lane), vat = v_place<DP>(lane);
 
-    // The elements that `put` left out, for the rows that see their keys: an infinity
+    // The elements that `screen` left out, for the rows that see their keys: an infinity
     // or NaN with a weight above 0 is the sum it joins.
     auto add_odd = [&](uint32_t j0) __attribute__((always_inline)) {
 #pragma unroll 1
@@ -217,19 +169,6 @@ __device__ __forceinline__ void packed_tile(const AttnPackedArgs &a, const float
 
     f32x16 s[2];
     u32x4 qf[NK];
-    // operand k (of NK) of the K tile in `buf`, key half h; of V's, 16-key step st and
-    // 32-dim block d
-    auto k_frag = [&](const uint8_t *buf, uint32_t at, int k, int h) __attribute__((always_inline)) {
-        return *reinterpret_cast<const lds_u32x4 *>((const lds_u8 *)buf + (at ^ (32u * k)) + 32u * RB * h);
-    };
-    auto v_frag = [&](const uint8_t *buf, uint32_t at, int st, int d) __attribute__((always_inline)) {
-        const lds_u8 *p = (const lds_u8 *)buf + (at ^ (64u * d)) + 16u * RB * st;
-        const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            reinterpret_cast<lds_i16x4 *>(const_cast<lds_u8 *>(p)));
-        const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            reinterpret_cast<lds_i16x4 *>(const_cast<lds_u8 *>(p + 8u * RB)));
-        return __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-    };
     auto limit = [&](uint32_t j0) __attribute__((always_inline)) {   // keys the row does not see
         if (j0 + kKeys <= wmin) return;
         int sees = int(lim) - int(j0) - 4 * lg;
@@ -279,7 +218,7 @@ __device__ __forceinline__ void packed_tile(const AttnPackedArgs &a, const float
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) kf[k][h] = k_frag(buf, at, k, h);
+            for (int h = 0; h < 2; ++h) kf[k][h] = k_frag<DP>(buf, at, k, h);
         const float ref = reference();
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -292,7 +231,7 @@ __device__ __forceinline__ void packed_tile(const AttnPackedArgs &a, const float
             for (int h = 0; h < 2; ++h) to[h] = mfma<E>(kf[k & 1][h], qf[k], to[h]);
             if (k + 2 < NK)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) kf[k & 1][h] = k_frag(buf, at, k + 2, h);
+                for (int h = 0; h < 2; ++h) kf[k & 1][h] = k_frag<DP>(buf, at, k + 2, h);
             if (weigh)
 #pragma unroll
                 for (int i = kPairs * k; i < kPairs * (k + 1); ++i) weight_pair(i, ref);
@@ -308,7 +247,7 @@ __device__ __forceinline__ void packed_tile(const AttnPackedArgs &a, const float
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) vf[i][h] = v_frag(buf, at, i / (DB / 2), 2 * (i % (DB / 2)) + h);
+            for (int h = 0; h < 2; ++h) vf[i][h] = v_frag<DP>(buf, at, i / (DB / 2), 2 * (i % (DB / 2)) + h);
         float mt = -INFINITY;
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
@@ -319,7 +258,7 @@ __device__ __forceinline__ void packed_tile(const AttnPackedArgs &a, const float
             if (i + 2 < kSteps)
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
-                    vf[i & 1][h] = v_frag(buf, at, (i + 2) / (DB / 2), 2 * ((i + 2) % (DB / 2)) + h);
+                    vf[i & 1][h] = v_frag<DP>(buf, at, (i + 2) / (DB / 2), 2 * ((i + 2) % (DB / 2)) + h);
 #pragma unroll
             for (int r = kMax * i; r < kMax * (i + 1); ++r) mt = fmaxf(mt, s[r >> 4][r & 15]);
         }
