@@ -375,24 +375,20 @@ __device__ __forceinline__ void sequence_quads(const AttnBlocksArgs &a, uint32_t
     *quads = len ? (len + kQuad - 1) / kQuad : 1u;
 }
 
+// The sequences' costs laid end to end.
 struct Line {
-    uint64_t total;      // quads of all units of all kv heads
+    uint64_t total;
     uint64_t at;         // where sequence b's begin
     uint32_t b;
 };
-// Where the sequence that holds quad `want(total)` of the line begins: 256 threads sum
-// a run of sequences each, the run that holds it is walked. A sequence's quads come
-// unit by unit, kv head by kv head.
-template <class F>
-__device__ __forceinline__ Line find_line(const AttnBlocksArgs &a, F want, uint64_t *sums, Line *found) {
-    const uint32_t tid = threadIdx.x, per = (a.pb.batch + 255) / 256;
-    const uint32_t b0 = tid * per, b1 = b0 + per < a.pb.batch ? b0 + per : a.pb.batch;
+// Where the sequence that holds place `want(total)` of the line begins: 256 threads sum
+// a run of sequences each, the run that holds it is walked.
+template <class C, class F>
+__device__ __forceinline__ Line find_line(uint32_t batch, C cost, F want, uint64_t *sums, Line *found) {
+    const uint32_t tid = threadIdx.x, per = (batch + 255) / 256;
+    const uint32_t b0 = tid * per, b1 = b0 + per < batch ? b0 + per : batch;
     uint64_t sum = 0;
-    uint32_t u, q;
-    for (uint32_t b = b0; b < b1; ++b) {
-        sequence_quads(a, b, &u, &q);
-        sum += uint64_t(u) * q * a.Hkv;
-    }
+    for (uint32_t b = b0; b < b1; ++b) sum += cost(b);
     // running sums: within a wavefront, then over the four
     uint64_t run = sum;
 #pragma unroll
@@ -414,8 +410,7 @@ __device__ __forceinline__ Line find_line(const AttnBlocksArgs &a, F want, uint6
     if (at >= base && at < base + sum) {
         uint64_t here = base;
         for (uint32_t b = b0; b < b1; ++b) {
-            sequence_quads(a, b, &u, &q);
-            const uint64_t all = uint64_t(u) * q * a.Hkv;
+            const uint64_t all = cost(b);
             if (at < here + all) {
                 *found = Line{total, here, b};
                 break;
@@ -440,7 +435,12 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void few_shares_kernel(Block
     const AttnBlocksArgs &a = k.a;
     if (blockIdx.x == 0) check_starts(a.pb);
     const uint32_t G = a.H / a.Hkv;
-    const Line ln = find_line(a, [&](uint64_t total) { return blockIdx.x * share_of(total); }, sums, &found);
+    // a sequence's quads come unit by unit, kv head by kv head
+    const Line ln = find_line(a.pb.batch, [&](uint32_t b) {
+        uint32_t units, quads;
+        sequence_quads(a, b, &units, &quads);
+        return uint64_t(units) * quads * a.Hkv;
+    }, [&](uint64_t total) { return blockIdx.x * share_of(total); }, sums, &found);
     const uint64_t share = share_of(ln.total);
     uint64_t pos = blockIdx.x * share, end = pos + share < ln.total ? pos + share : ln.total;
     uint64_t base = ln.at;
@@ -536,15 +536,20 @@ __global__ __launch_bounds__(256) void merge_kernel(Blocks k) {
 // zero V scale makes them zeros, on the way into LDS.
 // In a tile that some row does not see to its end, s is scaled and limited first (c = 1),
 // and a step that a row does not see brings it no scale.
-// Where the rows give too few workgroups, a row tile's keys are cut into `splits` shares
-// of whole tiles, whose partials join_kernel joins.
-constexpr uint32_t kRows = 128, kKeys = 64, kResident = 512, kMaxSplits = 32;
+// A workgroup a row tile and kv head where that gives many times what the GPU holds at
+// once. Fewer are dealt as equal shares of a line of keys, one share for each workgroup
+// that the GPU holds: unit u (a row tile) of a sequence costs past' + S (u + 1) keys,
+// past' what its rows see before their own to a multiple of 64 and S = ceil(128 / G)
+// the tokens that a unit spans at most, so that a sequence's cost and the unit at a
+// place of the line are closed forms; cuts fall on tiles. A unit that is cut leaves
+// partials for join_kernel.
+constexpr uint32_t kRows = 128, kKeys = 64, kManyRounds = 4, kMinKeys = 256;
 
 struct Chunk {
     AttnBlocksArgs a;
     float mul;
-    uint32_t shift, places, splits;
-    float *part;         // [places * Hkv * splits][kRows][DP + 2], as Blocks::part
+    uint32_t shift, places, shares;
+    float *part;         // [places * Hkv + shares][kRows][DP + 2], as Blocks::part
 };
 
 // Four int8 (xor 0x80) as f16.
@@ -566,21 +571,24 @@ __device__ __forceinline__ float largest(const float (&mg)[4], const float (&c)[
     return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
 }
 
+template <int DP>
+struct ChunkLds {
+    uint8_t k0[128 * DP], k1[128 * DP], v0[128 * DP], v1[128 * DP];   // kKeys rows of 2 DP bytes each
+};
+
+// Keys [c0, c1) (whole tiles, but for the last) of row tile at.unit of sequence at.b and
+// kv head kh, to the output (whole) or to a partial at dst.
 template <class E, int DP>
-__device__ __forceinline__ void chunk_tile(const Chunk &k) {
+__device__ __forceinline__ void chunk_segment(const Chunk &k, const Place &at, uint32_t kh, uint32_t c0, uint32_t c1,
+                                              bool whole, float *dst, ChunkLds<DP> &lds) {
     constexpr int RB = 2 * DP, NK = DP / 16, DB = DP / 32, CT = DP / 64;   // CT: 16-byte chunks a thread widens
     constexpr bool kF32 = std::is_same_v<E, F32>;
     constexpr int P = kF32 ? 2 : 1;
     constexpr float kLag = 8.0f;
     typedef typename E::T T;
-    typedef uint8_t Buf[kKeys * RB];
-    __shared__ __attribute__((aligned(1024))) Buf kb0, kb1, vb0, vb1;
+    uint8_t *const kb0 = lds.k0, *const kb1 = lds.k1, *const vb0 = lds.v0, *const vb1 = lds.v1;
     const AttnBlocksArgs &a = k.a;
-    if (blockIdx.x == 0) check_starts(a.pb);
-    const uint32_t G = a.H / a.Hkv, kh = blockIdx.x % a.Hkv, rest = blockIdx.x / a.Hkv;
-    const uint32_t split = rest % k.splits, place = k.places - 1 - rest / k.splits;
-    Place at;
-    if (!place_of(a.pb, G, kRows, place, &at)) return;
+    const uint32_t G = a.H / a.Hkv;
     const uint32_t t0 = at.lo, n = at.hi - at.lo, R = n * G, r0 = at.unit * kRows;
     const int tid = threadIdx.x, lane = tid & 63, lr = lane & 31, lg = lane >> 5;
     const uint32_t wave = pk_uni(uint32_t(tid) >> 6);
@@ -588,10 +596,8 @@ __device__ __forceinline__ void chunk_tile(const Chunk &k) {
     auto sees = [&](uint32_t r) { return visible_keys(len, n, (r < R ? r : R - 1) / G, a.bucket); };
     const uint32_t wr0 = r0 + 32 * wave, row = wr0 + lr < R ? wr0 + lr : R - 1, tok = row / G;
     const uint32_t lim = sees(row), wmin = pk_uni(sees(wr0));
-    const uint32_t kall = pk_uni(sees(r0 + kRows - 1)), tiles = (kall + kKeys - 1) / kKeys;
-    const uint32_t per = (tiles + k.splits - 1) / k.splits * kKeys;
-    const uint32_t j1 = split * per < kall ? split * per : kall;                  // this share's keys
-    const uint32_t kmax = j1 + per < kall ? j1 + per : kall;
+    const uint32_t kall = pk_uni(sees(r0 + kRows - 1));
+    const uint32_t j1 = c0 < kall ? c0 : kall, kmax = c1 < kall ? c1 : kall;
     const bool live = pk_uni(wr0 < R);
 
     // the tile's bytes: key tid / 4, chunks tid % 4 + 4 i of its row; its step's scales
@@ -709,13 +715,18 @@ __device__ __forceinline__ void chunk_tile(const Chunk &k) {
     float c[4], fr[4], lf[4];
     int ex[4];
 
+    float nk[4], nv[4];      // the next tile's scales, loaded a tile's scores ahead of their use
+    auto load_scales = [&](uint32_t j) __attribute__((always_inline)) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) nk[g] = scale_at(ks, j + 16 * g), nv[g] = scale_at(vs, j + 16 * g);
+    };
     // the scales of tile j, and s limited; the largest exponent of the steps the row sees
     auto limit = [&](uint32_t j, int *top) __attribute__((always_inline)) {
         *top = kVeMin;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            float v = fabsf(scale_at(vs, j + 16 * g));
-            c[g] = fabsf(scale_at(ks, j + 16 * g)) * mul;
+            float v = fabsf(nv[g]);
+            c[g] = fabsf(nk[g]) * mul;
             v = v == 0.0f ? 1.0f : v;      // (its bytes are zeros)
             const bool finite = v <= 3.4028235e38f;
             ex[g] = 0;
@@ -754,7 +765,7 @@ __device__ __forceinline__ void chunk_tile(const Chunk &k) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             up[g] = (lf[g] + float(ex[g] + 7 - ve)) - ref;
-            back[g] = ldexpf(1.0f / fr[g], ve - 7 - ex[g]);
+            back[g] = ldexpf(__builtin_amdgcn_rcpf(fr[g]), ve - 7 - ex[g]);   // (exact for powers of two)
         }
     };
     auto weight_pair = [&](int i) __attribute__((always_inline)) {
@@ -840,6 +851,7 @@ __device__ __forceinline__ void chunk_tile(const Chunk &k) {
         lds_barrier();     // k_next and v_this are filled, k_this and v_next are done with
         const bool more = j + kKeys < kmax;
         if (more) {
+            load_scales(j + kKeys);
             put_k(k_this);
             put_v(v_next);
             fetch_k(j + 3 * kKeys);
@@ -861,6 +873,7 @@ __device__ __forceinline__ void chunk_tile(const Chunk &k) {
         if (more) rescale(mt, top);
     };
     if (j1 < kmax) {
+        load_scales(j1);
         put_k(kb0);
         put_v(vb0);
         fetch_k(j1 + kKeys);
@@ -882,9 +895,9 @@ __device__ __forceinline__ void chunk_tile(const Chunk &k) {
     }
     l += __shfl_xor(l, 32, 64);
     const float unit = ldexpf(1.0f, ve - 7);
-    if (k.splits > 1) {
+    if (!whole) {
         if (wr0 + lr >= R) return;
-        float *dst = k.part + (((uint64_t(place) * a.Hkv + kh) * k.splits + split) * kRows + 32 * wave + lr) * (DP + 2);
+        dst += (32 * wave + lr) * (DP + 2);
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -933,42 +946,138 @@ __device__ __forceinline__ void chunk_tile(const Chunk &k) {
     }
 }
 
+// A row tile a workgroup: grid places * Hkv, those that see most keys first.
 template <class E, int DP>
 __global__ __launch_bounds__(256, (DP > 128 || sizeof(typename E::T) == 4 ? 1 : 2)) void chunk_tile_kernel(Chunk k) {
-    chunk_tile<E, DP>(k);
+    __shared__ __attribute__((aligned(1024))) ChunkLds<DP> lds;
+    if (blockIdx.x == 0) check_starts(k.a.pb);
+    Place at;
+    if (!place_of(k.a.pb, k.a.H / k.a.Hkv, kRows, k.places - 1 - blockIdx.x / k.a.Hkv, &at)) return;
+    chunk_segment<E, DP>(k, at, blockIdx.x % k.a.Hkv, 0, k.a.bucket, true, nullptr, lds);
 }
 
-// Joins a row tile's shares: grid places * Hkv * (kRows / 4), a wavefront a row.
+// The row tiles of sequence b and the line of their costs, one kv head's.
+struct Units {
+    uint32_t units, past, S;
+    __device__ __forceinline__ uint64_t before(uint32_t u) const {   // cost of units 0 .. u - 1
+        return uint64_t(u) * past + uint64_t(S) * (uint64_t(u) * (u + 1) / 2);
+    }
+    __device__ __forceinline__ uint32_t holding(uint64_t at) const {   // the unit at place `at`
+        uint32_t lo = 0, hi = units;
+        while (hi - lo > 1) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            if (before(mid) <= at) lo = mid;
+            else hi = mid;
+        }
+        return lo;
+    }
+};
+__device__ __forceinline__ Units sequence_units(const AttnBlocksArgs &a, uint32_t b) {
+    const uint32_t lo = start_of(a.pb, b), hi = start_of(a.pb, b + 1), G = a.H / a.Hkv, n = hi > lo ? hi - lo : 0u;
+    const uint32_t past = visible_keys(int64_t(a.lens[b]) - n, 1, 0, a.bucket);
+    return Units{(n * G + kRows - 1) / kRows, (past + kKeys - 1) / kKeys * kKeys, (kRows + G - 1) / G};
+}
+__device__ __forceinline__ uint64_t keys_of(uint64_t total, uint32_t shares) {
+    const uint64_t s = (total + shares - 1) / shares;
+    return s < kMinKeys ? kMinKeys : s;
+}
+
+template <class E, int DP>
+__global__ __launch_bounds__(256, (DP > 128 || sizeof(typename E::T) == 4 ? 1 : 2)) void chunk_shares_kernel(Chunk k) {
+    __shared__ __attribute__((aligned(1024))) ChunkLds<DP> lds;
+    __shared__ uint64_t sums[4];
+    __shared__ Line found;
+    const AttnBlocksArgs &a = k.a;
+    if (blockIdx.x == 0) check_starts(a.pb);
+    const uint32_t G = a.H / a.Hkv;
+    const Line ln = find_line(a.pb.batch, [&](uint32_t b) {
+        const Units u = sequence_units(a, b);
+        return u.before(u.units) * a.Hkv;
+    }, [&](uint64_t total) { return blockIdx.x * keys_of(total, k.shares); }, sums, &found);
+    const uint64_t share = keys_of(ln.total, k.shares);
+    uint64_t pos = blockIdx.x * share, base = ln.at;
+    const uint64_t end = pos + share < ln.total ? pos + share : ln.total;
+    for (uint32_t b = ln.b; pos < end && b < a.pb.batch; ++b) {
+        const Units u = sequence_units(a, b);
+        const uint64_t one = u.before(u.units), all = one * a.Hkv;
+        while (pos < end && pos < base + all) {
+            const uint32_t kh = pk_uni(uint32_t((pos - base) / one));
+            const uint64_t in = pos - base - kh * one;            // place in the head's line
+            const uint32_t unit = pk_uni(u.holding(in));
+            const uint64_t from = u.before(unit), cost = u.before(unit + 1) - from;
+            const uint64_t left = in - from, right = left + (end - pos) < cost ? left + (end - pos) : cost;
+            // cuts at the next tile's end; the unit's own end takes what is left
+            const uint32_t c0 = pk_uni(uint32_t((left + kKeys - 1) / kKeys * kKeys));
+            const uint32_t c1 = pk_uni(right == cost ? 0xffffffffu : uint32_t((right + kKeys - 1) / kKeys * kKeys));
+            const Place at{pk_uni(b), pk_uni(start_of(a.pb, b)), pk_uni(start_of(a.pb, b + 1)), unit};
+            const uint64_t id = uint64_t(at.lo * G / kRows + at.b) * a.Hkv + uint64_t(kh) * u.units + unit;
+            lds_barrier();     // the segment before is done with the buffers
+            chunk_segment<E, DP>(k, at, kh, c0, c1, pk_uni(left == 0 && right == cost),
+                                 k.part + (id + blockIdx.x) * (kRows * (DP + 2)), lds);
+            pos += right - left;
+        }
+        base += all;
+    }
+}
+
+// Joins the partials of a row tile that shares cut: grid places * Hkv * kJoin, a
+// wavefront a row in turn.
+constexpr uint32_t kJoin = 8;
 template <class E, int DP>
 __global__ __launch_bounds__(256) void join_kernel(Chunk k) {
+    __shared__ uint64_t sums[4], alls[4];
     const AttnBlocksArgs &a = k.a;
-    const uint32_t G = a.H / a.Hkv, kh = blockIdx.x % a.Hkv, rest = blockIdx.x / a.Hkv;
-    const uint32_t place = rest / (kRows / 4), c = rest % (kRows / 4) * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63u;
+    const uint32_t G = a.H / a.Hkv, kh = blockIdx.x % a.Hkv, rest = blockIdx.x / a.Hkv, lane = threadIdx.x & 63u;
     Place at;
-    if (!place_of(a.pb, G, kRows, place, &at)) return;
-    const uint32_t n = at.hi - at.lo, rr = at.unit * kRows + c;
-    if (rr >= n * G) return;
-    const uint32_t t = rr / G;
-    const bool none = visible_keys(a.lens[at.b], n, t, a.bucket) == 0;
-    const float *p = k.part + ((uint64_t(place) * a.Hkv + kh) * k.splits * kRows + c) * (DP + 2);
-    constexpr uint32_t kStride = kRows * (DP + 2);
-    float M = -INFINITY;
-    for (uint32_t w = 0; w < k.splits; ++w) M = fmaxf(M, p[w * kStride + DP]);
-    const float ref = M == -INFINITY ? 0.0f : M;
-    float l = 0.0f, o[DP / 64];
-#pragma unroll
-    for (int i = 0; i < DP / 64; ++i) o[i] = 0.0f;
-    for (uint32_t w = 0; w < k.splits; ++w) {
-        const float *x = p + w * kStride;
-        const float e = __builtin_amdgcn_exp2f(x[DP] - ref);
-        l = fmaf(x[DP + 1], e, l);
-#pragma unroll
-        for (int i = 0; i < DP / 64; ++i) o[i] = fmaf(x[lane + 64 * i], e, o[i]);
+    if (!place_of(a.pb, G, kRows, rest / kJoin, &at)) return;
+    uint64_t sum = 0, all = 0;       // costs before sequence at.b, and of all
+    for (uint32_t b = threadIdx.x; b < a.pb.batch; b += 256) {
+        const Units u = sequence_units(a, b);
+        const uint64_t c = u.before(u.units) * a.Hkv;
+        all += c;
+        sum += b < at.b ? c : 0;
     }
-    auto *out = static_cast<typename E::T *>(a.out) + (uint64_t(at.lo + t) * a.H + kh * G + (rr - t * G)) * a.D;
 #pragma unroll
-    for (int i = 0; i < DP / 64; ++i)
-        if (lane + 64 * i < a.D) out[lane + 64 * i] = E::narrow(none ? 0.0f : o[i] / l);
+    for (int o = 32; o >= 1; o >>= 1) {
+        sum += __shfl_xor(sum, o, 64);
+        all += __shfl_xor(all, o, 64);
+    }
+    if (lane == 0) sums[threadIdx.x >> 6] = sum, alls[threadIdx.x >> 6] = all;
+    __syncthreads();
+    sum = sums[0] + sums[1] + sums[2] + sums[3];
+    all = alls[0] + alls[1] + alls[2] + alls[3];
+    const Units u = sequence_units(a, at.b);
+    const uint64_t share = keys_of(all, k.shares), q0 = sum + kh * u.before(u.units) + u.before(at.unit);
+    const uint64_t w0 = q0 / share, w1 = (sum + kh * u.before(u.units) + u.before(at.unit + 1) - 1) / share;
+    if (w0 == w1) return;            // one workgroup had all of it
+    const uint32_t np = uint32_t(w1 - w0 + 1), n = at.hi - at.lo, R = n * G;
+    const uint64_t id = uint64_t(at.lo * G / kRows + at.b) * a.Hkv + uint64_t(kh) * u.units + at.unit;
+    constexpr uint32_t kStride = kRows * (DP + 2);
+    const float *src = k.part + (id + w0) * kStride;
+    for (uint32_t c = rest % kJoin * 4 + (threadIdx.x >> 6); c < kRows; c += 4 * kJoin) {
+        const uint32_t rr = at.unit * kRows + c;
+        if (rr >= R) return;
+        const uint32_t t = rr / G;
+        const bool none = visible_keys(a.lens[at.b], n, t, a.bucket) == 0;
+        const float *p = src + c * (DP + 2);
+        float M = -INFINITY;
+        for (uint32_t w = 0; w < np; ++w) M = fmaxf(M, p[w * kStride + DP]);
+        const float ref = M == -INFINITY ? 0.0f : M;
+        float l = 0.0f, o[DP / 64];
+#pragma unroll
+        for (int i = 0; i < DP / 64; ++i) o[i] = 0.0f;
+        for (uint32_t w = 0; w < np; ++w) {
+            const float *x = p + w * kStride;
+            const float e = __builtin_amdgcn_exp2f(x[DP] - ref);
+            l = fmaf(x[DP + 1], e, l);
+#pragma unroll
+            for (int i = 0; i < DP / 64; ++i) o[i] = fmaf(x[lane + 64 * i], e, o[i]);
+        }
+        auto *out = static_cast<typename E::T *>(a.out) + (uint64_t(at.lo + t) * a.H + kh * G + (rr - t * G)) * a.D;
+#pragma unroll
+        for (int i = 0; i < DP / 64; ++i)
+            if (lane + 64 * i < a.D) out[lane + 64 * i] = E::narrow(none ? 0.0f : o[i] / l);
+    }
 }
 
 // What the matrix forms take: 16-byte rows of q and the caches, whole 16-key steps in
@@ -1002,20 +1111,22 @@ void launch_few(const Blocks &k, hipStream_t stream) {
 uint32_t chunk_places(const AttnBlocksArgs &a) {
     return uint32_t(uint64_t(a.pb.tokens) * (a.H / a.Hkv) / kRows) + a.pb.batch;
 }
-// Shares of a row tile's keys: as many as let the grid fill the GPU, none shorter than
-// four tiles of a full bucket.
-uint32_t chunk_splits(const AttnBlocksArgs &a) {
-    const uint64_t grid = uint64_t(chunk_places(a)) * a.Hkv;
-    const uint64_t most = a.bucket / (4 * kKeys), want = kResident / (grid ? grid : 1);
-    const uint64_t s = want < most ? want : most;
-    return uint32_t(s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s);
+// Workgroups that the GPU holds at once (two a CU, one of f32 rows or 256 dims); 0 where
+// the row tiles are many times as many and need no shares.
+uint32_t chunk_shares(const AttnBlocksArgs &a) {
+    const uint32_t held = a.dtype == 8 || a.D > 128 ? 256 : 512;
+    return uint64_t(chunk_places(a)) * a.Hkv >= uint64_t(kManyRounds) * held ? 0 : held;
 }
 
 template <class E, int DP>
 void launch_chunk(const Chunk &k, hipStream_t stream) {
     const uint32_t grid = k.places * k.a.Hkv;
-    chunk_tile_kernel<E, DP><<<grid * k.splits, 256, 0, stream>>>(k);
-    if (k.splits > 1) join_kernel<E, DP><<<grid * (kRows / 4), 256, 0, stream>>>(k);
+    if (k.shares == 0) {
+        chunk_tile_kernel<E, DP><<<grid, 256, 0, stream>>>(k);
+        return;
+    }
+    chunk_shares_kernel<E, DP><<<k.shares, 256, 0, stream>>>(k);
+    join_kernel<E, DP><<<grid * kJoin, 256, 0, stream>>>(k);
 }
 template <class E>
 void launch_chunk(const Chunk &k, hipStream_t stream) {
@@ -1077,8 +1188,8 @@ void launch_rows(const AttnBlocksArgs &a, float mul, hipStream_t stream) {
 size_t attn_blocks_scratch_bytes(const AttnBlocksArgs &a) {
     if (!matrix_applies(a)) return 0;
     if (!few_rows(a)) {
-        const uint64_t s = chunk_splits(a);
-        return s == 1 ? 0 : uint64_t(chunk_places(a)) * a.Hkv * s * kRows * (padded(a.D) + 2) * 4;
+        const uint64_t s = chunk_shares(a);
+        return s == 0 ? 0 : (uint64_t(chunk_places(a)) * a.Hkv + s) * kRows * (padded(a.D) + 2) * 4;
     }
     if (a.bucket <= kDirect) return 0;
     return (uint64_t(few_places(a)) * a.Hkv + kShares) * kUnit * (padded(a.D) + 2) * 4;
@@ -1088,7 +1199,7 @@ hipError_t launch_attn_blocks(const AttnBlocksArgs &a, void *scratch, hipStream_
     const float mul = kLog2e / a.score_scale;
     if (matrix_applies(a) && !few_rows(a)) {
         Chunk k;
-        k.a = a, k.mul = mul, k.places = chunk_places(a), k.splits = chunk_splits(a);
+        k.a = a, k.mul = mul, k.places = chunk_places(a), k.shares = chunk_shares(a);
         k.part = static_cast<float *>(scratch), k.shift = uint32_t(__builtin_ctz(a.block));
         if (a.dtype == 7) launch_chunk<Bf16>(k, stream);
         else if (a.dtype == 6) launch_chunk<F16>(k, stream);
