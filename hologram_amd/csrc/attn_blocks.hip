@@ -500,24 +500,46 @@ __global__ __launch_bounds__(256) void merge_kernel(Blocks k) {
     const uint32_t np = uint32_t(w1 - w0 + 1), n = at.hi - at.lo, R = n * G;
     const uint32_t rows = R - at.unit * kUnit < kUnit ? R - at.unit * kUnit : kUnit;
     typedef typename E::T T;
-    const int64_t len = a.lens[at.b];
-    for (uint32_t i = threadIdx.x; i < rows * a.D; i += 256) {
-        const uint32_t c = i / a.D, d = i - c * a.D;
+    constexpr uint32_t kStride = kUnit * (DP + 2);
+    const uint32_t wave = pk_uni(threadIdx.x >> 6), lane = threadIdx.x & 63u;
+    // a wavefront a row: its lanes take the partials' weights, 64 at a time, then the dims
+    for (uint32_t c = wave; c < rows; c += 4) {
         const float *p = src + c * (DP + 2);
-        float M = -INFINITY;
-        for (uint32_t w = 0; w < np; ++w) M = fmaxf(M, p[w * (kUnit * (DP + 2)) + DP]);
+        float M = -INFINITY, l = 0.0f, o[DP / 64];
+        for (uint32_t w = lane; w < np; w += 64) M = fmaxf(M, p[w * kStride + DP]);
+#pragma unroll
+        for (int x = 32; x >= 1; x >>= 1) M = fmaxf(M, __shfl_xor(M, x, 64));
         const float ref = M == -INFINITY ? 0.0f : M;
-        float o = 0.0f, l = 0.0f;
-        for (uint32_t w = 0; w < np; ++w) {
-            const float *x = p + w * (kUnit * (DP + 2));
-            const float e = __builtin_amdgcn_exp2f(x[DP] - ref);
-            o = fmaf(x[d], e, o);
-            l = fmaf(x[DP + 1], e, l);
+#pragma unroll
+        for (int i = 0; i < DP / 64; ++i) o[i] = 0.0f;
+        for (uint32_t w0 = 0; w0 < np; w0 += 64) {
+            const bool in = w0 + lane < np;
+            const float e = in ? __builtin_amdgcn_exp2f(p[(w0 + lane) * kStride + DP] - ref) : 0.0f;
+            const float le = in ? p[(w0 + lane) * kStride + DP + 1] * e : 0.0f;
+            const uint32_t many = np - w0 < 64 ? np - w0 : 64;
+            for (uint32_t w = 0; w < many; w += 8) {
+                float x[8][DP / 64];
+#pragma unroll
+                for (uint32_t q = 0; q < 8; ++q)
+#pragma unroll
+                    for (int i = 0; i < DP / 64; ++i)
+                        x[q][i] = w + q < many ? p[(w0 + w + q) * kStride + lane + 64 * i] : 0.0f;
+#pragma unroll
+                for (uint32_t q = 0; q < 8; ++q) {
+                    if (w + q >= many) break;
+                    const float ew = __shfl(e, int(w + q), 64);
+                    l += __shfl(le, int(w + q), 64);
+#pragma unroll
+                    for (int i = 0; i < DP / 64; ++i) o[i] = fmaf(x[q][i], ew, o[i]);
+                }
+            }
         }
         const uint32_t rr = at.unit * kUnit + c, t = rr / G;
-        const bool none = visible_keys(len, n, t, a.bucket) == 0;
-        static_cast<T *>(a.out)[(uint64_t(at.lo + t) * a.H + kh * G + (rr - t * G)) * a.D + d] =
-            E::narrow(none ? 0.0f : o / l);
+        const bool none = visible_keys(a.lens[at.b], n, t, a.bucket) == 0;
+        T *out = static_cast<T *>(a.out) + (uint64_t(at.lo + t) * a.H + kh * G + (rr - t * G)) * a.D;
+#pragma unroll
+        for (int i = 0; i < DP / 64; ++i)
+            if (lane + 64 * i < a.D) out[lane + 64 * i] = E::narrow(none ? 0.0f : o[i] / l);
     }
 }
 
@@ -538,12 +560,13 @@ __global__ __launch_bounds__(256) void merge_kernel(Blocks k) {
 // and a step that a row does not see brings it no scale.
 // A workgroup a row tile and kv head where that gives many times what the GPU holds at
 // once. Fewer are dealt as equal shares of a line of keys, one share for each workgroup
-// that the GPU holds: unit u (a row tile) of a sequence costs past' + S (u + 1) keys,
-// past' what its rows see before their own to a multiple of 64 and S = ceil(128 / G)
-// the tokens that a unit spans at most, so that a sequence's cost and the unit at a
-// place of the line are closed forms; cuts fall on tiles. A unit that is cut leaves
-// partials for join_kernel.
-constexpr uint32_t kRows = 128, kKeys = 64, kManyRounds = 4, kMinKeys = 256;
+// that the GPU holds: unit u (a row tile) of a sequence costs kStart + past' + S (u + 1)
+// keys, past' what its rows see before their own to a multiple of 64, S = ceil(128 / G)
+// the tokens that a unit spans at most, and kStart what starting and ending a unit
+// takes in keys' time, so that a sequence's cost and the unit at a place of the line
+// are closed forms. A unit's keys begin at its place kStart; cuts fall on tiles. A unit
+// that is cut leaves partials for join_kernel.
+constexpr uint32_t kRows = 128, kKeys = 64, kManyRounds = 4, kMinKeys = 256, kStart = 192;
 
 struct Chunk {
     AttnBlocksArgs a;
@@ -642,19 +665,37 @@ __device__ __forceinline__ void chunk_segment(const Chunk &k, const Place &at, u
     fetch_k(j1);
     fetch_v(j1);
 
-    // Q's parts
+    // Q's parts, by way of LDS: whole rows into 32 QB bytes of the wavefront's own, a row
+    // past R a copy of the last
+    constexpr uint32_t QB = sizeof(T) * DP, QC = QB / 16, QR = 1024 / QB;
+    uint8_t *qbuf = kF32 ? (wave & 2 ? (wave & 1 ? vb1 : vb0) : (wave & 1 ? kb1 : kb0))
+                         : (wave & 2 ? vb1 : kb1) + (wave & 1) * (32 * QB);
+    auto chunk_at = [](uint32_t bytes, uint32_t r, uint32_t q) {   // 16-byte chunk q of row r
+        return r * bytes + (q ^ (r & (bytes / 16 - 1u) & 15u)) * 16u;
+    };
+    {
+        const uint32_t tok0 = r0 / G;
+        const auto r = range(static_cast<const T *>(a.q) + uint64_t(t0 + tok0) * a.q_stride + kh * G * a.D, kOob);
+#pragma unroll
+        for (uint32_t i = 0; i < 32 / QR; ++i) {
+            const uint32_t at_row = i * QR + lane / QC, rr = wr0 + at_row < R ? wr0 + at_row : R - 1, t = rr / G;
+            const uint32_t q = (lane % QC) ^ (at_row & (QC - 1u) & 15u);
+            const uint32_t off = ((t - tok0) * a.q_stride + (rr - t * G) * a.D) * uint32_t(sizeof(T)) + 16 * q;
+            load_to_lds(r, qbuf + 1024 * i, 16 * q < a.D * sizeof(T) ? off : kOob);
+        }
+    }
     u32x4 qf[P][NK];
     float mul;
     {
-        const T *q = static_cast<const T *>(a.q) + uint64_t(t0 + tok) * a.q_stride + (uint64_t(kh) * G + (row - tok * G)) * a.D;
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt((15 << 8) | (7 << 4));   // vmcnt(0)
+        asm volatile("" ::: "memory");
         float top = 0.0f;
         bool bad = false;
-        // a chunk of 8 elements, dims 16 i + 8 lg on
-        auto chunk = [&](int i, float (&x)[8]) {
+        auto chunk = [&](int i, float (&x)[8]) {   // dims 16 i + 8 lg on
 #pragma unroll
             for (int w = 0; w < int(sizeof(T)) / 2; ++w) {
-                u32x4 v = {0, 0, 0, 0};
-                if (uint32_t(16 * i + 8 * lg) < a.D) v = *reinterpret_cast<const u32x4 *>(q + 16 * i + 8 * lg + 4 * w);
+                const u32x4 v = *reinterpret_cast<const u32x4 *>(qbuf + chunk_at(QB, lr, (2 * i + lg) * (sizeof(T) / 2) + w));
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     if constexpr (kF32) {
@@ -666,7 +707,7 @@ __device__ __forceinline__ void chunk_segment(const Chunk &k, const Place &at, u
                 }
             }
         };
-#pragma unroll 2
+#pragma unroll
         for (int i = 0; i < NK; ++i) {
             float x[8];
             chunk(i, x);
@@ -689,17 +730,11 @@ __device__ __forceinline__ void chunk_segment(const Chunk &k, const Place &at, u
             float x[8];
             chunk(i, x);
 #pragma unroll
-            for (int p = 0; p < P; ++p)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float y[2];
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float v = bad ? 0.0f : ldexpf(x[2 * e + h], qe);
-                        y[h] = p == 0 ? v : v - float(_Float16(v));
-                    }
-                    qf[p][i][e] = pack2<F16>(y[0], y[1]);
-                }
+            for (int e = 0; e < 4; ++e) {
+                const float y0 = bad ? 0.0f : ldexpf(x[2 * e], qe), y1 = bad ? 0.0f : ldexpf(x[2 * e + 1], qe);
+                qf[0][i][e] = pack2<F16>(y0, y1);
+                if constexpr (kF32) qf[P - 1][i][e] = pack2<F16>(y0 - float(_Float16(y0)), y1 - float(_Float16(y1)));
+            }
         }
     }
 
@@ -874,13 +909,14 @@ __device__ __forceinline__ void chunk_segment(const Chunk &k, const Place &at, u
     };
     if (j1 < kmax) {
         load_scales(j1);
+        if constexpr (kF32) lds_barrier();   // Q has been read where these go
         put_k(kb0);
         put_v(vb0);
         fetch_k(j1 + kKeys);
         fetch_v(j1 + kKeys);
+        lds_barrier();     // and here
         put_k(kb1);
         fetch_k(j1 + 2 * kKeys);
-        lds_barrier();
         scores(kb0, s, false);
         int top;
         limit(j1, &top);
@@ -926,12 +962,11 @@ __device__ __forceinline__ void chunk_segment(const Chunk &k, const Place &at, u
         lds_barrier();
         uint8_t *turn = (wave & 2 ? kb1 : kb0) + (wave & 1) * (32 * RB);
         constexpr uint32_t CPR = RB / 16, RPL = 1024 / RB;
-        auto chunk_at = [&](uint32_t r, uint32_t q) { return r * RB + (q ^ (r & (CPR - 1u) & 15u)) * 16u; };
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int g = 0; g < 4; ++g)
-                *reinterpret_cast<uint2 *>(turn + chunk_at(lr, 4 * d + g) + 8 * lg) =
+                *reinterpret_cast<uint2 *>(turn + chunk_at(RB, lr, 4 * d + g) + 8 * lg) =
                     make_uint2(pack2<E>(o[d][4 * g] * inv, o[d][4 * g + 1] * inv),
                                pack2<E>(o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv));
         __builtin_amdgcn_wave_barrier();
@@ -941,7 +976,7 @@ __device__ __forceinline__ void chunk_segment(const Chunk &k, const Place &at, u
             const uint32_t r = i * RPL + lane / CPR, rr = wr0 + r, t = rr / G;
             if (rr < R && 8 * q < a.D)
                 *reinterpret_cast<u32x4 *>(out + (uint64_t(t) * a.H + (rr - t * G)) * a.D + 8 * q) =
-                    *reinterpret_cast<const u32x4 *>(turn + chunk_at(r, q));
+                    *reinterpret_cast<const u32x4 *>(turn + chunk_at(RB, r, q));
         }
     }
 }
@@ -960,7 +995,7 @@ __global__ __launch_bounds__(256, (DP > 128 || sizeof(typename E::T) == 4 ? 1 : 
 struct Units {
     uint32_t units, past, S;
     __device__ __forceinline__ uint64_t before(uint32_t u) const {   // cost of units 0 .. u - 1
-        return uint64_t(u) * past + uint64_t(S) * (uint64_t(u) * (u + 1) / 2);
+        return uint64_t(u) * (kStart + past) + uint64_t(S) * (uint64_t(u) * (u + 1) / 2);
     }
     __device__ __forceinline__ uint32_t holding(uint64_t at) const {   // the unit at place `at`
         uint32_t lo = 0, hi = units;
@@ -1006,15 +1041,17 @@ __global__ __launch_bounds__(256, (DP > 128 || sizeof(typename E::T) == 4 ? 1 : 
             const uint32_t unit = pk_uni(u.holding(in));
             const uint64_t from = u.before(unit), cost = u.before(unit + 1) - from;
             const uint64_t left = in - from, right = left + (end - pos) < cost ? left + (end - pos) : cost;
-            // cuts at the next tile's end; the unit's own end takes what is left
-            const uint32_t c0 = pk_uni(uint32_t((left + kKeys - 1) / kKeys * kKeys));
-            const uint32_t c1 = pk_uni(right == cost ? 0xffffffffu : uint32_t((right + kKeys - 1) / kKeys * kKeys));
+            pos += right - left;
+            // cuts at the next tile's end; the unit's own end takes what is left, and one
+            // before its keys begin leaves them to the share behind it
+            auto cut = [](uint64_t x) { return x <= kStart ? 0u : uint32_t((x - kStart + kKeys - 1) / kKeys * kKeys); };
+            const uint32_t c0 = pk_uni(cut(left)), c1 = pk_uni(right == cost ? 0xffffffffu : cut(right));
+            if (c1 == 0) continue;
             const Place at{pk_uni(b), pk_uni(start_of(a.pb, b)), pk_uni(start_of(a.pb, b + 1)), unit};
             const uint64_t id = uint64_t(at.lo * G / kRows + at.b) * a.Hkv + uint64_t(kh) * u.units + unit;
             lds_barrier();     // the segment before is done with the buffers
-            chunk_segment<E, DP>(k, at, kh, c0, c1, pk_uni(left == 0 && right == cost),
+            chunk_segment<E, DP>(k, at, kh, c0, c1, pk_uni(c0 == 0 && right == cost),
                                  k.part + (id + blockIdx.x) * (kRows * (DP + 2)), lds);
-            pos += right - left;
         }
         base += all;
     }
@@ -1047,8 +1084,9 @@ __global__ __launch_bounds__(256) void join_kernel(Chunk k) {
     sum = sums[0] + sums[1] + sums[2] + sums[3];
     all = alls[0] + alls[1] + alls[2] + alls[3];
     const Units u = sequence_units(a, at.b);
+    // the share that holds the unit's first keys, and its last
     const uint64_t share = keys_of(all, k.shares), q0 = sum + kh * u.before(u.units) + u.before(at.unit);
-    const uint64_t w0 = q0 / share, w1 = (sum + kh * u.before(u.units) + u.before(at.unit + 1) - 1) / share;
+    const uint64_t w0 = (q0 + kStart) / share, w1 = (sum + kh * u.before(u.units) + u.before(at.unit + 1) - 1) / share;
     if (w0 == w1) return;            // one workgroup had all of it
     const uint32_t np = uint32_t(w1 - w0 + 1), n = at.hi - at.lo, R = n * G;
     const uint64_t id = uint64_t(at.lo * G / kRows + at.b) * a.Hkv + uint64_t(kh) * u.units + at.unit;
@@ -1080,13 +1118,13 @@ __global__ __launch_bounds__(256) void join_kernel(Chunk k) {
     }
 }
 
-// What the matrix forms take: 16-byte rows of q and the caches, whole 16-key steps in
-// a block.
+// What the matrix forms take: 16-byte rows of q, the caches and the output, offsets
+// within a row tile's q below 2^30 bytes, whole 16-key steps in a block.
 bool matrix_applies(const AttnBlocksArgs &a) {
     auto at16 = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
     const uint32_t es = a.dtype == 8 ? 4 : 2;
     return a.D % 16 == 0 && a.D <= 256 && a.block >= 16 && (a.block & (a.block - 1)) == 0 && at16(a.kq) &&
-           at16(a.vq) && at16(a.q) && at16(a.out) && uint64_t(a.q_stride) * es % 16 == 0;
+           at16(a.vq) && at16(a.q) && at16(a.out) && uint64_t(a.q_stride) * es % 16 == 0 && a.q_stride < (1u << 21);
 }
 uint32_t few_places(const AttnBlocksArgs &a) {
     return uint32_t(uint64_t(a.pb.tokens) * (a.H / a.Hkv) / kUnit) + a.pb.batch;

@@ -89,9 +89,8 @@ __device__ __forceinline__ void packed_tile(const AttnPackedArgs &a, const float
         const uint32_t left = j0 < n ? (n - j0 < kKeys ? n - j0 : kKeys) : 0u;
         const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(base + uint64_t(left ? j0 : 0u) * stride), 0,
                                                          left ? int(((left - 1) * stride + a.D) * 2u) : 0, 0x00020000);
-        lds_u8 *to = (lds_u8 *)buf + wave * (LPW * 1024u);
 #pragma unroll
-        for (int t = 0; t < LPW; ++t) __builtin_amdgcn_raw_ptr_buffer_load_lds(r, to + 1024 * t, 16, off[t], 0, 0, 0);
+        for (int t = 0; t < LPW; ++t) load_to_lds(r, buf + (wave * LPW + t) * 1024u, off[t]);
     };
     auto load_k = [&](uint32_t j0, uint8_t *buf) { load_tile(kp, a.k_stride, j0, koff, buf); };
     auto load_v = [&](uint32_t j0, uint8_t *buf) { load_tile(vp, a.v_stride, j0, voff, buf); };
@@ -110,7 +109,7 @@ __device__ __forceinline__ void packed_tile(const AttnPackedArgs &a, const float
             const uint32_t at = t * RPL + lane / CPR, rr = wr0 + at < R ? wr0 + at : R - 1, tq = rr / G;
             const uint32_t c = (lane % CPR) ^ (at & (CPR - 1u) & 15u);
             const uint32_t off = ((tq - tok0) * a.q_stride + (rr - tq * G) * a.D + 8 * c) * 2u;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_u8 *)qbuf + 1024 * t, 16, 8 * c < a.D ? off : kOob, 0, 0, 0);
+            load_to_lds(r, qbuf + 1024 * t, 8 * c < a.D ? off : kOob);
         }
     }
     load_k(0, kb0);

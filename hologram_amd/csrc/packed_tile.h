@@ -40,6 +40,12 @@ __device__ __forceinline__ void all_barrier() {
     asm volatile("" ::: "memory");
 }
 
+// A wavefront's 1 KiB straight into LDS: each lane's 16 bytes at byte `off` of r, lane i's
+// to dst + 16 i.
+__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t r, uint8_t *dst, uint32_t off) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_u8 *)dst, 16, off, 0, 0, 0);
+}
+
 // Two weights narrowed to nearest.
 template <class E>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
