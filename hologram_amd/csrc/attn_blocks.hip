@@ -463,6 +463,46 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void few_shares_kernel(Block
     }
 }
 
+// One row of `np` partials, `stride` floats from one to the next, joined in order by a
+// wavefront: its lanes take the partials' weights, 64 at a time, then the dims, eight
+// partials in flight.
+template <class E, int DP>
+__device__ __forceinline__ void join_row(const float *p, uint32_t stride, uint32_t np, uint32_t D, bool none,
+                                         typename E::T *out) {
+    const uint32_t lane = threadIdx.x & 63u;
+    float M = -INFINITY, l = 0.0f, o[DP / 64];
+    for (uint32_t w = lane; w < np; w += 64) M = fmaxf(M, p[w * stride + DP]);
+#pragma unroll
+    for (int x = 32; x >= 1; x >>= 1) M = fmaxf(M, __shfl_xor(M, x, 64));
+    const float ref = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+    for (int i = 0; i < DP / 64; ++i) o[i] = 0.0f;
+    for (uint32_t w0 = 0; w0 < np; w0 += 64) {
+        const bool in = w0 + lane < np;
+        const float e = in ? __builtin_amdgcn_exp2f(p[(w0 + lane) * stride + DP] - ref) : 0.0f;
+        const float le = in ? p[(w0 + lane) * stride + DP + 1] * e : 0.0f;
+        const uint32_t many = np - w0 < 64 ? np - w0 : 64;
+        for (uint32_t w = 0; w < many; w += 8) {
+            float x[8][DP / 64];
+#pragma unroll
+            for (uint32_t q = 0; q < 8; ++q)
+#pragma unroll
+                for (int i = 0; i < DP / 64; ++i) x[q][i] = w + q < many ? p[(w0 + w + q) * stride + lane + 64 * i] : 0.0f;
+#pragma unroll
+            for (uint32_t q = 0; q < 8; ++q) {
+                if (w + q >= many) break;
+                const float ew = __shfl(e, int(w + q), 64);
+                l += __shfl(le, int(w + q), 64);
+#pragma unroll
+                for (int i = 0; i < DP / 64; ++i) o[i] = fmaf(x[q][i], ew, o[i]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < DP / 64; ++i)
+        if (lane + 64 * i < D) out[lane + 64 * i] = E::narrow(none ? 0.0f : o[i] / l);
+}
+
 // Joins the partials of a unit that shares cut: grid places * Hkv.
 template <class E, int DP>
 __global__ __launch_bounds__(256) void merge_kernel(Blocks k) {
@@ -501,45 +541,12 @@ __global__ __launch_bounds__(256) void merge_kernel(Blocks k) {
     const uint32_t rows = R - at.unit * kUnit < kUnit ? R - at.unit * kUnit : kUnit;
     typedef typename E::T T;
     constexpr uint32_t kStride = kUnit * (DP + 2);
-    const uint32_t wave = pk_uni(threadIdx.x >> 6), lane = threadIdx.x & 63u;
-    // a wavefront a row: its lanes take the partials' weights, 64 at a time, then the dims
+    const uint32_t wave = pk_uni(threadIdx.x >> 6);
     for (uint32_t c = wave; c < rows; c += 4) {
-        const float *p = src + c * (DP + 2);
-        float M = -INFINITY, l = 0.0f, o[DP / 64];
-        for (uint32_t w = lane; w < np; w += 64) M = fmaxf(M, p[w * kStride + DP]);
-#pragma unroll
-        for (int x = 32; x >= 1; x >>= 1) M = fmaxf(M, __shfl_xor(M, x, 64));
-        const float ref = M == -INFINITY ? 0.0f : M;
-#pragma unroll
-        for (int i = 0; i < DP / 64; ++i) o[i] = 0.0f;
-        for (uint32_t w0 = 0; w0 < np; w0 += 64) {
-            const bool in = w0 + lane < np;
-            const float e = in ? __builtin_amdgcn_exp2f(p[(w0 + lane) * kStride + DP] - ref) : 0.0f;
-            const float le = in ? p[(w0 + lane) * kStride + DP + 1] * e : 0.0f;
-            const uint32_t many = np - w0 < 64 ? np - w0 : 64;
-            for (uint32_t w = 0; w < many; w += 8) {
-                float x[8][DP / 64];
-#pragma unroll
-                for (uint32_t q = 0; q < 8; ++q)
-#pragma unroll
-                    for (int i = 0; i < DP / 64; ++i)
-                        x[q][i] = w + q < many ? p[(w0 + w + q) * kStride + lane + 64 * i] : 0.0f;
-#pragma unroll
-                for (uint32_t q = 0; q < 8; ++q) {
-                    if (w + q >= many) break;
-                    const float ew = __shfl(e, int(w + q), 64);
-                    l += __shfl(le, int(w + q), 64);
-#pragma unroll
-                    for (int i = 0; i < DP / 64; ++i) o[i] = fmaf(x[q][i], ew, o[i]);
-                }
-            }
-        }
         const uint32_t rr = at.unit * kUnit + c, t = rr / G;
         const bool none = visible_keys(a.lens[at.b], n, t, a.bucket) == 0;
         T *out = static_cast<T *>(a.out) + (uint64_t(at.lo + t) * a.H + kh * G + (rr - t * G)) * a.D;
-#pragma unroll
-        for (int i = 0; i < DP / 64; ++i)
-            if (lane + 64 * i < a.D) out[lane + 64 * i] = E::narrow(none ? 0.0f : o[i] / l);
+        join_row<E, DP>(src + c * (DP + 2), kStride, np, a.D, none, out);
     }
 }
 
@@ -634,6 +641,11 @@ __device__ __forceinline__ void chunk_segment(const Chunk &k, const Place &at, u
         const uint32_t i = j >> k.shift;
         return x[i < nb ? i : nb - 1];
     };
+    auto uniform_at = [&](const float *x, uint32_t j) {   // alike in all lanes: a scalar load
+        const uint32_t i = j >> k.shift;
+        return reinterpret_cast<const __attribute__((address_space(4))) float *>(
+            reinterpret_cast<uintptr_t>(x))[i < nb ? i : nb - 1];
+    };
     u32x4 kr[CT], vr[CT];
     float ksk, vsk;
     auto fetch = [&](const __amdgpu_buffer_rsrc_t r, uint32_t j, u32x4 (&x)[CT]) {
@@ -645,7 +657,7 @@ __device__ __forceinline__ void chunk_segment(const Chunk &k, const Place &at, u
     };
     auto fetch_k = [&](uint32_t j) { fetch(rk, j, kr), ksk = scale_at(ks, j + key); };
     auto fetch_v = [&](uint32_t j) { fetch(rv, j, vr), vsk = scale_at(vs, j + key); };
-    auto put = [&](uint8_t *buf, const u32x4 (&x)[CT], float scale, bool zero, auto swz) {
+    auto put = [&](uint8_t *buf, const u32x4 (&x)[CT], float scale, bool zero, const uint32_t (&to)[2]) {
         const uint32_t flip = __float_as_uint(scale) >> 31 ? 0x80008000u : 0u;
         const bool plain = !__any(flip != 0 || zero);
 #pragma unroll
@@ -654,14 +666,23 @@ __device__ __forceinline__ void chunk_segment(const Chunk &k, const Place &at, u
             for (int h = 0; h < 2; ++h) {
                 const uint2 lo = widen4(x[i][2 * h]), hi = widen4(x[i][2 * h + 1]);
                 u32x4 v = {lo.x, lo.y, hi.x, hi.y};
-                if (!plain)
+                if (!plain) {
+                    asm volatile("");      // a branch of its own
 #pragma unroll
                     for (int w = 0; w < 4; ++w) v[w] = zero ? 0u : v[w] ^ flip;
-                *reinterpret_cast<u32x4 *>(buf + key * RB + (((2u * (part + 4u * i) + h) ^ swz(key)) * 16u)) = v;
+                }
+                *reinterpret_cast<u32x4 *>(buf + (to[h] ^ (128u * i))) = v;
             }
     };
-    auto put_k = [&](uint8_t *buf) { put(buf, kr, ksk, false, [](uint32_t r) { return swz_k<DP>(r); }); };
-    auto put_v = [&](uint8_t *buf) { put(buf, vr, vsk, vsk == 0.0f, [](uint32_t r) { return swz_v<DP>(r); }); };
+    // chunk 2 (part + 4 i) + h of the key's row, swizzled
+    uint32_t kto[2], vto[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        kto[h] = key * RB + (((2u * part + h) ^ swz_k<DP>(key)) * 16u);
+        vto[h] = key * RB + (((2u * part + h) ^ swz_v<DP>(key)) * 16u);
+    }
+    auto put_k = [&](uint8_t *buf) { put(buf, kr, ksk, false, kto); };
+    auto put_v = [&](uint8_t *buf) { put(buf, vr, vsk, vsk == 0.0f, vto); };
     fetch_k(j1);
     fetch_v(j1);
 
@@ -753,24 +774,38 @@ __device__ __forceinline__ void chunk_segment(const Chunk &k, const Place &at, u
     float nk[4], nv[4];      // the next tile's scales, loaded a tile's scores ahead of their use
     auto load_scales = [&](uint32_t j) __attribute__((always_inline)) {
 #pragma unroll
-        for (int g = 0; g < 4; ++g) nk[g] = scale_at(ks, j + 16 * g), nv[g] = scale_at(vs, j + 16 * g);
+        for (int g = 0; g < 4; ++g) nk[g] = uniform_at(ks, j + 16 * g), nv[g] = uniform_at(vs, j + 16 * g);
     };
     // the scales of tile j, and s limited; the largest exponent of the steps the row sees
+    auto take = [&](int g) __attribute__((always_inline)) {
+        c[g] = fabsf(nk[g]) * mul;
+        float v = fabsf(nv[g]);
+        v = v == 0.0f ? 1.0f : v;      // (its bytes are zeros)
+        ex[g] = 0;
+        fr[g] = v <= 3.4028235e38f ? frexpf(v, &ex[g]) : v;        // fr in [0.5, 1)
+        lf[g] = __builtin_amdgcn_logf(fr[g]);
+    };
     auto limit = [&](uint32_t j, int *top) __attribute__((always_inline)) {
+        take(0);
+        if (k.shift >= 6) {            // one block holds the tile
+            asm volatile("");
+#pragma unroll
+            for (int g = 1; g < 4; ++g) c[g] = c[0], fr[g] = fr[0], lf[g] = lf[0], ex[g] = ex[0];
+        } else {
+#pragma unroll
+            for (int g = 1; g < 4; ++g) take(g);
+        }
+        const bool all = j + kKeys <= wmin;
+        if (!all) {
+            asm volatile("");
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                if (j + 16 * g >= lim) fr[g] = 0.5f, lf[g] = -1.0f, ex[g] = kVeMin;
+        }
         *top = kVeMin;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            float v = fabsf(nv[g]);
-            c[g] = fabsf(nk[g]) * mul;
-            v = v == 0.0f ? 1.0f : v;      // (its bytes are zeros)
-            const bool finite = v <= 3.4028235e38f;
-            ex[g] = 0;
-            fr[g] = finite ? frexpf(v, &ex[g]) : v;        // fr in [0.5, 1)
-            if (j + kKeys > wmin && j + 16 * g >= lim) fr[g] = 0.5f, ex[g] = kVeMin;
-            lf[g] = __builtin_amdgcn_logf(fr[g]);
-            *top = finite && ex[g] > *top ? ex[g] : *top;
-        }
-        if (j + kKeys <= wmin) return;
+        for (int g = 0; g < 4; ++g) *top = fr[g] < 1.0f && ex[g] > *top ? ex[g] : *top;   // (not of an infinity or NaN)
+        if (all) return;
         int see = int(lim < kmax ? lim : kmax) - int(j) - 4 * lg;
         asm volatile("" : "+v"(see));
 #pragma unroll
@@ -1059,7 +1094,7 @@ __global__ __launch_bounds__(256, (DP > 128 || sizeof(typename E::T) == 4 ? 1 : 
 
 // Joins the partials of a row tile that shares cut: grid places * Hkv * kJoin, a
 // wavefront a row in turn.
-constexpr uint32_t kJoin = 8;
+constexpr uint32_t kJoin = 16;
 template <class E, int DP>
 __global__ __launch_bounds__(256) void join_kernel(Chunk k) {
     __shared__ uint64_t sums[4], alls[4];
@@ -1097,24 +1132,8 @@ __global__ __launch_bounds__(256) void join_kernel(Chunk k) {
         if (rr >= R) return;
         const uint32_t t = rr / G;
         const bool none = visible_keys(a.lens[at.b], n, t, a.bucket) == 0;
-        const float *p = src + c * (DP + 2);
-        float M = -INFINITY;
-        for (uint32_t w = 0; w < np; ++w) M = fmaxf(M, p[w * kStride + DP]);
-        const float ref = M == -INFINITY ? 0.0f : M;
-        float l = 0.0f, o[DP / 64];
-#pragma unroll
-        for (int i = 0; i < DP / 64; ++i) o[i] = 0.0f;
-        for (uint32_t w = 0; w < np; ++w) {
-            const float *x = p + w * kStride;
-            const float e = __builtin_amdgcn_exp2f(x[DP] - ref);
-            l = fmaf(x[DP + 1], e, l);
-#pragma unroll
-            for (int i = 0; i < DP / 64; ++i) o[i] = fmaf(x[lane + 64 * i], e, o[i]);
-        }
         auto *out = static_cast<typename E::T *>(a.out) + (uint64_t(at.lo + t) * a.H + kh * G + (rr - t * G)) * a.D;
-#pragma unroll
-        for (int i = 0; i < DP / 64; ++i)
-            if (lane + 64 * i < a.D) out[lane + 64 * i] = E::narrow(none ? 0.0f : o[i] / l);
+        join_row<E, DP>(src + c * (DP + 2), kStride, np, a.D, none, out);
     }
 }
 
