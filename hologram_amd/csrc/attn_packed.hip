@@ -342,13 +342,206 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void packed_tile_kernel(Attn
     packed_tile<E, DP>(a, mul, places);
 }
 
+// --------------------------------------------------------- tiled form, f32 ----
+// f32 rows on the f32 matrix cores (32x32x2, 64 cycles): products and sums in f32
+// throughout. They run at a sixteenth of the 16-bit rate, so a workgroup takes 32 rows
+// and its wavefronts share the rows' keys, 32-key tiles in turn: four times the
+// workgroups, a quarter of the chain. Each wavefront loads its own tiles into LDS, K's
+// next while V is multiplied and V's next while K is, and meets the others once, at the
+// end. A lane's scores are keys 8 (r / 4) + 4 (lane / 32) + r % 4 of row lane % 32, which
+// is the order V's operands are read in; Q's dims go to the steps in the order in which
+// 16-byte reads of K bring them. V that is not finite: as in the 16-bit form.
+constexpr uint32_t kRows32 = 32, kKeys32 = 32;
+
+template <int DP, int W>
+struct F32Lds {
+    // K and V, [32 keys][DP], chunk c of row r at c ^ (r & 15); then O, [32 rows][DP] likewise
+    float k[W][kKeys32 * DP], v[W][kKeys32 * DP];
+    float m[W][kRows32], l[W][kRows32];
+};
+
+// DC: the dims that are multiplied, of rows of DP.
+template <int DP, int DC, int W>
+__device__ __forceinline__ void packed_f32(const AttnPackedArgs &a, const float mul, const uint32_t places) {
+    constexpr int NC = DC / 8, DB = DC / 32;              // 16-byte chunks a lane reads of a key; 32-dim blocks
+    constexpr uint32_t CPR = DP / 4, RPL = 256 / DP, kOob = 0x80000000u;
+    __shared__ __attribute__((aligned(1024))) F32Lds<DP, W> lds;
+    if (blockIdx.x == 0) check_starts(a.pb);
+    const uint32_t G = a.H / a.Hkv, kh = blockIdx.x % a.Hkv;
+    Place at;
+    if (!place_of(a.pb, G, kRows32, places - 1 - blockIdx.x / a.Hkv, &at)) return;
+    const uint32_t t0 = at.lo, n = at.hi - at.lo, R = n * G, r0 = at.unit * kRows32;
+    const int tid = threadIdx.x, lane = tid & 63, lr = lane & 31, lg = lane >> 5;
+    const uint32_t wave = pk_uni(uint32_t(tid) >> 6);
+    const uint32_t row = r0 + lr < R ? r0 + lr : R - 1, tok = row / G, lim = tok + 1;
+    const uint32_t kmin = pk_uni(r0 / G + 1), kmax = pk_uni((r0 + kRows32 - 1 < R ? r0 + kRows32 - 1 : R - 1) / G + 1);
+    const float *kp = static_cast<const float *>(a.k) + uint64_t(t0) * a.k_stride + uint64_t(kh) * a.D;
+    const float *vp = static_cast<const float *>(a.v) + uint64_t(t0) * a.v_stride + uint64_t(kh) * a.D;
+    float *const kb = lds.k[wave], *const vb = lds.v[wave];
+    auto place = [](uint32_t r, uint32_t c) { return r * DP + (c ^ (r & 15u)) * 4u; };   // of a 16-byte chunk
+
+    auto load_tile = [&](const float *base, uint32_t stride, uint32_t j0, float *buf) {
+        const uint32_t left = j0 < n ? (n - j0 < kKeys32 ? n - j0 : kKeys32) : 0u;
+        const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(base + uint64_t(left ? j0 : 0u) * stride), 0,
+                                                         left ? int(((left - 1) * stride + a.D) * 4u) : 0, 0x00020000);
+#pragma unroll
+        for (uint32_t t = 0; t < kKeys32 / RPL; ++t) {
+            const uint32_t kr = t * RPL + lane / CPR, c = (lane % CPR) ^ (kr & 15u);
+            load_to_lds(r, reinterpret_cast<uint8_t *>(buf) + 1024 * t, 4 * c < a.D ? (kr * stride + 4 * c) * 4u : kOob);
+        }
+    };
+    load_tile(kp, a.k_stride, wave * kKeys32, kb);
+    load_tile(vp, a.v_stride, wave * kKeys32, vb);
+
+    // dims 8 i + 4 lg + e of the lane's row
+    float4 q[NC];
+    {
+        const float *qp = static_cast<const float *>(a.q) + uint64_t(t0 + tok) * a.q_stride + (uint64_t(kh) * G + (row - tok * G)) * a.D;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const uint32_t d = 8 * i + 4 * lg;
+            q[i] = d < a.D ? *reinterpret_cast<const float4 *>(qp + d) : float4{0, 0, 0, 0};
+        }
+    }
+    auto odd = [](float x) { return !(fabsf(x) <= 3.4028235e38f); };
+
+    f32x16 o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+    for (uint32_t j0 = wave * kKeys32; j0 < kmax; j0 += W * kKeys32) {
+        // K has landed (V's loads, the later ones, may not have)
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt((15 << 8) | (7 << 4) | ((kKeys32 / RPL) & 15) | (((kKeys32 / RPL) >> 4) << 14));
+        asm volatile("" ::: "memory");
+        f32x16 s;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const float4 x = *reinterpret_cast<const float4 *>(kb + place(lr, 2 * i + lg));
+            s = __builtin_amdgcn_mfma_f32_32x32x2f32(x.x, q[i].x, s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x2f32(x.y, q[i].y, s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x2f32(x.z, q[i].z, s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x2f32(x.w, q[i].w, s, 0, 0, 0);
+        }
+        // V has landed; K's reads are done, its next tile may come
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(7 << 4);   // vmcnt(0) lgkmcnt(0)
+        asm volatile("" ::: "memory");
+        load_tile(kp, a.k_stride, j0 + W * kKeys32, kb);
+        const bool full = j0 + kKeys32 <= kmin;
+        bool found = false;
+        if (!full) {
+            const int see = int(lim) - int(j0) - 4 * lg;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = 8 * (r >> 2) + (r & 3) < see ? s[r] : -INFINITY;
+#pragma unroll 1
+            for (uint32_t i = lane; i < kKeys32 * DP / 4; i += 64) {
+                float4 x = *reinterpret_cast<float4 *>(vb + 4 * i);
+                const bool here = odd(x.x) || odd(x.y) || odd(x.z) || odd(x.w);
+                found |= here;
+                if (!here) continue;
+                x.x = odd(x.x) ? 0.0f : x.x, x.y = odd(x.y) ? 0.0f : x.y;
+                x.z = odd(x.z) ? 0.0f : x.z, x.w = odd(x.w) ? 0.0f : x.w;
+                *reinterpret_cast<float4 *>(vb + 4 * i) = x;
+            }
+            found = __ballot(found) != 0;
+        }
+        float mt = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[r]);
+        mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * mul;
+        if (__any(mt > m)) {
+            const float mn = fmaxf(m, mt);
+            const float al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            l *= al;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) o[d] *= al;
+            m = mn;
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], mul, -ref));
+            l += s[r];
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const uint32_t kr = 8 * (r >> 2) + 4 * lg + (r & 3);
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vb[place(kr, 8 * d + (lr >> 2)) + (lr & 3)], s[r], o[d], 0, 0, 0);
+        }
+        if (__builtin_expect(found, 0)) {
+#pragma unroll 1
+            for (uint32_t j = j0; j < j0 + kKeys32 && j < n; ++j)
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const uint32_t dim = 32u * d + 8u * c + 4u * lg;
+                        if (j >= lim || dim >= a.D) continue;
+                        const float4 x = *reinterpret_cast<const float4 *>(vp + uint64_t(j) * a.v_stride + dim);
+                        o[d][4 * c] += odd(x.x) ? x.x : 0.0f;
+                        o[d][4 * c + 1] += odd(x.y) ? x.y : 0.0f;
+                        o[d][4 * c + 2] += odd(x.z) ? x.z : 0.0f;
+                        o[d][4 * c + 3] += odd(x.w) ? x.w : 0.0f;
+                    }
+        }
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4));   // lgkmcnt(0): V's reads are done
+        asm volatile("" ::: "memory");
+        load_tile(vp, a.v_stride, j0 + W * kKeys32, vb);
+    }
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(7 << 4);   // (the loads past the last tile still write LDS)
+    asm volatile("" ::: "memory");
+    l += __shfl_xor(l, 32, 64);
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            *reinterpret_cast<float4 *>(kb + place(lr, 8 * d + 2 * c + lg)) =
+                float4{o[d][4 * c], o[d][4 * c + 1], o[d][4 * c + 2], o[d][4 * c + 3]};
+    if (lg == 0) lds.m[wave][lr] = m, lds.l[wave][lr] = l;
+    __syncthreads();
+    float *out = static_cast<float *>(a.out) + (uint64_t(t0) * a.H + kh * G) * a.D;
+    for (uint32_t i = tid; i < kRows32 * CPR; i += 64 * W) {
+        const uint32_t r = i / CPR, c = i % CPR, rr = r0 + r, t = rr / G;
+        if (rr >= R || 4 * c >= a.D) continue;
+        float M = lds.m[0][r];
+#pragma unroll
+        for (int w = 1; w < W; ++w) M = fmaxf(M, lds.m[w][r]);
+        const float ref = M == -INFINITY ? 0.0f : M;
+        float4 x = {0, 0, 0, 0};
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float e = __builtin_amdgcn_exp2f(lds.m[w][r] - ref);
+            const float4 y = *reinterpret_cast<const float4 *>(lds.k[w] + place(r, c));
+            sum = fmaf(lds.l[w][r], e, sum);
+            x.x = fmaf(y.x, e, x.x), x.y = fmaf(y.y, e, x.y), x.z = fmaf(y.z, e, x.z), x.w = fmaf(y.w, e, x.w);
+        }
+        *reinterpret_cast<float4 *>(out + (uint64_t(t) * a.H + (rr - t * G)) * a.D + 4 * c) =
+            float4{x.x / sum, x.y / sum, x.z / sum, x.w / sum};
+    }
+}
+
+template <int DP, int DC, int W>
+__global__ __launch_bounds__(64 * W, 1) void packed_f32_kernel(AttnPackedArgs a, float mul, uint32_t places) {
+    packed_f32<DP, DC, W>(a, mul, places);
+}
+
 // What the tiles take: 16-byte rows of q, k, v and out, offsets within a tile's 64 keys
 // and a workgroup's 128 rows below 2^31 bytes.
 bool tiles_apply(const AttnPackedArgs &a) {
     auto at16 = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
     const uint32_t far = std::max({a.q_stride, a.k_stride, a.v_stride});
-    return a.dtype != 8 && a.D % 8 == 0 && a.D <= 256 && a.q_stride % 8 == 0 && a.k_stride % 8 == 0 &&
-           a.v_stride % 8 == 0 && at16(a.q) && at16(a.k) && at16(a.v) && at16(a.out) && far < (1u << 23);
+    const uint32_t e = a.dtype == 8 ? 4 : 8;      // elements of 16 bytes
+    return a.D % e == 0 && a.D <= 256 && a.q_stride % e == 0 && a.k_stride % e == 0 && a.v_stride % e == 0 && at16(a.q) && at16(a.k) && at16(a.v) && at16(a.out) && far < (1u << 23);
 }
 
 template <class E>
@@ -358,6 +551,15 @@ void launch_tiles(const AttnPackedArgs &a, float mul, hipStream_t stream) {
     if (a.D <= 64) packed_tile_kernel<E, 64><<<grid, 256, 0, stream>>>(a, mul, places);
     else if (a.D <= 128) packed_tile_kernel<E, 128><<<grid, 256, 0, stream>>>(a, mul, places);
     else packed_tile_kernel<E, 256><<<grid, 256, 0, stream>>>(a, mul, places);
+}
+
+void launch_f32(const AttnPackedArgs &a, float mul, hipStream_t stream) {
+    const uint32_t G = a.H / a.Hkv;
+    const uint32_t places = uint32_t(uint64_t(a.pb.tokens) * G / kRows32) + a.pb.batch, grid = places * a.Hkv;
+    if (a.D <= 64) packed_f32_kernel<64, 64, 4><<<grid, 256, 0, stream>>>(a, mul, places);
+    else if (a.D <= 96) packed_f32_kernel<128, 96, 4><<<grid, 256, 0, stream>>>(a, mul, places);
+    else if (a.D <= 128) packed_f32_kernel<128, 128, 4><<<grid, 256, 0, stream>>>(a, mul, places);
+    else packed_f32_kernel<256, 256, 2><<<grid, 128, 0, stream>>>(a, mul, places);      // (LDS for two wavefronts)
 }
 
 // ---------------------------------------------------------- general form ----
@@ -407,7 +609,8 @@ hipError_t launch_attn_packed(const AttnPackedArgs &a, hipStream_t stream) {
     const float mul = kLog2e / a.score_scale;
     if (tiles_apply(a)) {
         if (a.dtype == 7) launch_tiles<Bf16>(a, mul, stream);
-        else launch_tiles<F16>(a, mul, stream);
+        else if (a.dtype == 6) launch_tiles<F16>(a, mul, stream);
+        else launch_f32(a, mul, stream);
         return hipGetLastError();
     }
     if (a.dtype == 7) launch_rows<Bf16>(a, mul, stream);

@@ -7,46 +7,75 @@
 namespace holo {
 namespace {
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
 // A workgroup takes kCols columns of a row. What the rules say of a column is one
 // word in LDS: bits 0-18 how often it was generated, bits 19-30 one more than the
 // place of its summed bias, bit 31 seen in the prompt. Every workgroup reads the
 // row's whole history (it stays in L2) and keeps what falls into its columns, so
 // counts are integers whose order does not matter, and no column's rule leaves
-// the workgroup that writes it.
-constexpr uint32_t kCols = 4096, kThreads = 256;
+// the workgroup that writes it. Bound by the logits' own bytes where there are many
+// rows (128 rows of 128000 bf16 with masks, biases and 4096 tokens of history each):
+// 16384 columns and 1024 threads a workgroup then read the history eight times a row,
+// 4096 and 256 thirty-two times. Few rows take the small ones, to spread over the GPU.
+template <int kCols>
+constexpr uint32_t threads_of() { return kCols / 16; }
 
+// 16 bytes of elements.
 template <class E>
-__global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a, uint32_t chunks) {
-    __shared__ uint32_t word[kCols];
-    __shared__ int32_t ids[kLogitsMaxBiases];
-    __shared__ float sums[kLogitsMaxBiases];
-    const uint32_t row = blockIdx.x / chunks, c0 = (blockIdx.x % chunks) * kCols, tid = threadIdx.x;
-    const uint32_t cols = a.cols - c0 < kCols ? a.cols - c0 : kCols;
-    for (uint32_t c = tid; c < kCols; c += kThreads) word[c] = 0;
-    const int32_t *bi = a.bias_ids + uint64_t(row) * a.biases;
-    const float *bv = a.bias_values + uint64_t(row) * a.biases;
+union Vec {
+    u32x4 v;
+    typename E::T e[16 / sizeof(typename E::T)];
+};
+
+template <class E, int kCols>
+__global__ __launch_bounds__(threads_of<kCols>()) void logits_kernel(LogitsArgs a, uint32_t chunks, bool wide) {
+    constexpr uint32_t kThreads = threads_of<kCols>(), kV = 16 / sizeof(typename E::T);
+    __shared__ __attribute__((aligned(16))) uint32_t word[kCols];
+    extern __shared__ int32_t ids[];                    // [biases], then their sums
+    float *sums = reinterpret_cast<float *>(ids + a.biases);
+    const uint32_t row = blockIdx.x / chunks, tid = threadIdx.x;
+    const uint64_t at = uint64_t(row) * a.cols;
+    const auto *in = static_cast<const typename E::T *>(a.logits) + at;
+    auto *out = static_cast<typename E::T *>(a.out) + at;
+    // columns [c0, c0 + kCols) of which those in [0, cols) are there; c0 falls on 16 bytes
+    const uint32_t skew = wide ? uint32_t(reinterpret_cast<uintptr_t>(in) / sizeof(typename E::T)) % kV : 0u;
+    const int64_t c0 = int64_t(blockIdx.x % chunks) * kCols - skew;
+    auto place = [&](int32_t id) -> uint32_t {          // in word, kCols for none of them
+        const int64_t p = int64_t(id) - c0;
+        return id >= 0 && uint32_t(id) < a.cols && p >= 0 && p < kCols ? uint32_t(p) : uint32_t(kCols);
+    };
+    for (uint32_t c = 4 * tid; c < kCols; c += 4 * kThreads) *reinterpret_cast<u32x4 *>(word + c) = u32x4{0, 0, 0, 0};
     if (a.bias_ids)
-        for (uint32_t j = tid; j < a.biases; j += kThreads) ids[j] = bi[j];
+        for (uint32_t j = tid; j < a.biases; j += kThreads) ids[j] = a.bias_ids[uint64_t(row) * a.biases + j];
     __syncthreads();
     float rep = 1.0f, freq = 0.0f, pres = 0.0f;
     if (a.history) {
         const int32_t *h = a.history + uint64_t(row) * a.history_len;
-        const uint32_t n = a.spans[2 * row + 1] < a.history_len ? a.spans[2 * row + 1] : a.history_len;
-        const uint32_t prompt = a.spans[2 * row];
-        for (uint32_t i = tid; i < n; i += kThreads) {
-            const uint32_t c = uint32_t(h[i]) - c0;
-            if (h[i] < 0 || uint32_t(h[i]) < c0 || c >= cols) continue;
-            if (i < prompt) atomicOr(&word[c], 0x80000000u);
-            else atomicAdd(&word[c], 1u);
+        const uint32_t n = a.spans[2 * uint64_t(row) + 1] < a.history_len ? a.spans[2 * uint64_t(row) + 1] : a.history_len;
+        const uint32_t prompt = a.spans[2 * uint64_t(row)];
+        auto count = [&](int32_t id, uint32_t i) {
+            const uint32_t p = place(id);
+            if (p == kCols) return;
+            if (i < prompt) atomicOr(&word[p], 0x80000000u);
+            else atomicAdd(&word[p], 1u);
+        };
+        const uint32_t quads = reinterpret_cast<uintptr_t>(h) % 16 == 0 ? n / 4 : 0u;
+        for (uint32_t q = tid; q < quads; q += kThreads) {
+            const int4 x = reinterpret_cast<const int4 *>(h)[q];
+            count(x.x, 4 * q), count(x.y, 4 * q + 1), count(x.z, 4 * q + 2), count(x.w, 4 * q + 3);
         }
+        for (uint32_t k = 4 * quads + tid; k < n; k += kThreads) count(h[k], k);
         rep = a.params[3 * uint64_t(row)];
         freq = a.params[3 * uint64_t(row) + 1];
         pres = a.params[3 * uint64_t(row) + 2];
     }
-    if (a.bias_ids)
+    if (a.bias_ids) {
+        const float *bv = a.bias_values + uint64_t(row) * a.biases;
         for (uint32_t j = tid; j < a.biases; j += kThreads) {
             const int32_t id = ids[j];
-            if (id < 0 || uint32_t(id) < c0 || uint32_t(id) - c0 >= cols) continue;
+            const uint32_t p = place(id);
+            if (p == kCols) continue;
             bool first = true;
             for (uint32_t k = 0; k < j; ++k) first &= ids[k] != id;
             if (!first) continue;
@@ -54,36 +83,73 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a, uint32_t
             for (uint32_t k = j + 1; k < a.biases; ++k)
                 if (ids[k] == id) s += bv[k];
             sums[j] = s;
-            atomicOr(&word[uint32_t(id) - c0], (j + 1) << 19);
+            atomicOr(&word[p], (j + 1) << 19);
         }
+    }
     __syncthreads();
-    const auto *in = static_cast<const typename E::T *>(a.logits) + uint64_t(row) * a.cols + c0;
-    auto *out = static_cast<typename E::T *>(a.out) + uint64_t(row) * a.cols + c0;
+    auto rule = [&](typename E::T bits, uint32_t w, bool allowed) {
+        if (w == 0 && allowed) return bits;
+        float x = E::widen(bits);
+        const uint32_t n = w & 0x7ffffu, b = (w >> 19) & 0xfffu;
+        if (n || (w >> 31)) x = x > 0.0f ? x / rep : x * rep;
+        if (n) x = x - (freq * float(n) + pres);
+        if (b) x = x + sums[b - 1];
+        return E::narrow(allowed ? x : -INFINITY);
+    };
     const uint32_t *mask = a.mask ? a.mask + uint64_t(row) * ((a.cols + 31) / 32) : nullptr;
-    for (uint32_t c = tid; c < cols; c += kThreads) {
-        const uint32_t w = word[c];
-        const bool allowed = !mask || ((mask[(c0 + c) >> 5] >> ((c0 + c) & 31u)) & 1u);
-        typename E::T bits = in[c];
-        if (w || !allowed) {
-            float x = E::widen(bits);
-            const uint32_t n = w & 0x7ffffu, at = (w >> 19) & 0xfffu;
-            if (n || (w >> 31)) x = x > 0.0f ? x / rep : x * rep;
-            if (n) x = x - (freq * float(n) + pres);
-            if (at) x = x + sums[at - 1];
-            bits = E::narrow(allowed ? x : -INFINITY);
+    auto allowed = [&](uint32_t c) { return !mask || ((mask[c >> 5] >> (c & 31u)) & 1u); };
+    for (uint32_t p = kV * tid; p < kCols; p += kV * kThreads) {
+        const int64_t c = c0 + p;
+        if (wide && c >= 0 && c + kV <= a.cols) {
+            Vec<E> x;
+            x.v = *reinterpret_cast<const u32x4 *>(in + c);
+            uint32_t bits = 0xffffffffu;
+            if (mask) {
+                const uint32_t sh = uint32_t(c) & 31u;
+                bits = mask[c >> 5] >> sh;
+                if (sh + kV > 32) bits |= mask[(c >> 5) + 1] << (32 - sh);
+            }
+            uint32_t w[kV], any = 0;
+#pragma unroll
+            for (uint32_t e = 0; e < kV; e += 4) {
+                const u32x4 q = *reinterpret_cast<const u32x4 *>(word + p + e);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) any |= w[e + i] = q[i];
+            }
+            constexpr uint32_t kAll = (1u << kV) - 1;
+            if (any || (bits & kAll) != kAll)
+#pragma unroll
+                for (uint32_t e = 0; e < kV; ++e) x.e[e] = rule(x.e[e], w[e], (bits >> e) & 1u);
+            *reinterpret_cast<u32x4 *>(out + c) = x.v;
+        } else {
+            for (uint32_t e = 0; e < kV; ++e)
+                if (c + e >= 0 && c + e < a.cols) out[c + e] = rule(in[c + e], word[p + e], allowed(uint32_t(c + e)));
         }
-        out[c] = bits;
+    }
+}
+
+template <class E>
+void launch(const LogitsArgs &a, hipStream_t stream) {
+    const uint32_t kV = 16 / sizeof(typename E::T);
+    // the logits and the result as far past 16 bytes as each other
+    const bool wide = (reinterpret_cast<uintptr_t>(a.logits) - reinterpret_cast<uintptr_t>(a.out)) % 16 == 0;
+    const size_t lds = size_t(a.biases) * 8;
+    auto chunks = [&](uint32_t cols) { return uint32_t((uint64_t(a.cols) + kV - 1 + cols - 1) / cols); };
+    if (uint64_t(a.rows) * chunks(16384) >= 256) {
+        const uint32_t n = chunks(16384);
+        logits_kernel<E, 16384><<<a.rows * n, threads_of<16384>(), lds, stream>>>(a, n, wide);
+    } else {
+        const uint32_t n = chunks(4096);
+        logits_kernel<E, 4096><<<a.rows * n, threads_of<4096>(), lds, stream>>>(a, n, wide);
     }
 }
 
 }  // namespace
 
 hipError_t launch_logits(const LogitsArgs &a, hipStream_t stream) {
-    const uint32_t chunks = (a.cols + kCols - 1) / kCols;
-    const dim3 grid(a.rows * chunks);
-    if (a.dtype == 7) logits_kernel<Bf16><<<grid, kThreads, 0, stream>>>(a, chunks);
-    else if (a.dtype == 6) logits_kernel<F16><<<grid, kThreads, 0, stream>>>(a, chunks);
-    else logits_kernel<F32><<<grid, kThreads, 0, stream>>>(a, chunks);
+    if (a.dtype == 7) launch<Bf16>(a, stream);
+    else if (a.dtype == 6) launch<F16>(a, stream);
+    else launch<F32>(a, stream);
     return hipGetLastError();
 }
 
