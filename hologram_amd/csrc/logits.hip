@@ -45,6 +45,27 @@ __global__ __launch_bounds__(threads_of<kCols>()) void logits_kernel(LogitsArgs 
         const int64_t p = int64_t(id) - c0;
         return id >= 0 && uint32_t(id) < a.cols && p >= 0 && p < kCols ? uint32_t(p) : uint32_t(kCols);
     };
+    // the thread's logits and their mask bits, on their way while the rules are gathered
+    constexpr int kMine = kCols / (kV * kThreads);
+    const uint32_t *mask = a.mask ? a.mask + uint64_t(row) * ((a.cols + 31) / 32) : nullptr;
+    Vec<E> x[kMine];
+    uint32_t bits[kMine];
+    auto whole = [&](int i) {
+        const int64_t c = c0 + kV * (tid + uint32_t(i) * kThreads);
+        return wide && c >= 0 && c + kV <= a.cols;
+    };
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+        const int64_t c = c0 + kV * (tid + uint32_t(i) * kThreads);
+        bits[i] = 0xffffffffu;
+        if (!whole(i)) continue;
+        x[i].v = *reinterpret_cast<const u32x4 *>(in + c);
+        if (mask) {
+            const uint32_t sh = uint32_t(c) & 31u;
+            bits[i] = mask[c >> 5] >> sh;
+            if (sh + kV > 32) bits[i] |= mask[(c >> 5) + 1] << (32 - sh);
+        }
+    }
     for (uint32_t c = 4 * tid; c < kCols; c += 4 * kThreads) *reinterpret_cast<u32x4 *>(word + c) = u32x4{0, 0, 0, 0};
     if (a.bias_ids)
         for (uint32_t j = tid; j < a.biases; j += kThreads) ids[j] = a.bias_ids[uint64_t(row) * a.biases + j];
@@ -96,34 +117,29 @@ __global__ __launch_bounds__(threads_of<kCols>()) void logits_kernel(LogitsArgs 
         if (b) x = x + sums[b - 1];
         return E::narrow(allowed ? x : -INFINITY);
     };
-    const uint32_t *mask = a.mask ? a.mask + uint64_t(row) * ((a.cols + 31) / 32) : nullptr;
-    auto allowed = [&](uint32_t c) { return !mask || ((mask[c >> 5] >> (c & 31u)) & 1u); };
-    for (uint32_t p = kV * tid; p < kCols; p += kV * kThreads) {
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+        const uint32_t p = kV * (tid + uint32_t(i) * kThreads);
         const int64_t c = c0 + p;
-        if (wide && c >= 0 && c + kV <= a.cols) {
-            Vec<E> x;
-            x.v = *reinterpret_cast<const u32x4 *>(in + c);
-            uint32_t bits = 0xffffffffu;
-            if (mask) {
-                const uint32_t sh = uint32_t(c) & 31u;
-                bits = mask[c >> 5] >> sh;
-                if (sh + kV > 32) bits |= mask[(c >> 5) + 1] << (32 - sh);
-            }
+        if (whole(i)) {
             uint32_t w[kV], any = 0;
 #pragma unroll
             for (uint32_t e = 0; e < kV; e += 4) {
                 const u32x4 q = *reinterpret_cast<const u32x4 *>(word + p + e);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) any |= w[e + i] = q[i];
+                for (int k = 0; k < 4; ++k) any |= w[e + k] = q[k];
             }
             constexpr uint32_t kAll = (1u << kV) - 1;
-            if (any || (bits & kAll) != kAll)
+            if (any || (bits[i] & kAll) != kAll)
 #pragma unroll
-                for (uint32_t e = 0; e < kV; ++e) x.e[e] = rule(x.e[e], w[e], (bits >> e) & 1u);
-            *reinterpret_cast<u32x4 *>(out + c) = x.v;
+                for (uint32_t e = 0; e < kV; ++e) x[i].e[e] = rule(x[i].e[e], w[e], (bits[i] >> e) & 1u);
+            *reinterpret_cast<u32x4 *>(out + c) = x[i].v;
         } else {
-            for (uint32_t e = 0; e < kV; ++e)
-                if (c + e >= 0 && c + e < a.cols) out[c + e] = rule(in[c + e], word[p + e], allowed(uint32_t(c + e)));
+            for (uint32_t e = 0; e < kV; ++e) {
+                const int64_t d = c + e;
+                if (d < 0 || d >= a.cols) continue;
+                out[d] = rule(in[d], word[p + e], !mask || ((mask[d >> 5] >> (d & 31)) & 1u));
+            }
         }
     }
 }

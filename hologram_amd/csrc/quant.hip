@@ -766,6 +766,43 @@ __global__ __launch_bounds__(256) void dequant_kernel(DqArgs d) {
     }
 }
 
+// The same, element for element, 16 int8 a thread: runs of one channel that hold whole
+// 16-byte chunks (a block-scaled cache's blocks, a weight's rows), so that a chunk has one
+// scale and zero point. Bound by the bytes: 33.5 M int8 to bf16 in 524 k channels of 64 x
+// 128, 59.6 us an element a thread.
+template <class T, class F>
+__device__ __forceinline__ void dequant_chunk(const DqArgs &d, uint64_t c, F narrow) {
+    const u32x4 q = reinterpret_cast<const u32x4 *>(d.in)[c];
+    float s = d.scale;
+    int32_t z = d.zp;
+    if (d.scales) {
+        const uint64_t run = 16 * c / d.inner;
+        const uint32_t ch = uint32_t(run % d.channels);
+        s = d.scales[ch];
+        z = d.zps[ch];
+    }
+    union {
+        u32x4 v[sizeof(T)];
+        T e[16];
+    } o;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int32_t level = int32_t(int8_t(q[i >> 2] >> (8 * (i & 3))));
+        o.e[i] = narrow(float(int32_t(uint32_t(level) - uint32_t(z))) * s);
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < sizeof(T); ++i) reinterpret_cast<u32x4 *>(d.out)[c * sizeof(T) + i] = o.v[i];
+}
+
+__global__ __launch_bounds__(256) void dequant16_kernel(DqArgs d) {
+    const uint64_t stride = uint64_t(gridDim.x) * 256;
+    for (uint64_t c = uint64_t(blockIdx.x) * 256 + threadIdx.x; c < d.n / 16; c += stride) {
+        if (d.dtype == 8) dequant_chunk<float>(d, c, [](float v) { return v; });
+        else if (d.dtype == 7) dequant_chunk<uint16_t>(d, c, [](float v) { return uint16_t(__float_as_uint(v) >> 16); });
+        else dequant_chunk<uint16_t>(d, c, [](float v) { return f32_to_f16_bits(v); });
+    }
+}
+
 // ------------------------------------------------------- DequantActivation --
 struct DqActTable {
     float t[256];
@@ -927,6 +964,12 @@ hipError_t launch_dequantize(const DequantArgs &a, hipStream_t stream) {
     d.dtype = a.dtype;
     d.scale = a.scale;
     d.zp = a.zp;
+    if (d.quant == 2 && d.n % 16 == 0 && (!d.scales || d.inner % 16 == 0) &&
+        ((reinterpret_cast<uintptr_t>(d.in) | reinterpret_cast<uintptr_t>(d.out)) & 15) == 0) {
+        const uint64_t b = (d.n / 16 + 255) / 256;
+        hipLaunchKernelGGL(dequant16_kernel, dim3(uint32_t(b < (1u << 20) ? b : (1u << 20))), dim3(256), 0, stream, d);
+        return hipGetLastError();
+    }
     hipLaunchKernelGGL(dequant_kernel, dim3(grid_for(a.n)), dim3(256), 0, stream, d);
     return hipGetLastError();
 }

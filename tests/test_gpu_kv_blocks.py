@@ -150,3 +150,27 @@ def test_dropped_rows_leave_the_rest_exact(torch_cuda, backend):
         backend.synchronize()
     assert np.array_equal(from_dev(ts[3], np.int8).reshape(want[0].shape), want[0])
     assert np.array_equal(from_dev(ts[4], np.float32).reshape(want[1].shape), want[1])
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("off", [0, 16, 5])
+@pytest.mark.parametrize("channels,inner", [(6, 4096), (7, 16), (1, 48), (3, 24)])
+def test_a_cache_reads_back_through_dequantize(torch_cuda, backend, dtype, off, channels, inner):
+    """Runs of whole 16-byte chunks and others, aligned and not, with more runs than channels:
+    (q - zero point) * scale, narrowed as the reference narrows, bit for bit."""
+    import oracle
+    from hologram_amd import DTYPE_I8, DequantizeCall
+    rng = np.random.default_rng(channels)
+    n = 2 * channels * inner
+    q = rng.integers(0, 256, n + off, dtype=np.uint8)
+    scales = (2.0 ** rng.integers(-9, 3, channels)).astype(np.float32)
+    zps = rng.integers(-300, 300, channels).astype(np.int32)
+    out = torch_cuda.zeros(n * (4 if dtype == DTYPE_F32 else 2) + off * 4, dtype=torch_cuda.uint8, device="cuda")
+    ws = DeviceWorkspace()
+    for s, t in enumerate((to_dev(torch_cuda, q), to_dev(torch_cuda, scales), to_dev(torch_cuda, zps), out)):
+        ws.bind(s, t)
+    backend.dispatch(KernelCall.Dequantize(DequantizeCall(
+        BufferRef(0, off), BufferRef(1), BufferRef(2), BufferRef(3, off * 4), n, channels, inner, DTYPE_I8, dtype)), ws)
+    backend.synchronize()
+    want = oracle.dequantize(q[off:], n, DTYPE_I8, dtype, scales=scales, zps=zps, channels=channels, inner=inner)
+    assert np.array_equal(out.cpu().numpy()[off * 4:], np.ascontiguousarray(want).view(np.uint8).reshape(-1))
