@@ -32,8 +32,8 @@ template <class E, int kCols>
 __global__ __launch_bounds__(threads_of<kCols>()) void logits_kernel(LogitsArgs a, uint32_t chunks, bool wide) {
     constexpr uint32_t kThreads = threads_of<kCols>(), kV = 16 / sizeof(typename E::T);
     __shared__ __attribute__((aligned(16))) uint32_t word[kCols];
-    extern __shared__ int32_t ids[];                    // [biases], then their sums
-    float *sums = reinterpret_cast<float *>(ids + a.biases);
+    extern __shared__ __attribute__((aligned(16))) int32_t ids[];     // [biases] in fours, then their sums
+    float *sums = reinterpret_cast<float *>(ids + (a.biases + 3) / 4 * 4);
     const uint32_t row = blockIdx.x / chunks, tid = threadIdx.x;
     const uint64_t at = uint64_t(row) * a.cols;
     const auto *in = static_cast<const typename E::T *>(a.logits) + at;
@@ -66,30 +66,39 @@ __global__ __launch_bounds__(threads_of<kCols>()) void logits_kernel(LogitsArgs 
             if (sh + kV > 32) bits[i] |= mask[(c >> 5) + 1] << (32 - sh);
         }
     }
-    for (uint32_t c = 4 * tid; c < kCols; c += 4 * kThreads) *reinterpret_cast<u32x4 *>(word + c) = u32x4{0, 0, 0, 0};
-    if (a.bias_ids)
-        for (uint32_t j = tid; j < a.biases; j += kThreads) ids[j] = a.bias_ids[uint64_t(row) * a.biases + j];
-    __syncthreads();
+    // and its first tokens (as long as the row may be: what counts of it comes with them)
+    const int32_t *h = a.history ? a.history + uint64_t(row) * a.history_len : nullptr;
+    const bool by16 = reinterpret_cast<uintptr_t>(h) % 16 == 0;
+    int4 tokens = {-1, -1, -1, -1};
+    uint32_t n = 0, prompt = 0;
     float rep = 1.0f, freq = 0.0f, pres = 0.0f;
-    if (a.history) {
-        const int32_t *h = a.history + uint64_t(row) * a.history_len;
-        const uint32_t n = a.spans[2 * uint64_t(row) + 1] < a.history_len ? a.spans[2 * uint64_t(row) + 1] : a.history_len;
-        const uint32_t prompt = a.spans[2 * uint64_t(row)];
+    if (h) {
+        if (by16 && tid < a.history_len / 4) tokens = reinterpret_cast<const int4 *>(h)[tid];
+        prompt = a.spans[2 * uint64_t(row)];
+        n = a.spans[2 * uint64_t(row) + 1];
+        rep = a.params[3 * uint64_t(row)];
+        freq = a.params[3 * uint64_t(row) + 1];
+        pres = a.params[3 * uint64_t(row) + 2];
+    }
+    for (uint32_t c = 4 * tid; c < kCols; c += 4 * kThreads) *reinterpret_cast<u32x4 *>(word + c) = u32x4{0, 0, 0, 0};
+    const uint32_t padded = (a.biases + 3) / 4 * 4;      // ids in fours, -1 behind the last
+    for (uint32_t j = tid; j < padded; j += kThreads)
+        ids[j] = j < a.biases ? a.bias_ids[uint64_t(row) * a.biases + j] : -1;
+    __syncthreads();
+    if (h) {
+        n = n < a.history_len ? n : a.history_len;
         auto count = [&](int32_t id, uint32_t i) {
             const uint32_t p = place(id);
             if (p == kCols) return;
             if (i < prompt) atomicOr(&word[p], 0x80000000u);
             else atomicAdd(&word[p], 1u);
         };
-        const uint32_t quads = reinterpret_cast<uintptr_t>(h) % 16 == 0 ? n / 4 : 0u;
+        const uint32_t quads = by16 ? n / 4 : 0u;
         for (uint32_t q = tid; q < quads; q += kThreads) {
-            const int4 x = reinterpret_cast<const int4 *>(h)[q];
-            count(x.x, 4 * q), count(x.y, 4 * q + 1), count(x.z, 4 * q + 2), count(x.w, 4 * q + 3);
+            if (q != tid) tokens = reinterpret_cast<const int4 *>(h)[q];
+            count(tokens.x, 4 * q), count(tokens.y, 4 * q + 1), count(tokens.z, 4 * q + 2), count(tokens.w, 4 * q + 3);
         }
         for (uint32_t k = 4 * quads + tid; k < n; k += kThreads) count(h[k], k);
-        rep = a.params[3 * uint64_t(row)];
-        freq = a.params[3 * uint64_t(row) + 1];
-        pres = a.params[3 * uint64_t(row) + 2];
     }
     if (a.bias_ids) {
         const float *bv = a.bias_values + uint64_t(row) * a.biases;
@@ -97,48 +106,66 @@ __global__ __launch_bounds__(threads_of<kCols>()) void logits_kernel(LogitsArgs 
             const int32_t id = ids[j];
             const uint32_t p = place(id);
             if (p == kCols) continue;
-            bool first = true;
-            for (uint32_t k = 0; k < j; ++k) first &= ids[k] != id;
-            if (!first) continue;
+            // the first of its id has them all, in the list's order
+            uint32_t first = j;
+            bool more = false;
+#pragma unroll 4
+            for (uint32_t k = 0; k < padded; k += 4) {
+                const int4 x = *reinterpret_cast<const int4 *>(ids + k);
+                const int32_t e[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    first = e[i] == id && k + i < first ? k + i : first;
+                    more |= e[i] == id && k + i > j;
+                }
+            }
+            if (first != j) continue;
             float s = bv[j];
-            for (uint32_t k = j + 1; k < a.biases; ++k)
-                if (ids[k] == id) s += bv[k];
+            if (more)
+                for (uint32_t k = j + 1; k < a.biases; ++k)
+                    if (ids[k] == id) s += bv[k];
             sums[j] = s;
             atomicOr(&word[p], (j + 1) << 19);
         }
     }
     __syncthreads();
-    auto rule = [&](typename E::T bits, uint32_t w, bool allowed) {
-        if (w == 0 && allowed) return bits;
+    const typename E::T none = E::narrow(-INFINITY);
+    auto rule = [&](typename E::T bits, uint32_t w) {      // w != 0
         float x = E::widen(bits);
         const uint32_t n = w & 0x7ffffu, b = (w >> 19) & 0xfffu;
         if (n || (w >> 31)) x = x > 0.0f ? x / rep : x * rep;
         if (n) x = x - (freq * float(n) + pres);
         if (b) x = x + sums[b - 1];
-        return E::narrow(allowed ? x : -INFINITY);
+        return E::narrow(x);
     };
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
         const uint32_t p = kV * (tid + uint32_t(i) * kThreads);
         const int64_t c = c0 + p;
         if (whole(i)) {
+            // what the mask leaves out is done at a select; few of the rest have a rule
             uint32_t w[kV], any = 0;
 #pragma unroll
             for (uint32_t e = 0; e < kV; e += 4) {
                 const u32x4 q = *reinterpret_cast<const u32x4 *>(word + p + e);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) any |= w[e + k] = q[k];
+                for (int k = 0; k < 4; ++k) {
+                    const bool in = (bits[i] >> (e + k)) & 1u;
+                    any |= w[e + k] = in ? q[k] : 0u;
+                    x[i].e[e + k] = in ? x[i].e[e + k] : none;
+                }
             }
-            constexpr uint32_t kAll = (1u << kV) - 1;
-            if (any || (bits[i] & kAll) != kAll)
+            if (any)
 #pragma unroll
-                for (uint32_t e = 0; e < kV; ++e) x[i].e[e] = rule(x[i].e[e], w[e], (bits[i] >> e) & 1u);
+                for (uint32_t e = 0; e < kV; ++e)
+                    if (w[e]) x[i].e[e] = rule(x[i].e[e], w[e]);
             *reinterpret_cast<u32x4 *>(out + c) = x[i].v;
         } else {
             for (uint32_t e = 0; e < kV; ++e) {
                 const int64_t d = c + e;
                 if (d < 0 || d >= a.cols) continue;
-                out[d] = rule(in[d], word[p + e], !mask || ((mask[d >> 5] >> (d & 31)) & 1u));
+                const bool there = !mask || ((mask[d >> 5] >> (d & 31)) & 1u);
+                out[d] = !there ? none : word[p + e] ? rule(in[d], word[p + e]) : in[d];
             }
         }
     }
@@ -149,7 +176,7 @@ void launch(const LogitsArgs &a, hipStream_t stream) {
     const uint32_t kV = 16 / sizeof(typename E::T);
     // the logits and the result as far past 16 bytes as each other
     const bool wide = (reinterpret_cast<uintptr_t>(a.logits) - reinterpret_cast<uintptr_t>(a.out)) % 16 == 0;
-    const size_t lds = size_t(a.biases) * 8;
+    const size_t lds = size_t((a.biases + 3) / 4 * 4) * 8;
     auto chunks = [&](uint32_t cols) { return uint32_t((uint64_t(a.cols) + kV - 1 + cols - 1) / cols); };
     if (uint64_t(a.rows) * chunks(16384) >= 256) {
         const uint32_t n = chunks(16384);
