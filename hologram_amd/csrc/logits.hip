@@ -16,7 +16,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 // counts are integers whose order does not matter, and no column's rule leaves
 // the workgroup that writes it. Bound by the logits' own bytes where there are many
 // rows (128 rows of 128000 bf16 with masks, biases and 4096 tokens of history each):
-// 16384 columns and 1024 threads a workgroup then read the history eight times a row,
+// 8192 columns and 1024 threads a workgroup then read the history eight times a row,
 // 4096 and 256 thirty-two times. Few rows take the small ones, to spread over the GPU.
 template <int kCols>
 constexpr uint32_t threads_of() { return kCols / 16; }
@@ -32,8 +32,9 @@ template <class E, int kCols>
 __global__ __launch_bounds__(threads_of<kCols>()) void logits_kernel(LogitsArgs a, uint32_t chunks, bool wide) {
     constexpr uint32_t kThreads = threads_of<kCols>(), kV = 16 / sizeof(typename E::T);
     __shared__ __attribute__((aligned(16))) uint32_t word[kCols];
-    extern __shared__ __attribute__((aligned(16))) int32_t ids[];     // [biases] in fours, then their sums
-    float *sums = reinterpret_cast<float *>(ids + (a.biases + 3) / 4 * 4);
+    __shared__ uint32_t twice;                          // some token of the workgroup's has two biases
+    extern __shared__ int32_t ids[];                    // [biases], then their sums
+    float *sums = reinterpret_cast<float *>(ids + a.biases);
     const uint32_t row = blockIdx.x / chunks, tid = threadIdx.x;
     const uint64_t at = uint64_t(row) * a.cols;
     const auto *in = static_cast<const typename E::T *>(a.logits) + at;
@@ -41,9 +42,9 @@ __global__ __launch_bounds__(threads_of<kCols>()) void logits_kernel(LogitsArgs 
     // columns [c0, c0 + kCols) of which those in [0, cols) are there; c0 falls on 16 bytes
     const uint32_t skew = wide ? uint32_t(reinterpret_cast<uintptr_t>(in) / sizeof(typename E::T)) % kV : 0u;
     const int64_t c0 = int64_t(blockIdx.x % chunks) * kCols - skew;
-    auto place = [&](int32_t id) -> uint32_t {          // in word, kCols for none of them
-        const int64_t p = int64_t(id) - c0;
-        return id >= 0 && uint32_t(id) < a.cols && p >= 0 && p < kCols ? uint32_t(p) : uint32_t(kCols);
+    auto place = [&](int32_t id) -> uint32_t {          // in word, kCols or more for none of them
+        const uint32_t p = uint32_t(id) - uint32_t(int32_t(c0));
+        return uint32_t(id) < a.cols ? p : uint32_t(kCols);
     };
     // the thread's logits and their mask bits, on their way while the rules are gathered
     constexpr int kMine = kCols / (kV * kThreads);
@@ -81,15 +82,14 @@ __global__ __launch_bounds__(threads_of<kCols>()) void logits_kernel(LogitsArgs 
         pres = a.params[3 * uint64_t(row) + 2];
     }
     for (uint32_t c = 4 * tid; c < kCols; c += 4 * kThreads) *reinterpret_cast<u32x4 *>(word + c) = u32x4{0, 0, 0, 0};
-    const uint32_t padded = (a.biases + 3) / 4 * 4;      // ids in fours, -1 behind the last
-    for (uint32_t j = tid; j < padded; j += kThreads)
-        ids[j] = j < a.biases ? a.bias_ids[uint64_t(row) * a.biases + j] : -1;
+    for (uint32_t j = tid; j < a.biases; j += kThreads) ids[j] = a.bias_ids[uint64_t(row) * a.biases + j];
+    if (tid == 0) twice = 0;
     __syncthreads();
     if (h) {
         n = n < a.history_len ? n : a.history_len;
         auto count = [&](int32_t id, uint32_t i) {
             const uint32_t p = place(id);
-            if (p == kCols) return;
+            if (p >= kCols) return;
             if (i < prompt) atomicOr(&word[p], 0x80000000u);
             else atomicAdd(&word[p], 1u);
         };
@@ -100,35 +100,38 @@ __global__ __launch_bounds__(threads_of<kCols>()) void logits_kernel(LogitsArgs 
         }
         for (uint32_t k = 4 * quads + tid; k < n; k += kThreads) count(h[k], k);
     }
-    if (a.bias_ids) {
-        const float *bv = a.bias_values + uint64_t(row) * a.biases;
+    // A bias is its token's sum where the token has one; where a second is found, the
+    // workgroup starts over with sums in the list's order.
+    constexpr uint32_t kSlot = 0xfffu << 19;
+    const float *bv = a.bias_values + uint64_t(row) * a.biases;
+    for (uint32_t j = tid; j < a.biases; j += kThreads) {
+        const uint32_t p = place(ids[j]);
+        if (p >= kCols) continue;
+        sums[j] = bv[j];
+        if (atomicOr(&word[p], (j + 1) << 19) & kSlot) twice = 1;
+    }
+    __syncthreads();
+    if (twice) {
+        for (uint32_t j = tid; j < a.biases; j += kThreads) {
+            const uint32_t p = place(ids[j]);
+            if (p < kCols) atomicAnd(&word[p], ~kSlot);
+        }
+        __syncthreads();
         for (uint32_t j = tid; j < a.biases; j += kThreads) {
             const int32_t id = ids[j];
             const uint32_t p = place(id);
-            if (p == kCols) continue;
-            // the first of its id has them all, in the list's order
-            uint32_t first = j;
-            bool more = false;
-#pragma unroll 4
-            for (uint32_t k = 0; k < padded; k += 4) {
-                const int4 x = *reinterpret_cast<const int4 *>(ids + k);
-                const int32_t e[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    first = e[i] == id && k + i < first ? k + i : first;
-                    more |= e[i] == id && k + i > j;
-                }
-            }
-            if (first != j) continue;
+            if (p >= kCols) continue;
+            bool first = true;
+            for (uint32_t k = 0; k < j; ++k) first &= ids[k] != id;
+            if (!first) continue;
             float s = bv[j];
-            if (more)
-                for (uint32_t k = j + 1; k < a.biases; ++k)
-                    if (ids[k] == id) s += bv[k];
+            for (uint32_t k = j + 1; k < a.biases; ++k)
+                if (ids[k] == id) s += bv[k];
             sums[j] = s;
             atomicOr(&word[p], (j + 1) << 19);
         }
+        __syncthreads();
     }
-    __syncthreads();
     const typename E::T none = E::narrow(-INFINITY);
     auto rule = [&](typename E::T bits, uint32_t w) {      // w != 0
         float x = E::widen(bits);
@@ -176,11 +179,11 @@ void launch(const LogitsArgs &a, hipStream_t stream) {
     const uint32_t kV = 16 / sizeof(typename E::T);
     // the logits and the result as far past 16 bytes as each other
     const bool wide = (reinterpret_cast<uintptr_t>(a.logits) - reinterpret_cast<uintptr_t>(a.out)) % 16 == 0;
-    const size_t lds = size_t((a.biases + 3) / 4 * 4) * 8;
+    const size_t lds = size_t(a.biases) * 8;
     auto chunks = [&](uint32_t cols) { return uint32_t((uint64_t(a.cols) + kV - 1 + cols - 1) / cols); };
-    if (uint64_t(a.rows) * chunks(16384) >= 256) {
-        const uint32_t n = chunks(16384);
-        logits_kernel<E, 16384><<<a.rows * n, threads_of<16384>(), lds, stream>>>(a, n, wide);
+    if (uint64_t(a.rows) * chunks(8192) >= 256) {
+        const uint32_t n = chunks(8192);
+        logits_kernel<E, 8192><<<a.rows * n, threads_of<8192>(), lds, stream>>>(a, n, wide);
     } else {
         const uint32_t n = chunks(4096);
         logits_kernel<E, 4096><<<a.rows * n, threads_of<4096>(), lds, stream>>>(a, n, wide);
