@@ -1092,16 +1092,17 @@ __global__ __launch_bounds__(256, (DP > 128 || sizeof(typename E::T) == 4 ? 1 : 
     }
 }
 
-// Joins the partials of a row tile that shares cut: grid places * Hkv * kJoin, a
-// wavefront a row in turn.
-constexpr uint32_t kJoin = 16;
+// Joins the partials of a row tile that shares cut: grid places * Hkv * joins, a
+// wavefront a row in turn. `joins` fills 1024 workgroups with the places that there are,
+// between 4 and 32 (a row a wavefront) of them a place: one sequence of 64 rows 49 us
+// with 8, 41 with 16, 38 with 32; 4 of 301 to 1024 rows 200 us with 16, 194 with 4 or 8.
 template <class E, int DP>
-__global__ __launch_bounds__(256) void join_kernel(Chunk k) {
+__global__ __launch_bounds__(256) void join_kernel(Chunk k, uint32_t joins) {
     __shared__ uint64_t sums[4], alls[4];
     const AttnBlocksArgs &a = k.a;
     const uint32_t G = a.H / a.Hkv, kh = blockIdx.x % a.Hkv, rest = blockIdx.x / a.Hkv, lane = threadIdx.x & 63u;
     Place at;
-    if (!place_of(a.pb, G, kRows, rest / kJoin, &at)) return;
+    if (!place_of(a.pb, G, kRows, rest / joins, &at)) return;
     uint64_t sum = 0, all = 0;       // costs before sequence at.b, and of all
     for (uint32_t b = threadIdx.x; b < a.pb.batch; b += 256) {
         const Units u = sequence_units(a, b);
@@ -1127,7 +1128,7 @@ __global__ __launch_bounds__(256) void join_kernel(Chunk k) {
     const uint64_t id = uint64_t(at.lo * G / kRows + at.b) * a.Hkv + uint64_t(kh) * u.units + at.unit;
     constexpr uint32_t kStride = kRows * (DP + 2);
     const float *src = k.part + (id + w0) * kStride;
-    for (uint32_t c = rest % kJoin * 4 + (threadIdx.x >> 6); c < kRows; c += 4 * kJoin) {
+    for (uint32_t c = rest % joins * 4 + (threadIdx.x >> 6); c < kRows; c += 4 * joins) {
         const uint32_t rr = at.unit * kRows + c;
         if (rr >= R) return;
         const uint32_t t = rr / G;
@@ -1183,7 +1184,8 @@ void launch_chunk(const Chunk &k, hipStream_t stream) {
         return;
     }
     chunk_shares_kernel<E, DP><<<k.shares, 256, 0, stream>>>(k);
-    join_kernel<E, DP><<<grid * kJoin, 256, 0, stream>>>(k);
+    const uint32_t joins = grid >= 256 ? 4 : grid <= 32 ? 32 : 1024 / grid;
+    join_kernel<E, DP><<<grid * joins, 256, 0, stream>>>(k, joins);
 }
 template <class E>
 void launch_chunk(const Chunk &k, hipStream_t stream) {
