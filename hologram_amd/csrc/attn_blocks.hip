@@ -582,6 +582,14 @@ struct Chunk {
     float *part;         // [places * Hkv + shares][kRows][DP + 2], as Blocks::part
 };
 
+// A partial: O as the lanes hold it, 4 dims (8 g + 4 (lane / 32) on) of row lane % 32 a
+// 16-byte element, wavefront by wavefront and 8 dims by 8 dims (q), so that every access
+// is 1 KB of whole lines; then the rows' maxima, then their sums.
+template <int DP>
+__device__ __forceinline__ uint32_t part_of(uint32_t wave, uint32_t q, uint32_t lane) {
+    return ((wave * (DP / 8) + q) * 64 + lane) * 4;
+}
+
 // Four int8 (xor 0x80) as f16.
 __device__ __forceinline__ uint2 widen4(uint32_t w) {
     typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
@@ -967,15 +975,17 @@ __device__ __forceinline__ void chunk_segment(const Chunk &k, const Place &at, u
     l += __shfl_xor(l, 32, 64);
     const float unit = ldexpf(1.0f, ve - 7);
     if (!whole) {
-        if (wr0 + lr >= R) return;
-        dst += (32 * wave + lr) * (DP + 2);
+        if (!live) return;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
+            for (int g = 0; g < 4; ++g) {
+                f32x4 x;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) dst[32 * d + 8 * g + 4 * lg + e] = o[d][4 * g + e] * unit;
-        if (lg == 0) dst[DP] = m, dst[DP + 1] = l;
+                for (int e = 0; e < 4; ++e) x[e] = o[d][4 * g + e] * unit;
+                *reinterpret_cast<f32x4 *>(dst + part_of<DP>(wave, 4 * d + g, lane)) = x;
+            }
+        if (lg == 0) dst[kRows * DP + 32 * wave + lr] = m, dst[kRows * (DP + 1) + 32 * wave + lr] = l;
         return;
     }
     // rows stored whole through LDS (16-bit), or as they are (f32)
@@ -1093,9 +1103,8 @@ __global__ __launch_bounds__(256, (DP > 128 || sizeof(typename E::T) == 4 ? 1 : 
 }
 
 // Joins the partials of a row tile that shares cut: grid places * Hkv * joins, a
-// wavefront a row in turn. `joins` fills 1024 workgroups with the places that there are,
-// between 4 and 32 (a row a wavefront) of them a place: one sequence of 64 rows 49 us
-// with 8, 41 with 16, 38 with 32; 4 of 301 to 1024 rows 200 us with 16, 194 with 4 or 8.
+// wavefront 32 rows and, in turn, 8 of their dims. `joins` fills 1024 workgroups with the
+// places that there are, up to 8 dims a workgroup.
 template <class E, int DP>
 __global__ __launch_bounds__(256) void join_kernel(Chunk k, uint32_t joins) {
     __shared__ uint64_t sums[4], alls[4];
@@ -1128,13 +1137,54 @@ __global__ __launch_bounds__(256) void join_kernel(Chunk k, uint32_t joins) {
     const uint64_t id = uint64_t(at.lo * G / kRows + at.b) * a.Hkv + uint64_t(kh) * u.units + at.unit;
     constexpr uint32_t kStride = kRows * (DP + 2);
     const float *src = k.part + (id + w0) * kStride;
-    for (uint32_t c = rest % joins * 4 + (threadIdx.x >> 6); c < kRows; c += 4 * joins) {
-        const uint32_t rr = at.unit * kRows + c;
-        if (rr >= R) return;
-        const uint32_t t = rr / G;
-        const bool none = visible_keys(a.lens[at.b], n, t, a.bucket) == 0;
-        auto *out = static_cast<typename E::T *>(a.out) + (uint64_t(at.lo + t) * a.H + kh * G + (rr - t * G)) * a.D;
-        join_row<E, DP>(src + c * (DP + 2), kStride, np, a.D, none, out);
+    const uint32_t wave = pk_uni(threadIdx.x >> 6), in = 32 * wave + (lane & 31u), rr = at.unit * kRows + in;
+    if (at.unit * kRows + 32 * wave >= R) return;
+    const float *ms = src + kRows * DP + in, *ls = ms + kRows;
+    float M = -INFINITY, l = 0.0f;
+    for (uint32_t w = 0; w < np; w += 8) {
+        float x[8], y[8], mx = M;
+#pragma unroll
+        for (uint32_t q = 0; q < 8; ++q) {
+            const bool is = w + q < np;
+            x[q] = is ? ms[(w + q) * kStride] : -INFINITY, y[q] = is ? ls[(w + q) * kStride] : 0.0f;
+        }
+#pragma unroll
+        for (uint32_t q = 0; q < 8; ++q) mx = fmaxf(mx, x[q]);
+        const float ref = mx == -INFINITY ? 0.0f : mx;
+        l *= __builtin_amdgcn_exp2f(M - ref);
+#pragma unroll
+        for (uint32_t q = 0; q < 8; ++q) l = fmaf(y[q], __builtin_amdgcn_exp2f(x[q] - ref), l);
+        M = mx;
+    }
+    const float ref = M == -INFINITY ? 0.0f : M;
+    const uint32_t t = (rr < R ? rr : R - 1) / G;
+    const bool none = visible_keys(a.lens[at.b], n, t, a.bucket) == 0;
+    auto *out = static_cast<typename E::T *>(a.out) + (uint64_t(at.lo + t) * a.H + kh * G + (rr - t * G)) * a.D;
+    for (uint32_t c = rest % joins; 8 * c < a.D; c += joins) {
+        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+        const float *po = src + part_of<DP>(wave, c, lane);
+        for (uint32_t w = 0; w < np; w += 8) {
+            f32x4 x[8];
+            float e[8];
+#pragma unroll
+            for (uint32_t q = 0; q < 8; ++q) {
+                const uint32_t at_w = w + q < np ? w + q : np - 1;
+                x[q] = *reinterpret_cast<const f32x4 *>(po + at_w * kStride);
+                e[q] = ms[at_w * kStride];
+            }
+#pragma unroll
+            for (uint32_t q = 0; q < 8; ++q) {
+                const bool is = w + q < np;
+                const float ew = is ? __builtin_amdgcn_exp2f(e[q] - ref) : 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i] = fmaf(is ? x[q][i] : 0.0f, ew, o[i]);
+            }
+        }
+        if (rr >= R) continue;
+        typename E::T v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = E::narrow(none ? 0.0f : o[i] / l);
+        __builtin_memcpy(out + 8 * c + 4 * (lane >> 5), v, sizeof v);
     }
 }
 
@@ -1184,7 +1234,7 @@ void launch_chunk(const Chunk &k, hipStream_t stream) {
         return;
     }
     chunk_shares_kernel<E, DP><<<k.shares, 256, 0, stream>>>(k);
-    const uint32_t joins = grid >= 256 ? 4 : grid <= 32 ? 32 : 1024 / grid;
+    const uint32_t joins = grid * (DP / 8) <= 1024 ? DP / 8 : grid >= 256 ? 4 : 1024 / grid;
     join_kernel<E, DP><<<grid * joins, 256, 0, stream>>>(k, joins);
 }
 template <class E>
