@@ -43,15 +43,19 @@ __device__ __forceinline__ uint32_t visible_keys(int64_t len, uint32_t n, uint32
 // the scales of steps it does not see left out, so nothing reaches another row.
 //
 // Two splits. Direct: a workgroup of eight wavefronts a unit, no second launch; for
-// buckets up to kDirect rows, where a share of a unit would not fill a wavefront's
-// pipeline. Balanced: all units' 128-key quads laid end to end and cut into equal
+// buckets up to kDirect rows (one token of 8 kv heads of 128 dims for 8, 32 and 64 full
+// sequences: 11, 13 and 23 us against the shares' 13, 18 and 20 at 512 rows, 15, 17 and
+// 33 against 14, 22 and 30 at 1024, 23, 27 and 52 against 17, 31 and 49 at 2048, and 20
+// against 16 where 4 of them are ragged). Balanced: all units' 128-key quads laid end to end and cut into equal
 // shares, one for each of the workgroups that the GPU holds at once, whatever the
 // lengths; a unit that is cut leaves partials, which merge_kernel joins in order (a
 // launch of its own: partials pass between XCDs' L2s at its boundary).
+// Bound by the cache's bytes: 32 sequences of up to 8192 keys, 528 MB, 106 us or 5.0
+// TB/s, merge_kernel 5 us of them; 6.6 TB/s where 128 of them are full.
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 constexpr uint32_t kUnit = 16, kStep = 32, kQuad = 128, kOob = 1u << 30;   // past every plane, twice it too
-constexpr uint32_t kDirect = 2048, kShares = 512, kMinQuads = 2;
+constexpr uint32_t kDirect = 1024, kShares = 512, kMinQuads = 2;
 constexpr int kVeMin = -100;   // 2^ve's floor keeps 2^-ve finite
 
 struct Blocks {
@@ -565,8 +569,11 @@ __global__ __launch_bounds__(256) void merge_kernel(Blocks k) {
 // zero V scale makes them zeros, on the way into LDS.
 // In a tile that some row does not see to its end, s is scaled and limited first (c = 1),
 // and a step that a row does not see brings it no scale.
-// A workgroup a row tile and kv head where that gives many times what the GPU holds at
-// once. Fewer are dealt as equal shares of a line of keys, one share for each workgroup
+// A row tile and kv head is a workgroup's, whole (chunk_tile_kernel), where that gives
+// kManyRounds times what the GPU holds at once, or where the longest tile's keys are few
+// beside the tiles there are (tiles_whole: known on the device, so all three kernels are
+// launched and those not needed return; 7 us of the other split's 164). Else the tiles
+// are dealt as equal shares of a line of keys, one share for each workgroup
 // that the GPU holds: unit u (a row tile) of a sequence costs kStart + past' + S (u + 1)
 // keys, past' what its rows see before their own to a multiple of 64, S = ceil(128 / G)
 // the tokens that a unit spans at most, and kStart what starting and ending a unit
@@ -1035,16 +1042,6 @@ __device__ __forceinline__ void chunk_segment(const Chunk &k, const Place &at, u
     }
 }
 
-// A row tile a workgroup: grid places * Hkv, those that see most keys first.
-template <class E, int DP>
-__global__ __launch_bounds__(256, (DP > 128 || sizeof(typename E::T) == 4 ? 1 : 2)) void chunk_tile_kernel(Chunk k) {
-    __shared__ __attribute__((aligned(1024))) ChunkLds<DP> lds;
-    if (blockIdx.x == 0) check_starts(k.a.pb);
-    Place at;
-    if (!place_of(k.a.pb, k.a.H / k.a.Hkv, kRows, k.places - 1 - blockIdx.x / k.a.Hkv, &at)) return;
-    chunk_segment<E, DP>(k, at, blockIdx.x % k.a.Hkv, 0, k.a.bucket, true, nullptr, lds);
-}
-
 // The row tiles of sequence b and the line of their costs, one kv head's.
 struct Units {
     uint32_t units, past, S;
@@ -1071,13 +1068,53 @@ __device__ __forceinline__ uint64_t keys_of(uint64_t total, uint32_t shares) {
     return s < kMinKeys ? kMinKeys : s;
 }
 
+// Whether the row tiles go whole to workgroups. Whole, the GPU waits for the last long
+// one, about half of its time; cut, each share starts one tile more and the partials are
+// joined. 4 sequences of 301 to 1024 rows, the longest tile's keys 1.7 for each tile:
+// 43 us whole, 73 cut; behind up to 6000 keys, 11 for each: 258 and 164; 16 of 200 to
+// 500 rows behind up to 3000, 2.5 for each: 121 and 156; 8, 4.7 for each: 117 and 96.
+// The threads of a workgroup call it; all get the answer.
+__device__ __forceinline__ bool tiles_whole(const AttnBlocksArgs &a, uint32_t (&most)[4], uint32_t (&many)[4]) {
+    uint32_t keys = 0, units = 0;
+    for (uint32_t b = threadIdx.x; b < a.pb.batch; b += 256) {
+        const Units u = sequence_units(a, b);
+        const uint32_t x = u.units ? u.past + u.S * u.units : 0u;
+        keys = x > keys ? x : keys;
+        units += u.units;
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+        const uint32_t x = __shfl_xor(keys, o, 64);
+        keys = x > keys ? x : keys;
+        units += __shfl_xor(units, o, 64);
+    }
+    if ((threadIdx.x & 63u) == 0) most[threadIdx.x >> 6] = keys, many[threadIdx.x >> 6] = units;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 4; ++w) keys = most[w] > keys ? most[w] : keys;
+    return keys <= 1000 + 2 * a.Hkv * (many[0] + many[1] + many[2] + many[3]);
+}
+
+// A row tile a workgroup: grid places * Hkv, those that see most keys first.
+template <class E, int DP>
+__global__ __launch_bounds__(256, (DP > 128 || sizeof(typename E::T) == 4 ? 1 : 2)) void chunk_tile_kernel(Chunk k) {
+    __shared__ __attribute__((aligned(1024))) ChunkLds<DP> lds;
+    if (blockIdx.x == 0) check_starts(k.a.pb);
+    __shared__ uint32_t most[4], many[4];
+    if (k.shares && !tiles_whole(k.a, most, many)) return;
+    Place at;
+    if (!place_of(k.a.pb, k.a.H / k.a.Hkv, kRows, k.places - 1 - blockIdx.x / k.a.Hkv, &at)) return;
+    chunk_segment<E, DP>(k, at, blockIdx.x % k.a.Hkv, 0, k.a.bucket, true, nullptr, lds);
+}
+
 template <class E, int DP>
 __global__ __launch_bounds__(256, (DP > 128 || sizeof(typename E::T) == 4 ? 1 : 2)) void chunk_shares_kernel(Chunk k) {
     __shared__ __attribute__((aligned(1024))) ChunkLds<DP> lds;
     __shared__ uint64_t sums[4];
+    __shared__ uint32_t most[4], many[4];
     __shared__ Line found;
     const AttnBlocksArgs &a = k.a;
-    if (blockIdx.x == 0) check_starts(a.pb);
+    if (tiles_whole(a, most, many)) return;
     const uint32_t G = a.H / a.Hkv;
     const Line ln = find_line(a.pb.batch, [&](uint32_t b) {
         const Units u = sequence_units(a, b);
@@ -1117,10 +1154,11 @@ __global__ __launch_bounds__(256, (DP > 128 || sizeof(typename E::T) == 4 ? 1 : 
 template <class E, int DP>
 __global__ __launch_bounds__(256) void join_kernel(Chunk k, uint32_t joins) {
     __shared__ uint64_t sums[4], alls[4];
+    __shared__ uint32_t most[4], many[4];
     const AttnBlocksArgs &a = k.a;
     const uint32_t G = a.H / a.Hkv, kh = blockIdx.x % a.Hkv, rest = blockIdx.x / a.Hkv, lane = threadIdx.x & 63u;
     Place at;
-    if (!place_of(a.pb, G, kRows, rest / joins, &at)) return;
+    if (!place_of(a.pb, G, kRows, rest / joins, &at) || tiles_whole(a, most, many)) return;
     uint64_t sum = 0, all = 0;       // costs before sequence at.b, and of all
     for (uint32_t b = threadIdx.x; b < a.pb.batch; b += 256) {
         const Units u = sequence_units(a, b);
@@ -1209,9 +1247,13 @@ uint32_t few_places(const AttnBlocksArgs &a) {
     return uint32_t(uint64_t(a.pb.tokens) * (a.H / a.Hkv) / kUnit) + a.pb.batch;
 }
 uint32_t padded(uint32_t D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
-// At most 16 packed rows a sequence on average.
+// At most 16 packed rows a sequence on average, 32 where no shares are cut: 32 sequences of
+// 4000 keys, 58 us against the tiles' 94 with 16 rows, 80 and 95 with 32, 157 and 115 with
+// 64, but 61 and 42 with 32 rows and 1 to 4000 keys; of 900 keys, 32 rows, 4 and 16
+// sequences 17 and 32 us against 23 and 35.
 bool few_rows(const AttnBlocksArgs &a) {
-    return uint64_t(a.pb.tokens) * (a.H / a.Hkv) <= uint64_t(kUnit) * a.pb.batch;
+    const uint32_t rows = a.bucket <= kDirect ? 2 * kUnit : kUnit;
+    return uint64_t(a.pb.tokens) * (a.H / a.Hkv) <= uint64_t(rows) * a.pb.batch;
 }
 
 template <class E, int DP>
@@ -1238,10 +1280,8 @@ uint32_t chunk_shares(const AttnBlocksArgs &a) {
 template <class E, int DP>
 void launch_chunk(const Chunk &k, hipStream_t stream) {
     const uint32_t grid = k.places * k.a.Hkv;
-    if (k.shares == 0) {
-        chunk_tile_kernel<E, DP><<<grid, 256, 0, stream>>>(k);
-        return;
-    }
+    chunk_tile_kernel<E, DP><<<grid, 256, 0, stream>>>(k);
+    if (k.shares == 0) return;
     chunk_shares_kernel<E, DP><<<k.shares, 256, 0, stream>>>(k);
     const uint32_t joins = grid * (DP / 8) <= 1024 ? DP / 8 : grid >= 256 ? 4 : 1024 / grid;
     join_kernel<E, DP><<<grid * joins, 256, 0, stream>>>(k, joins);
