@@ -15,11 +15,11 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 // row's whole history (it stays in L2) and keeps what falls into its columns, so
 // counts are integers whose order does not matter, and no column's rule leaves
 // the workgroup that writes it. Bound by the logits' own bytes where there are many
-// rows (128 rows of 128000 bf16 with masks, biases and 4096 tokens of history each):
-// 8192 columns and 1024 threads a workgroup then read the history eight times a row,
-// 4096 and 256 thirty-two times. Few rows take the small ones, to spread over the GPU.
-template <int kCols>
-constexpr uint32_t threads_of() { return kCols / 16; }
+// rows: 128 rows of 128000 bf16 with masks, biases and 4096 tokens of
+// history each, 70 MB, 22 us or 3.2 TB/s (every row's history is read 16 times, once a
+// workgroup; 4096 columns and 256 threads, 32 times: 23 us; 64 rows 12.3 and 13.3, one row
+// 6.1 and 6.1, the launch's own time).
+constexpr uint32_t kCols = 8192, kThreads = kCols / 16;
 
 // 16 bytes of elements.
 template <class E>
@@ -28,9 +28,9 @@ union Vec {
     typename E::T e[16 / sizeof(typename E::T)];
 };
 
-template <class E, int kCols>
-__global__ __launch_bounds__(threads_of<kCols>()) void logits_kernel(LogitsArgs a, uint32_t chunks, bool wide) {
-    constexpr uint32_t kThreads = threads_of<kCols>(), kV = 16 / sizeof(typename E::T);
+template <class E>
+__global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a, uint32_t chunks, bool wide) {
+    constexpr uint32_t kV = 16 / sizeof(typename E::T);
     __shared__ __attribute__((aligned(16))) uint32_t word[kCols];
     __shared__ uint32_t twice;                          // some token of the workgroup's has two biases
     extern __shared__ int32_t ids[];                    // [biases], then their sums
@@ -180,14 +180,8 @@ void launch(const LogitsArgs &a, hipStream_t stream) {
     // the logits and the result as far past 16 bytes as each other
     const bool wide = (reinterpret_cast<uintptr_t>(a.logits) - reinterpret_cast<uintptr_t>(a.out)) % 16 == 0;
     const size_t lds = size_t(a.biases) * 8;
-    auto chunks = [&](uint32_t cols) { return uint32_t((uint64_t(a.cols) + kV - 1 + cols - 1) / cols); };
-    if (uint64_t(a.rows) * chunks(8192) >= 256) {
-        const uint32_t n = chunks(8192);
-        logits_kernel<E, 8192><<<a.rows * n, threads_of<8192>(), lds, stream>>>(a, n, wide);
-    } else {
-        const uint32_t n = chunks(4096);
-        logits_kernel<E, 4096><<<a.rows * n, threads_of<4096>(), lds, stream>>>(a, n, wide);
-    }
+    const uint32_t chunks = uint32_t((uint64_t(a.cols) + kV - 1 + kCols - 1) / kCols);
+    logits_kernel<E><<<a.rows * chunks, kThreads, lds, stream>>>(a, chunks, wide);
 }
 
 }  // namespace
