@@ -1588,8 +1588,11 @@ int do_kv_block_append(holo_backend *be, const SlotTable &st, const holo_kv_bloc
     const uint64_t es = dtype_size(c.dtype), D = c.head_dim;
     const uint64_t planes = uint64_t(c.batch) * c.kv_heads;
     const uint64_t nb = (uint64_t(c.bucket_rows) + c.block_rows - 1) / c.block_rows;
-    if (uint64_t(c.bucket_rows) * D > (uint64_t(1) << 40))
-        return fail(HOLO_ERR_UNSUPPORTED_OP, "kv_block_append: bucket_rows * head_dim above 2^40");
+    // a block's elements are counted in 32 bits, a cache's bytes in 64
+    if (uint64_t(std::min(c.block_rows, c.bucket_rows)) * D > (uint64_t(1) << 30))
+        return fail(HOLO_ERR_UNSUPPORTED_OP, "kv_block_append: a block of more than 2^30 elements");
+    if (planes * c.bucket_rows > (uint64_t(1) << 50))
+        return fail(HOLO_ERR_UNSUPPORTED_OP, "kv_block_append: a cache of more than 2^50 rows");
     const uint64_t qbytes = planes * c.bucket_rows * D, sbytes = planes * nb * 4;
     const bool in_place = c.output.slot == c.cache.slot && c.output.offset == c.cache.offset &&
                           c.output_scales.slot == c.cache_scales.slot &&

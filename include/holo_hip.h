@@ -467,7 +467,7 @@ typedef struct holo_attention_packed_call {
  * rarely. A NaN or infinite value makes its block's scale NaN: the block reads
  * as NaN until a row is appended at its first row again. Rows at and past
  * pos[b] that this call does not write keep their bytes; a block's scale is no
- * input where pos[b] is its first row.
+ * input where pos[b] is its first row. A block holds at most 2^30 elements.
  *   output == cache and output_scales == cache_scales (same slot and offset):
  *       in place; otherwise the caches are copied first. */
 typedef struct holo_kv_block_append_call {
@@ -492,7 +492,8 @@ typedef struct holo_kv_block_append_call {
  * step and many are a prompt's next chunk, whose own rows were appended before.
  * Scores, softmax and rounding as in 126; a row that sees no key is zeros. What
  * an invisible row or block scale holds does not reach a result. dtype (q,
- * output): bf16, f16 or f32; kv_heads 0 means heads; head_dim <= 1024. */
+ * output): bf16, f16 or f32; kv_heads 0 means heads; head_dim <= 1024;
+ * bucket_rows * head_dim <= 2^30. Long buckets and many rows take scratch. */
 typedef struct holo_attention_i8_blocks_call {
     holo_buffer_ref q;
     holo_buffer_ref k_cache;
@@ -619,7 +620,8 @@ int holo_hip_slot_unbind(holo_backend *be, uint32_t slot);
  * before the host reads any output. Unsupported tags return
  * HOLO_ERR_UNSUPPORTED_OP so the caller can route the call elsewhere, as the
  * reference's GPU backends do (src/metal_backend/mod.rs:172-180).
- * Calls that need split-K scratch share the backend's, which grows to the
+ * Calls that need scratch (split-K products, attention that splits a row's
+ * keys) share the backend's, which grows to the
  * largest request: on several streams the caller orders them, as it orders the
  * replays of graphs it captured them into. Under capture it must be large
  * enough already (dispatch the call once before; HOLO_ERR_DISPATCH otherwise);

@@ -172,3 +172,20 @@ def test_a_graph_of_them_loads_and_its_appends_move_in_place():
             assert (a.output.slot, a.output_scales.slot) == (a.cache.slot, a.cache_scales.slot)
     labels = s.output_labels(["blake3:%064x" % i for i in range(12)])
     assert len(set(labels)) == len(labels) == 7
+
+
+def test_sizes_that_would_wrap_are_refused():
+    """A cache whose bytes pass 64 bits does not wrap to one that fits, and a block whose elements
+    pass 32 bits is not taken."""
+    sizes = [1 << 40, 1 << 40, 1 << 40, 0, 1 << 40]
+    big = replace(APPEND, tokens=1, batch=1 << 24, kv_heads=1, bucket_rows=1 << 31, head_dim=512)
+    with pytest.raises(UnsupportedOp, match="2\\^50"):
+        validate(KernelCall.KvBlockAppend(big), sizes)
+    for block, bucket in ((1 << 22, 1 << 23), (1 << 31, (1 << 20) + 1)):
+        with pytest.raises(UnsupportedOp, match="2\\^30"):
+            validate(KernelCall.KvBlockAppend(replace(APPEND, block_rows=block, bucket_rows=bucket,
+                                                      head_dim=1024)), [1 << 50] * 5)
+    with pytest.raises(UnsupportedOp):
+        validate(KernelCall.AttentionI8Blocks(replace(BLOCKS, batch=1 << 30)), [1 << 40] * 8)
+    with pytest.raises(UnsupportedOp):
+        validate(KernelCall.LogitsProcess(replace(LOGITS, rows=1 << 31, cols=1 << 20)), [1 << 62] * 8)
