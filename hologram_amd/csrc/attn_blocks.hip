@@ -43,10 +43,11 @@ __device__ __forceinline__ uint32_t visible_keys(int64_t len, uint32_t n, uint32
 // the scales of steps it does not see left out, so nothing reaches another row.
 //
 // Two splits. Direct: a workgroup of eight wavefronts a unit, no second launch; for
-// buckets up to kDirect rows (one token of 8 kv heads of 128 dims for 8, 32 and 64 full
-// sequences: 11, 13 and 23 us against the shares' 13, 18 and 20 at 512 rows, 15, 17 and
-// 33 against 14, 22 and 30 at 1024, 23, 27 and 52 against 17, 31 and 49 at 2048, and 20
-// against 16 where 4 of them are ragged). Balanced: all units' 128-key quads laid end to end and cut into equal
+// buckets up to kDirect rows and kDirectUnits units (one token of 8 kv heads of 128 dims
+// for 8, 32 and 128 full sequences: 11, 13 and 47 us against the shares' 13, 18 and 34 at
+// 512 rows, 15, 17 and 64 against 14, 22 and 52 at 1024, 23, 27 and 103 against 17, 31
+// and 90 at 2048; ragged ones of up to 512 rows, 64 and 128 of them: 18 and 33 against 20
+// and 29). Balanced: all units' 128-key quads laid end to end and cut into equal
 // shares, one for each of the workgroups that the GPU holds at once, whatever the
 // lengths; a unit that is cut leaves partials, which merge_kernel joins in order (a
 // launch of its own: partials pass between XCDs' L2s at its boundary).
@@ -55,7 +56,7 @@ __device__ __forceinline__ uint32_t visible_keys(int64_t len, uint32_t n, uint32
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 constexpr uint32_t kUnit = 16, kStep = 32, kQuad = 128, kOob = 1u << 30;   // past every plane, twice it too
-constexpr uint32_t kDirect = 1024, kShares = 512, kMinQuads = 2;
+constexpr uint32_t kDirect = 1024, kDirectUnits = 640, kShares = 512, kMinQuads = 2;
 constexpr int kVeMin = -100;   // 2^ve's floor keeps 2^-ve finite
 
 struct Blocks {
@@ -1247,19 +1248,22 @@ uint32_t few_places(const AttnBlocksArgs &a) {
     return uint32_t(uint64_t(a.pb.tokens) * (a.H / a.Hkv) / kUnit) + a.pb.batch;
 }
 uint32_t padded(uint32_t D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
+bool few_direct(const AttnBlocksArgs &a) {
+    return a.bucket <= kDirect && uint64_t(few_places(a)) * a.Hkv <= kDirectUnits;
+}
 // At most 16 packed rows a sequence on average, 32 where no shares are cut: 32 sequences of
 // 4000 keys, 58 us against the tiles' 94 with 16 rows, 80 and 95 with 32, 157 and 115 with
 // 64, but 61 and 42 with 32 rows and 1 to 4000 keys; of 900 keys, 32 rows, 4 and 16
 // sequences 17 and 32 us against 23 and 35.
 bool few_rows(const AttnBlocksArgs &a) {
-    const uint32_t rows = a.bucket <= kDirect ? 2 * kUnit : kUnit;
+    const uint32_t rows = few_direct(a) ? 2 * kUnit : kUnit;
     return uint64_t(a.pb.tokens) * (a.H / a.Hkv) <= uint64_t(rows) * a.pb.batch;
 }
 
 template <class E, int DP>
 void launch_few(const Blocks &k, hipStream_t stream) {
     const uint32_t grid = k.places * k.a.Hkv;
-    if (k.a.bucket <= kDirect) {
+    if (few_direct(k.a)) {
         constexpr int W = DP > 128 ? 4 : 8;
         few_direct_kernel<E, DP, W><<<grid, 64 * W, 0, stream>>>(k);
         return;
@@ -1349,7 +1353,7 @@ size_t attn_blocks_scratch_bytes(const AttnBlocksArgs &a) {
         const uint64_t s = chunk_shares(a);
         return s == 0 ? 0 : (uint64_t(chunk_places(a)) * a.Hkv + s) * kRows * (padded(a.D) + 2) * 4;
     }
-    if (a.bucket <= kDirect) return 0;
+    if (few_direct(a)) return 0;
     return (uint64_t(few_places(a)) * a.Hkv + kShares) * kUnit * (padded(a.D) + 2) * 4;
 }
 

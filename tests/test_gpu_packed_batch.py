@@ -318,3 +318,104 @@ def test_another_stream_and_replays(torch_cuda):
         assert np.array_equal(run_blocks(torch, eager, cases[turn]), want[turn])
     be.close()
     eager.close()
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("rows,lens,H,Hkv,D,bucket,block", [
+    ([1, 3], [300, 40], 8, 2, 128, 512, 32),          # a unit a workgroup
+    ([1, 3], [1500, 40], 8, 2, 128, 1536, 32),        # shares of units
+    ([70, 33], [70, 400], 8, 2, 64, 512, 64),         # row tiles
+    ([150, 33], [4000, 400], 4, 2, 64, 4096, 64),     # cut row tiles
+    ([3, 20], [30, 90], 2, 1, 72, 100, 10),           # a row a wavefront
+])
+def test_rows_outside_the_sequences_stay_as_they_were(torch_cuda, backend, rows, lens, H, Hkv, D, bucket,
+                                                      block, dtype):
+    rng = np.random.default_rng(bucket)
+    c = blocks_case(rng, rows, lens, H, Hkv, D, bucket, block, dtype)
+    width, n = c["q"].shape[1], sum(rows)
+    c["q"] = np.concatenate([encode(np.full((2, width), np.nan), dtype).reshape(2, width), c["q"],
+                             encode(np.full((3, width), np.nan), dtype).reshape(3, width)])
+    c["starts"] = starts_of(rows, 2)
+    got = run_blocks(torch_cuda, backend, c)
+    assert (got[:2] == 7).all() and (got[2 + n:] == 7).all()
+    check_blocks(got[2:2 + n], {**c, "q": c["q"][2:2 + n]})
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("n", [4, 70])
+def test_unseen_rows_and_blocks_stay_out_of_split_keys(torch_cuda, backend, dtype, n):
+    """As above where a row's keys are several workgroups'."""
+    rng = np.random.default_rng(n)
+    c = blocks_case(rng, [n, n], [2500, 2990], 4, 2, 64, 3008, 16, dtype)
+    clean = run_blocks(torch_cuda, backend, c)
+    for s in ("ks", "vs"):
+        c[s] = c[s].copy()
+        c[s][1, :, 187:] = np.nan         # rows 2992 on
+        c[s][0, :, 157:] = np.inf         # rows 2512 on
+    assert np.array_equal(run_blocks(torch_cuda, backend, c), clean)
+    c["vs"][1, 0, 186] = np.nan           # rows 2976-2991 of kv head 0: the last 14 rows' keys
+    got = run_blocks(torch_cuda, backend, c)
+    sees = np.arange(2 * n) - n >= n - 14
+    sees[:n] = False
+    assert np.array_equal(got[~sees], clean[~sees])
+    assert np.array_equal(got[:, 2:], clean[:, 2:])
+    assert np.isnan(decode(got[sees][:, :2], dtype)).all()
+
+
+def test_a_graph_of_two_calls_over_changing_lengths(torch_cuda):
+    """A chunk and a decode step over one cache in one graph, both in the backend's scratch:
+    replayed with lengths that a workgroup takes whole, that several split, and none at all, each
+    replay is the eager result, and within the bound."""
+    torch = torch_cuda
+    from hologram_amd import HipBackend
+    rng = np.random.default_rng(5)
+    rows, H, Hkv, D, bucket, block = [70, 33], 8, 2, 64, 4096, 32
+    chunks = [blocks_case(rng, rows, lens, H, Hkv, D, bucket, block, DTYPE_F16)
+              for lens in ([70, 120], [4000, 3000], [0, 33], [2100, 33])]
+    steps = [blocks_case(rng, [1, 1], c["lens"] + 1, H, Hkv, D, bucket, block, DTYPE_F16) for c in chunks]
+    for c, s in zip(chunks, steps):
+        for name in ("k", "v", "ks", "vs"):
+            s[name] = c[name]
+    stream = torch.cuda.Stream()
+    be, eager = HipBackend(0, stream.cuda_stream), HipBackend(0, torch.cuda.current_stream().cuda_stream)
+    want = [(run_blocks(torch, eager, c), run_blocks(torch, eager, s)) for c, s in zip(chunks, steps)]
+    for (a, b), c, s in zip(want, chunks, steps):
+        check_blocks(a, c)
+        check_blocks(b, s)
+    ws, ts, calls = DeviceWorkspace(), {}, []
+    for tag, c in (("chunk", chunks[0]), ("step", steps[0])):
+        names = ["q", "k", "v", "ks", "vs", "starts", "lens"]
+        at = []
+        for name in names:
+            key = name if name in ("k", "v", "ks", "vs") else tag + name
+            if key not in ts:
+                ts[key] = (len(ts), to_dev(torch, c[name]))
+            at.append(BufferRef(ts[key][0]))
+        ts[tag + "out"] = (len(ts), torch.zeros(c["q"].nbytes, dtype=torch.uint8, device="cuda"))
+        calls.append(KernelCall.AttentionI8Blocks(AttentionI8BlocksCall(
+            *at, BufferRef(ts[tag + "out"][0]), sum(c["rows"]), 2, H, Hkv, bucket, block, D, 0, 0, DTYPE_F16)))
+    for slot, t in ts.values():
+        ws.bind(slot, t)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        for call in calls:
+            be.dispatch(call, ws)          # sizes the scratch
+    be.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        for call in calls:
+            be.dispatch(call, ws)
+    for turn in (0, 1, 2, 3, 1, 0):
+        for tag, c in (("chunk", chunks[turn]), ("step", steps[turn])):
+            for name in ("q", "k", "v", "ks", "vs", "starts", "lens"):
+                key = name if name in ("k", "v", "ks", "vs") else tag + name
+                ts[key][1].copy_(to_dev(torch, c[name]))
+            ts[tag + "out"][1].zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for tag, w in zip(("chunk", "step"), want[turn]):
+            assert np.array_equal(from_dev(ts[tag + "out"][1], w.dtype).reshape(w.shape), w), (turn, tag)
+        assert np.array_equal(run_blocks(torch, eager, chunks[turn]), want[turn][0])
+    be.close()
+    eager.close()
