@@ -51,8 +51,9 @@ __device__ __forceinline__ uint32_t visible_keys(int64_t len, uint32_t n, uint32
 // shares, one for each of the workgroups that the GPU holds at once, whatever the
 // lengths; a unit that is cut leaves partials, which merge_kernel joins in order (a
 // launch of its own: partials pass between XCDs' L2s at its boundary).
-// Bound by the cache's bytes: 32 sequences of up to 8192 keys, 528 MB, 106 us or 5.0
-// TB/s, merge_kernel 5 us of them; 6.6 TB/s where 128 of them are full.
+// Bound by the cache's bytes: 32 sequences of 512 to 32767 keys, 8 kv heads of 128 dims,
+// 528 MB, 106 us or 5.0 TB/s, merge_kernel 5 us of them; 128 of 8192 keys, 2.2 GB, 6.6 TB/s.
+// Short ones by their latency: 8 of 30 to 700 keys 9 us.
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 constexpr uint32_t kUnit = 16, kStep = 32, kQuad = 128, kOob = 1u << 30;   // past every plane, twice it too
@@ -582,6 +583,11 @@ __global__ __launch_bounds__(256) void merge_kernel(Blocks k) {
 // workgroups a CU; 4 chunks of 301 to 1024 rows 188 us with 192 keys, 181 with 384), so that a sequence's cost and the unit at a place of the line
 // are closed forms. A unit's keys begin at its place kStart; cuts fall on tiles. A unit
 // that is cut leaves partials for join_kernel.
+// Bound by the vector units beside the matrix cores (440 vector instructions a wavefront
+// and tile, a third of them the widening and the scales, against 32 matrix instructions:
+// those are busy 28% of the cycles) and by the units' starts: 4 chunks of 301 to 1024 rows
+// behind up to 6000 keys, 32 heads on 8 of 128 dims, 171 us, 0.51 PFLOP/s, join_kernel 15
+// to 20 us of them; one of 1024 rows 0.60. A wavefront a row (below) took 793 us.
 constexpr uint32_t kRows = 128, kKeys = 64, kManyRounds = 4, kMinKeys = 256, kStart = 384;
 
 struct Chunk {
@@ -1304,7 +1310,9 @@ void launch_few(const Blocks &k, hipStream_t stream) {
 }
 
 // ---------------------------------------------------------- general form ----
-// One wavefront a token and head, any head_dim, block and alignment.
+// One wavefront a token and head, any head_dim, block and alignment: for what the matrix
+// forms do not take (32 sequences of up to 32768 keys, one token each: 18.7 ms, 0.11 on
+// those).
 struct BlockSrc {
     const int8_t *kp, *vp;
     const float *ks, *vs;

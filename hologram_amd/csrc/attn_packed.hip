@@ -18,8 +18,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 // ------------------------------------------------------------ tiled form ----
 // bf16 and f16 rows. A sequence's n * G query rows of a kv head (G = H / Hkv; row
 // r = token r / G, head r % G) go 128 to a workgroup, 32 to a wavefront, over
-// 64-key tiles of the sequence, staged through registers a tile ahead into one of
-// two LDS buffers while the other is multiplied. Per tile and wavefront:
+// 64-key tiles of the sequence, which come by LDS DMA, K's two tiles ahead and V's one,
+// into one of two buffers while the other is multiplied. Per tile and wavefront:
 //     S^T[64 keys x 32 rows] = K . Q^T    32x32x16, a row is a lane column
 //     causal limit, online softmax in f32 (a row's keys are in its lane and in
 //                                         the lane 32 apart)
@@ -351,6 +351,10 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void packed_tile_kernel(Attn
 // end. A lane's scores are keys 8 (r / 4) + 4 (lane / 32) + r % 4 of row lane % 32, which
 // is the order V's operands are read in; Q's dims go to the steps in the order in which
 // 16-byte reads of K bring them. V that is not finite: as in the 16-bit form.
+// 5 prompts of 33 to 1000 rows, 8 heads on 2 of 96 dims: 44 us, of which the longest
+// prompt's last rows take most, 8 tiles a wavefront one after the other (1.9 GFLOP are 12
+// us at the rate of an f32 product); a wavefront a row (below) took 583. 96 dims of rows of
+// 128 are multiplied as 96: a quarter less of them.
 constexpr uint32_t kRows32 = 32, kKeys32 = 32;
 
 template <int DP, int W>
@@ -541,7 +545,8 @@ bool tiles_apply(const AttnPackedArgs &a) {
     auto at16 = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
     const uint32_t far = std::max({a.q_stride, a.k_stride, a.v_stride});
     const uint32_t e = a.dtype == 8 ? 4 : 8;      // elements of 16 bytes
-    return a.D % e == 0 && a.D <= 256 && a.q_stride % e == 0 && a.k_stride % e == 0 && a.v_stride % e == 0 && at16(a.q) && at16(a.k) && at16(a.v) && at16(a.out) && far < (1u << 23);
+    return a.D % e == 0 && a.D <= 256 && a.q_stride % e == 0 && a.k_stride % e == 0 && a.v_stride % e == 0 &&
+           at16(a.q) && at16(a.k) && at16(a.v) && at16(a.out) && far < (1u << 23);
 }
 
 template <class E>
@@ -563,7 +568,8 @@ void launch_f32(const AttnPackedArgs &a, float mul, hipStream_t stream) {
 }
 
 // ---------------------------------------------------------- general form ----
-// One wavefront a token and head, any head_dim, stride and alignment.
+// One wavefront a token and head, any head_dim, stride and alignment: for what the tiles
+// do not take, 30 to 130 times as long where they do.
 template <class E>
 struct RowSrc {
     const typename E::T *kp, *vp;
