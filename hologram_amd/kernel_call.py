@@ -1,9 +1,10 @@
 """KernelCall: the reference's closed kernel-call surface, for the hot ops.
 
 Mirrors crates/hologram-compute/src/kernel_call.rs (field names, order and
-widths) for the variants this backend executes, plus the two new int8-KV
-capabilities, which take new archive discriminants (122, 123) as the
-reference's codec rule requires (crates/hologram-archive/src/kernel_codec.rs:124-128).
+widths) for the variants this backend executes, plus the new capabilities (the
+int8 caches, ArgMax, the packed batch and the logits' rules), which take new
+archive discriminants (122-129) as the reference's codec rule requires
+(crates/hologram-archive/src/kernel_codec.rs:124-128).
 `KernelCall.encode()` writes the archive wire form (u16 LE discriminant + LE
 payload, kernel_codec.rs:557-813).
 """

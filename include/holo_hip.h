@@ -67,7 +67,7 @@ typedef enum holo_status {
 #define HOLO_FUSED_EXP 8
 
 /* KernelCall tags = the archive wire discriminants,
- * crates/hologram-archive/src/kernel_codec.rs:18-128. 122 and 123 are new
+ * crates/hologram-archive/src/kernel_codec.rs:18-128. 122 to 129 are new
  * capabilities and take new discriminants (kernel_codec.rs:124-128). */
 #define HOLO_OP_ADD 5u
 #define HOLO_OP_MUL 7u
@@ -515,7 +515,7 @@ typedef struct holo_attention_i8_blocks_call {
  *   x = logits[r][c]
  *   c among the row's history:            x = x > 0 ? x / rep : x * rep
  *   c generated n >= 1 times:             x = x - (freq * n + pres)
- *   each of the row's biases for c:       x = x + bias, in the list's order
+ *   the row's list has biases for c:      x = x + their sum, in the list's order
  *   mask given and its bit of c clear:    x = -inf
  * history is i32 [rows, history_len] token ids, of which the first
  * min(spans[r][1], history_len) count, the first spans[r][0] of those as prompt
@@ -809,7 +809,7 @@ int holo_hip_derive_label(uint16_t opcode, const uint8_t *params, uint64_t n_par
                           const char *labels, uint64_t n_labels, char out[72]);
 /* KernelCall::op_signature (crates/hologram-compute/src/kernel_call.rs:
  * 1321-1500): the opcode and LE parameter bytes a call's label is derived
- * with. The new calls (122-125) take their discriminant as opcode and their
+ * with. The new calls (122-129) take their discriminant as opcode and their
  * scalar fields in struct order. UnsupportedOp for a call not served here. */
 int holo_hip_op_signature(const holo_kernel_call *call, uint16_t *opcode, uint8_t params[64],
                           uint32_t *n_params);
