@@ -121,20 +121,24 @@ __device__ __forceinline__ void packed_tile(const AttnPackedArgs &a, const float
     // V of a tile that some row does not see to its end: elements that are not finite
     // become zeros; whether there were any is *flag's.
     auto screen = [&](uint8_t *buf, uint32_t *flag) {
+        constexpr int kMine = kKeys * RB / 4096;
+        u32x4 x[kMine];
         bool any = false;
-#pragma unroll 1
-        for (uint32_t at = uint32_t(tid) * 16u; at < kKeys * RB; at += 4096u) {
-            u32x4 x = *reinterpret_cast<u32x4 *>(buf + at);
-            const bool here = odd(x[0]) || odd(x[1]) || odd(x[2]) || odd(x[3]);
-            any |= here;
-            if (!here) continue;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                x[w] = (x[w] & kExp) == kExp ? x[w] & 0xffff0000u : x[w];
-                x[w] = ((x[w] >> 16) & kExp) == kExp ? x[w] & 0xffffu : x[w];
-            }
-            *reinterpret_cast<u32x4 *>(buf + at) = x;
+        for (int i = 0; i < kMine; ++i) {
+            x[i] = *reinterpret_cast<u32x4 *>(buf + tid * 16u + 4096u * i);
+            any |= odd(x[i][0]) || odd(x[i][1]) || odd(x[i][2]) || odd(x[i][3]);
         }
+        if (any)
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    x[i][w] = (x[i][w] & kExp) == kExp ? x[i][w] & 0xffff0000u : x[i][w];
+                    x[i][w] = ((x[i][w] >> 16) & kExp) == kExp ? x[i][w] & 0xffffu : x[i][w];
+                }
+                *reinterpret_cast<u32x4 *>(buf + tid * 16u + 4096u * i) = x[i];
+            }
         const bool found = __ballot(any) != 0;
         if (lane == 0) flag[wave] = found;
     };
