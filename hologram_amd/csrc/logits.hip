@@ -14,12 +14,12 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 // place of its summed bias, bit 31 seen in the prompt. Every workgroup reads the
 // row's whole history (it stays in L2) and keeps what falls into its columns, so
 // counts are integers whose order does not matter, and no column's rule leaves
-// the workgroup that writes it. Bound by the logits' own bytes where there are many
-// rows: 128 rows of 128000 bf16 with masks, biases and 4096 tokens of
-// history each, 70 MB, 22 us or 3.2 TB/s (every row's history is read 16 times, once a
-// workgroup; 4096 columns and 256 threads, 32 times: 23 us; 64 rows 12.3 and 13.3, one row
-// 6.1 and 6.1, the launch's own time).
-constexpr uint32_t kCols = 8192, kThreads = kCols / 16;
+// the workgroup that writes it. The logits are copied, masked, while the rules are
+// gathered; then the columns that a rule names, which their first finder listed, are
+// written again, a thread each: few of a row's columns have one, and a division for
+// every column that shares its 64 lanes with one took longer than the bytes. Bound by
+// @@
+constexpr uint32_t kCols = 8192, kThreads = kCols / 16, kList = 2048;
 
 // 16 bytes of elements.
 template <class E>
@@ -32,7 +32,8 @@ template <class E>
 __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a, uint32_t chunks, bool wide) {
     constexpr uint32_t kV = 16 / sizeof(typename E::T);
     __shared__ __attribute__((aligned(16))) uint32_t word[kCols];
-    __shared__ uint32_t twice;                          // some token of the workgroup's has two biases
+    __shared__ uint16_t list[kList];                    // places that a rule names
+    __shared__ uint32_t listed, twice;                  // so many; some token of the workgroup's has two biases
     extern __shared__ int32_t ids[];                    // [biases], then their sums
     float *sums = reinterpret_cast<float *>(ids + a.biases);
     const uint32_t row = blockIdx.x / chunks, tid = threadIdx.x;
@@ -70,11 +71,14 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a, uint32_t
     // and its first tokens (as long as the row may be: what counts of it comes with them)
     const int32_t *h = a.history ? a.history + uint64_t(row) * a.history_len : nullptr;
     const bool by16 = reinterpret_cast<uintptr_t>(h) % 16 == 0;
-    int4 tokens = {-1, -1, -1, -1};
+    constexpr uint32_t kFirst = 2;
+    int4 tokens[kFirst];
     uint32_t n = 0, prompt = 0;
     float rep = 1.0f, freq = 0.0f, pres = 0.0f;
     if (h) {
-        if (by16 && tid < a.history_len / 4) tokens = reinterpret_cast<const int4 *>(h)[tid];
+#pragma unroll
+        for (uint32_t u = 0; u < kFirst; ++u)
+            if (by16 && tid + u * kThreads < a.history_len / 4) tokens[u] = reinterpret_cast<const int4 *>(h)[tid + u * kThreads];
         prompt = a.spans[2 * uint64_t(row)];
         n = a.spans[2 * uint64_t(row) + 1];
         rep = a.params[3 * uint64_t(row)];
@@ -83,21 +87,44 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a, uint32_t
     }
     for (uint32_t c = 4 * tid; c < kCols; c += 4 * kThreads) *reinterpret_cast<u32x4 *>(word + c) = u32x4{0, 0, 0, 0};
     for (uint32_t j = tid; j < a.biases; j += kThreads) ids[j] = a.bias_ids[uint64_t(row) * a.biases + j];
-    if (tid == 0) twice = 0;
+    if (tid == 0) listed = 0, twice = 0;
     __syncthreads();
+    // what no rule names is done: the mask's select
+    const typename E::T none = E::narrow(-INFINITY);
+    auto there = [&](uint32_t c) { return !mask || ((mask[c >> 5] >> (c & 31)) & 1u); };
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+        const int64_t c = c0 + kV * (tid + uint32_t(i) * kThreads);
+        if (whole(i)) {
+#pragma unroll
+            for (uint32_t e = 0; e < kV; ++e) x[i].e[e] = (bits[i] >> e) & 1u ? x[i].e[e] : none;
+            *reinterpret_cast<u32x4 *>(out + c) = x[i].v;
+        } else {
+            for (uint32_t e = 0; e < kV; ++e)
+                if (c + e >= 0 && c + e < a.cols) out[c + e] = there(uint32_t(c + e)) ? in[c + e] : none;
+        }
+    }
+    // the one who finds a place without a rule lists it
+    auto name = [&](uint32_t old, uint32_t p) {
+        if (old) return;
+        const uint32_t i = atomicAdd(&listed, 1u);
+        if (i < kList) list[i] = uint16_t(p);
+    };
     if (h) {
         n = n < a.history_len ? n : a.history_len;
         auto count = [&](int32_t id, uint32_t i) {
             const uint32_t p = place(id);
             if (p >= kCols) return;
-            if (i < prompt) atomicOr(&word[p], 0x80000000u);
-            else atomicAdd(&word[p], 1u);
+            name(i < prompt ? atomicOr(&word[p], 0x80000000u) : atomicAdd(&word[p], 1u), p);
         };
         const uint32_t quads = by16 ? n / 4 : 0u;
-        for (uint32_t q = tid; q < quads; q += kThreads) {
-            if (q != tid) tokens = reinterpret_cast<const int4 *>(h)[q];
-            count(tokens.x, 4 * q), count(tokens.y, 4 * q + 1), count(tokens.z, 4 * q + 2), count(tokens.w, 4 * q + 3);
-        }
+        auto four = [&](const int4 &x, uint32_t q) {
+            count(x.x, 4 * q), count(x.y, 4 * q + 1), count(x.z, 4 * q + 2), count(x.w, 4 * q + 3);
+        };
+#pragma unroll
+        for (uint32_t u = 0; u < kFirst; ++u)
+            if (tid + u * kThreads < quads) four(tokens[u], tid + u * kThreads);
+        for (uint32_t q = tid + kFirst * kThreads; q < quads; q += kThreads) four(reinterpret_cast<const int4 *>(h)[q], q);
         for (uint32_t k = 4 * quads + tid; k < n; k += kThreads) count(h[k], k);
     }
     // A bias is its token's sum where the token has one; where a second is found, the
@@ -108,7 +135,9 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a, uint32_t
         const uint32_t p = place(ids[j]);
         if (p >= kCols) continue;
         sums[j] = bv[j];
-        if (atomicOr(&word[p], (j + 1) << 19) & kSlot) twice = 1;
+        const uint32_t old = atomicOr(&word[p], (j + 1) << 19);
+        if (old & kSlot) twice = 1;
+        name(old, p);
     }
     __syncthreads();
     if (twice) {
@@ -132,45 +161,20 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a, uint32_t
         }
         __syncthreads();
     }
-    const typename E::T none = E::narrow(-INFINITY);
-    auto rule = [&](typename E::T bits, uint32_t w) {      // w != 0
-        float x = E::widen(bits);
-        const uint32_t n = w & 0x7ffffu, b = (w >> 19) & 0xfffu;
+    auto rule = [&](uint32_t p) {
+        const uint32_t c = uint32_t(c0 + p), w = word[p], n = w & 0x7ffffu, b = (w >> 19) & 0xfffu;
+        if (!there(c)) return;
+        float x = E::widen(in[c]);
         if (n || (w >> 31)) x = x > 0.0f ? x / rep : x * rep;
         if (n) x = x - (freq * float(n) + pres);
         if (b) x = x + sums[b - 1];
-        return E::narrow(x);
+        out[c] = E::narrow(x);
     };
-#pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-        const uint32_t p = kV * (tid + uint32_t(i) * kThreads);
-        const int64_t c = c0 + p;
-        if (whole(i)) {
-            // what the mask leaves out is done at a select; few of the rest have a rule
-            uint32_t w[kV], any = 0;
-#pragma unroll
-            for (uint32_t e = 0; e < kV; e += 4) {
-                const u32x4 q = *reinterpret_cast<const u32x4 *>(word + p + e);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const bool in = (bits[i] >> (e + k)) & 1u;
-                    any |= w[e + k] = in ? q[k] : 0u;
-                    x[i].e[e + k] = in ? x[i].e[e + k] : none;
-                }
-            }
-            if (any)
-#pragma unroll
-                for (uint32_t e = 0; e < kV; ++e)
-                    if (w[e]) x[i].e[e] = rule(x[i].e[e], w[e]);
-            *reinterpret_cast<u32x4 *>(out + c) = x[i].v;
-        } else {
-            for (uint32_t e = 0; e < kV; ++e) {
-                const int64_t d = c + e;
-                if (d < 0 || d >= a.cols) continue;
-                const bool there = !mask || ((mask[d >> 5] >> (d & 31)) & 1u);
-                out[d] = !there ? none : word[p + e] ? rule(in[d], word[p + e]) : in[d];
-            }
-        }
+    if (listed <= kList) {
+        for (uint32_t i = tid; i < listed; i += kThreads) rule(list[i]);
+    } else {
+        for (uint32_t p = tid; p < kCols; p += kThreads)
+            if (word[p]) rule(p);
     }
 }
 

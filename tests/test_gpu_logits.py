@@ -139,3 +139,15 @@ def test_biases_of_one_token_add_in_the_lists_order(torch_cuda, backend):
              values=np.array([[1e8, 2.0, -1e8, 1.0, 3.0]], np.float32))
     got = run(torch_cuda, backend, c, DTYPE_F32)
     assert got[0, 3] == 1.0 and got[0, 5] == 5.0 and np.count_nonzero(got) == 2
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("offset", [0, 3])
+def test_more_columns_with_a_rule_than_are_listed(torch_cuda, backend, dtype, offset):
+    """Histories that name most of a workgroup's 8192 columns, beside ones that name few."""
+    rng = np.random.default_rng(offset)
+    c = make(rng, 4, 17000, 9001, 30, True, dtype)
+    c["history"][1] = rng.integers(8000, 8400, 9001)      # one workgroup's end and the next one's start
+    c["history"][2] = rng.integers(0, 2100, 9001)
+    c["spans"][:, 1] = [9001, 9000, 9001, 8192]
+    check(run(torch_cuda, backend, c, dtype, offset), c, dtype)
