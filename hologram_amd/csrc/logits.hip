@@ -143,6 +143,8 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a, uint32_t
         if (old & kSlot) twice = 1;
         name(old, p);
     }
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((15 << 8) | (7 << 4));   // vmcnt(0): the copies are there, to be written over
     __syncthreads();
     if (twice) {
         for (uint32_t j = tid; j < a.biases; j += kThreads) {
