@@ -419,3 +419,15 @@ def test_a_graph_of_two_calls_over_changing_lengths(torch_cuda):
         assert np.array_equal(run_blocks(torch, eager, chunks[turn]), want[turn][0])
     be.close()
     eager.close()
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_blocks_more_sequences_than_a_workgroup_has_threads(torch_cuda, backend, n):
+    """Shares cut on a line of 300 sequences, several a thread, some of them empty."""
+    rng = np.random.default_rng(n)
+    B, bucket = 300, 2600
+    rows = [0 if b % 7 == 3 else n for b in range(B)]
+    lens = rng.integers(0, bucket + 1, B)
+    lens[[0, 255, 256, 299]] = [bucket, 1, 2599, 1300]
+    c = blocks_case(rng, rows, lens, 4, 1, 64, bucket, 32, DTYPE_BF16)
+    check_blocks(run_blocks(torch_cuda, backend, c), c, sequences=(0, 1, 2, 150, 254, 255, 256, 257, 298, 299))
