@@ -13,6 +13,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <initializer_list>
 #include <string>
 #include <vector>
 
@@ -57,6 +58,18 @@ Sig p_attn_i8(const holo_decode_attention_i8_call &c) {
     Sig s;
     return s.u32(c.batch).u32(c.heads).u32(c.kv_heads).u32(c.bucket_rows).u32(c.head_dim)
         .u32(c.scale_bits).u8(c.dtype);
+}
+// Where each operand of a packed-batch call starts (all ones for one that is
+// absent), as the first 16 bytes of a BLAKE3 digest, for 64 bytes do not hold
+// them: their q, k and v are views of one value, and any other operand may be,
+// and an absent operand has no label to stand in its place. (The session
+// computes calls of one label once.)
+void p_views(Sig *s, std::initializer_list<holo_buffer_ref> refs) {
+    std::vector<uint64_t> at;
+    for (const auto &b : refs) at.push_back(b.slot == HOLO_SLOT_ABSENT ? ~uint64_t(0) : b.offset);
+    uint8_t digest[32];
+    blake3_hash(at.data(), at.size() * 8, digest);
+    s->raw(digest, 16);
 }
 
 bool per_channel(uint32_t channels, const holo_buffer_ref &scales) {
@@ -239,20 +252,20 @@ bool op_signature(const holo_kernel_call &c, uint16_t *opcode, uint8_t params[64
         case HOLO_OP_ATTN_I8_ROWS:
             s = p_attn_i8(c.u.attn_i8_rows.attn), s.u32(c.u.attn_i8_rows.q_rows), op = 125;
             break;
-        // (q, k, v and the new rows may be views of one value: where a view starts is
-        // a parameter, so that calls over different views derive different labels)
         case HOLO_OP_ATTN_PACKED: {
             const auto &a = c.u.attn_packed;
             s.u32(a.tokens).u32(a.batch).u32(a.heads).u32(a.kv_heads).u32(a.head_dim)
-                .u32(a.q_stride).u32(a.k_stride).u32(a.v_stride).u32(a.scale_bits).u8(a.dtype)
-                .u64(a.q.offset).u64(a.k.offset).u64(a.v.offset);
+                .u32(a.q_stride).u32(a.k_stride).u32(a.v_stride).u32(a.scale_bits).u8(a.dtype);
+            p_views(&s, {a.q, a.k, a.v, a.starts, a.output});
             op = 126;
             break;
         }
         case HOLO_OP_KV_BLOCK_APPEND: {
             const auto &a = c.u.kv_block_append;
             s.u32(a.tokens).u32(a.batch).u32(a.kv_heads).u32(a.bucket_rows).u32(a.block_rows)
-                .u32(a.head_dim).u32(a.new_stride).u8(a.dtype).u64(a.new_rows_buf.offset);
+                .u32(a.head_dim).u32(a.new_stride).u8(a.dtype);
+            p_views(&s, {a.new_rows_buf, a.starts, a.pos, a.cache, a.cache_scales, a.output,
+                         a.output_scales});
             op = 127;
             break;
         }
@@ -260,14 +273,15 @@ bool op_signature(const holo_kernel_call &c, uint16_t *opcode, uint8_t params[64
             const auto &a = c.u.attn_i8_blocks;
             s.u32(a.tokens).u32(a.batch).u32(a.heads).u32(a.kv_heads).u32(a.bucket_rows)
                 .u32(a.block_rows).u32(a.head_dim).u32(a.q_stride).u32(a.scale_bits)
-                .u8(a.dtype)
-                .u64(a.q.offset);
+                .u8(a.dtype);
+            p_views(&s, {a.q, a.k_cache, a.v_cache, a.k_scales, a.v_scales, a.starts, a.lens, a.output});
             op = 128;
             break;
         }
         case HOLO_OP_LOGITS_PROCESS: {
             const auto &a = c.u.logits_process;
             s.u32(a.rows).u32(a.cols).u32(a.history_len).u32(a.biases).u8(a.dtype);
+            p_views(&s, {a.logits, a.history, a.spans, a.params, a.bias_ids, a.bias_values, a.mask, a.output});
             op = 129;
             break;
         }

@@ -810,7 +810,10 @@ int holo_hip_derive_label(uint16_t opcode, const uint8_t *params, uint64_t n_par
 /* KernelCall::op_signature (crates/hologram-compute/src/kernel_call.rs:
  * 1321-1500): the opcode and LE parameter bytes a call's label is derived
  * with. The new calls (122-129) take their discriminant as opcode and their
- * scalar fields in struct order. UnsupportedOp for a call not served here. */
+ * scalar fields in struct order; 126-129 then the first 16 bytes of the BLAKE3
+ * digest of their operands' offsets, u64 LE each in struct order, 2^64 - 1 for
+ * an absent one: calls over different views of one slot, or with other operands
+ * absent, have different labels. UnsupportedOp for a call not served here. */
 int holo_hip_op_signature(const holo_kernel_call *call, uint16_t *opcode, uint8_t params[64],
                           uint32_t *n_params);
 
