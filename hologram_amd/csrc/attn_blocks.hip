@@ -791,7 +791,10 @@ __device__ __forceinline__ void chunk_segment(const Chunk &k, const Place &at, u
     float m = -INFINITY, l = 0.0f;
     int ve = kVeMin;
     const uint32_t kat = k_place<DP>(lane), vat = v_place<DP>(lane);
-    // of the steps of the tile in s: K's factor; |vs| = fr 2^ex, log2(fr)
+    // of the steps of the tile in s: K's factor; |vs| = fr 2^ex, log2(fr); ex is kNone of a
+    // step that adds nothing (a scale of zero; none of its keys seen), whose weights go by
+    // the row's own ve, clear of f16's ends
+    constexpr int kNone = -1000;
     float c[4], fr[4], lf[4];
     int ex[4];
 
@@ -803,10 +806,10 @@ __device__ __forceinline__ void chunk_segment(const Chunk &k, const Place &at, u
     // the scales of tile j, and s limited; the largest exponent of the steps the row sees
     auto take = [&](int g) __attribute__((always_inline)) {
         c[g] = fabsf(nk[g]) * mul;
-        float v = fabsf(nv[g]);
-        v = v == 0.0f ? 1.0f : v;      // (its bytes are zeros)
+        const float v = fabsf(nv[g]);
         ex[g] = 0;
         fr[g] = v <= 3.4028235e38f ? frexpf(v, &ex[g]) : v;        // fr in [0.5, 1)
+        if (v == 0.0f) fr[g] = 0.5f, ex[g] = kNone;                // (its bytes are zeros)
         lf[g] = __builtin_amdgcn_logf(fr[g]);
     };
     auto limit = [&](uint32_t j, int *top) __attribute__((always_inline)) {
@@ -824,7 +827,7 @@ __device__ __forceinline__ void chunk_segment(const Chunk &k, const Place &at, u
             asm volatile("");
 #pragma unroll
             for (int g = 0; g < 4; ++g)
-                if (j + 16 * g >= lim) fr[g] = 0.5f, lf[g] = -1.0f, ex[g] = kVeMin;
+                if (j + 16 * g >= lim) fr[g] = 0.5f, lf[g] = -1.0f, ex[g] = kNone;
         }
         *top = kVeMin;
 #pragma unroll
@@ -857,8 +860,9 @@ __device__ __forceinline__ void chunk_segment(const Chunk &k, const Place &at, u
     auto prepare = [&]() __attribute__((always_inline)) {
         const float ref = m == -INFINITY ? 0.0f : m;
         auto one = [&](int g) __attribute__((always_inline)) {
-            up[g] = (lf[g] + float(ex[g] + 7 - ve)) - ref;
-            back[g] = ldexpf(__builtin_amdgcn_rcpf(fr[g]), ve - 7 - ex[g]);   // (exact for powers of two)
+            const int e = ex[g] == kNone ? 0 : ex[g] - ve;
+            up[g] = (lf[g] + float(e + 7)) - ref;
+            back[g] = ldexpf(__builtin_amdgcn_rcpf(fr[g]), -7 - e);   // (exact for powers of two)
         };
         one(0);
         if (k.shift >= 6) {            // (a row that sees none of the block has weights of 0)

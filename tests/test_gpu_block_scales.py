@@ -1,0 +1,49 @@
+"""AttentionI8Blocks (128) over caches whose V scales are zero, far apart, tiny or not finite, in
+each of its forms, against 64 bits."""
+import numpy as np
+import pytest
+
+from hologram_amd import DTYPE_BF16, DTYPE_F16, DTYPE_F32
+from packed_reference import ALL, attend, bound, decode
+from test_gpu_packed_batch import blocks_case, run_blocks
+
+pytestmark = pytest.mark.gpu
+
+# half the least step of the result's type
+FLOOR = {DTYPE_BF16: 2.0 ** -134, DTYPE_F16: 2.0 ** -25, DTYPE_F32: 2.0 ** -150}
+# rows of each of two sequences, their lengths, the bucket: a unit a workgroup, shares of units, row
+# tiles whole, row tiles cut
+FORMS = [(1, [400, 90], 400), (1, [2500, 90], 2512), (80, [400, 90], 400), (80, [4000, 300], 4000)]
+
+
+def make(rng, n, lens, bucket, dtype, D=64):
+    return blocks_case(rng, [n, n], lens, 4, 2, D, bucket, 16, dtype)
+
+
+def check(got, c):
+    """Within packed_reference's bound and half a least step of the type."""
+    dtype, H, Hkv, D = c["dtype"], c["H"], c["Hkv"], c["D"]
+    q = decode(c["q"], dtype).reshape(c["q"].shape)[:, c["pad"]:].reshape(-1, H, D)
+    at = 0
+    for b, n in enumerate(c["rows"]):
+        keys = np.clip(int(c["lens"][b]) - (n - 1 - np.arange(n)), 0, c["bucket"])
+        of = np.arange(int(keys.max())) // c["block"]
+        k, v = ((c[x][b, :, :len(of)].astype(np.float64) * c[x + "s"][b][:, of, None].astype(np.float64))
+                .transpose(1, 0, 2) for x in "kv")
+        want, slack, top = attend(q[at:at + n], k, v, keys, H, Hkv, np.sqrt(D))
+        err = np.abs(decode(got[at:at + n], dtype).reshape(want.shape) - want)
+        tol = bound(slack, top, dtype) + FLOOR[dtype]
+        assert (err <= tol).all(), (b, float(np.nanmax(err / tol)))
+        at += n
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("exponent", [-13, -20, -24, -34, -40])
+@pytest.mark.parametrize("n,lens,bucket", FORMS)
+def test_a_zero_v_scale_costs_the_other_blocks_nothing(torch_cuda, backend, n, lens, bucket, exponent, dtype):
+    """A block of zeros, as KvBlockAppend writes it (scale 0), among blocks of one small scale."""
+    c = make(np.random.default_rng(-exponent), n, lens, bucket, dtype)
+    c["vs"][:] = 2.0 ** exponent
+    c["vs"][:, :, 3] = 0.0
+    c["vs"][1, 0, 0] = -0.0
+    check(run_blocks(torch_cuda, backend, c), c)
