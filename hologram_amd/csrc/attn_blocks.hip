@@ -565,11 +565,12 @@ __global__ __launch_bounds__(256) void merge_kernel(Blocks k) {
 // is in [2^14, 2^15): exact for 16-bit rows but for elements 2^-38 of the largest, and in
 // two parts, 22 bits, for f32 rows; a row's power and log2(e) / divisor join K's scales.
 // The scale of a 16-key step is one number: K's |ks| times the row's factor is the
-// step's c, with s c - m one instruction; V's joins the exponent, w = 2^(s c - m +
-// log2|vs| + 7 - ve) (log2 rounded to 2^-21 at worst, where it is 8 or less: a weight off
-// by 2^-21), and the sum l takes a step's weights back by 1 / |vs|. 2^ve is above every
-// finite |vs| of the steps the row sees so far. A scale's sign is put on the bytes, and a
-// zero V scale makes them zeros, on the way into LDS.
+// step's c, with s c - m one instruction; V's joins the weights as in the few-row form, w =
+// p |vs| 2^(7 - ve), and the sum l takes p itself, in f32, whatever the scales are. (V's
+// scale in the exponent and l's share of it taken back by 1 / |vs| was an instruction a
+// weight less; scales far below the row's largest lost their keys' part of l that way.)
+// 2^ve is above every finite |vs| of the steps the row sees so far. A scale's sign is put
+// on the bytes on the way into LDS.
 // In a tile that some row does not see to its end, s is scaled and limited first (c = 1),
 // and a step that a row does not see brings it no scale.
 // A row tile and kv head is a workgroup's, whole (chunk_tile_kernel), where that gives
@@ -681,9 +682,9 @@ __device__ __forceinline__ void chunk_segment(const Chunk &k, const Place &at, u
     };
     auto fetch_k = [&](uint32_t j) { fetch(rk, j, kr), ksk = scale_at(ks, j + key); };
     auto fetch_v = [&](uint32_t j) { fetch(rv, j, vr), vsk = scale_at(vs, j + key); };
-    auto put = [&](uint8_t *buf, const u32x4 (&x)[CT], float scale, bool zero, const uint32_t (&to)[2]) {
+    auto put = [&](uint8_t *buf, const u32x4 (&x)[CT], float scale, const uint32_t (&to)[2]) {
         const uint32_t flip = __float_as_uint(scale) >> 31 ? 0x80008000u : 0u;
-        const bool plain = !__any(flip != 0 || zero);
+        const bool plain = !__any(flip != 0);
 #pragma unroll
         for (int i = 0; i < CT; ++i)
 #pragma unroll
@@ -693,7 +694,7 @@ __device__ __forceinline__ void chunk_segment(const Chunk &k, const Place &at, u
                 if (!plain) {
                     asm volatile("");      // a branch of its own
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) v[w] = zero ? 0u : v[w] ^ flip;
+                    for (int w = 0; w < 4; ++w) v[w] ^= flip;
                 }
                 *reinterpret_cast<u32x4 *>(buf + (to[h] ^ (128u * i))) = v;
             }
@@ -705,8 +706,8 @@ __device__ __forceinline__ void chunk_segment(const Chunk &k, const Place &at, u
         kto[h] = key * RB + (((2u * part + h) ^ swz_k<DP>(key)) * 16u);
         vto[h] = key * RB + (((2u * part + h) ^ swz_v<DP>(key)) * 16u);
     }
-    auto put_k = [&](uint8_t *buf) { put(buf, kr, ksk, false, kto); };
-    auto put_v = [&](uint8_t *buf) { put(buf, vr, vsk, vsk == 0.0f, vto); };
+    auto put_k = [&](uint8_t *buf) { put(buf, kr, ksk, kto); };
+    auto put_v = [&](uint8_t *buf) { put(buf, vr, vsk, vto); };
     fetch_k(j1);
     fetch_v(j1);
 
@@ -791,12 +792,8 @@ __device__ __forceinline__ void chunk_segment(const Chunk &k, const Place &at, u
     float m = -INFINITY, l = 0.0f;
     int ve = kVeMin;
     const uint32_t kat = k_place<DP>(lane), vat = v_place<DP>(lane);
-    // of the steps of the tile in s: K's factor; |vs| = fr 2^ex, log2(fr); ex is kNone of a
-    // step that adds nothing (a scale of zero; none of its keys seen), whose weights go by
-    // the row's own ve, clear of f16's ends
-    constexpr int kNone = -1000;
-    float c[4], fr[4], lf[4];
-    int ex[4];
+    // of the steps of the tile in s: K's factor, and |vs| where the row sees a key of them, else 0
+    float c[4], v[4];
 
     float nk[4], nv[4];      // the next tile's scales, loaded a tile's scores ahead of their use
     auto load_scales = [&](uint32_t j) __attribute__((always_inline)) {
@@ -804,34 +801,32 @@ __device__ __forceinline__ void chunk_segment(const Chunk &k, const Place &at, u
         for (int g = 0; g < 4; ++g) nk[g] = uniform_at(ks, j + 16 * g), nv[g] = uniform_at(vs, j + 16 * g);
     };
     // the scales of tile j, and s limited; the largest exponent of the steps the row sees
-    auto take = [&](int g) __attribute__((always_inline)) {
-        c[g] = fabsf(nk[g]) * mul;
-        const float v = fabsf(nv[g]);
-        ex[g] = 0;
-        fr[g] = v <= 3.4028235e38f ? frexpf(v, &ex[g]) : v;        // fr in [0.5, 1)
-        if (v == 0.0f) fr[g] = 0.5f, ex[g] = kNone;                // (its bytes are zeros)
-        lf[g] = __builtin_amdgcn_logf(fr[g]);
+    auto take = [&](int g) __attribute__((always_inline)) { c[g] = fabsf(nk[g]) * mul, v[g] = fabsf(nv[g]); };
+    auto above = [&](float x) {        // the least 2^ve above x; kVeMin of a zero, an infinity or a NaN
+        return x > 0.0f && x <= 3.4028235e38f ? __builtin_amdgcn_frexp_expf(x) : kVeMin;
     };
     auto limit = [&](uint32_t j, int *top) __attribute__((always_inline)) {
         take(0);
+        const bool all = j + kKeys <= wmin;
         if (k.shift >= 6) {            // one block holds the tile
             asm volatile("");
+            if (j >= lim) v[0] = 0.0f;
 #pragma unroll
-            for (int g = 1; g < 4; ++g) c[g] = c[0], fr[g] = fr[0], lf[g] = lf[0], ex[g] = ex[0];
+            for (int g = 1; g < 4; ++g) c[g] = c[0], v[g] = v[0];
+            *top = above(v[0]);
         } else {
 #pragma unroll
             for (int g = 1; g < 4; ++g) take(g);
-        }
-        const bool all = j + kKeys <= wmin;
-        if (!all) {
-            asm volatile("");
+            if (!all) {
+                asm volatile("");
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
-                if (j + 16 * g >= lim) fr[g] = 0.5f, lf[g] = -1.0f, ex[g] = kNone;
-        }
-        *top = kVeMin;
+                for (int g = 0; g < 4; ++g)
+                    if (j + 16 * g >= lim) v[g] = 0.0f;
+            }
+            *top = kVeMin;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) *top = fr[g] < 1.0f && ex[g] > *top ? ex[g] : *top;   // (not of an infinity or NaN)
+            for (int g = 0; g < 4; ++g) *top = above(v[g]) > *top ? above(v[g]) : *top;
+        }
         if (all) return;
         int see = int(lim < kmax ? lim : kmax) - int(j) - 4 * lg;
         asm volatile("" : "+v"(see));
@@ -856,22 +851,17 @@ __device__ __forceinline__ void chunk_segment(const Chunk &k, const Place &at, u
         }
     };
     u32x4 pf[P][4];
-    float up[4], back[4];         // per step: log2|vs| + 7 - ve - m, and 2^(ve - 7) / |vs|
+    float ref, f[4];              // per step: |vs| 2^(7 - ve)
     auto prepare = [&]() __attribute__((always_inline)) {
-        const float ref = m == -INFINITY ? 0.0f : m;
-        auto one = [&](int g) __attribute__((always_inline)) {
-            const int e = ex[g] == kNone ? 0 : ex[g] - ve;
-            up[g] = (lf[g] + float(e + 7)) - ref;
-            back[g] = ldexpf(__builtin_amdgcn_rcpf(fr[g]), -7 - e);   // (exact for powers of two)
-        };
-        one(0);
-        if (k.shift >= 6) {            // (a row that sees none of the block has weights of 0)
+        ref = m == -INFINITY ? 0.0f : m;
+        f[0] = ldexpf(v[0], 7 - ve);
+        if (k.shift >= 6) {
             asm volatile("");
 #pragma unroll
-            for (int g = 1; g < 4; ++g) up[g] = up[0], back[g] = back[0];
+            for (int g = 1; g < 4; ++g) f[g] = f[0];
         } else {
 #pragma unroll
-            for (int g = 1; g < 4; ++g) one(g);
+            for (int g = 1; g < 4; ++g) f[g] = ldexpf(v[g], 7 - ve);
         }
     };
     auto weight_pair = [&](int i) __attribute__((always_inline)) {
@@ -879,10 +869,10 @@ __device__ __forceinline__ void chunk_segment(const Chunk &k, const Place &at, u
         float w[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const float x = s[i >> 3][2 * (i & 7) + e];
-            w[e] = __builtin_amdgcn_exp2f(fmaf(x, c[g], up[g]));
+            const float p = __builtin_amdgcn_exp2f(fmaf(s[i >> 3][2 * (i & 7) + e], c[g], -ref));
+            l += p;
+            w[e] = p * f[g];
         }
-        l = fmaf(w[0] + w[1], back[g], l);
         uint32_t hi = pack2<F16>(w[0], w[1]);
         if constexpr (kF32) {
             typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));

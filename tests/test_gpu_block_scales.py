@@ -47,3 +47,30 @@ def test_a_zero_v_scale_costs_the_other_blocks_nothing(torch_cuda, backend, n, l
     c["vs"][:, :, 3] = 0.0
     c["vs"][1, 0, 0] = -0.0
     check(run_blocks(torch_cuda, backend, c), c)
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("few", [[-149, -126, -6, 8], [-149], [-126], [-60, 8]])
+@pytest.mark.parametrize("n,lens,bucket", FORMS)
+def test_far_apart_v_scales(torch_cuda, backend, n, lens, bucket, few, dtype):
+    """Scales whose ratio passes what f32 holds: the keys of the small ones weigh in the softmax like
+    any other. (The first block's is ordinary, so every row that sees a key sees a value to measure
+    by.)"""
+    rng = np.random.default_rng(sum(few) + 1000)
+    c = make(rng, n, lens, bucket, dtype)
+    c["vs"] = np.ldexp(1.0, rng.choice(few, c["vs"].shape)).astype(np.float32)
+    c["vs"][:, :, 0] = 2.0 ** 8 if max(few) == 8 else 2.0 ** -6
+    check(run_blocks(torch_cuda, backend, c), c)
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("n,lens,bucket", FORMS)
+def test_a_zero_v_scale_is_a_block_of_zeros(torch_cuda, backend, n, lens, bucket, dtype):
+    """The same bits whichever of the two says so."""
+    c = make(np.random.default_rng(n), n, lens, bucket, dtype)
+    c["vs"][:] = 2.0 ** -9
+    by_scale = {**c, "vs": c["vs"].copy()}
+    by_scale["vs"][:, :, 3] = 0.0
+    by_bytes = {**c, "v": c["v"].copy()}
+    by_bytes["v"][:, :, 48:64] = 0
+    assert np.array_equal(run_blocks(torch_cuda, backend, by_scale), run_blocks(torch_cuda, backend, by_bytes))
