@@ -60,6 +60,16 @@ constexpr uint32_t kUnit = 16, kStep = 32, kQuad = 128, kOob = 1u << 30;   // pa
 constexpr uint32_t kDirect = 1024, kDirectUnits = 640, kShares = 512, kMinQuads = 2;
 constexpr int kVeMin = -100;   // 2^ve's floor keeps 2^-ve finite
 
+// A step's factor of its weights, v 2^(7 - ve). An infinite scale's is 2^100, whose weights
+// are infinite in f16 where p is not 0 and 0 where it is: a key that the row does not see
+// brings it no NaN.
+__device__ __forceinline__ float weight_factor(float v, int ve) {
+    const float f = ldexpf(v, 7 - ve);
+    return fabsf(f) == INFINITY ? copysignf(0x1p100f, f) : f;
+}
+// What a weight of at most 2^15 leaves over its f16, as f16; nothing of an infinite one's.
+__device__ __forceinline__ float left_over(float w, float hi) { return fminf(fmaxf(w - hi, -16.0f), 16.0f); }
+
 struct Blocks {
     AttnBlocksArgs a;
     float mul;           // log2(e) / divisor
@@ -293,14 +303,14 @@ __device__ __forceinline__ void few_segment(const Blocks &k, const Place &at, ui
         f16x8 hi, lo;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const float f = ldexpf(vs_h[h], 7 - ve);
+            const float f = weight_factor(vs_h[h], ve);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float p = __builtin_amdgcn_exp2f(s[4 * h + i] - ref);
                 st.l += p;
-                w[4 * h + i] = s[4 * h + i] == -INFINITY ? 0.0f : p * f;
+                w[4 * h + i] = p * f;
                 hi[4 * h + i] = _Float16(w[4 * h + i]);
-                if constexpr (kF32) lo[4 * h + i] = _Float16(w[4 * h + i] - float(hi[4 * h + i]));
+                if constexpr (kF32) lo[4 * h + i] = _Float16(left_over(w[4 * h + i], float(hi[4 * h + i])));
             }
         }
 #pragma unroll
@@ -854,14 +864,14 @@ __device__ __forceinline__ void chunk_segment(const Chunk &k, const Place &at, u
     float ref, f[4];              // per step: |vs| 2^(7 - ve)
     auto prepare = [&]() __attribute__((always_inline)) {
         ref = m == -INFINITY ? 0.0f : m;
-        f[0] = ldexpf(v[0], 7 - ve);
+        f[0] = weight_factor(v[0], ve);
         if (k.shift >= 6) {
             asm volatile("");
 #pragma unroll
             for (int g = 1; g < 4; ++g) f[g] = f[0];
         } else {
 #pragma unroll
-            for (int g = 1; g < 4; ++g) f[g] = ldexpf(v[g], 7 - ve);
+            for (int g = 1; g < 4; ++g) f[g] = weight_factor(v[g], ve);
         }
     };
     auto weight_pair = [&](int i) __attribute__((always_inline)) {
@@ -877,7 +887,7 @@ __device__ __forceinline__ void chunk_segment(const Chunk &k, const Place &at, u
         if constexpr (kF32) {
             typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
             const f16x2 f = __builtin_bit_cast(f16x2, hi);
-            uint32_t lo = pack2<F16>(w[0] - float(f[0]), w[1] - float(f[1]));
+            uint32_t lo = pack2<F16>(left_over(w[0], float(f[0])), left_over(w[1], float(f[1])));
             asm volatile("" : "+v"(lo));
             pf[P - 1][i >> 2][i & 3] = lo;
         }

@@ -74,3 +74,41 @@ def test_a_zero_v_scale_is_a_block_of_zeros(torch_cuda, backend, n, lens, bucket
     by_bytes = {**c, "v": c["v"].copy()}
     by_bytes["v"][:, :, 48:64] = 0
     assert np.array_equal(run_blocks(torch_cuda, backend, by_scale), run_blocks(torch_cuda, backend, by_bytes))
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("n,lens,bucket", FORMS)
+def test_an_infinite_v_scale(torch_cuda, backend, n, lens, bucket, dtype):
+    """Infinity times the bytes: infinite of their sign in a dim where all are of one, NaN where some
+    are zero, for the rows that see a key of the block; the rest as it was. (Q is small, so that no
+    weight is 0.)"""
+    c = make(np.random.default_rng(n), n, lens, bucket, dtype)
+    c["q"] = np.zeros_like(c["q"])
+    block = (lens[0] - 1 - n // 2) // 16        # half of the first sequence's rows see some of it
+    clean = decode(run_blocks(torch_cuda, backend, c), dtype).reshape(2 * n, 4, 64)
+    c["v"][0, 0, 16 * block:16 * block + 16] = np.array([3, -5, 0, 1], np.int8)[np.arange(64) % 4]
+    plain = decode(run_blocks(torch_cuda, backend, c), dtype).reshape(2 * n, 4, 64)
+    c["vs"][0, 0, block] = np.inf
+    got = decode(run_blocks(torch_cuda, backend, c), dtype).reshape(2 * n, 4, 64)
+    keys = np.concatenate([lens[0] - (n - 1 - np.arange(n)), np.zeros(n, int)])
+    sees = keys > 16 * block
+    assert sees.any()
+    assert np.array_equal(got[~sees], plain[~sees]) and np.array_equal(got[:, 2:], clean[:, 2:])
+    want = np.array([np.inf, -np.inf, np.nan, np.inf])[np.arange(64) % 4]
+    assert np.array_equal(got[sees][:, :2], np.broadcast_to(want, (sees.sum(), 2, 64)), equal_nan=True)
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("n,lens,bucket", FORMS)
+def test_a_nan_v_scale(torch_cuda, backend, n, lens, bucket, dtype):
+    """Every dim of the rows that see a key of the block is NaN, whatever its bytes."""
+    c = make(np.random.default_rng(n), n, lens, bucket, dtype)
+    block = (lens[0] - 1 - n // 2) // 16
+    clean = run_blocks(torch_cuda, backend, c)
+    c["v"][0, 0, 16 * block:16 * block + 16] = 0
+    plain = run_blocks(torch_cuda, backend, c)
+    c["vs"][0, 0, block] = np.nan
+    got = run_blocks(torch_cuda, backend, c)
+    sees = np.concatenate([lens[0] - (n - 1 - np.arange(n)), np.zeros(n, int)]) > 16 * block
+    assert np.array_equal(got[~sees], plain[~sees]) and np.array_equal(got[:, 2:], clean[:, 2:])
+    assert np.isnan(decode(got[sees][:, :2], dtype)).all()
