@@ -58,7 +58,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 constexpr uint32_t kUnit = 16, kStep = 32, kQuad = 128, kOob = 1u << 30;   // past every plane, twice it too
 constexpr uint32_t kDirect = 1024, kDirectUnits = 640, kShares = 512, kMinQuads = 2;
-constexpr int kVeMin = -100;   // 2^ve's floor keeps 2^-ve finite
+constexpr int kVeMin = -126;   // the floor of ve, where the result's own bits end
 
 // A step's factor of its weights, v 2^(7 - ve). An infinite scale's is 2^100, whose weights
 // are infinite in f16 where p is not 0 and 0 where it is: a key that the row does not see
@@ -1001,7 +1001,6 @@ __device__ __forceinline__ void chunk_segment(const Chunk &k, const Place &at, u
         }
     }
     l += __shfl_xor(l, 32, 64);
-    const float unit = ldexpf(1.0f, ve - 7);
     if (!whole) {
         if (!live) return;
 #pragma unroll
@@ -1010,14 +1009,16 @@ __device__ __forceinline__ void chunk_segment(const Chunk &k, const Place &at, u
             for (int g = 0; g < 4; ++g) {
                 f32x4 x;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = o[d][4 * g + e] * unit;
+                for (int e = 0; e < 4; ++e) x[e] = ldexpf(o[d][4 * g + e], ve - 7);
                 *reinterpret_cast<f32x4 *>(dst + part_of<DP>(wave, 4 * d + g, lane)) = x;
             }
         if (lg == 0) dst[kRows * DP + 32 * wave + lr] = m, dst[kRows * (DP + 1) + 32 * wave + lr] = l;
         return;
     }
-    // rows stored whole through LDS (16-bit), or as they are (f32)
-    const float inv = lim == 0 ? 0.0f : unit / l;
+    // rows stored whole through LDS (16-bit), or as they are (f32); 2^(ve - 7) last, for it
+    // may be a subnormal
+    const float inv = lim == 0 ? 0.0f : 1.0f / l;
+    auto result = [&](float x) { return ldexpf(x * inv, ve - 7); };
     T *out = static_cast<T *>(a.out) + (uint64_t(t0) * a.H + kh * G) * a.D;
     if constexpr (kF32) {
         if (wr0 + lr >= R) return;
@@ -1029,7 +1030,7 @@ __device__ __forceinline__ void chunk_segment(const Chunk &k, const Place &at, u
                 const uint32_t dim = 32 * d + 8 * g + 4 * lg;
                 if (dim < a.D)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) to[dim + e] = o[d][4 * g + e] * inv;
+                    for (int e = 0; e < 4; ++e) to[dim + e] = result(o[d][4 * g + e]);
             }
     } else {
         lds_barrier();
@@ -1040,8 +1041,8 @@ __device__ __forceinline__ void chunk_segment(const Chunk &k, const Place &at, u
 #pragma unroll
             for (int g = 0; g < 4; ++g)
                 *reinterpret_cast<uint2 *>(turn + chunk_at(RB, lr, 4 * d + g) + 8 * lg) =
-                    make_uint2(pack2<E>(o[d][4 * g] * inv, o[d][4 * g + 1] * inv),
-                               pack2<E>(o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv));
+                    make_uint2(pack2<E>(result(o[d][4 * g]), result(o[d][4 * g + 1])),
+                               pack2<E>(result(o[d][4 * g + 2]), result(o[d][4 * g + 3])));
         __builtin_amdgcn_wave_barrier();
         const uint32_t q = lane % CPR;
 #pragma unroll

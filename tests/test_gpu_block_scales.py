@@ -112,3 +112,13 @@ def test_a_nan_v_scale(torch_cuda, backend, n, lens, bucket, dtype):
     sees = np.concatenate([lens[0] - (n - 1 - np.arange(n)), np.zeros(n, int)]) > 16 * block
     assert np.array_equal(got[~sees], plain[~sees]) and np.array_equal(got[:, 2:], clean[:, 2:])
     assert np.isnan(decode(got[sees][:, :2], dtype)).all()
+
+
+@pytest.mark.parametrize("dtype", [DTYPE_BF16, DTYPE_F32])
+@pytest.mark.parametrize("exponent", [-126, -110, 100])
+@pytest.mark.parametrize("n,lens,bucket", FORMS)
+def test_v_scales_at_the_ends_of_f32(torch_cuda, backend, n, lens, bucket, exponent, dtype):
+    """2^-126 is the least scale that KvBlockAppend writes."""
+    c = make(np.random.default_rng(200 + exponent), n, lens, bucket, dtype)
+    c["vs"][:] = 2.0 ** exponent
+    check(run_blocks(torch_cuda, backend, c), c)
