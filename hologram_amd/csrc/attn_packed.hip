@@ -185,7 +185,7 @@ __device__ __forceinline__ void packed_tile(const AttnPackedArgs &a, const float
     // are rescaled only where a row passes that
     auto rescale = [&](float mt) __attribute__((always_inline)) {
         if (__any(mt > m + kLag)) {
-            const float mn = fmaxf(m, mt);
+            const float mn = mt > m + kLag ? mt : m;   // (the other rows' bits stay as they are)
             const float al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
             l *= al;
 #pragma unroll
