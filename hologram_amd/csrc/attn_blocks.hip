@@ -1371,6 +1371,11 @@ size_t attn_blocks_scratch_bytes(const AttnBlocksArgs &a) {
     return (uint64_t(few_places(a)) * a.Hkv + kShares) * kUnit * (padded(a.D) + 2) * 4;
 }
 
+uint64_t attn_blocks_threads(const AttnBlocksArgs &a) {
+    if (!matrix_applies(a)) return (uint64_t(a.pb.tokens) * a.H + 3) / 4 * 256;
+    return uint64_t(few_rows(a) ? few_places(a) : chunk_places(a)) * a.Hkv * 256;
+}
+
 hipError_t launch_attn_blocks(const AttnBlocksArgs &a, void *scratch, hipStream_t stream) {
     const float mul = kLog2e / a.score_scale;
     if (matrix_applies(a) && !few_rows(a)) {

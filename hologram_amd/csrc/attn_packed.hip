@@ -553,18 +553,20 @@ bool tiles_apply(const AttnPackedArgs &a) {
            at16(a.q) && at16(a.k) && at16(a.v) && at16(a.out) && far < (1u << 23);
 }
 
+uint32_t places_of(const AttnPackedArgs &a, uint32_t rows) {
+    return uint32_t(uint64_t(a.pb.tokens) * (a.H / a.Hkv) / rows) + a.pb.batch;
+}
+
 template <class E>
 void launch_tiles(const AttnPackedArgs &a, float mul, hipStream_t stream) {
-    const uint32_t G = a.H / a.Hkv;
-    const uint32_t places = uint32_t(uint64_t(a.pb.tokens) * G / kRows) + a.pb.batch, grid = places * a.Hkv;
+    const uint32_t places = places_of(a, kRows), grid = places * a.Hkv;
     if (a.D <= 64) packed_tile_kernel<E, 64><<<grid, 256, 0, stream>>>(a, mul, places);
     else if (a.D <= 128) packed_tile_kernel<E, 128><<<grid, 256, 0, stream>>>(a, mul, places);
     else packed_tile_kernel<E, 256><<<grid, 256, 0, stream>>>(a, mul, places);
 }
 
 void launch_f32(const AttnPackedArgs &a, float mul, hipStream_t stream) {
-    const uint32_t G = a.H / a.Hkv;
-    const uint32_t places = uint32_t(uint64_t(a.pb.tokens) * G / kRows32) + a.pb.batch, grid = places * a.Hkv;
+    const uint32_t places = places_of(a, kRows32), grid = places * a.Hkv;
     if (a.D <= 64) packed_f32_kernel<64, 64, 4><<<grid, 256, 0, stream>>>(a, mul, places);
     else if (a.D <= 96) packed_f32_kernel<128, 96, 4><<<grid, 256, 0, stream>>>(a, mul, places);
     else if (a.D <= 128) packed_f32_kernel<128, 128, 4><<<grid, 256, 0, stream>>>(a, mul, places);
@@ -614,6 +616,12 @@ void launch_rows(const AttnPackedArgs &a, float mul, hipStream_t stream) {
 }
 
 }  // namespace
+
+uint64_t attn_packed_threads(const AttnPackedArgs &a) {
+    if (!tiles_apply(a)) return (uint64_t(a.pb.tokens) * a.H + 3) / 4 * 256;
+    const bool f32 = a.dtype == 8;
+    return uint64_t(places_of(a, f32 ? kRows32 : kRows)) * a.Hkv * (f32 && a.D > 128 ? 128 : 256);
+}
 
 hipError_t launch_attn_packed(const AttnPackedArgs &a, hipStream_t stream) {
     const float mul = kLog2e / a.score_scale;

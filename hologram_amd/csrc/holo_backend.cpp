@@ -1527,6 +1527,13 @@ int strided(uint32_t tokens, uint64_t width, uint32_t *stride, uint64_t *span, c
     return HOLO_OK;
 }
 
+// A launch holds fewer than 2^32 threads.
+int one_launch(const char *op, uint64_t threads) {
+    if (threads >> 32)
+        return fail(HOLO_ERR_UNSUPPORTED_OP, std::string(op) + ": too many rows and heads for one launch");
+    return HOLO_OK;
+}
+
 // What the packed-batch calls ask of their sizes alike.
 int packed_shape(const char *op, uint32_t tokens, uint32_t batch, uint32_t heads, uint32_t hkv,
                  uint32_t head_dim, uint8_t dtype) {
@@ -1537,8 +1544,8 @@ int packed_shape(const char *op, uint32_t tokens, uint32_t batch, uint32_t heads
         return fail(HOLO_ERR_UNSUPPORTED_OP, std::string(op) + ": rows must be bf16, f16 or f32");
     if (head_dim > holo::kPackedMaxDim)
         return fail(HOLO_ERR_UNSUPPORTED_OP, std::string(op) + ": head_dim above 1024");
-    // a launch holds at most a workgroup for each row and head, and two for each
-    // sequence and head
+    // the kernels count rows and heads, and two places for each sequence and head, in
+    // 32 bits
     if ((uint64_t(tokens) + 2 * uint64_t(batch)) * heads > 0x3fffffffull)
         return fail(HOLO_ERR_UNSUPPORTED_OP, std::string(op) + ": (tokens + 2 batch) * heads above 2^30");
     return HOLO_OK;
@@ -1568,13 +1575,14 @@ int do_attn_packed(holo_backend *be, const SlotTable &st, const holo_attention_p
     if (!aligned(rv[0], es) || !aligned(rv[1], es) || !aligned(rv[2], es) || !aligned(out, es) ||
         !aligned(rv[3], 4))
         return fail(HOLO_ERR_UNSUPPORTED_OP, std::string(op) + ": operands must be element-aligned");
-    if (!be) return HOLO_OK;
-    OnDevice on(be->device);
-    a.pb = {reinterpret_cast<const uint32_t *>(rv[3].base), c.tokens, c.batch, be->dev_err};
+    a.pb = {reinterpret_cast<const uint32_t *>(rv[3].base), c.tokens, c.batch, be ? be->dev_err : nullptr};
     a.q = rv[0].base, a.k = rv[1].base, a.v = rv[2].base, a.out = out.base;
     a.H = c.heads, a.Hkv = hkv, a.D = c.head_dim;
     a.score_scale = score_divisor(c.head_dim, c.scale_bits);
     a.dtype = c.dtype;
+    HOLO_TRY(one_launch(op, holo::attn_packed_threads(a)));
+    if (!be) return HOLO_OK;
+    OnDevice on(be->device);
     return launched(holo::launch_attn_packed(a, be->stream), op);
 }
 
@@ -1620,6 +1628,14 @@ int do_kv_block_append(holo_backend *be, const SlotTable &st, const holo_kv_bloc
     if (!aligned(rv[0], es) || !aligned(rv[1], 4) || !aligned(rv[2], 4) || !aligned(os, 4) ||
         (!in_place && !aligned(rv[4], 4)))
         return fail(HOLO_ERR_UNSUPPORTED_OP, std::string(op) + ": operands must be element-aligned");
+    a.pb = {reinterpret_cast<const uint32_t *>(rv[1].base), c.tokens, c.batch, be ? be->dev_err : nullptr};
+    a.nw = rv[0].base;
+    a.pos = reinterpret_cast<const uint32_t *>(rv[2].base);
+    a.cache = reinterpret_cast<int8_t *>(oq.base);
+    a.scales = reinterpret_cast<float *>(os.base);
+    a.Hkv = c.kv_heads, a.bucket = c.bucket_rows, a.block = c.block_rows, a.D = c.head_dim;
+    a.dtype = c.dtype;
+    HOLO_TRY(one_launch(op, holo::kv_block_append_threads(a)));
     if (!be) return HOLO_OK;
     OnDevice on(be->device);
     if (!in_place && qbytes) {
@@ -1627,13 +1643,6 @@ int do_kv_block_append(holo_backend *be, const SlotTable &st, const holo_kv_bloc
         HOLO_TRY(launched(holo::launch_copy_bytes(rv[4].base, os.base, sbytes, be->stream), op));
     }
     if (c.tokens == 0 || c.batch == 0) return HOLO_OK;
-    a.pb = {reinterpret_cast<const uint32_t *>(rv[1].base), c.tokens, c.batch, be->dev_err};
-    a.nw = rv[0].base;
-    a.pos = reinterpret_cast<const uint32_t *>(rv[2].base);
-    a.cache = reinterpret_cast<int8_t *>(oq.base);
-    a.scales = reinterpret_cast<float *>(os.base);
-    a.Hkv = c.kv_heads, a.bucket = c.bucket_rows, a.block = c.block_rows, a.D = c.head_dim;
-    a.dtype = c.dtype;
     return launched(holo::launch_kv_block_append(a, be->stream), op);
 }
 
@@ -1668,9 +1677,7 @@ int do_attn_i8_blocks(holo_backend *be, const SlotTable &st, const holo_attentio
     if (!aligned(rv[0], es) || !aligned(out, es) || !aligned(rv[3], 4) || !aligned(rv[4], 4) ||
         !aligned(rv[5], 4) || !aligned(rv[6], 4))
         return fail(HOLO_ERR_UNSUPPORTED_OP, std::string(op) + ": operands must be element-aligned");
-    if (!be) return HOLO_OK;
-    OnDevice on(be->device);
-    a.pb = {reinterpret_cast<const uint32_t *>(rv[5].base), c.tokens, c.batch, be->dev_err};
+    a.pb = {reinterpret_cast<const uint32_t *>(rv[5].base), c.tokens, c.batch, be ? be->dev_err : nullptr};
     a.q = rv[0].base, a.out = out.base;
     a.kq = reinterpret_cast<const int8_t *>(rv[1].base);
     a.vq = reinterpret_cast<const int8_t *>(rv[2].base);
@@ -1680,6 +1687,9 @@ int do_attn_i8_blocks(holo_backend *be, const SlotTable &st, const holo_attentio
     a.H = c.heads, a.Hkv = hkv, a.bucket = c.bucket_rows, a.block = c.block_rows, a.D = c.head_dim;
     a.score_scale = score_divisor(c.head_dim, c.scale_bits);
     a.dtype = c.dtype;
+    HOLO_TRY(one_launch(op, holo::attn_blocks_threads(a)));
+    if (!be) return HOLO_OK;
+    OnDevice on(be->device);
     HOLO_TRY(ensure_scratch(be, holo::attn_blocks_scratch_bytes(a), op));
     return launched(holo::launch_attn_blocks(a, be->scratch, be->stream), op);
 }
@@ -1692,7 +1702,10 @@ int do_logits(holo_backend *be, const SlotTable &st, const holo_logits_process_c
     if (c.rows == 0 || c.cols == 0) return HOLO_OK;
     if (c.history_len > holo::kLogitsMaxHistory || c.biases > holo::kLogitsMaxBiases)
         return fail(HOLO_ERR_UNSUPPORTED_OP, "logits_process: history_len above 524287 or biases above 4095");
-    if (c.cols > 0x7fffffffu || uint64_t(c.rows) * ((uint64_t(c.cols) + 4095) / 4096) > 0x7fffffffull)
+    holo::LogitsArgs a;
+    a.rows = c.rows, a.cols = c.cols, a.history_len = c.history_len, a.biases = c.biases;
+    a.dtype = c.dtype;
+    if (c.cols > 0x7fffffffu || holo::logits_threads(a) >> 32)
         return fail(HOLO_ERR_UNSUPPORTED_OP, "logits_process: too many rows and columns for one launch");
     const uint64_t es = dtype_size(c.dtype), n = uint64_t(c.rows) * c.cols * es;
     const bool hist = c.history_len != 0, bias = c.biases != 0;
@@ -1728,7 +1741,6 @@ int do_logits(holo_backend *be, const SlotTable &st, const holo_logits_process_c
             return fail(HOLO_ERR_UNSUPPORTED_OP, std::string(op) + ": operands must be element-aligned");
     if (!be) return HOLO_OK;
     OnDevice on(be->device);
-    holo::LogitsArgs a;
     a.logits = rv[0].base, a.out = out.base;
     a.history = hist ? reinterpret_cast<const int32_t *>(rv[1].base) : nullptr;
     a.spans = reinterpret_cast<const uint32_t *>(rv[2].base);
@@ -1736,8 +1748,6 @@ int do_logits(holo_backend *be, const SlotTable &st, const holo_logits_process_c
     a.bias_ids = bias ? reinterpret_cast<const int32_t *>(rv[4].base) : nullptr;
     a.bias_values = reinterpret_cast<const float *>(rv[5].base);
     a.mask = mask ? reinterpret_cast<const uint32_t *>(rv[6].base) : nullptr;
-    a.rows = c.rows, a.cols = c.cols, a.history_len = c.history_len, a.biases = c.biases;
-    a.dtype = c.dtype;
     return launched(holo::launch_logits(a, be->stream), op);
 }
 

@@ -121,6 +121,7 @@ struct AttnPackedArgs {
     float score_scale;                // the divisor
     uint8_t dtype;
 };
+uint64_t attn_packed_threads(const AttnPackedArgs &a);   // of its largest launch
 hipError_t launch_attn_packed(const AttnPackedArgs &a, hipStream_t stream);
 // kv_blocks.hip — int8 append with one power-of-two scale a block of rows, in
 // place; bit 16 of *err for rows past the bucket.
@@ -133,6 +134,7 @@ struct KvBlockArgs {
     uint32_t Hkv, bucket, block, D, stride;
     uint8_t dtype;
 };
+uint64_t kv_block_append_threads(const KvBlockArgs &a);
 hipError_t launch_kv_block_append(const KvBlockArgs &a, hipStream_t stream);
 // attn_blocks.hip — attention of a packed batch over that cache. `scratch`
 // holds the split keys' partials, attn_blocks_scratch_bytes() of them.
@@ -148,6 +150,7 @@ struct AttnBlocksArgs {
     uint8_t dtype;
 };
 size_t attn_blocks_scratch_bytes(const AttnBlocksArgs &a);
+uint64_t attn_blocks_threads(const AttnBlocksArgs &a);
 hipError_t launch_attn_blocks(const AttnBlocksArgs &a, void *scratch, hipStream_t stream);
 // logits.hip — penalties, biases and a mask on logits. Null history, bias_ids
 // and mask: none.
@@ -164,6 +167,7 @@ struct LogitsArgs {
     uint32_t rows, cols, history_len, biases;
     uint8_t dtype;
 };
+uint64_t logits_threads(const LogitsArgs &a);
 hipError_t launch_logits(const LogitsArgs &a, hipStream_t stream);
 
 // quant.hip — MatMulDequant's output-major W8A8 GEMM (f32 A quantized per

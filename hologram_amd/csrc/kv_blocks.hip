@@ -161,9 +161,11 @@ __global__ __launch_bounds__(kThreads) void append_kernel(KvBlockArgs a) {
     }
 }
 
+uint32_t blocks_of(const KvBlockArgs &a) { return (a.pb.tokens / a.block + 2 * a.pb.batch) * a.Hkv; }
+
 template <class E>
 void launch(const KvBlockArgs &a, hipStream_t stream) {
-    const dim3 grid((a.pb.tokens / a.block + 2 * a.pb.batch) * a.Hkv);
+    const dim3 grid(blocks_of(a));
     const bool wide = a.D % 8 == 0 && a.stride * sizeof(typename E::T) % 16 == 0 &&
                       reinterpret_cast<uintptr_t>(a.nw) % 16 == 0 && reinterpret_cast<uintptr_t>(a.cache) % 8 == 0;
     if (wide) append_kernel<E, true><<<grid, kThreads, 0, stream>>>(a);
@@ -171,6 +173,8 @@ void launch(const KvBlockArgs &a, hipStream_t stream) {
 }
 
 }  // namespace
+
+uint64_t kv_block_append_threads(const KvBlockArgs &a) { return uint64_t(blocks_of(a)) * kThreads; }
 
 hipError_t launch_kv_block_append(const KvBlockArgs &a, hipStream_t stream) {
     if (a.dtype == 7) launch<Bf16>(a, stream);

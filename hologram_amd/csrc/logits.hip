@@ -184,17 +184,24 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a, uint32_t
     }
 }
 
+// Workgroups a row; its columns begin up to 15 bytes into the first one's.
+uint32_t chunks_of(const LogitsArgs &a) {
+    const uint32_t kV = a.dtype == 8 ? 4 : 8;
+    return uint32_t((uint64_t(a.cols) + kV - 1 + kCols - 1) / kCols);
+}
+
 template <class E>
 void launch(const LogitsArgs &a, hipStream_t stream) {
-    const uint32_t kV = 16 / sizeof(typename E::T);
     // the logits and the result as far past 16 bytes as each other
     const bool wide = (reinterpret_cast<uintptr_t>(a.logits) - reinterpret_cast<uintptr_t>(a.out)) % 16 == 0;
     const size_t lds = size_t(a.biases) * 8;
-    const uint32_t chunks = uint32_t((uint64_t(a.cols) + kV - 1 + kCols - 1) / kCols);
+    const uint32_t chunks = chunks_of(a);
     logits_kernel<E><<<a.rows * chunks, kThreads, lds, stream>>>(a, chunks, wide);
 }
 
 }  // namespace
+
+uint64_t logits_threads(const LogitsArgs &a) { return uint64_t(a.rows) * chunks_of(a) * kThreads; }
 
 hipError_t launch_logits(const LogitsArgs &a, hipStream_t stream) {
     if (a.dtype == 7) launch<Bf16>(a, stream);

@@ -426,7 +426,11 @@ typedef struct holo_attention_i8_rows_call {
  * sequence (before starts[0], from starts[batch] on) take no part and their
  * output rows stay as they were. Offsets that decrease or pass `tokens` are
  * reported (SlotOutOfRange) by the next holo_hip_synchronize; no access leaves
- * the operands, and the call's outputs are to be discarded. */
+ * the operands, and the call's outputs are to be discarded. (tokens + 2 batch) *
+ * heads is at most 2^30, and a call of these or of 129 whose launch would hold
+ * 2^32 threads is refused (UnsupportedOp). Below that whatever the form: tokens *
+ * heads < 2^26 with batch * kv_heads <= 2^23 (126, 128), (tokens / block_rows + 2
+ * batch) * kv_heads < 2^24 (127), rows * (cols / 8192 + 2) < 2^23 (129). */
 
 /* New (tag 126): causal grouped-query attention of a packed batch of prompts
  * over their own K and V, all of `dtype` (bf16, f16 or f32). q is [tokens,
