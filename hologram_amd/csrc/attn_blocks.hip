@@ -67,6 +67,13 @@ __device__ __forceinline__ float weight_factor(float v, int ve) {
     const float f = ldexpf(v, 7 - ve);
     return fabsf(f) == INFINITY ? copysignf(0x1p100f, f) : f;
 }
+// A product as it is rounded to f32: the conversion to f16 behind it would else take the
+// product unrounded, and its two parts, of which one does and the other not, be a step of
+// f16 apart.
+__device__ __forceinline__ float rounded(float w) {
+    asm volatile("" : "+v"(w));
+    return w;
+}
 // What a weight of at most 2^15 leaves over its f16, as f16; nothing of an infinite one's.
 __device__ __forceinline__ float left_over(float w, float hi) { return fminf(fmaxf(w - hi, -16.0f), 16.0f); }
 
@@ -308,7 +315,7 @@ __device__ __forceinline__ void few_segment(const Blocks &k, const Place &at, ui
             for (int i = 0; i < 4; ++i) {
                 const float p = __builtin_amdgcn_exp2f(s[4 * h + i] - ref);
                 st.l += p;
-                w[4 * h + i] = p * f;
+                w[4 * h + i] = kF32 ? rounded(p * f) : p * f;
                 hi[4 * h + i] = _Float16(w[4 * h + i]);
                 if constexpr (kF32) lo[4 * h + i] = _Float16(left_over(w[4 * h + i], float(hi[4 * h + i])));
             }
@@ -881,7 +888,7 @@ __device__ __forceinline__ void chunk_segment(const Chunk &k, const Place &at, u
         for (int e = 0; e < 2; ++e) {
             const float p = __builtin_amdgcn_exp2f(fmaf(s[i >> 3][2 * (i & 7) + e], c[g], -ref));
             l += p;
-            w[e] = p * f[g];
+            w[e] = kF32 ? rounded(p * f[g]) : p * f[g];
         }
         uint32_t hi = pack2<F16>(w[0], w[1]);
         if constexpr (kF32) {

@@ -122,3 +122,40 @@ def test_v_scales_at_the_ends_of_f32(torch_cuda, backend, n, lens, bucket, expon
     c = make(np.random.default_rng(200 + exponent), n, lens, bucket, dtype)
     c["vs"][:] = 2.0 ** exponent
     check(run_blocks(torch_cuda, backend, c), c)
+
+
+@pytest.mark.parametrize("B,n,H,Hkv,bucket", [
+    (20, 4, 64, 8, 128),          # a unit a workgroup
+    (100, 2, 64, 8, 1040),        # shares of units
+    (16, 128, 16, 2, 128),        # row tiles whole
+    (2, 200, 16, 2, 4000),        # row tiles cut
+])
+def test_f32_weights_keep_both_their_parts(torch_cuda, backend, B, n, H, Hkv, bucket):
+    """f32 rows against a bound without the scores' sums: q has one element, so a score is a product.
+    The 16-bit halves of a weight make it up to 2^-22 of itself, in every one of many rows whose few
+    largest weights are most of their sum."""
+    rng = np.random.default_rng(B + n)
+    D, dtype = 64, DTYPE_F32
+    c = blocks_case(rng, [n] * B, [min(bucket, 128 + 7 * b) for b in range(B)] if bucket != 4000 else [4000, 900],
+                    H, Hkv, D, bucket, 16, dtype, "any")
+    c["q"][:] = 0.0
+    c["q"][:, ::D] = rng.standard_normal((n * B, H)) * 30
+    got = run_blocks(torch_cuda, backend, c)
+    q = c["q"].astype(np.float64).reshape(B, n, Hkv, H // Hkv, D)[..., 0]
+    got = got.astype(np.float64).reshape(B, n, Hkv, H // Hkv, D)
+    of = np.arange(bucket) // 16
+    for b in range(B):
+        keys = int(c["lens"][b]) - (n - 1 - np.arange(n))
+        k, v = (c[x][b].astype(np.float64) * c[x + "s"][b][:, of, None].astype(np.float64) for x in "kv")
+        for kh in range(Hkv):
+            s = q[b, :, kh, :, None] * k[kh, :, 0] / np.sqrt(D)
+            s = np.where(np.arange(bucket) < keys[:, None, None], s, -np.inf)
+            p = np.exp(s - s.max(2, keepdims=True))
+            want = p @ v[kh] / p.sum(2, keepdims=True)
+            # the score's five roundings; exp2's argument and result, a weight's product and second
+            # part; the sums of keys that are not negligible, in f32, each by each
+            size = np.abs(np.where(np.isfinite(s), s, 0)).max(2, keepdims=True)
+            many = (p > 2.0 ** -24).sum(2, keepdims=True)
+            tol = (2 * 5 * 2.0 ** -24 * size + 2.0 ** -21 + 2 * (many + 8) * 2.0 ** -24) * np.abs(v[kh]).max()
+            err = np.abs(got[b, :, kh] - want)
+            assert (err <= tol).all(), (b, kh, float((err / tol).max()))
