@@ -52,8 +52,9 @@ __device__ __forceinline__ uint32_t visible_keys(int64_t len, uint32_t n, uint32
 // lengths; a unit that is cut leaves partials, which merge_kernel joins in order (a
 // launch of its own: partials pass between XCDs' L2s at its boundary).
 // Bound by the cache's bytes: 32 sequences of 512 to 32767 keys, 8 kv heads of 128 dims,
-// 528 MB, 106 us or 5.0 TB/s, merge_kernel 5 us of them; 128 of 8192 keys, 2.2 GB, 6.6 TB/s.
-// Short ones by their latency: 8 of 30 to 700 keys 9 us.
+// 528 MB, 106 us or 5.0 TB/s, merge_kernel 5 us of them, 108 us of f32 rows; 128 of 8192
+// keys, 2.2 GB, 6.6 TB/s. Short ones by their latency: 8 of 30 to 700 keys 9 us, up to three
+// rounds of a workgroup's 256 keys.
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 constexpr uint32_t kUnit = 16, kStep = 32, kQuad = 128, kOob = 1u << 30;   // past every plane, twice it too
@@ -599,14 +600,17 @@ __global__ __launch_bounds__(256) void merge_kernel(Blocks k) {
 // keys, past' what its rows see before their own to a multiple of 64, S = ceil(128 / G)
 // the tokens that a unit spans at most, and kStart what starting and ending a unit
 // takes in keys' time (14 to 17 us of head_dim 128 against 2.3 a 64-key tile with two
-// workgroups a CU; 4 chunks of 301 to 1024 rows 188 us with 192 keys, 181 with 384), so that a sequence's cost and the unit at a place of the line
-// are closed forms. A unit's keys begin at its place kStart; cuts fall on tiles. A unit
+// workgroups a CU; 4 chunks of 301 to 1024 rows behind up to 6000 keys with 192, 384 and 768
+// of them: 171, 165 and 179 us, 111, 117 and 129 of 64 dims, 434, 372 and 401 of 256, 287,
+// 298 and 322 of f32 rows), so that a sequence's cost and the unit at a place of the line are
+// closed forms. A unit's keys begin at its place kStart; cuts fall on tiles. A unit
 // that is cut leaves partials for join_kernel.
-// Bound by the vector units beside the matrix cores (440 vector instructions a wavefront
+// Bound by the vector units beside the matrix cores (450 vector instructions a wavefront
 // and tile, a third of them the widening and the scales, against 32 matrix instructions:
-// those are busy 28% of the cycles) and by the units' starts: 4 chunks of 301 to 1024 rows
-// behind up to 6000 keys, 32 heads on 8 of 128 dims, 171 us, 0.51 PFLOP/s, join_kernel 15
-// to 20 us of them; one of 1024 rows 0.60. A wavefront a row (below) took 793 us.
+// those are busy 29% of the cycles) and by the units' starts: 4 chunks of 301 to 1024 rows
+// behind up to 6000 keys, 32 heads on 8 of 128 dims, 165 us, 0.53 PFLOP/s, join_kernel 15
+// to 20 us of them; one of 1024 rows behind 4000 keys 0.57; f32 rows, whose every product is
+// two, 298 us. A wavefront a row (below) took 793 us.
 constexpr uint32_t kRows = 128, kKeys = 64, kManyRounds = 4, kMinKeys = 256, kStart = 384;
 
 struct Chunk {
@@ -1090,9 +1094,13 @@ __device__ __forceinline__ uint64_t keys_of(uint64_t total, uint32_t shares) {
 
 // Whether the row tiles go whole to workgroups. Whole, the GPU waits for the last long
 // one, about half of its time; cut, each share starts one tile more and the partials are
-// joined. 4 sequences of 301 to 1024 rows, the longest tile's keys 1.7 for each tile:
-// 43 us whole, 73 cut; behind up to 6000 keys, 11 for each: 258 and 164; 16 of 200 to
-// 500 rows behind up to 3000, 2.5 for each: 121 and 156; 8, 4.7 for each: 117 and 96.
+// joined. In us whole and cut, of 128 dims, 64, 256 and 128 of f32 rows: 4 sequences of 301
+// to 1024 rows, the longest tile's keys 1.7 for each tile: 45 and 76, 34 and 52, 100 and
+// 146, 79 and 106; behind up to 6000 keys, 11 for each: 263 and 164, 195 and 117, 420 and
+// 369, 333 and 298; 8 of 200 to 500 rows behind up to 3000, 4.7 for each: 120 and 94, 89 and
+// 68, 225 and 200, 182 and 159; 16, 2.5 for each: 126 and 160, 95 and 117 (256 dims and f32
+// are many times what the GPU holds). One of 1024 rows behind 4000, 20 for each: 159 and
+// 131, 120 and 91, but 272 and 292, 215 and 237.
 // The threads of a workgroup call it; all get the answer.
 __device__ __forceinline__ bool tiles_whole(const AttnBlocksArgs &a, uint32_t (&most)[4], uint32_t (&many)[4]) {
     uint32_t keys = 0, units = 0;
@@ -1273,7 +1281,10 @@ bool few_direct(const AttnBlocksArgs &a) {
 // At most 16 packed rows a sequence on average, 32 where no shares are cut: 32 sequences of
 // 4000 keys, 58 us against the tiles' 94 with 16 rows, 80 and 95 with 32, 157 and 115 with
 // 64, but 61 and 42 with 32 rows and 1 to 4000 keys; of 900 keys, 32 rows, 4 and 16
-// sequences 17 and 32 us against 23 and 35.
+// sequences 17 and 32 us against 23 and 35. An average: the lengths are on the device. Empty
+// sequences count (256 rows behind 4096 keys 54 us alone, 61 beside 63 of them), and rows of
+// both kinds in one call take one form: 64 decode rows over 8192 keys 169 us, a chunk of 512
+// rows 117, both in a call 443.
 bool few_rows(const AttnBlocksArgs &a) {
     const uint32_t rows = few_direct(a) ? 2 * kUnit : kUnit;
     return uint64_t(a.pb.tokens) * (a.H / a.Hkv) <= uint64_t(rows) * a.pb.batch;

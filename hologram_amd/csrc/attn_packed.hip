@@ -35,6 +35,12 @@ constexpr float kLog2e = 1.4426950408889634f;
 // V; late places, which see the most keys, go first. (All tiles of all sequences in
 // the order of what they see gained nothing: 24 sequences of 17 to 2000 rows 161
 // against 163 us, 60 of them 355 against 331.)
+// Bound by the matrix cores where sequences are long (one of 8192 rows, 32 heads on 8 of
+// 128 dims, 513 us, 1.07 PFLOP/s; of 96, 80 and 64 dims 485, 467 and 306: 80 and 96 are
+// multiplied as 128). Where they are short by a workgroup's start and end, 6.8 us beside
+// 2.0 us a 64-key step with two workgroups a CU (batches of equal sequences of 64 to 4096
+// rows fit that within 1%; below 128 rows the bytes bound too): 24 of 17 to 2000 rows 140
+// us, 37 of them starts and ends, 96 steps, 9% more of these than the visible pairs fill.
 // A masked key's weight is 0, and 0 times a V that is not finite is NaN: in a tile
 // that some row does not see to its end such elements are staged as 0, and then
 // added by the rows that see their keys (add_odd); the other rows' bits are what

@@ -44,9 +44,11 @@ struct Eight {
 // is wanted before its first byte: in the wide form (16-byte rows) a thread keeps its
 // eights of the rows in registers between the two, kHold of them, 64 rows of 128 dims;
 // what is past those it reads again. A power-of-two scale divides by its reciprocal,
-// exactly. Bound by the rows' bytes where they are many: 16 prompts of 100 to 1500 rows, 8
-// heads of 128 bf16, 17.6 MB in and 8.8 out, 11 us or 2.3 TB/s (31 us in the narrow form,
-// an element a thread); by the launch where each of 32 sequences has one, 4.6 us.
+// exactly. Bound by the rows' bytes where they are many: 32 prompts of 1500 rows, 8 heads of
+// 128 bf16, 98 MB in and 49 out, 29.5 us, 5.0 TB/s; by a launch and a workgroup's chain
+// (search, offsets, rows, barrier, store) where each of 32 sequences has one row, 4.8 us (an
+// empty launch, queued: 1.6). Between them both: 16 prompts of 100 to 1500 rows, 26 MB, 10 us,
+// 2.6 TB/s (31 us in the narrow form, an element a thread).
 constexpr uint32_t kHold = 4;
 template <class E, bool kWide>
 __global__ __launch_bounds__(kThreads) void append_kernel(KvBlockArgs a) {

@@ -20,7 +20,8 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 // column that shares its 64 lanes with one took longer than that. Bound by the logits' own
 // bytes, and by the gathering where many rows have long histories: 128 rows of 128000 bf16
 // with masks, biases and 4096 tokens of history each, 70 MB, 21 us or 3.3 TB/s; without
-// histories 14 us, 4.8 TB/s; one row 5 us, the launch's own time. 8192 columns read a row's
+// histories 14 us, 4.8 TB/s; one row 5 us, a workgroup's chain of history, barrier, copies
+// and listed columns (an empty launch, queued: 1.6). 8192 columns read a row's
 // history 16 times; 4096 and 256 threads, 32 times: 64 rows 13.3 us against 12.3, one row
 // the same; 16384 and 512 threads 25 against 22.
 constexpr uint32_t kCols = 8192, kThreads = kCols / 16, kList = 2048;

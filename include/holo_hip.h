@@ -437,11 +437,14 @@ typedef struct holo_attention_i8_rows_call {
  * heads, head_dim], k and v [tokens, kv_heads, head_dim], output [tokens, heads,
  * head_dim]. Row t of a sequence sees its rows 0..t, head h reads kv head h /
  * (heads / kv_heads): scores dot(q, k) / s with s as in DecodeAttentionValid,
- * f32 softmax, the result rounded to nearest. q_stride, k_stride and v_stride
- * are the elements from one token to the next (0: tight), so that q, k and v
- * may be views of one projection's output. What an invisible row holds, NaN and
- * infinity too, does not reach a result. kv_heads 0 means heads;
- * head_dim <= 1024. */
+ * f32 softmax, the result rounded to nearest. Scores, maxima and sums are f32; a
+ * weight of bf16 and f16 rows may be rounded once to the rows' type, to nearest,
+ * before it meets V (the softmax's sum takes it unrounded), of f32 rows not. Where
+ * |v| times a row's keys passes 2^119 the f32 sums may overflow. q_stride, k_stride
+ * and v_stride are the elements from one token to the next (0: tight), so that q,
+ * k and v may be views of one projection's output. What an invisible row holds,
+ * NaN and infinity too, does not reach a result, not its last bit. kv_heads 0
+ * means heads; head_dim <= 1024. */
 typedef struct holo_attention_packed_call {
     holo_buffer_ref q;
     holo_buffer_ref k;
@@ -494,10 +497,17 @@ typedef struct holo_kv_block_append_call {
  * least 0 and at most bucket_rows (lens u32 [batch], device-resident: the
  * visible length of the sequence's last row), so one row a sequence is a decode
  * step and many are a prompt's next chunk, whose own rows were appended before.
- * Scores, softmax and rounding as in 126; a row that sees no key is zeros. What
- * an invisible row or block scale holds does not reach a result. dtype (q,
- * output): bf16, f16 or f32; kv_heads 0 means heads; head_dim <= 1024;
- * bucket_rows * head_dim <= 2^30. Long buckets and many rows take scratch. */
+ * Scores, softmax and the result's rounding as in 126; a row that sees no key is
+ * zeros. What an invisible row or block scale holds does not reach a result. q may
+ * be held to 2^-22 of its row's largest element, and a weight times its V scale
+ * rounded to f16 (two f16 parts of f32 rows: 22 bits), no finer than 2^-32 of the
+ * largest |V scale| that the row sees: a block whose scale is below that may add
+ * nothing to the result, while its keys count in the softmax. |V| times a row's
+ * keys as in 126. A call takes one form for all its rows, chosen from tokens and
+ * batch as they are given: decode rows and a long chunk take less time in two
+ * calls than in one, and empty sequences count as short ones. dtype (q, output):
+ * bf16, f16 or f32; kv_heads 0 means heads; head_dim <= 1024; bucket_rows *
+ * head_dim <= 2^30. Long buckets and many rows take scratch. */
 typedef struct holo_attention_i8_blocks_call {
     holo_buffer_ref q;
     holo_buffer_ref k_cache;
