@@ -115,10 +115,10 @@ def test_a_nan_v_scale(torch_cuda, backend, n, lens, bucket, dtype):
 
 
 @pytest.mark.parametrize("dtype", [DTYPE_BF16, DTYPE_F32])
-@pytest.mark.parametrize("exponent", [-126, -110, 100])
+@pytest.mark.parametrize("exponent", [-140, -126, -110, 100])
 @pytest.mark.parametrize("n,lens,bucket", FORMS)
 def test_v_scales_at_the_ends_of_f32(torch_cuda, backend, n, lens, bucket, exponent, dtype):
-    """2^-126 is the least scale that KvBlockAppend writes."""
+    """2^-126 is the least scale that KvBlockAppend writes; 2^-140 a subnormal."""
     c = make(np.random.default_rng(200 + exponent), n, lens, bucket, dtype)
     c["vs"][:] = 2.0 ** exponent
     check(run_blocks(torch_cuda, backend, c), c)
