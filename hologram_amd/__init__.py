@@ -13,12 +13,14 @@ from .backend import (BackendError, DeviceWorkspace, DispatchError, HipBackend, 
                       validate)
 from .kernel_call import (DTYPE_BF16, DTYPE_E8CB, DTYPE_F16, DTYPE_F32, DTYPE_I4, DTYPE_I8,
                           DTYPE_I32, DTYPE_I64, DTYPE_U8, NO_BUFFER, SLOT_ABSENT, ArgMaxCall,
-                          AttentionI8BlocksCall, AttentionI8RowsCall, AttentionPackedCall,
-                          BinaryCall, BufferRef, DecodeAttentionCall,
+                          AttentionI8BlocksCall, AttentionI8RowsCall, AttentionI8SelectedCall,
+                          AttentionPackedCall, BinaryCall, BufferRef, DecodeAttentionCall,
                           DecodeAttentionI8Call, DecodeAttentionValidCall, DequantActivationCall,
-                          DequantizeCall, GatherCall, KernelCall, KvBlockAppendCall, KvCacheWriteCall,
-                          KvQuantAppendCall, LogitsProcessCall, MatMulActivationCall, MatMulAddActivationCall, MatMulAddCall,
-                          MatMulCall, MatMulDequantCall, NormCall, RoPECall, TransposeCall, LayoutCall,
+                          DequantizeCall, GatherCall, KernelCall, KvBlockAppendCall,
+                          KvBlockBoundsCall, KvBlockSelectCall, KvCacheWriteCall, KvQuantAppendCall,
+                          LogitsProcessCall, MatMulActivationCall, MatMulAddActivationCall, MatMulAddCall,
+                          MatMulCall, MatMulDequantCall, NormCall, QkNormRotaryCall, RoPECall, TransposeCall,
+                          LayoutCall,
                           UnaryCall, encode_calls, fused_activation, lut_act, mm_act_quant,
                           weight_layout)
 from .archive import ConstantEntry, HoloWriter, PortDescriptor, blake3
@@ -29,10 +31,10 @@ __all__ = [
     "ShapeMismatch", "SlotOutOfRange", "UnsupportedOp", "decode_call", "lut_table", "validate",
     "DTYPE_BF16", "DTYPE_E8CB", "DTYPE_F16", "DTYPE_F32", "DTYPE_I4", "DTYPE_I8", "DTYPE_I32",
     "DTYPE_I64", "DTYPE_U8", "NO_BUFFER", "SLOT_ABSENT", "ArgMaxCall", "AttentionI8BlocksCall",
-    "AttentionI8RowsCall", "AttentionPackedCall",
+    "AttentionI8RowsCall", "AttentionI8SelectedCall", "AttentionPackedCall",
     "BinaryCall", "BufferRef", "DecodeAttentionCall", "DecodeAttentionI8Call",
     "DecodeAttentionValidCall", "DequantActivationCall", "DequantizeCall", "GatherCall", "KernelCall", "KvCacheWriteCall",
-    "KvBlockAppendCall", "KvQuantAppendCall", "LogitsProcessCall", "MatMulActivationCall", "MatMulAddActivationCall", "MatMulAddCall",
+    "KvBlockAppendCall", "KvBlockBoundsCall", "KvBlockSelectCall", "QkNormRotaryCall", "KvQuantAppendCall", "LogitsProcessCall", "MatMulActivationCall", "MatMulAddActivationCall", "MatMulAddCall",
     "MatMulCall", "MatMulDequantCall", "NormCall", "RoPECall", "TransposeCall", "LayoutCall", "UnaryCall",
     "encode_calls", "fused_activation", "lut_act", "mm_act_quant", "weight_layout",
     "ConstantEntry", "HoloWriter", "PortDescriptor", "blake3", "HipSession",

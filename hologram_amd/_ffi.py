@@ -166,6 +166,48 @@ class LogitsProcessCallC(ctypes.Structure):
                 ctypes.c_uint8)]
 
 
+class QkNormRotaryCallC(ctypes.Structure):
+    _fields_ = [("q", BufferRefC), ("k", BufferRefC), ("q_gamma", BufferRefC),
+                ("k_gamma", BufferRefC), ("starts", BufferRefC), ("pos", BufferRefC),
+                ("freqs", BufferRefC), ("q_output", BufferRefC), ("k_output", BufferRefC),
+                ("tokens", ctypes.c_uint32), ("batch", ctypes.c_uint32), ("heads", ctypes.c_uint32),
+                ("kv_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32),
+                ("rotary_dim", ctypes.c_uint32), ("q_stride", ctypes.c_uint32),
+                ("k_stride", ctypes.c_uint32), ("epsilon_bits", ctypes.c_uint32),
+                ("magnitude_bits", ctypes.c_uint32), ("norms", ctypes.c_uint8),
+                ("interleaved", ctypes.c_uint8), ("dtype", ctypes.c_uint8)]
+
+
+class KvBlockBoundsCallC(ctypes.Structure):
+    _fields_ = [("cache", BufferRefC), ("starts", BufferRefC), ("pos", BufferRefC),
+                ("bounds", BufferRefC), ("output", BufferRefC), ("tokens", ctypes.c_uint32),
+                ("batch", ctypes.c_uint32), ("kv_heads", ctypes.c_uint32),
+                ("bucket_rows", ctypes.c_uint32), ("block_rows", ctypes.c_uint32),
+                ("head_dim", ctypes.c_uint32)]
+
+
+class KvBlockSelectCallC(ctypes.Structure):
+    _fields_ = [("q", BufferRefC), ("bounds", BufferRefC), ("k_scales", BufferRefC),
+                ("starts", BufferRefC), ("lens", BufferRefC), ("output", BufferRefC),
+                ("tokens", ctypes.c_uint32), ("batch", ctypes.c_uint32), ("heads", ctypes.c_uint32),
+                ("kv_heads", ctypes.c_uint32), ("bucket_rows", ctypes.c_uint32),
+                ("block_rows", ctypes.c_uint32), ("head_dim", ctypes.c_uint32),
+                ("q_stride", ctypes.c_uint32), ("top", ctypes.c_uint32),
+                ("keep_first", ctypes.c_uint32), ("keep_last", ctypes.c_uint32),
+                ("dtype", ctypes.c_uint8)]
+
+
+class AttentionI8SelectedCallC(ctypes.Structure):
+    _fields_ = [("q", BufferRefC), ("k_cache", BufferRefC), ("v_cache", BufferRefC),
+                ("k_scales", BufferRefC), ("v_scales", BufferRefC), ("blocks", BufferRefC),
+                ("starts", BufferRefC), ("lens", BufferRefC), ("output", BufferRefC),
+                ("tokens", ctypes.c_uint32), ("batch", ctypes.c_uint32), ("heads", ctypes.c_uint32),
+                ("kv_heads", ctypes.c_uint32), ("bucket_rows", ctypes.c_uint32),
+                ("block_rows", ctypes.c_uint32), ("head_dim", ctypes.c_uint32),
+                ("q_stride", ctypes.c_uint32), ("top", ctypes.c_uint32),
+                ("scale_bits", ctypes.c_uint32), ("dtype", ctypes.c_uint8)]
+
+
 class TransposeCallC(ctypes.Structure):
     _fields_ = [("input", BufferRefC), ("output", BufferRefC), ("rank", ctypes.c_uint8),
                 ("dims", ctypes.c_uint32 * 8), ("perm", ctypes.c_uint8 * 8),
@@ -218,7 +260,11 @@ class CallUnion(ctypes.Union):
                 ("layout", LayoutCallC), ("attn_packed", AttentionPackedCallC),
                 ("kv_block_append", KvBlockAppendCallC),
                 ("attn_i8_blocks", AttentionI8BlocksCallC),
-                ("logits_process", LogitsProcessCallC)]
+                ("logits_process", LogitsProcessCallC),
+                ("qk_norm_rotary", QkNormRotaryCallC),
+                ("kv_block_bounds", KvBlockBoundsCallC),
+                ("kv_block_select", KvBlockSelectCallC),
+                ("attn_i8_selected", AttentionI8SelectedCallC)]
 
 
 class KernelCallC(ctypes.Structure):

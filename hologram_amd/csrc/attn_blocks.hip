@@ -14,12 +14,6 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// Keys that row t of sequence b's n rows sees.
-__device__ __forceinline__ uint32_t visible_keys(int64_t len, uint32_t n, uint32_t t, uint32_t bucket) {
-    const int64_t v = len - int64_t(n - 1 - t);
-    return v < 0 ? 0u : v > int64_t(bucket) ? bucket : uint32_t(v);
-}
-
 // ---------------------------------------------------------- few-row form ----
 // Decode and drafts. Sixteen packed rows of a sequence and kv head (row r = token r /
 // G, head r % G) are a unit: the columns of the matrix instructions, which read each

@@ -1751,6 +1751,223 @@ int do_logits(holo_backend *be, const SlotTable &st, const holo_logits_process_c
     return launched(holo::launch_logits(a, be->stream), op);
 }
 
+// ------------------------------------------------------- QkNormRotary ----
+int do_qk_norm_rotary(holo_backend *be, const SlotTable &st, const holo_qk_norm_rotary_call &c) {
+    const char *op = "qk_norm_rotary";
+    if (c.tokens == 0 || c.batch == 0 || c.heads == 0 || c.head_dim == 0) return HOLO_OK;
+    const bool has_k = c.k.slot != HOLO_SLOT_ABSENT;
+    const uint32_t hkv = !has_k ? 0 : c.kv_heads == 0 ? c.heads : c.kv_heads;
+    HOLO_TRY(packed_shape(op, c.tokens, c.batch, c.heads, has_k ? hkv : 1, c.head_dim, c.dtype));
+    if (c.rotary_dim > c.head_dim)
+        return fail(HOLO_ERR_SHAPE_MISMATCH, "qk_norm_rotary: rotary_dim above head_dim");
+    if (c.rotary_dim % 2 != 0) return fail(HOLO_ERR_UNSUPPORTED_OP, "qk_norm_rotary: rotary_dim must be even");
+    if (c.norms > 3 || c.interleaved > 1)
+        return fail(HOLO_ERR_UNSUPPORTED_OP, "qk_norm_rotary: norms is 0 to 3, interleaved 0 or 1");
+    holo::QkNormRotaryArgs a;
+    a.eps = 1e-9f, a.magnitude = 1.0f;
+    if (c.epsilon_bits) memcpy(&a.eps, &c.epsilon_bits, 4);
+    if (c.magnitude_bits) memcpy(&a.magnitude, &c.magnitude_bits, 4);
+    if (!(a.eps > 0.0f) || std::isinf(a.eps))
+        return fail(HOLO_ERR_UNSUPPORTED_OP,
+                    "qk_norm_rotary: epsilon must be a positive finite f32 (0 selects the default)");
+    if (!(a.magnitude > 0.0f) || std::isinf(a.magnitude))
+        return fail(HOLO_ERR_UNSUPPORTED_OP, "qk_norm_rotary: magnitude must be a positive finite f32 (0 selects 1)");
+    const uint64_t es = dtype_size(c.dtype), D = c.head_dim;
+    a.stride[0] = c.q_stride, a.stride[1] = c.k_stride;
+    uint64_t span[2] = {0, 0};
+    HOLO_TRY(strided(c.tokens, c.heads * D, &a.stride[0], &span[0], op, "q"));
+    if (has_k) HOLO_TRY(strided(c.tokens, hkv * D, &a.stride[1], &span[1], op, "k"));
+    const bool norm_q = (c.norms & 1) && c.q_gamma.slot != HOLO_SLOT_ABSENT;
+    const bool norm_k = has_k && (c.norms & 2) && c.k_gamma.slot != HOLO_SLOT_ABSENT;
+    const bool turn = c.rotary_dim != 0;
+    // absent operands stand as q in the list of reads
+    holo_buffer_ref reads[7] = {c.q, has_k ? c.k : c.q, norm_q ? c.q_gamma : c.q, norm_k ? c.k_gamma : c.q,
+                                c.starts, turn ? c.pos : c.q, turn ? c.freqs : c.q};
+    View rv[7], oq, ok;
+    HOLO_TRY(split_borrow(st, reads, rv, 7, c.q_output, &oq, op));
+    if (has_k) {
+        HOLO_TRY(split_borrow(st, reads, rv, 7, c.k_output, &ok, op));
+        if (overlaps(oq, ok)) return fail(HOLO_ERR_SLOT_OUT_OF_RANGE, "qk_norm_rotary: the outputs overlap");
+    }
+    HOLO_TRY(need(rv[0], span[0] * es, c.q.slot, op, "q"));
+    HOLO_TRY(need(oq, uint64_t(c.tokens) * c.heads * D * es, c.q_output.slot, op, "q_output"));
+    HOLO_TRY(need(rv[4], (uint64_t(c.batch) + 1) * 4, c.starts.slot, op, "starts"));
+    if (has_k) {
+        HOLO_TRY(need(rv[1], span[1] * es, c.k.slot, op, "k"));
+        HOLO_TRY(need(ok, uint64_t(c.tokens) * hkv * D * es, c.k_output.slot, op, "k_output"));
+    }
+    if (norm_q) HOLO_TRY(need(rv[2], D * es, c.q_gamma.slot, op, "q_gamma"));
+    if (norm_k) HOLO_TRY(need(rv[3], D * es, c.k_gamma.slot, op, "k_gamma"));
+    if (turn) {
+        HOLO_TRY(need(rv[5], uint64_t(c.batch) * 4, c.pos.slot, op, "pos"));
+        HOLO_TRY(need(rv[6], uint64_t(c.rotary_dim / 2) * 4, c.freqs.slot, op, "freqs"));
+    }
+    if (!aligned(rv[0], es) || !aligned(oq, es) || !aligned(rv[1], es) || (has_k && !aligned(ok, es)) ||
+        !aligned(rv[2], es) || !aligned(rv[3], es) || !aligned(rv[4], 4) ||
+        (turn && (!aligned(rv[5], 4) || !aligned(rv[6], 4))))
+        return fail(HOLO_ERR_UNSUPPORTED_OP, std::string(op) + ": operands must be element-aligned");
+    a.pb = {reinterpret_cast<const uint32_t *>(rv[4].base), c.tokens, c.batch, be ? be->dev_err : nullptr};
+    a.x[0] = rv[0].base, a.x[1] = has_k ? rv[1].base : nullptr;
+    a.gamma[0] = norm_q ? rv[2].base : nullptr, a.gamma[1] = norm_k ? rv[3].base : nullptr;
+    a.out[0] = oq.base, a.out[1] = has_k ? ok.base : nullptr;
+    a.pos = turn ? reinterpret_cast<const uint32_t *>(rv[5].base) : nullptr;
+    a.freqs = turn ? reinterpret_cast<const float *>(rv[6].base) : nullptr;
+    a.H = c.heads, a.Hkv = hkv, a.D = c.head_dim, a.rot = c.rotary_dim;
+    a.norms = c.norms, a.interleaved = c.interleaved, a.dtype = c.dtype;
+    HOLO_TRY(one_launch(op, holo::qk_norm_rotary_threads(a)));
+    if (!be) return HOLO_OK;
+    OnDevice on(be->device);
+    return launched(holo::launch_qk_norm_rotary(a, be->stream), op);
+}
+
+// A cache's planes of blocks, within what the kernels count.
+int block_planes(const char *op, uint64_t planes, uint32_t bucket_rows, uint32_t block_rows) {
+    if (bucket_rows == 0 || block_rows == 0)
+        return fail(HOLO_ERR_UNSUPPORTED_OP, std::string(op) + ": bucket_rows and block_rows must be >= 1");
+    if (planes * bucket_rows > (uint64_t(1) << 50))
+        return fail(HOLO_ERR_UNSUPPORTED_OP, std::string(op) + ": a cache of more than 2^50 rows");
+    return HOLO_OK;
+}
+
+// ------------------------------------------------------ KvBlockBounds ----
+int do_kv_block_bounds(holo_backend *be, const SlotTable &st, const holo_kv_block_bounds_call &c) {
+    const char *op = "kv_block_bounds";
+    if (c.head_dim == 0 || c.kv_heads == 0)
+        return fail(HOLO_ERR_UNSUPPORTED_OP, "kv_block_bounds: kv_heads and head_dim must be >= 1");
+    HOLO_TRY(packed_shape(op, c.tokens, c.batch, c.kv_heads, c.kv_heads, c.head_dim, HOLO_DTYPE_F32));
+    const uint64_t D = c.head_dim, planes = uint64_t(c.batch) * c.kv_heads;
+    HOLO_TRY(block_planes(op, planes, c.bucket_rows, c.block_rows));
+    if (uint64_t(std::min(c.block_rows, c.bucket_rows)) * D > (uint64_t(1) << 30))
+        return fail(HOLO_ERR_UNSUPPORTED_OP, "kv_block_bounds: a block of more than 2^30 elements");
+    const uint64_t nb = (uint64_t(c.bucket_rows) + c.block_rows - 1) / c.block_rows;
+    const uint64_t bytes = planes * nb * 2 * D;
+    const bool in_place = c.output.slot == c.bounds.slot && c.output.offset == c.bounds.offset;
+    holo_buffer_ref reads[4] = {c.cache, c.starts, c.pos, c.bounds};
+    View rv[4], out;
+    HOLO_TRY(split_borrow(st, reads, rv, in_place ? 3 : 4, c.output, &out, op));
+    HOLO_TRY(need(rv[0], planes * c.bucket_rows * D, c.cache.slot, op, "cache"));
+    HOLO_TRY(need(rv[1], (uint64_t(c.batch) + 1) * 4, c.starts.slot, op, "starts"));
+    HOLO_TRY(need(rv[2], uint64_t(c.batch) * 4, c.pos.slot, op, "pos"));
+    if (!in_place) HOLO_TRY(need(rv[3], bytes, c.bounds.slot, op, "bounds"));
+    HOLO_TRY(need(out, bytes, c.output.slot, op, "output"));
+    if (!aligned(rv[1], 4) || !aligned(rv[2], 4))
+        return fail(HOLO_ERR_UNSUPPORTED_OP, std::string(op) + ": operands must be element-aligned");
+    holo::KvBoundsArgs a;
+    a.pb = {reinterpret_cast<const uint32_t *>(rv[1].base), c.tokens, c.batch, be ? be->dev_err : nullptr};
+    a.cache = reinterpret_cast<const int8_t *>(rv[0].base);
+    a.pos = reinterpret_cast<const uint32_t *>(rv[2].base);
+    a.bounds = reinterpret_cast<int8_t *>(out.base);
+    a.Hkv = c.kv_heads, a.bucket = c.bucket_rows, a.block = c.block_rows, a.D = c.head_dim;
+    HOLO_TRY(one_launch(op, holo::kv_bounds_threads(a)));
+    if (!be) return HOLO_OK;
+    OnDevice on(be->device);
+    if (!in_place && bytes) HOLO_TRY(launched(holo::launch_copy_bytes(rv[3].base, out.base, bytes, be->stream), op));
+    if (c.tokens == 0 || c.batch == 0) return HOLO_OK;
+    return launched(holo::launch_kv_bounds(a, be->stream), op);
+}
+
+// ------------------------------------------------------ KvBlockSelect ----
+int do_kv_block_select(holo_backend *be, const SlotTable &st, const holo_kv_block_select_call &c) {
+    const char *op = "kv_block_select";
+    if (c.tokens == 0 || c.batch == 0 || c.heads == 0 || c.head_dim == 0) return HOLO_OK;
+    const uint32_t hkv = c.kv_heads == 0 ? c.heads : c.kv_heads;
+    HOLO_TRY(packed_shape(op, c.tokens, c.batch, c.heads, hkv, c.head_dim, c.dtype));
+    const uint64_t es = dtype_size(c.dtype), D = c.head_dim, planes = uint64_t(c.batch) * hkv;
+    HOLO_TRY(block_planes(op, planes, c.bucket_rows, c.block_rows));
+    const uint64_t nb = (uint64_t(c.bucket_rows) + c.block_rows - 1) / c.block_rows;
+    // a score's whole number is counted in 32 bits, 127 * 128 an element at most
+    if (c.heads / hkv * D > (1u << 17))
+        return fail(HOLO_ERR_UNSUPPORTED_OP, "kv_block_select: heads / kv_heads * head_dim above 2^17");
+    if (nb > (1u << 20) || hkv * nb > (1u << 28))
+        return fail(HOLO_ERR_UNSUPPORTED_OP, "kv_block_select: more than 2^20 blocks a plane, or 2^28 a row's kv heads");
+    if (c.keep_last == 0)
+        return fail(HOLO_ERR_UNSUPPORTED_OP,
+                    "kv_block_select: keep_last must be >= 1 (the last block may hold later rows)");
+    if (c.top > (1u << 20)) return fail(HOLO_ERR_UNSUPPORTED_OP, "kv_block_select: top above 2^20");
+    if (uint64_t(c.keep_first) + c.keep_last > c.top)
+        return fail(HOLO_ERR_SHAPE_MISMATCH, "kv_block_select: keep_first + keep_last above top");
+    holo::KvSelectArgs a;
+    a.q_stride = c.q_stride;
+    uint64_t qn;
+    HOLO_TRY(strided(c.tokens, c.heads * D, &a.q_stride, &qn, op, "q"));
+    holo_buffer_ref reads[5] = {c.q, c.bounds, c.k_scales, c.starts, c.lens};
+    View rv[5], out;
+    HOLO_TRY(split_borrow(st, reads, rv, 5, c.output, &out, op));
+    HOLO_TRY(need(rv[0], qn * es, c.q.slot, op, "q"));
+    HOLO_TRY(need(rv[1], planes * nb * 2 * D, c.bounds.slot, op, "bounds"));
+    HOLO_TRY(need(rv[2], planes * nb * 4, c.k_scales.slot, op, "k_scales"));
+    HOLO_TRY(need(rv[3], (uint64_t(c.batch) + 1) * 4, c.starts.slot, op, "starts"));
+    HOLO_TRY(need(rv[4], uint64_t(c.batch) * 4, c.lens.slot, op, "lens"));
+    HOLO_TRY(need(out, uint64_t(c.tokens) * hkv * c.top * 4, c.output.slot, op, "output"));
+    if (!aligned(rv[0], es) || !aligned(rv[2], 4) || !aligned(rv[3], 4) || !aligned(rv[4], 4) || !aligned(out, 4))
+        return fail(HOLO_ERR_UNSUPPORTED_OP, std::string(op) + ": operands must be element-aligned");
+    a.pb = {reinterpret_cast<const uint32_t *>(rv[3].base), c.tokens, c.batch, be ? be->dev_err : nullptr};
+    a.q = rv[0].base;
+    a.bounds = reinterpret_cast<const int8_t *>(rv[1].base);
+    a.ks = reinterpret_cast<const float *>(rv[2].base);
+    a.lens = reinterpret_cast<const uint32_t *>(rv[4].base);
+    a.out = reinterpret_cast<int32_t *>(out.base);
+    a.H = c.heads, a.Hkv = hkv, a.bucket = c.bucket_rows, a.block = c.block_rows, a.D = c.head_dim;
+    a.top = c.top, a.first = c.keep_first, a.last = c.keep_last;
+    a.dtype = c.dtype;
+    HOLO_TRY(one_launch(op, holo::kv_select_threads(a)));
+    if (!be) return HOLO_OK;
+    OnDevice on(be->device);
+    HOLO_TRY(ensure_scratch(be, holo::kv_select_scratch_bytes(a), op));
+    return launched(holo::launch_kv_select(a, be->scratch, be->stream), op);
+}
+
+// ------------------------------------------------ AttentionI8Selected ----
+int do_attn_i8_selected(holo_backend *be, const SlotTable &st, const holo_attention_i8_selected_call &c) {
+    const char *op = "attention_i8_selected";
+    if (c.tokens == 0 || c.batch == 0 || c.heads == 0 || c.head_dim == 0) return HOLO_OK;
+    const uint32_t hkv = c.kv_heads == 0 ? c.heads : c.kv_heads;
+    HOLO_TRY(packed_shape(op, c.tokens, c.batch, c.heads, hkv, c.head_dim, c.dtype));
+    const uint64_t es = dtype_size(c.dtype), D = c.head_dim, planes = uint64_t(c.batch) * hkv;
+    HOLO_TRY(block_planes(op, planes, c.bucket_rows, c.block_rows));
+    if (c.bucket_rows * D > (uint64_t(1) << 30))
+        return fail(HOLO_ERR_UNSUPPORTED_OP, "attention_i8_selected: bucket_rows * head_dim above 2^30");
+    if (c.top == 0 || c.top > (1u << 20))
+        return fail(HOLO_ERR_UNSUPPORTED_OP, "attention_i8_selected: top must be 1 to 2^20");
+    const uint64_t nb = (uint64_t(c.bucket_rows) + c.block_rows - 1) / c.block_rows;
+    holo::AttnSelectedArgs s;
+    holo::AttnBlocksArgs &a = s.a;
+    a.q_stride = c.q_stride;
+    uint64_t qn;
+    HOLO_TRY(strided(c.tokens, c.heads * D, &a.q_stride, &qn, op, "q"));
+    holo_buffer_ref reads[8] = {c.q, c.k_cache, c.v_cache, c.k_scales, c.v_scales, c.starts, c.lens, c.blocks};
+    View rv[8], out;
+    HOLO_TRY(split_borrow(st, reads, rv, 8, c.output, &out, op));
+    HOLO_TRY(need(rv[0], qn * es, c.q.slot, op, "q"));
+    HOLO_TRY(need(rv[1], planes * c.bucket_rows * D, c.k_cache.slot, op, "k_cache"));
+    HOLO_TRY(need(rv[2], planes * c.bucket_rows * D, c.v_cache.slot, op, "v_cache"));
+    HOLO_TRY(need(rv[3], planes * nb * 4, c.k_scales.slot, op, "k_scales"));
+    HOLO_TRY(need(rv[4], planes * nb * 4, c.v_scales.slot, op, "v_scales"));
+    HOLO_TRY(need(rv[5], (uint64_t(c.batch) + 1) * 4, c.starts.slot, op, "starts"));
+    HOLO_TRY(need(rv[6], uint64_t(c.batch) * 4, c.lens.slot, op, "lens"));
+    HOLO_TRY(need(rv[7], uint64_t(c.tokens) * hkv * c.top * 4, c.blocks.slot, op, "blocks"));
+    HOLO_TRY(need(out, uint64_t(c.tokens) * c.heads * D * es, c.output.slot, op, "output"));
+    if (!aligned(rv[0], es) || !aligned(out, es) || !aligned(rv[3], 4) || !aligned(rv[4], 4) ||
+        !aligned(rv[5], 4) || !aligned(rv[6], 4) || !aligned(rv[7], 4))
+        return fail(HOLO_ERR_UNSUPPORTED_OP, std::string(op) + ": operands must be element-aligned");
+    a.pb = {reinterpret_cast<const uint32_t *>(rv[5].base), c.tokens, c.batch, be ? be->dev_err : nullptr};
+    a.q = rv[0].base, a.out = out.base;
+    a.kq = reinterpret_cast<const int8_t *>(rv[1].base);
+    a.vq = reinterpret_cast<const int8_t *>(rv[2].base);
+    a.ks = reinterpret_cast<const float *>(rv[3].base);
+    a.vs = reinterpret_cast<const float *>(rv[4].base);
+    a.lens = reinterpret_cast<const uint32_t *>(rv[6].base);
+    a.H = c.heads, a.Hkv = hkv, a.bucket = c.bucket_rows, a.block = c.block_rows, a.D = c.head_dim;
+    a.score_scale = score_divisor(c.head_dim, c.scale_bits);
+    a.dtype = c.dtype;
+    s.blocks = reinterpret_cast<const int32_t *>(rv[7].base), s.top = c.top;
+    HOLO_TRY(one_launch(op, holo::attn_selected_threads(s)));
+    if (!be) return HOLO_OK;
+    OnDevice on(be->device);
+    HOLO_TRY(ensure_scratch(be, holo::attn_selected_scratch_bytes(s), op));
+    return launched(holo::launch_attn_selected(s, be->scratch, be->stream), op);
+}
+
 int dispatch_impl(holo_backend *be, const SlotTable &st, const holo_kernel_call *call) {
     if (!call) return fail(HOLO_ERR_DISPATCH, "dispatch: null call");
     switch (call->tag) {
@@ -1794,6 +2011,10 @@ int dispatch_impl(holo_backend *be, const SlotTable &st, const holo_kernel_call 
         case HOLO_OP_KV_BLOCK_APPEND: return do_kv_block_append(be, st, call->u.kv_block_append);
         case HOLO_OP_ATTN_I8_BLOCKS: return do_attn_i8_blocks(be, st, call->u.attn_i8_blocks);
         case HOLO_OP_LOGITS_PROCESS: return do_logits(be, st, call->u.logits_process);
+        case HOLO_OP_QK_NORM_ROTARY: return do_qk_norm_rotary(be, st, call->u.qk_norm_rotary);
+        case HOLO_OP_KV_BLOCK_BOUNDS: return do_kv_block_bounds(be, st, call->u.kv_block_bounds);
+        case HOLO_OP_KV_BLOCK_SELECT: return do_kv_block_select(be, st, call->u.kv_block_select);
+        case HOLO_OP_ATTN_I8_SELECTED: return do_attn_i8_selected(be, st, call->u.attn_i8_selected);
         case HOLO_OP_TRANSPOSE: return do_transpose(be, st, call->u.transpose);
         case HOLO_OP_RESHAPE:
         case HOLO_OP_SLICE: return do_layout(be, st, call->tag, call->u.layout);
@@ -2177,6 +2398,93 @@ int decode_impl(const uint8_t *wire, size_t len, holo_kernel_call *out, size_t *
             c.cols = r.get<uint32_t>();
             c.history_len = r.get<uint32_t>();
             c.biases = r.get<uint32_t>();
+            c.dtype = r.get<uint8_t>();
+            break;
+        }
+        case HOLO_OP_QK_NORM_ROTARY: {  // field order of holo_qk_norm_rotary_call
+            auto &c = out->u.qk_norm_rotary;
+            c.q = r.buf();
+            c.k = r.buf();
+            c.q_gamma = r.buf();
+            c.k_gamma = r.buf();
+            c.starts = r.buf();
+            c.pos = r.buf();
+            c.freqs = r.buf();
+            c.q_output = r.buf();
+            c.k_output = r.buf();
+            c.tokens = r.get<uint32_t>();
+            c.batch = r.get<uint32_t>();
+            c.heads = r.get<uint32_t>();
+            c.kv_heads = r.get<uint32_t>();
+            c.head_dim = r.get<uint32_t>();
+            c.rotary_dim = r.get<uint32_t>();
+            c.q_stride = r.get<uint32_t>();
+            c.k_stride = r.get<uint32_t>();
+            c.epsilon_bits = r.get<uint32_t>();
+            c.magnitude_bits = r.get<uint32_t>();
+            c.norms = r.get<uint8_t>();
+            c.interleaved = r.get<uint8_t>();
+            c.dtype = r.get<uint8_t>();
+            break;
+        }
+        case HOLO_OP_KV_BLOCK_BOUNDS: {  // field order of holo_kv_block_bounds_call
+            auto &c = out->u.kv_block_bounds;
+            c.cache = r.buf();
+            c.starts = r.buf();
+            c.pos = r.buf();
+            c.bounds = r.buf();
+            c.output = r.buf();
+            c.tokens = r.get<uint32_t>();
+            c.batch = r.get<uint32_t>();
+            c.kv_heads = r.get<uint32_t>();
+            c.bucket_rows = r.get<uint32_t>();
+            c.block_rows = r.get<uint32_t>();
+            c.head_dim = r.get<uint32_t>();
+            break;
+        }
+        case HOLO_OP_KV_BLOCK_SELECT: {  // field order of holo_kv_block_select_call
+            auto &c = out->u.kv_block_select;
+            c.q = r.buf();
+            c.bounds = r.buf();
+            c.k_scales = r.buf();
+            c.starts = r.buf();
+            c.lens = r.buf();
+            c.output = r.buf();
+            c.tokens = r.get<uint32_t>();
+            c.batch = r.get<uint32_t>();
+            c.heads = r.get<uint32_t>();
+            c.kv_heads = r.get<uint32_t>();
+            c.bucket_rows = r.get<uint32_t>();
+            c.block_rows = r.get<uint32_t>();
+            c.head_dim = r.get<uint32_t>();
+            c.q_stride = r.get<uint32_t>();
+            c.top = r.get<uint32_t>();
+            c.keep_first = r.get<uint32_t>();
+            c.keep_last = r.get<uint32_t>();
+            c.dtype = r.get<uint8_t>();
+            break;
+        }
+        case HOLO_OP_ATTN_I8_SELECTED: {  // field order of holo_attention_i8_selected_call
+            auto &c = out->u.attn_i8_selected;
+            c.q = r.buf();
+            c.k_cache = r.buf();
+            c.v_cache = r.buf();
+            c.k_scales = r.buf();
+            c.v_scales = r.buf();
+            c.blocks = r.buf();
+            c.starts = r.buf();
+            c.lens = r.buf();
+            c.output = r.buf();
+            c.tokens = r.get<uint32_t>();
+            c.batch = r.get<uint32_t>();
+            c.heads = r.get<uint32_t>();
+            c.kv_heads = r.get<uint32_t>();
+            c.bucket_rows = r.get<uint32_t>();
+            c.block_rows = r.get<uint32_t>();
+            c.head_dim = r.get<uint32_t>();
+            c.q_stride = r.get<uint32_t>();
+            c.top = r.get<uint32_t>();
+            c.scale_bits = r.get<uint32_t>();
             c.dtype = r.get<uint8_t>();
             break;
         }

@@ -285,6 +285,41 @@ bool op_signature(const holo_kernel_call &c, uint16_t *opcode, uint8_t params[64
             op = 129;
             break;
         }
+        case HOLO_OP_QK_NORM_ROTARY: {
+            const auto &a = c.u.qk_norm_rotary;
+            s.u32(a.tokens).u32(a.batch).u32(a.heads).u32(a.kv_heads).u32(a.head_dim)
+                .u32(a.rotary_dim).u32(a.q_stride).u32(a.k_stride).u32(a.epsilon_bits)
+                .u32(a.magnitude_bits).u8(a.norms).u8(a.interleaved).u8(a.dtype);
+            p_views(&s, {a.q, a.k, a.q_gamma, a.k_gamma, a.starts, a.pos, a.freqs, a.q_output, a.k_output});
+            op = 130;
+            break;
+        }
+        case HOLO_OP_KV_BLOCK_BOUNDS: {
+            const auto &a = c.u.kv_block_bounds;
+            s.u32(a.tokens).u32(a.batch).u32(a.kv_heads).u32(a.bucket_rows).u32(a.block_rows)
+                .u32(a.head_dim);
+            p_views(&s, {a.cache, a.starts, a.pos, a.bounds, a.output});
+            op = 131;
+            break;
+        }
+        case HOLO_OP_KV_BLOCK_SELECT: {
+            const auto &a = c.u.kv_block_select;
+            s.u32(a.tokens).u32(a.batch).u32(a.heads).u32(a.kv_heads).u32(a.bucket_rows)
+                .u32(a.block_rows).u32(a.head_dim).u32(a.q_stride).u32(a.top).u32(a.keep_first)
+                .u32(a.keep_last).u8(a.dtype);
+            p_views(&s, {a.q, a.bounds, a.k_scales, a.starts, a.lens, a.output});
+            op = 132;
+            break;
+        }
+        case HOLO_OP_ATTN_I8_SELECTED: {
+            const auto &a = c.u.attn_i8_selected;
+            s.u32(a.tokens).u32(a.batch).u32(a.heads).u32(a.kv_heads).u32(a.bucket_rows)
+                .u32(a.block_rows).u32(a.head_dim).u32(a.q_stride).u32(a.top).u32(a.scale_bits)
+                .u8(a.dtype);
+            p_views(&s, {a.q, a.k_cache, a.v_cache, a.k_scales, a.v_scales, a.blocks, a.starts, a.lens, a.output});
+            op = 133;
+            break;
+        }
         default: return false;
     }
     if (s.n > 64) return false;
@@ -388,6 +423,29 @@ bool label_operands(const holo_kernel_call &c, std::vector<uint32_t> *ins,
             const auto &a = c.u.logits_process;
             r(a.logits), r(a.history), r(a.spans), r(a.params), r(a.bias_ids), r(a.bias_values),
             r(a.mask), w(a.output);
+            break;
+        }
+        case HOLO_OP_QK_NORM_ROTARY: {
+            const auto &a = c.u.qk_norm_rotary;
+            r(a.q), r(a.k), r(a.q_gamma), r(a.k_gamma), r(a.starts), r(a.pos), r(a.freqs);
+            w(a.q_output);
+            if (a.k_output.slot != HOLO_SLOT_ABSENT) w(a.k_output);
+            break;
+        }
+        case HOLO_OP_KV_BLOCK_BOUNDS: {
+            const auto &a = c.u.kv_block_bounds;
+            r(a.cache), r(a.starts), r(a.pos), r(a.bounds), w(a.output);
+            break;
+        }
+        case HOLO_OP_KV_BLOCK_SELECT: {
+            const auto &a = c.u.kv_block_select;
+            r(a.q), r(a.bounds), r(a.k_scales), r(a.starts), r(a.lens), w(a.output);
+            break;
+        }
+        case HOLO_OP_ATTN_I8_SELECTED: {
+            const auto &a = c.u.attn_i8_selected;
+            r(a.q), r(a.k_cache), r(a.v_cache), r(a.k_scales), r(a.v_scales), r(a.blocks),
+            r(a.starts), r(a.lens), w(a.output);
             break;
         }
         case HOLO_OP_ARGMAX: r(c.u.argmax.input), w(c.u.argmax.output); break;

@@ -152,6 +152,55 @@ struct AttnBlocksArgs {
 size_t attn_blocks_scratch_bytes(const AttnBlocksArgs &a);
 uint64_t attn_blocks_threads(const AttnBlocksArgs &a);
 hipError_t launch_attn_blocks(const AttnBlocksArgs &a, void *scratch, hipStream_t stream);
+// qk_norm_rotary.hip — q and k of a packed batch normed by the head and rotated by
+// position. Hkv 0: q alone; null gamma: 1; null freqs: no rotation.
+struct QkNormRotaryArgs {
+    PackedBatch pb;
+    const void *x[2];                 // q [tokens, H, D], k [tokens, Hkv, D]
+    const void *gamma[2];             // [D]
+    void *out[2];
+    const uint32_t *pos;              // [batch]
+    const float *freqs;               // [rot / 2]
+    uint32_t stride[2];               // elements a token
+    uint32_t H, Hkv, D, rot;
+    float eps, magnitude;
+    uint8_t norms, interleaved, dtype;
+};
+uint64_t qk_norm_rotary_threads(const QkNormRotaryArgs &a);
+hipError_t launch_qk_norm_rotary(const QkNormRotaryArgs &a, hipStream_t stream);
+// kv_select.hip — the bounds of the blocks that an append wrote to, in place, and the
+// blocks that each row attends to, by those bounds.
+struct KvBoundsArgs {
+    PackedBatch pb;
+    const int8_t *cache;              // [batch * Hkv, bucket, D]
+    const uint32_t *pos;              // [batch]
+    int8_t *bounds;                   // [batch * Hkv, ceil(bucket / block), 2, D]
+    uint32_t Hkv, bucket, block, D;
+};
+uint64_t kv_bounds_threads(const KvBoundsArgs &a);
+hipError_t launch_kv_bounds(const KvBoundsArgs &a, hipStream_t stream);
+struct KvSelectArgs {
+    PackedBatch pb;
+    const void *q;                    // [tokens, H, D]
+    const int8_t *bounds;
+    const float *ks;                  // [batch * Hkv, ceil(bucket / block)]
+    const uint32_t *lens;             // [batch]
+    int32_t *out;                     // [tokens, Hkv, top]
+    uint32_t H, Hkv, bucket, block, D, q_stride, top, first, last;
+    uint8_t dtype;
+};
+size_t kv_select_scratch_bytes(const KvSelectArgs &a);
+uint64_t kv_select_threads(const KvSelectArgs &a);
+hipError_t launch_kv_select(const KvSelectArgs &a, void *scratch, hipStream_t stream);
+// attn_selected.hip — attn_blocks.hip over the blocks that each row's list names.
+struct AttnSelectedArgs {
+    AttnBlocksArgs a;
+    const int32_t *blocks;            // [tokens, Hkv, top]
+    uint32_t top;
+};
+size_t attn_selected_scratch_bytes(const AttnSelectedArgs &a);
+uint64_t attn_selected_threads(const AttnSelectedArgs &a);
+hipError_t launch_attn_selected(const AttnSelectedArgs &a, void *scratch, hipStream_t stream);
 // logits.hip — penalties, biases and a mask on logits. Null history, bias_ids
 // and mask: none.
 constexpr uint32_t kLogitsMaxHistory = 524287, kLogitsMaxBiases = 4095;

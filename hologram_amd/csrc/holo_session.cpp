@@ -215,6 +215,29 @@ void call_operands(const holo_kernel_call &c, std::vector<holo_buffer_ref> *read
             r(a.mask); w(a.output);
             break;
         }
+        case HOLO_OP_QK_NORM_ROTARY: {
+            const auto &a = c.u.qk_norm_rotary;
+            r(a.q); r(a.k); r(a.q_gamma); r(a.k_gamma); r(a.starts); r(a.pos); r(a.freqs);
+            w(a.q_output);
+            if (a.k_output.slot != HOLO_SLOT_ABSENT) w(a.k_output);
+            break;
+        }
+        case HOLO_OP_KV_BLOCK_BOUNDS: {
+            const auto &a = c.u.kv_block_bounds;
+            r(a.cache); r(a.starts); r(a.pos); r(a.bounds); w(a.output);
+            break;
+        }
+        case HOLO_OP_KV_BLOCK_SELECT: {
+            const auto &a = c.u.kv_block_select;
+            r(a.q); r(a.bounds); r(a.k_scales); r(a.starts); r(a.lens); w(a.output);
+            break;
+        }
+        case HOLO_OP_ATTN_I8_SELECTED: {
+            const auto &a = c.u.attn_i8_selected;
+            r(a.q); r(a.k_cache); r(a.v_cache); r(a.k_scales); r(a.v_scales); r(a.blocks);
+            r(a.starts); r(a.lens); w(a.output);
+            break;
+        }
         default: break;
     }
 }
@@ -1298,6 +1321,7 @@ void elide_steps(holo_session *s, const std::vector<uint8_t> &is_output,
             const auto &k = c.u.kv_block_append;
             mark(k.cache), mark(k.cache_scales), mark(k.output), mark(k.output_scales);
         }
+        if (c.tag == HOLO_OP_KV_BLOCK_BOUNDS) mark(c.u.kv_block_bounds.bounds), mark(c.u.kv_block_bounds.output);
     }
     for (const auto &a : s->aliases) {
         if (a.first < nslots) kv[a.first] = 1;
@@ -1305,7 +1329,7 @@ void elide_steps(holo_session *s, const std::vector<uint8_t> &is_output,
     }
     auto is_kv_op = [](uint32_t tag) {
         return tag == HOLO_OP_KV_CACHE_WRITE || tag == HOLO_OP_KV_QUANT_APPEND ||
-               tag == HOLO_OP_KV_BLOCK_APPEND;
+               tag == HOLO_OP_KV_BLOCK_APPEND || tag == HOLO_OP_KV_BLOCK_BOUNDS;
     };
     // a slot only this step writes, that no port, constant or KV op touches
     auto plain = [&](uint32_t sl) {
@@ -1918,6 +1942,15 @@ plan_moves:
             s->aliases.push_back({os, cs});
             k.output = k.cache;
             k.output_scales = k.cache_scales;
+        } else if (call.tag == HOLO_OP_KV_BLOCK_BOUNDS) {
+            auto &k = call.u.kv_block_bounds;
+            const uint32_t bs = k.bounds.slot, os = k.output.slot;
+            if (bs == HOLO_SLOT_ABSENT || bs == os || readers[bs] != 1 || is_output[bs] || is_const[bs] ||
+                k.bounds.offset != 0 || k.output.offset != 0)
+                continue;
+            if (k.cache.slot == bs || k.starts.slot == bs || k.pos.slot == bs) continue;
+            s->aliases.push_back({os, bs});
+            k.output = k.bounds;
         }
     }
     // every call must be one this backend runs (validated on the slot sizes)

@@ -10,32 +10,9 @@ namespace {
 
 constexpr uint32_t kThreads = 256;
 
-// The least 2^e, e >= -126, with v <= 127 * 2^e, for a finite v > 0 given by its
-// bits: 127 is 1.984375 * 2^6, so e is v's exponent less 6, one more where v's
-// mantissa passes 1.984375. Exact, subnormal v included (the floor takes them).
-__device__ __forceinline__ float block_scale(uint32_t bits) {
-    const int e = int(bits >> 23) - 127 - 6 + ((bits & 0x7fffffu) > 0x7e0000u);
-    return __uint_as_float(uint32_t((e < -126 ? -126 : e) + 127) << 23);
-}
-
 __device__ __forceinline__ int8_t to_i8(float r) {   // r finite
     return int8_t(rintf(fminf(fmaxf(r, -127.0f), 127.0f)));
 }
-
-// Eight elements: their largest magnitude's bits, and them over a scale as int8.
-template <class E>
-struct Eight {
-    uint4 raw[sizeof(typename E::T) / 2];
-    __device__ __forceinline__ void load(const typename E::T *p) {
-#pragma unroll
-        for (uint32_t i = 0; i < sizeof raw / 16; ++i) raw[i] = reinterpret_cast<const uint4 *>(p)[i];
-    }
-    __device__ __forceinline__ float get(int i) const {
-        const uint32_t *w = reinterpret_cast<const uint32_t *>(raw);
-        if constexpr (sizeof(typename E::T) == 4) return __uint_as_float(w[i]);
-        else return E::widen(uint16_t(w[i >> 1] >> (16 * (i & 1))));
-    }
-};
 
 // One workgroup a touched block and head. Sequence s owns the places [floor(
 // starts[s] / block) + 2 s, floor(starts[s + 1] / block) + 2 (s + 1)) of the grid: n

@@ -1,5 +1,5 @@
 // packed_batch.h — what the packed-batch kernels (attn_packed.hip, attn_blocks.hip,
-// kv_blocks.hip) share: finding a workgroup's sequence among the device-resident
+// attn_selected.hip, kv_blocks.hip, kv_select.hip, qk_norm_rotary.hip) share: finding a workgroup's sequence among the device-resident
 // offsets, widening and narrowing, and the attention of one row at a time.
 #pragma once
 
@@ -100,50 +100,94 @@ struct F32 {
     typedef float T;
 };
 
-// One wavefront's query row over `keys` keys: q (D floats in LDS, scaled by
-// log2(e) / s), K row j's elements src.k(j, d) times src.k_scale(j), V's likewise.
-// A lane takes one key of 64 for the scores and every 64th dim of the result, so
-// any D and any layout go. Softmax in f32 with a running maximum and sum; keys at
-// and past `keys` are not read. A row whose scores are all -inf is NaN (0 / 0), a
-// row without keys zeros.
-template <int kDims, class Src, class Put>
-__device__ __forceinline__ void attend_row(const float *q, uint32_t D, uint32_t keys, const Src &src, Put put) {
-    const uint32_t lane = threadIdx.x & 63u;
-    float m = -INFINITY, l = 0.0f, acc[kDims];
+// Eight elements, 16 bytes a load.
+template <class E>
+struct Eight {
+    uint4 raw[sizeof(typename E::T) / 2];
+    __device__ __forceinline__ void load(const typename E::T *p) {
 #pragma unroll
-    for (int i = 0; i < kDims; ++i) acc[i] = 0.0f;
-    for (uint32_t j0 = 0; j0 < keys; j0 += 64) {
-        const uint32_t n = keys - j0 < 64 ? keys - j0 : 64;
-        float s = -INFINITY;
-        if (lane < n) {
-            float dot = 0.0f;
-            for (uint32_t d = 0; d < D; ++d) dot = fmaf(q[d], src.k(j0 + lane, d), dot);
-            s = dot * src.k_scale(j0 + lane);
-        }
-        float mn = s;
+        for (uint32_t i = 0; i < sizeof raw / 16; ++i) raw[i] = reinterpret_cast<const uint4 *>(p)[i];
+    }
+    __device__ __forceinline__ float get(int i) const {
+        const uint32_t *w = reinterpret_cast<const uint32_t *>(raw);
+        if constexpr (sizeof(typename E::T) == 4) return __uint_as_float(w[i]);
+        else return E::widen(uint16_t(w[i >> 1] >> (16 * (i & 1))));
+    }
+};
+
+// The least 2^e, e >= -126, with v <= 127 * 2^e, for a finite v > 0 given by its
+// bits: 127 is 1.984375 * 2^6, so e is v's exponent less 6, one more where v's
+// mantissa passes 1.984375. Exact, subnormal v included (the floor takes them).
+__device__ __forceinline__ float block_scale(uint32_t bits) {
+    const int e = int(bits >> 23) - 127 - 6 + ((bits & 0x7fffffu) > 0x7e0000u);
+    return __uint_as_float(uint32_t((e < -126 ? -126 : e) + 127) << 23);
+}
+
+// Keys that row t of sequence b's n rows sees.
+__device__ __forceinline__ uint32_t visible_keys(int64_t len, uint32_t n, uint32_t t, uint32_t bucket) {
+    const int64_t v = len - int64_t(n - 1 - t);
+    return v < 0 ? 0u : v > int64_t(bucket) ? bucket : uint32_t(v);
+}
+
+// One wavefront's query row: q (D floats in LDS, scaled by log2(e) / s), K row j's
+// elements src.k(j, d) times src.k_scale(j), V's likewise. A lane takes one key of 64 for
+// the scores and every 64th dim of the result, so any D and any layout go. Softmax in f32
+// with a running maximum and sum. A row whose scores are all -inf is NaN (0 / 0), a row
+// without keys zeros.
+template <int kDims>
+struct RowState {
+    float m = -INFINITY, l = 0.0f, acc[kDims] = {};
+    bool any = false;
+
+    // Keys [from, to); no other is read.
+    template <class Src>
+    __device__ __forceinline__ void keys(const float *q, uint32_t D, uint32_t from, uint32_t to, const Src &src) {
+        const uint32_t lane = threadIdx.x & 63u;
+        any |= from < to;
+        for (uint32_t j0 = from; j0 < to; j0 += 64) {
+            const uint32_t n = to - j0 < 64 ? to - j0 : 64;
+            float s = -INFINITY;
+            if (lane < n) {
+                float dot = 0.0f;
+                for (uint32_t d = 0; d < D; ++d) dot = fmaf(q[d], src.k(j0 + lane, d), dot);
+                s = dot * src.k_scale(j0 + lane);
+            }
+            float mn = s;
 #pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) mn = fmaxf(mn, __shfl_xor(mn, o, 64));
-        mn = fmaxf(mn, m);
-        const float ref = mn == -INFINITY ? 0.0f : mn;
-        const float al = m == -INFINITY ? 0.0f : exp2f(m - ref);
-        const float p = lane < n ? (s == -INFINITY ? 0.0f : exp2f(s - ref)) : 0.0f;
-        float sum = p;
+            for (int o = 32; o >= 1; o >>= 1) mn = fmaxf(mn, __shfl_xor(mn, o, 64));
+            mn = fmaxf(mn, m);
+            const float ref = mn == -INFINITY ? 0.0f : mn;
+            const float al = m == -INFINITY ? 0.0f : exp2f(m - ref);
+            const float p = lane < n ? (s == -INFINITY ? 0.0f : exp2f(s - ref)) : 0.0f;
+            float sum = p;
 #pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
-        l = l * al + sum;
-        m = mn;
+            for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
+            l = l * al + sum;
+            m = mn;
 #pragma unroll
-        for (int i = 0; i < kDims; ++i) acc[i] *= al;
-        for (uint32_t j = 0; j < n; ++j) {
-            const float w = __shfl(p, int(j), 64) * src.v_scale(j0 + j);
+            for (int i = 0; i < kDims; ++i) acc[i] *= al;
+            for (uint32_t j = 0; j < n; ++j) {
+                const float w = __shfl(p, int(j), 64) * src.v_scale(j0 + j);
 #pragma unroll
-            for (int i = 0; i < kDims; ++i)
-                if (lane + 64u * i < D) acc[i] = fmaf(w, src.v(j0 + j, lane + 64u * i), acc[i]);
+                for (int i = 0; i < kDims; ++i)
+                    if (lane + 64u * i < D) acc[i] = fmaf(w, src.v(j0 + j, lane + 64u * i), acc[i]);
+            }
         }
     }
+    template <class Put>
+    __device__ __forceinline__ void write(uint32_t D, Put put) const {
+        const uint32_t lane = threadIdx.x & 63u;
 #pragma unroll
-    for (int i = 0; i < kDims; ++i)
-        if (lane + 64u * i < D) put(lane + 64u * i, keys ? acc[i] / l : 0.0f);
+        for (int i = 0; i < kDims; ++i)
+            if (lane + 64u * i < D) put(lane + 64u * i, any ? acc[i] / l : 0.0f);
+    }
+};
+
+template <int kDims, class Src, class Put>
+__device__ __forceinline__ void attend_row(const float *q, uint32_t D, uint32_t keys, const Src &src, Put put) {
+    RowState<kDims> st;
+    st.keys(q, D, 0, keys, src);
+    st.write(D, put);
 }
 
 }  // namespace holo

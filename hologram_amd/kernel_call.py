@@ -75,6 +75,10 @@ D_APK = 126     # new: causal attention of a packed batch of prompts
 D_KVBA = 127    # new: int8 append, one scale a block of rows
 D_AI8B = 128    # new: attention over the cache D_KVBA fills
 D_LOGITS = 129  # new: penalties, biases and a mask on logits
+D_QKNR = 130    # new: q and k normed and rotated by position
+D_KVBB = 131    # new: smallest and largest bytes of a cache's blocks
+D_KVBS = 132    # new: the blocks a row attends to
+D_AI8S = 133    # new: attention over those blocks
 D_TRANSPOSE = 61
 D_RESHAPE = 60
 D_SLICE = 63
@@ -631,6 +635,131 @@ class LogitsProcessCall:
 
 
 @dataclass(frozen=True)
+class QkNormRotaryCall:
+    """New (discriminant 130): q and k normed by the head and rotated by position
+    (include/holo_hip.h); NO_BUFFER for k, a gamma or freqs that a call does not use."""
+    q: BufferRef
+    k: BufferRef
+    q_gamma: BufferRef
+    k_gamma: BufferRef
+    starts: BufferRef
+    pos: BufferRef
+    freqs: BufferRef
+    q_output: BufferRef
+    k_output: BufferRef
+    tokens: int
+    batch: int
+    heads: int
+    kv_heads: int
+    head_dim: int
+    rotary_dim: int
+    q_stride: int = 0
+    k_stride: int = 0
+    epsilon_bits: int = 0
+    magnitude_bits: int = 0
+    norms: int = 3
+    interleaved: int = 0
+    dtype: int = DTYPE_BF16
+
+    def wire(self) -> bytes:
+        return (self.q.wire() + self.k.wire() + self.q_gamma.wire() + self.k_gamma.wire()
+                + self.starts.wire() + self.pos.wire() + self.freqs.wire() + self.q_output.wire()
+                + self.k_output.wire()
+                + struct.pack("<IIIIIIIIIIBBB", self.tokens, self.batch, self.heads, self.kv_heads,
+                              self.head_dim, self.rotary_dim, self.q_stride, self.k_stride,
+                              self.epsilon_bits, self.magnitude_bits, self.norms, self.interleaved,
+                              self.dtype))
+
+
+@dataclass(frozen=True)
+class KvBlockBoundsCall:
+    """New (discriminant 131): the smallest and largest bytes of the blocks that a
+    KvBlockAppend wrote to (include/holo_hip.h)."""
+    cache: BufferRef
+    starts: BufferRef
+    pos: BufferRef
+    bounds: BufferRef
+    output: BufferRef
+    tokens: int
+    batch: int
+    kv_heads: int
+    bucket_rows: int
+    block_rows: int
+    head_dim: int
+
+    def wire(self) -> bytes:
+        return (self.cache.wire() + self.starts.wire() + self.pos.wire() + self.bounds.wire()
+                + self.output.wire()
+                + struct.pack("<IIIIII", self.tokens, self.batch, self.kv_heads, self.bucket_rows,
+                              self.block_rows, self.head_dim))
+
+
+@dataclass(frozen=True)
+class KvBlockSelectCall:
+    """New (discriminant 132): the blocks each row attends to, by the scores that their
+    bounds allow (include/holo_hip.h)."""
+    q: BufferRef
+    bounds: BufferRef
+    k_scales: BufferRef
+    starts: BufferRef
+    lens: BufferRef
+    output: BufferRef
+    tokens: int
+    batch: int
+    heads: int
+    kv_heads: int
+    bucket_rows: int
+    block_rows: int
+    head_dim: int
+    q_stride: int
+    top: int
+    keep_first: int
+    keep_last: int
+    dtype: int = DTYPE_BF16
+
+    def wire(self) -> bytes:
+        return (self.q.wire() + self.bounds.wire() + self.k_scales.wire() + self.starts.wire()
+                + self.lens.wire() + self.output.wire()
+                + struct.pack("<IIIIIIIIIIIB", self.tokens, self.batch, self.heads, self.kv_heads,
+                              self.bucket_rows, self.block_rows, self.head_dim, self.q_stride,
+                              self.top, self.keep_first, self.keep_last, self.dtype))
+
+
+@dataclass(frozen=True)
+class AttentionI8SelectedCall:
+    """New (discriminant 133): AttentionI8Blocks over the blocks of each row's list
+    (include/holo_hip.h)."""
+    q: BufferRef
+    k_cache: BufferRef
+    v_cache: BufferRef
+    k_scales: BufferRef
+    v_scales: BufferRef
+    blocks: BufferRef
+    starts: BufferRef
+    lens: BufferRef
+    output: BufferRef
+    tokens: int
+    batch: int
+    heads: int
+    kv_heads: int
+    bucket_rows: int
+    block_rows: int
+    head_dim: int
+    q_stride: int
+    top: int
+    scale_bits: int = 0
+    dtype: int = DTYPE_BF16
+
+    def wire(self) -> bytes:
+        return (self.q.wire() + self.k_cache.wire() + self.v_cache.wire() + self.k_scales.wire()
+                + self.v_scales.wire() + self.blocks.wire() + self.starts.wire()
+                + self.lens.wire() + self.output.wire()
+                + struct.pack("<IIIIIIIIIIB", self.tokens, self.batch, self.heads, self.kv_heads,
+                              self.bucket_rows, self.block_rows, self.head_dim, self.q_stride,
+                              self.top, self.scale_bits, self.dtype))
+
+
+@dataclass(frozen=True)
 class TransposeCall:
     """kernel_call.rs:487-499: output axis i is input axis perm[i]."""
     input: BufferRef
@@ -670,7 +799,9 @@ _NAMES = {D_RESHAPE: "Reshape", D_SLICE: "Slice", D_ADD: "Add", D_MUL: "Mul", D_
           D_MATMUL: "MatMul", D_MMA: "MatMulActivation", D_MMADD: "MatMulAdd",
           D_MMAA: "MatMulAddActivation", D_KVWR: "KvCacheWrite", D_KVQA: "KvQuantAppend",
           D_DECATTN: "DecodeAttention", D_DAVL: "DecodeAttentionValid", D_DAI8: "DecodeAttentionI8", D_AI8R: "AttentionI8Rows", D_TRANSPOSE: "Transpose",
-          D_APK: "AttentionPacked", D_KVBA: "KvBlockAppend", D_AI8B: "AttentionI8Blocks", D_LOGITS: "LogitsProcess"}
+          D_APK: "AttentionPacked", D_KVBA: "KvBlockAppend", D_AI8B: "AttentionI8Blocks", D_LOGITS: "LogitsProcess",
+          D_QKNR: "QkNormRotary", D_KVBB: "KvBlockBounds", D_KVBS: "KvBlockSelect",
+          D_AI8S: "AttentionI8Selected"}
 
 
 @dataclass(frozen=True)
@@ -813,6 +944,22 @@ class KernelCall:
         return cls(D_LOGITS, c)
 
     @classmethod
+    def QkNormRotary(cls, c: QkNormRotaryCall) -> "KernelCall":  # noqa: N802
+        return cls(D_QKNR, c)
+
+    @classmethod
+    def KvBlockBounds(cls, c: KvBlockBoundsCall) -> "KernelCall":  # noqa: N802
+        return cls(D_KVBB, c)
+
+    @classmethod
+    def KvBlockSelect(cls, c: KvBlockSelectCall) -> "KernelCall":  # noqa: N802
+        return cls(D_KVBS, c)
+
+    @classmethod
+    def AttentionI8Selected(cls, c: AttentionI8SelectedCall) -> "KernelCall":  # noqa: N802
+        return cls(D_AI8S, c)
+
+    @classmethod
     def Transpose(cls, c: TransposeCall) -> "KernelCall":  # noqa: N802
         return cls(D_TRANSPOSE, c)
 
@@ -897,6 +1044,26 @@ class KernelCall:
                 p.logits.c(), p.history.c(), p.spans.c(), p.params.c(), p.bias_ids.c(),
                 p.bias_values.c(), p.mask.c(), p.output.c(), p.rows, p.cols, p.history_len,
                 p.biases, p.dtype)
+        elif isinstance(p, QkNormRotaryCall):
+            kc.u.qk_norm_rotary = _ffi.QkNormRotaryCallC(
+                p.q.c(), p.k.c(), p.q_gamma.c(), p.k_gamma.c(), p.starts.c(), p.pos.c(),
+                p.freqs.c(), p.q_output.c(), p.k_output.c(), p.tokens, p.batch, p.heads, p.kv_heads,
+                p.head_dim, p.rotary_dim, p.q_stride, p.k_stride, p.epsilon_bits, p.magnitude_bits,
+                p.norms, p.interleaved, p.dtype)
+        elif isinstance(p, KvBlockBoundsCall):
+            kc.u.kv_block_bounds = _ffi.KvBlockBoundsCallC(
+                p.cache.c(), p.starts.c(), p.pos.c(), p.bounds.c(), p.output.c(), p.tokens, p.batch,
+                p.kv_heads, p.bucket_rows, p.block_rows, p.head_dim)
+        elif isinstance(p, KvBlockSelectCall):
+            kc.u.kv_block_select = _ffi.KvBlockSelectCallC(
+                p.q.c(), p.bounds.c(), p.k_scales.c(), p.starts.c(), p.lens.c(), p.output.c(),
+                p.tokens, p.batch, p.heads, p.kv_heads, p.bucket_rows, p.block_rows, p.head_dim,
+                p.q_stride, p.top, p.keep_first, p.keep_last, p.dtype)
+        elif isinstance(p, AttentionI8SelectedCall):
+            kc.u.attn_i8_selected = _ffi.AttentionI8SelectedCallC(
+                p.q.c(), p.k_cache.c(), p.v_cache.c(), p.k_scales.c(), p.v_scales.c(), p.blocks.c(),
+                p.starts.c(), p.lens.c(), p.output.c(), p.tokens, p.batch, p.heads, p.kv_heads,
+                p.bucket_rows, p.block_rows, p.head_dim, p.q_stride, p.top, p.scale_bits, p.dtype)
         elif isinstance(p, TransposeCall):
             rank = len(p.dims)
             kc.u.transpose = _ffi.TransposeCallC(
@@ -998,6 +1165,10 @@ _FLAT = {cls: _flat_form(ctype) for cls, ctype in (
     (KvBlockAppendCall, _ffi.KvBlockAppendCallC),
     (AttentionI8BlocksCall, _ffi.AttentionI8BlocksCallC),
     (LogitsProcessCall, _ffi.LogitsProcessCallC),
+    (QkNormRotaryCall, _ffi.QkNormRotaryCallC),
+    (KvBlockBoundsCall, _ffi.KvBlockBoundsCallC),
+    (KvBlockSelectCall, _ffi.KvBlockSelectCallC),
+    (AttentionI8SelectedCall, _ffi.AttentionI8SelectedCallC),
     (MatMulDequantCall, _ffi.MatMulDequantCallC))}
 
 

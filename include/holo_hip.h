@@ -67,7 +67,7 @@ typedef enum holo_status {
 #define HOLO_FUSED_EXP 8
 
 /* KernelCall tags = the archive wire discriminants,
- * crates/hologram-archive/src/kernel_codec.rs:18-128. 122 to 129 are new
+ * crates/hologram-archive/src/kernel_codec.rs:18-128. 122 to 133 are new
  * capabilities and take new discriminants (kernel_codec.rs:124-128). */
 #define HOLO_OP_ADD 5u
 #define HOLO_OP_MUL 7u
@@ -102,6 +102,10 @@ typedef enum holo_status {
 #define HOLO_OP_KV_BLOCK_APPEND 127u      /* new: int8 append, one scale a block of rows */
 #define HOLO_OP_ATTN_I8_BLOCKS 128u       /* new: attention over the cache 127 fills */
 #define HOLO_OP_LOGITS_PROCESS 129u       /* new: penalties, biases and a mask on logits */
+#define HOLO_OP_QK_NORM_ROTARY 130u       /* new: q and k normed and rotated by position */
+#define HOLO_OP_KV_BLOCK_BOUNDS 131u      /* new: smallest and largest bytes of a cache's blocks */
+#define HOLO_OP_KV_BLOCK_SELECT 132u      /* new: the blocks a row attends to */
+#define HOLO_OP_ATTN_I8_SELECTED 133u     /* new: attention over those blocks */
 #define HOLO_OP_TRANSPOSE 61u             /* Transpose (kernel_codec.rs:80)     */
 #define HOLO_OP_RESHAPE 60u               /* Reshape (kernel_codec.rs:79, D_RESHAPE) */
 #define HOLO_OP_SLICE 63u                 /* Slice (kernel_codec.rs:82, D_SLICE)     */
@@ -419,7 +423,7 @@ typedef struct holo_attention_i8_rows_call {
     uint32_t q_rows;
 } holo_attention_i8_rows_call;
 
-/* The packed batch of the next three calls: the rows of `batch` sequences lie
+/* The packed batch of the next three calls and of 130 to 133: the rows of `batch` sequences lie
  * end to end, sequence b's at rows [starts[b], starts[b + 1]) of `tokens`.
  * starts is u32 [batch + 1], device-resident and non-decreasing, with
  * starts[batch] <= tokens; a sequence may be empty. Rows outside every
@@ -430,7 +434,8 @@ typedef struct holo_attention_i8_rows_call {
  * heads is at most 2^30, and a call of these or of 129 whose launch would hold
  * 2^32 threads is refused (UnsupportedOp). Below that whatever the form: tokens *
  * heads < 2^26 with batch * kv_heads <= 2^23 (126, 128), (tokens / block_rows + 2
- * batch) * kv_heads < 2^24 (127), rows * (cols / 8192 + 2) < 2^23 (129). */
+ * batch) * kv_heads < 2^24 (127, 131), rows * (cols / 8192 + 2) < 2^23 (129). Of 130,
+ * 132 and 133 where each describes it. */
 
 /* New (tag 126): causal grouped-query attention of a packed batch of prompts
  * over their own K and V, all of `dtype` (bf16, f16 or f32). q is [tokens,
@@ -552,6 +557,118 @@ typedef struct holo_logits_process_call {
     uint8_t dtype;
 } holo_logits_process_call;
 
+/* New (tag 130): what stands between a packed batch's projections and its
+ * attention. Each head's row of q [tokens, heads, head_dim] and k [tokens,
+ * kv_heads, head_dim], of bf16, f16 or f32, is normed where its bit of `norms` is
+ * set (1: q, 2: k), y = x * (1 / sqrtf(mean(x^2) + eps)) * gamma, gamma of the
+ * rows' type [head_dim] (absent: 1), eps as in NormCall; then the pairs of its
+ * first rotary_dim elements are turned by the angle p * freqs[i]:
+ *   (a, b) -> magnitude * (a cos - b sin, b cos + a sin)
+ * pair i being elements i and i + rotary_dim / 2, or 2 i and 2 i + 1 where
+ * `interleaved` is 1; the elements behind rotary_dim stay as they are. p is pos[b] +
+ * t for row t of sequence b (pos u32 [batch], device-resident: what 127 takes), freqs
+ * f32 [rotary_dim / 2] radians a position, device-resident: any schedule of
+ * frequencies, those scaled for long contexts among them; magnitude =
+ * f32(magnitude_bits), 0: 1. Angles are taken in f64 and reduced there, so they keep
+ * f32's precision at every position while |p * freq| < 2^50; everything else is f32,
+ * rounded to nearest once. rotary_dim 0: no rotation, freqs may be absent. k may be
+ * absent (with k_output, k_gamma): q alone. q_stride and k_stride are the elements
+ * from one token to the next (0: tight); the outputs are tight, and neither overlaps
+ * an input or the other. kv_heads 0 means heads; head_dim <= 1024. tokens * (heads +
+ * kv_heads) < 2^26 in any form. */
+typedef struct holo_qk_norm_rotary_call {
+    holo_buffer_ref q;
+    holo_buffer_ref k;
+    holo_buffer_ref q_gamma;
+    holo_buffer_ref k_gamma;
+    holo_buffer_ref starts;
+    holo_buffer_ref pos;
+    holo_buffer_ref freqs;
+    holo_buffer_ref q_output;
+    holo_buffer_ref k_output;
+    uint32_t tokens, batch, heads, kv_heads, head_dim, rotary_dim;
+    uint32_t q_stride, k_stride;
+    uint32_t epsilon_bits, magnitude_bits;
+    uint8_t norms, interleaved, dtype;
+} holo_qk_norm_rotary_call;
+
+/* New (tag 131): the bounds of a cache's blocks, brought up to date behind 127 on
+ * the same starts and pos: for every block that holds one of the rows [pos[b], pos[b]
+ * + n) of sequence b's planes (n its rows; those at and past bucket_rows take no
+ * part), the smallest and the largest byte of each dim over the block's rows before
+ * pos[b] + n. cache int8 [batch * kv_heads, bucket_rows, head_dim]; bounds int8 [batch
+ * * kv_heads, ceil(bucket_rows / block_rows), 2, head_dim], smallest first, in the
+ * cache's units: the block's scale makes values of them, so they are what Dequantize
+ * (118) reads with one channel a block. Other blocks keep their bounds.
+ *   output == bounds (same slot and offset): in place; otherwise they are copied
+ *   first. A block holds at most 2^30 elements. */
+typedef struct holo_kv_block_bounds_call {
+    holo_buffer_ref cache;
+    holo_buffer_ref starts;
+    holo_buffer_ref pos;
+    holo_buffer_ref bounds;
+    holo_buffer_ref output;
+    uint32_t tokens, batch, kv_heads, bucket_rows, block_rows, head_dim;
+} holo_kv_block_bounds_call;
+
+/* New (tag 132): the blocks of the K cache that each row attends to, one list for a
+ * row and kv head, by the largest score that a block's bounds allow. Row t of the n
+ * rows of sequence b sees v = min(max(lens[b] - (n - 1 - t), 0), bucket_rows) rows of
+ * its planes, as in 128, and so ceil(v / block_rows) blocks. Of those the list names
+ * `top`, all where they are not more: the first keep_first, the last keep_last, and of
+ * the others those of the largest score, the lower block of equal ones. In ascending
+ * order, -1 behind them. output i32 [tokens, kv_heads, top].
+ * A block's score is k_scale * sum over the kv head's heads h and dims d of the larger
+ * (k_scale < 0: the smaller) of Q[h][d] * lo[d] and Q[h][d] * hi[d], with lo and hi its
+ * bounds (131) and Q = rne(q / 2^e), 2^e the least power of two, e >= -126, with max|q|
+ * <= 127 * 2^e over the group's finite elements (those that are not count as 0). Whole
+ * numbers times an f32: scores are compared exactly. One that is NaN ranks as positive
+ * infinity. keep_last >= 1, keep_first + keep_last <= top: the block that holds a row's
+ * last key may hold later rows, so its bounds and scale are never looked at.
+ * q of bf16, f16 or f32 (q_stride as in 128); bounds int8 [batch * kv_heads,
+ * ceil(bucket_rows / block_rows), 2, head_dim]; k_scales f32 [batch * kv_heads,
+ * ceil(bucket_rows / block_rows)]; lens u32 [batch], device-resident. kv_heads 0 means
+ * heads; head_dim <= 1024, heads / kv_heads * head_dim <= 2^17, at most 2^20 blocks a
+ * plane, kv_heads times those at most 2^28, top <= 2^20; (tokens + 16 batch) * kv_heads *
+ * (blocks / 64 + 1) < 2^24 in any form. Takes scratch. */
+typedef struct holo_kv_block_select_call {
+    holo_buffer_ref q;
+    holo_buffer_ref bounds;
+    holo_buffer_ref k_scales;
+    holo_buffer_ref starts;
+    holo_buffer_ref lens;
+    holo_buffer_ref output;
+    uint32_t tokens, batch, heads, kv_heads, bucket_rows, block_rows, head_dim;
+    uint32_t q_stride;
+    uint32_t top, keep_first, keep_last;
+    uint8_t dtype;
+} holo_kv_block_select_call;
+
+/* New (tag 133): 128 over the blocks that a list names: a row of head h sees, of the
+ * rows that it sees in 128, those of the blocks in `blocks` i32 [tokens, kv_heads, top]
+ * of its kv head, in any order. An entry below 0 or past the plane's blocks is passed
+ * over, a block listed twice counts twice. Scores, softmax, roundings and the result as
+ * in 128; a row that sees no key is zeros, and what a row does not see, blocks that its
+ * list does not name among it, does not reach its result. kv_heads 0 means heads; head_dim
+ * <= 1024; bucket_rows * head_dim <= 2^30; top <= 2^20; tokens * heads * (top / 4 + 1) <
+ * 2^24 in any form. Long lists and few rows take scratch. */
+typedef struct holo_attention_i8_selected_call {
+    holo_buffer_ref q;
+    holo_buffer_ref k_cache;
+    holo_buffer_ref v_cache;
+    holo_buffer_ref k_scales;
+    holo_buffer_ref v_scales;
+    holo_buffer_ref blocks;
+    holo_buffer_ref starts;
+    holo_buffer_ref lens;
+    holo_buffer_ref output;
+    uint32_t tokens, batch, heads, kv_heads, bucket_rows, block_rows, head_dim;
+    uint32_t q_stride;
+    uint32_t top;
+    uint32_t scale_bits;
+    uint8_t dtype;
+} holo_attention_i8_selected_call;
+
 /* TransposeCall, kernel_call.rs:487-499 (transpose_float,
  * src/cpu/float_kernels.rs:2980-3028): output axis i is input axis perm[i] of
  * the row-major input of shape dims[0..rank). rank 1..8; f16/bf16/f32 elements;
@@ -608,6 +725,10 @@ typedef struct holo_kernel_call {
         holo_kv_block_append_call kv_block_append;
         holo_attention_i8_blocks_call attn_i8_blocks;
         holo_logits_process_call logits_process;
+        holo_qk_norm_rotary_call qk_norm_rotary;
+        holo_kv_block_bounds_call kv_block_bounds;
+        holo_kv_block_select_call kv_block_select;
+        holo_attention_i8_selected_call attn_i8_selected;
         holo_transpose_call transpose;
         holo_layout_call layout;
     } u;
@@ -823,8 +944,8 @@ int holo_hip_derive_label(uint16_t opcode, const uint8_t *params, uint64_t n_par
                           const char *labels, uint64_t n_labels, char out[72]);
 /* KernelCall::op_signature (crates/hologram-compute/src/kernel_call.rs:
  * 1321-1500): the opcode and LE parameter bytes a call's label is derived
- * with. The new calls (122-129) take their discriminant as opcode and their
- * scalar fields in struct order; 126-129 then the first 16 bytes of the BLAKE3
+ * with. The new calls (122-133) take their discriminant as opcode and their
+ * scalar fields in struct order; 126-133 then the first 16 bytes of the BLAKE3
  * digest of their operands' offsets, u64 LE each in struct order, 2^64 - 1 for
  * an absent one: calls over different views of one slot, or with other operands
  * absent, have different labels. UnsupportedOp for a call not served here. */
