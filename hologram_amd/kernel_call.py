@@ -1173,9 +1173,34 @@ _FLAT = {cls: _flat_form(ctype) for cls, ctype in (
 
 
 def dispatch_form(call: "KernelCall"):
-    """What a dispatch passes: to_c()'s bytes, or to_c() by reference."""
-    form = _FLAT.get(type(call.payload))
-    return form and form(call.tag, call.payload) or ctypes.byref(call.to_c())
+    """What a dispatch passes: to_c()'s bytes, or to_c() by reference. The bytes stay with the
+    call where it and all it holds are frozen: packing nine BufferRefs and thirteen numbers takes
+    longer than a small kernel runs (3 to 6 us; looking them up 0.3)."""
+    kept = call.__dict__.get("_packed")
+    if kept is not None:
+        return kept
+    payload = call.payload
+    form = _FLAT.get(type(payload))
+    packed = form and form(call.tag, payload)
+    if not packed:
+        return ctypes.byref(call.to_c())
+    if type(call) is KernelCall and _all_frozen(payload):
+        object.__setattr__(call, "_packed", packed)
+    return packed
+
+
+def _all_frozen(payload) -> bool:
+    """Whether what a payload of _FLAT holds is numbers, BufferRefs and payloads of _FLAT."""
+    for v in payload.__dict__.values():
+        t = type(v)
+        if t in _INTS:
+            continue
+        if t is BufferRef:
+            if not _INTS.issuperset(map(type, v.__dict__.values())):
+                return False
+        elif t not in _FLAT or not _all_frozen(v):
+            return False
+    return True
 
 
 def _attn_c(p: DecodeAttentionI8Call) -> _ffi.DecodeAttentionI8CallC:
