@@ -1773,7 +1773,7 @@ int do_qk_norm_rotary(holo_backend *be, const SlotTable &st, const holo_qk_norm_
     if (!(a.magnitude > 0.0f) || std::isinf(a.magnitude))
         return fail(HOLO_ERR_UNSUPPORTED_OP, "qk_norm_rotary: magnitude must be a positive finite f32 (0 selects 1)");
     const uint64_t es = dtype_size(c.dtype), D = c.head_dim;
-    a.stride[0] = c.q_stride, a.stride[1] = c.k_stride;
+    a.stride[0] = c.q_stride, a.stride[1] = has_k ? c.k_stride : 0;
     uint64_t span[2] = {0, 0};
     HOLO_TRY(strided(c.tokens, c.heads * D, &a.stride[0], &span[0], op, "q"));
     if (has_k) HOLO_TRY(strided(c.tokens, hkv * D, &a.stride[1], &span[1], op, "k"));

@@ -68,6 +68,34 @@ __device__ __forceinline__ bool place_of(const PackedBatch &pb, uint32_t m, uint
     return o->hi > o->lo && t >= first && o->unit * unit < (o->hi - o->lo) * m;
 }
 
+// The sequence that holds row `t`: its number, its first and one-past-last row and its
+// element of `per` (u32 [batch], or null), loaded beside the offsets; false for a row
+// outside every sequence. As place_of.
+struct RowAt {
+    uint32_t b, lo, hi, of;
+};
+__device__ __forceinline__ bool row_of(const PackedBatch &pb, const uint32_t *per, uint32_t t, RowAt *o) {
+    const uint32_t lane = threadIdx.x & 63u;
+    uint32_t lo = 0, n = pb.batch, v, x;
+    int at;
+    for (;;) {
+        const uint32_t step = (n + 63) / 64;
+        const uint64_t s = lo + uint64_t(lane) * step;
+        v = start_of(pb, s < pb.batch ? uint32_t(s) : pb.batch);
+        x = per ? per[s < pb.batch ? uint32_t(s) : pb.batch - 1] : 0u;
+        const uint64_t hit = __ballot(lane * uint64_t(step) < n && v <= t);
+        at = hit ? 63 - __builtin_clzll(hit) : 0;
+        lo = pk_uni(lo + at * step);
+        if (step == 1) break;
+        n = pk_uni(pb.batch - lo < step ? pb.batch - lo : step);
+    }
+    o->b = lo;
+    o->lo = __builtin_amdgcn_readlane(v, at);
+    o->hi = at < 63 ? __builtin_amdgcn_readlane(v, at + 1) : pk_uni(start_of(pb, lo + 1));
+    o->of = __builtin_amdgcn_readlane(x, at);
+    return t >= o->lo && t < o->hi;
+}
+
 // Bit 8 of *err if the offsets decrease or pass `tokens`; the threads of one
 // workgroup call it.
 __device__ __forceinline__ void check_starts(const PackedBatch &pb) {
