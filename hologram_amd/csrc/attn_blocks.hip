@@ -2,39 +2,15 @@
 // one scale a block of rows (AttentionI8Blocks, 128).
 #include <hip/hip_runtime.h>
 
-#include <math.h>
-
-#include <type_traits>
-
-#include "holo_kernels.h"
-#include "packed_tile.h"
+#include "i8_rows.h"
 
 namespace holo {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
-
 // ---------------------------------------------------------- few-row form ----
 // Decode and drafts. Sixteen packed rows of a sequence and kv head (row r = token r /
-// G, head r % G) are a unit: the columns of the matrix instructions, which read each
-// byte of K and V once for all of them. The wavefronts of a workgroup take the 32-key
-// blocks of its share in turn. Per block and wavefront:
-//     S^T[32 keys x 16 rows] = K . Q^T    16x16x64 i8 on the cache's own bytes; a row
-//                                         of Q as 23-bit integers in three int8
-//                                         parts, its largest in [2^21, 2^22), so
-//                                         the products are exact
-//     scores, limits, online softmax      f32; a row is a lane column
-//     O^T[DP x 16 rows] += V^T . P^T      16x16x32 f16; an int8 is an exact f16, built
-//                                         by placing its byte under the exponent of
-//                                         1024
-// The scale of a 16-key step is one number (blocks are multiples of 16 keys): K's
-// joins the scores, V's the weights, w = p vs 2^(7 - ve) with 2^ve above every finite
-// |vs| of the keys the row sees so far. p is at most 2^8 (a row's maximum may lag that
-// far behind before its sums are rescaled), so |w| <= 2^15, and weights down to 2^-31
-// of the largest stay clear of f16's subnormals. 16-bit rows round w to f16 once, 11
-// bits where the result has 8 or 11; f32 rows hold it in two parts, 22 bits.
-// A row's sums, maximum and ve are its lanes' own, and a masked key's weight is 0 with
-// the scales of steps it does not see left out, so nothing reaches another row.
+// G, head r % G) are a unit, the columns of the matrix instructions (i8_rows.h). The
+// wavefronts of a workgroup take the 32-key blocks of its share in turn.
 //
 // Two splits. Direct: a workgroup of eight wavefronts a unit, no second launch; for
 // buckets up to kDirect rows and kDirectUnits units (one token of 8 kv heads of 128 dims
@@ -49,28 +25,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 // 528 MB, 106 us or 5.0 TB/s, merge_kernel 5 us of them, 108 us of f32 rows; 128 of 8192
 // keys, 2.2 GB, 6.6 TB/s. Short ones by their latency: 8 of 30 to 700 keys 9 us, up to three
 // rounds of a workgroup's 256 keys.
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef int i32x4 __attribute__((ext_vector_type(4)));
-constexpr uint32_t kUnit = 16, kStep = 32, kQuad = 128, kOob = 1u << 30;   // past every plane, twice it too
+constexpr uint32_t kQuad = 128;
 constexpr uint32_t kDirect = 1024, kDirectUnits = 640, kShares = 512, kMinQuads = 2;
-constexpr int kVeMin = -126;   // the floor of ve, where the result's own bits end
-
-// A step's factor of its weights, v 2^(7 - ve). An infinite scale's is 2^100, whose weights
-// are infinite in f16 where p is not 0 and 0 where it is: a key that the row does not see
-// brings it no NaN.
-__device__ __forceinline__ float weight_factor(float v, int ve) {
-    const float f = ldexpf(v, 7 - ve);
-    return fabsf(f) == INFINITY ? copysignf(0x1p100f, f) : f;
-}
-// A product as it is rounded to f32: the conversion to f16 behind it would else take the
-// product unrounded, and its two parts, of which one does and the other not, be a step of
-// f16 apart.
-__device__ __forceinline__ float rounded(float w) {
-    asm volatile("" : "+v"(w));
-    return w;
-}
-// What a weight of at most 2^15 leaves over its f16, as f16; nothing of an infinite one's.
-__device__ __forceinline__ float left_over(float w, float hi) { return fminf(fmaxf(w - hi, -16.0f), 16.0f); }
 
 struct Blocks {
     AttnBlocksArgs a;
@@ -80,58 +36,15 @@ struct Blocks {
     float *part;         // [places * Hkv + kShares][kUnit][DP + 2]: O, then the maximum and the sum
 };
 
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t range(const void *base, uint32_t bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, int(bytes), 0x00020000);
-}
-
-// The largest over a column's four lanes.
-__device__ __forceinline__ float column_max(float v) {
-    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-
-// Dim t of four (bytes of words w[0..7], one a key, xor 0x80) for the eight keys, as
-// f16: 1024 + byte by placement, less 1152.
-__device__ __forceinline__ f16x8 key_column(const uint32_t (&w)[8], int t) {
-    u32x4 m;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t two = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], t < 2 ? 0x05010400u : 0x07030602u);
-        m[i] = __builtin_amdgcn_perm(0x64646464u, two, t & 1 ? 0x04030402u : 0x04010400u);
-    }
-    return __builtin_bit_cast(f16x8, m) - (f16x8)(_Float16)1152.0f;
-}
-
-// One wavefront's state of a unit's 16 rows: O^T (dim NDB * (4 g + i) + d of row r in
-// o[d][i]), maximum, sum, ve.
-template <int DP>
-struct State {
-    f32x4 o[DP / 16];
-    float m, l;
-    int ve;
-};
-
-template <class E, int DP, int W>
-struct FewLds {
-    float o[W][kUnit][DP + 4];
-    float m[W][kUnit], l[W][kUnit];
-    int ve[W][kUnit];
-};
-
 // Keys [c0, c1) of unit `at.unit` of sequence at.b and kv head kh, by W wavefronts; the
 // joined result goes to `out` (whole) or to a partial at dst.
 template <class E, int DP, int W>
 __device__ __forceinline__ void few_segment(const Blocks &k, const Place &at, uint32_t kh, uint32_t c0, uint32_t c1,
                                             bool whole, float *dst, FewLds<E, DP, W> &lds) {
-    constexpr int NKS = DP / 64, NDB = DP / 16, VW = NDB / 4;
-    constexpr bool kF32 = std::is_same_v<E, F32>;
     typedef typename E::T T;
     const AttnBlocksArgs &a = k.a;
     const uint32_t G = a.H / a.Hkv, n = at.hi - at.lo, R = n * G;
-    const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
-    const uint32_t wave = pk_uni(uint32_t(tid) >> 6);
+    const uint32_t r = threadIdx.x & 15u, wave = pk_uni(threadIdx.x >> 6);
     const uint32_t row = at.unit * kUnit + r, tok = row / G;
     const bool live = row < R;
     const int64_t len = a.lens[at.b];
@@ -140,193 +53,29 @@ __device__ __forceinline__ void few_segment(const Blocks &k, const Place &at, ui
     const uint32_t kmin = visible_keys(len, n, first, a.bucket), kmax = visible_keys(len, n, last, a.bucket);
     const uint32_t end = pk_uni(c1 < kmax ? c1 : kmax);
     const uint64_t plane = uint64_t(at.b) * a.Hkv + kh;
-    const auto rk = range(a.kq + plane * a.bucket * a.D, a.bucket * a.D);
-    const auto rv = range(a.vq + plane * a.bucket * a.D, a.bucket * a.D);
+    const KvPlane<DP> kv(a.kq + plane * a.bucket * a.D, a.vq + plane * a.bucket * a.D, a.bucket, a.D);
     const uint32_t nb = (a.bucket + a.block - 1) >> k.shift;
     const float *ks = a.ks + plane * nb, *vs = a.vs + plane * nb;
-
-    // K: keys 16 h + r, bytes 64 s + 16 g on. V: keys 16 (j / 4) + 4 g + j % 4, bytes
-    // NDB r on.
-    uint32_t koff[NKS];
-#pragma unroll
-    for (int s = 0; s < NKS; ++s) koff[s] = uint32_t(64 * s + 16 * g) < a.D ? r * a.D + 64 * s + 16 * g : kOob;
-    const uint32_t voff = uint32_t(NDB * r) < a.D ? 4 * g * a.D + NDB * r : kOob;
-    struct Bytes {
-        u32x4 k[2][NKS];
-        uint32_t v[8][VW];
-        float ks[2], vs[2];
-    };
-    // (non-temporal: the cache is read once)
-    auto load = [&](uint32_t blk, Bytes &x) __attribute__((always_inline)) {
+    auto load = [&](uint32_t blk, KvStep<DP> &x) __attribute__((always_inline)) {
         const uint32_t so = blk < end ? blk * a.D : kOob;   // past the share: nothing is read
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int s = 0; s < NKS; ++s)
-                x.k[h][s] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, koff[s] + (so + 16 * h * a.D), 0, 2));
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const uint32_t o = voff + (so + (16 * (j >> 2) + (j & 3)) * a.D);
-            if constexpr (VW == 1) {
-                x.v[j][0] = __builtin_amdgcn_raw_buffer_load_b32(rv, o, 0, 2);
-            } else if constexpr (VW == 2) {
-                const auto w = __builtin_amdgcn_raw_buffer_load_b64(rv, o, 0, 2);
-                x.v[j][0] = w[0], x.v[j][1] = w[1];
-            } else {
-                const auto w = __builtin_amdgcn_raw_buffer_load_b128(rv, o, 0, 2);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x.v[j][i] = w[i];
-            }
-        }
+        kv.load({so, so + 16 * a.D}, x);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const uint32_t i = (blk + 16 * h) >> k.shift, c = i < nb ? i : nb - 1;
             x.ks[h] = ks[c], x.vs[h] = vs[c];
         }
     };
-    Bytes ring[2];
+    KvStep<DP> ring[2];
     const uint32_t mine = c0 + wave * kStep;
     load(mine, ring[0]);
-
-    // Q: dims 64 s + 16 g + e of the lane's row
-    float qv[16 * NKS], top = 0.0f;
-    {
-        const T *q = static_cast<const T *>(a.q) + uint64_t(at.lo + (live ? tok : 0u)) * a.q_stride +
-                     (uint64_t(kh) * G + (live ? row - tok * G : 0u)) * a.D;
-#pragma unroll
-        for (int s = 0; s < NKS; ++s) {
-            const uint32_t d = 64 * s + 16 * g;
-            const bool in = live && d < a.D;
-#pragma unroll
-            for (int w = 0; w < int(sizeof(T)); ++w) {
-                u32x4 x = {0, 0, 0, 0};
-                if (in) x = *reinterpret_cast<const u32x4 *>(q + d + w * (16 / sizeof(T)));
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float *to = qv + 16 * s + w * (16 / sizeof(T));
-                    if constexpr (kF32) {
-                        to[i] = __uint_as_float(x[i]);
-                    } else {
-                        to[2 * i] = E::widen(uint16_t(x[i]));
-                        to[2 * i + 1] = E::widen(uint16_t(x[i] >> 16));
-                    }
-                }
-            }
-        }
-    }
-    bool bad = false;      // a row with a NaN or infinity is NaN throughout
-#pragma unroll
-    for (int e = 0; e < 16 * NKS; ++e) {
-        top = fmaxf(top, fabsf(qv[e]));
-        bad |= !(fabsf(qv[e]) <= 3.4028235e38f);
-    }
-    top = column_max(top);
-    bad = column_max(bad ? 1.0f : 0.0f) != 0.0f;
-    int qe = 0;
-    if (top > 0.0f && top <= 3.4028235e38f) {
-        (void)frexpf(top, &qe);     // top < 2^qe
-        qe = 22 - qe;
-    }
-    i32x4 qp[3][NKS];
-#pragma unroll
-    for (int s = 0; s < NKS; ++s)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            uint32_t part[3] = {0, 0, 0};
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                int v = bad ? 0 : int(rintf(ldexpf(qv[16 * s + 4 * w + t], qe)));
-#pragma unroll
-                for (int p = 2; p >= 0; --p) {
-                    const int up = (v + 128) >> 8;
-                    part[p] |= uint32_t((p ? v - up * 256 : v) & 0xff) << (8 * t);
-                    v = up;
-                }
-            }
-#pragma unroll
-            for (int p = 0; p < 3; ++p) qp[p][s][w] = int(part[p]);
-        }
-    const float mul = bad ? __uint_as_float(0x7fc00000u) : ldexpf(k.mul, -qe);
-
+    RowQ<E, DP> q;
+    q.load(static_cast<const T *>(a.q) + uint64_t(at.lo + (live ? tok : 0u)) * a.q_stride +
+               (uint64_t(kh) * G + (live ? row - tok * G : 0u)) * a.D,
+           live, a.D, k.mul);
     State<DP> st;
-#pragma unroll
-    for (int d = 0; d < NDB; ++d) st.o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    st.m = -INFINITY, st.l = 0.0f, st.ve = kVeMin;
-    constexpr float kLag = 8.0f;
-    auto block = [&](uint32_t blk, const Bytes &x) __attribute__((always_inline)) {
-        float s[8], w[8];
-        float vs_h[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            i32x4 a0 = {0, 0, 0, 0}, a1 = {0, 0, 0, 0}, a2 = {0, 0, 0, 0};
-#pragma unroll
-            for (int c = 0; c < NKS; ++c) {
-                const i32x4 kf = __builtin_bit_cast(i32x4, x.k[h][c]);
-                a0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf, qp[0][c], a0, 0, 0, 0);
-                a1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf, qp[1][c], a1, 0, 0, 0);
-                a2 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf, qp[2][c], a2, 0, 0, 0);
-            }
-            const float c = x.ks[h] * mul;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[4 * h + i] = fmaf(float(a0[i]), 65536.0f, float(a1[i] * 256 + a2[i])) * c;
-            vs_h[h] = x.vs[h];
-        }
-        if (blk + kStep > kmin || blk + kStep > end) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t key = blk + 16 * h + 4 * g + i;
-                    s[4 * h + i] = key < lim && key < end ? s[4 * h + i] : -INFINITY;
-                }
-                vs_h[h] = blk + 16 * h < lim ? vs_h[h] : 0.0f;
-            }
-        }
-        float mt = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
-        mt = column_max(mt);
-        int ve = st.ve;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const float v = fabsf(vs_h[h]);
-            int e = kVeMin;
-            if (v > 0.0f && v <= 3.4028235e38f) (void)frexpf(v, &e);   // v < 2^e
-            ve = e > ve ? e : ve;
-        }
-        if (__any(mt > st.m + kLag || ve > st.ve)) {
-            const float mn = mt > st.m + kLag ? mt : st.m;
-            const float al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(st.m - mn);
-            st.l *= al;
-            const float sh = ldexpf(al, st.ve - ve);
-#pragma unroll
-            for (int d = 0; d < NDB; ++d) st.o[d] *= sh;
-            st.m = mn, st.ve = ve;
-        }
-        const float ref = st.m == -INFINITY ? 0.0f : st.m;
-        f16x8 hi, lo;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const float f = weight_factor(vs_h[h], ve);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float p = __builtin_amdgcn_exp2f(s[4 * h + i] - ref);
-                st.l += p;
-                w[4 * h + i] = kF32 ? rounded(p * f) : p * f;
-                hi[4 * h + i] = _Float16(w[4 * h + i]);
-                if constexpr (kF32) lo[4 * h + i] = _Float16(left_over(w[4 * h + i], float(hi[4 * h + i])));
-            }
-        }
-#pragma unroll
-        for (int q = 0; q < VW; ++q) {
-            uint32_t words[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) words[j] = x.v[j][q] ^ 0x80808080u;
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const f16x8 v = key_column(words, t);
-                st.o[4 * q + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, hi, st.o[4 * q + t], 0, 0, 0);
-                if constexpr (kF32) st.o[4 * q + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo, st.o[4 * q + t], 0, 0, 0);
-            }
-        }
+    st.clear();
+    auto block = [&](uint32_t blk, const KvStep<DP> &x) __attribute__((always_inline)) {
+        few_step<E, DP>(st, x, q, {blk, blk + 16}, blk + kStep > kmin || blk + kStep > end, lim, end);
     };
     for (uint32_t blk = mine; blk < end; blk += 2 * W * kStep) {
         load(blk + W * kStep, ring[1]);
@@ -335,31 +84,8 @@ __device__ __forceinline__ void few_segment(const Blocks &k, const Place &at, ui
         load(blk + 2 * W * kStep, ring[0]);
         block(blk + W * kStep, ring[1]);
     }
-
-    // The wavefronts' states joined: 2^(m_w - M) of each, their units of 2^(ve - 7) made
-    // one
-    st.l += __shfl_xor(st.l, 16, 64);
-    st.l += __shfl_xor(st.l, 32, 64);
-#pragma unroll
-    for (int d = 0; d < NDB; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) lds.o[wave][r][NDB * (4 * g + i) + d] = st.o[d][i];
-    if (g == 0) lds.m[wave][r] = st.m, lds.l[wave][r] = st.l, lds.ve[wave][r] = st.ve;
-    __syncthreads();
     const uint32_t rows = R - at.unit * kUnit < kUnit ? R - at.unit * kUnit : kUnit;
-    for (uint32_t i = tid; i < rows * a.D; i += 64 * W) {
-        const uint32_t c = i / a.D, d = i - c * a.D;
-        float M = lds.m[0][c];
-#pragma unroll
-        for (int w = 1; w < W; ++w) M = fmaxf(M, lds.m[w][c]);
-        const float ref = M == -INFINITY ? 0.0f : M;
-        float o = 0.0f, l = 0.0f;
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const float e = __builtin_amdgcn_exp2f(lds.m[w][c] - ref);
-            l += lds.l[w][c] * e;
-            o += ldexpf(lds.o[w][c][d], lds.ve[w][c] - 7) * e;
-        }
+    join_waves<E, DP, W>(st, rows, a.D, lds, [&](uint32_t c, uint32_t d, float o, float M, float l) {
         const uint32_t rr = at.unit * kUnit + c, t = rr / G;
         if (whole) {
             const bool none = visible_keys(len, n, t, a.bucket) == 0;
@@ -369,8 +95,7 @@ __device__ __forceinline__ void few_segment(const Blocks &k, const Place &at, ui
             dst[c * (DP + 2) + d] = o;
             if (d == 0) dst[c * (DP + 2) + DP] = M, dst[c * (DP + 2) + DP + 1] = l;
         }
-    }
-    __syncthreads();
+    });
 }
 
 // Direct: grid places * Hkv. Eight wavefronts a unit, past 128 dims four, whose registers
@@ -480,46 +205,6 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void few_shares_kernel(Block
         }
         base += all;
     }
-}
-
-// One row of `np` partials, `stride` floats from one to the next, joined in order by a
-// wavefront: its lanes take the partials' weights, 64 at a time, then the dims, eight
-// partials in flight.
-template <class E, int DP>
-__device__ __forceinline__ void join_row(const float *p, uint32_t stride, uint32_t np, uint32_t D, bool none,
-                                         typename E::T *out) {
-    const uint32_t lane = threadIdx.x & 63u;
-    float M = -INFINITY, l = 0.0f, o[DP / 64];
-    for (uint32_t w = lane; w < np; w += 64) M = fmaxf(M, p[w * stride + DP]);
-#pragma unroll
-    for (int x = 32; x >= 1; x >>= 1) M = fmaxf(M, __shfl_xor(M, x, 64));
-    const float ref = M == -INFINITY ? 0.0f : M;
-#pragma unroll
-    for (int i = 0; i < DP / 64; ++i) o[i] = 0.0f;
-    for (uint32_t w0 = 0; w0 < np; w0 += 64) {
-        const bool in = w0 + lane < np;
-        const float e = in ? __builtin_amdgcn_exp2f(p[(w0 + lane) * stride + DP] - ref) : 0.0f;
-        const float le = in ? p[(w0 + lane) * stride + DP + 1] * e : 0.0f;
-        const uint32_t many = np - w0 < 64 ? np - w0 : 64;
-        for (uint32_t w = 0; w < many; w += 8) {
-            float x[8][DP / 64];
-#pragma unroll
-            for (uint32_t q = 0; q < 8; ++q)
-#pragma unroll
-                for (int i = 0; i < DP / 64; ++i) x[q][i] = w + q < many ? p[(w0 + w + q) * stride + lane + 64 * i] : 0.0f;
-#pragma unroll
-            for (uint32_t q = 0; q < 8; ++q) {
-                if (w + q >= many) break;
-                const float ew = __shfl(e, int(w + q), 64);
-                l += __shfl(le, int(w + q), 64);
-#pragma unroll
-                for (int i = 0; i < DP / 64; ++i) o[i] = fmaf(x[q][i], ew, o[i]);
-            }
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < DP / 64; ++i)
-        if (lane + 64 * i < D) out[lane + 64 * i] = E::narrow(none ? 0.0f : o[i] / l);
 }
 
 // Joins the partials of a unit that shares cut: grid places * Hkv.

@@ -2,15 +2,175 @@
 // cache that each row's list names (AttentionI8Selected, 133).
 #include <hip/hip_runtime.h>
 
-#include "holo_kernels.h"
-#include "packed_batch.h"
+#include <algorithm>
+
+#include "i8_rows.h"
 
 namespace holo {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
+// -------------------------------------------------------------- matrix form ----
+// A unit is a token, a kv head and sixteen of its heads: the columns of the matrix
+// instructions (i8_rows.h). Its workgroup reads the list with the blocks' scales into LDS,
+// drops the tail that names nothing, and its wavefronts take the 32-key steps of the
+// blocks in turn.
+constexpr uint32_t kMaxList = 512;            // entries a workgroup takes
+constexpr uint32_t kNone = 0x80000000u;       // past every key
 
-// General form: one wavefront a token and head, any head_dim, block and alignment.
+struct Selected {
+    AttnSelectedArgs s;
+    float mul;           // log2(e) / divisor
+    uint32_t shift;      // block == 1 << shift
+    uint32_t tiles;      // of sixteen heads a kv head
+    uint32_t shares, per;   // of a list, and its entries each
+    float *part;         // [units][shares][kUnit][DP + 2]: O, then the maximum and the sum (-1: no key)
+};
+
+struct Entry {
+    uint32_t key;        // the block's first, kNone for none
+    float ks, vs;
+};
+
+template <class E, int DP, int W>
+__global__ __launch_bounds__(64 * W) void few_kernel(Selected k) {
+    typedef typename E::T T;
+    __shared__ FewLds<E, DP, W> lds;
+    __shared__ Entry list[kMaxList];
+    __shared__ uint32_t last;
+    const AttnBlocksArgs &a = k.s.a;
+    const uint32_t tid = threadIdx.x, wave = pk_uni(tid >> 6), share = blockIdx.y;
+    if (blockIdx.x == 0 && share == 0) check_starts(a.pb);
+    const uint32_t kh = blockIdx.x % a.Hkv, tile = blockIdx.x / a.Hkv % k.tiles, tok = blockIdx.x / a.Hkv / k.tiles;
+    RowAt at;
+    if (!row_of(a.pb, a.lens, tok, &at)) return;
+    const uint32_t sees = visible_keys(at.of, at.hi - at.lo, tok - at.lo, a.bucket), G = a.H / a.Hkv;
+    const uint64_t plane = uint64_t(at.b) * a.Hkv + kh, nb = (uint64_t(a.bucket) + a.block - 1) >> k.shift;
+    const uint32_t e0 = share * k.per, n = k.s.top - e0 < k.per ? k.s.top - e0 : k.per;
+    const int32_t *ids = k.s.blocks + (uint64_t(tok) * a.Hkv + kh) * k.s.top + e0;
+    if (tid == 0) last = 0;
+    __syncthreads();
+    for (uint32_t i = tid; i < n; i += 64 * W) {
+        const int32_t id = ids[i];
+        const bool ok = id >= 0 && uint64_t(id) << k.shift < sees;
+        const uint64_t j = plane * nb + (ok ? uint32_t(id) : 0u);
+        list[i] = Entry{ok ? uint32_t(id) << k.shift : kNone, a.ks[j], a.vs[j]};
+        if (ok) atomicMax(&last, i + 1);
+    }
+    const uint32_t r = tid & 15u, h0 = kh * G + tile * kUnit, rows = G - tile * kUnit < kUnit ? G - tile * kUnit : kUnit;
+    const bool live = r < rows;
+    RowQ<E, DP> q;
+    q.load(static_cast<const T *>(a.q) + uint64_t(tok) * a.q_stride + uint64_t(h0 + (live ? r : 0u)) * a.D, live, a.D, k.mul);
+    __syncthreads();
+    const uint32_t count = pk_uni(last), deep = k.shift - 4;              // 2^deep halves a block
+    const uint32_t halves = count << deep, steps = (halves + 1) / 2;
+    const KvPlane<DP> kv(a.kq + plane * a.bucket * a.D, a.vq + plane * a.bucket * a.D, a.bucket, a.D);
+    struct Keys {
+        uint32_t key[2];
+    };
+    auto load = [&](uint32_t step, KvStep<DP> &x, Keys &o) __attribute__((always_inline)) {
+        uint32_t so[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t half = 2 * step + h, i = half < halves ? half >> deep : 0u;
+            const Entry e = list[i];
+            const bool in = half < halves && e.key != kNone;
+            o.key[h] = pk_uni(in ? e.key + 16 * (half & ((1u << deep) - 1)) : kNone);
+            so[h] = o.key[h] == kNone ? kOob : o.key[h] * a.D;
+            x.ks[h] = e.ks, x.vs[h] = e.vs;
+        }
+        kv.load(so, x);
+    };
+    State<DP> st;
+    st.clear();
+    auto take = [&](const KvStep<DP> &x, const Keys &o) __attribute__((always_inline)) {
+        few_step<E, DP>(st, x, q, o.key, o.key[0] + 16 > sees || o.key[1] + 16 > sees, sees, sees);
+    };
+    KvStep<DP> ring[2];
+    Keys key[2];
+    if (wave < steps) load(wave, ring[0], key[0]);
+    for (uint32_t i = wave; i < steps; i += 2 * W) {
+        if (i + W < steps) load(i + W, ring[1], key[1]);
+        take(ring[0], key[0]);
+        if (i + W >= steps) break;
+        if (i + 2 * W < steps) load(i + 2 * W, ring[0], key[0]);
+        take(ring[1], key[1]);
+    }
+    float *dst = k.part + (uint64_t(blockIdx.x) * k.shares + share) * (kUnit * (DP + 2));
+    join_waves<E, DP, W>(st, rows, a.D, lds, [&](uint32_t c, uint32_t d, float o, float M, float l) {
+        if (k.shares == 1) {
+            static_cast<T *>(a.out)[(uint64_t(tok) * a.H + h0 + c) * a.D + d] = E::narrow(count ? o / l : 0.0f);
+        } else {
+            dst[c * (DP + 2) + d] = o;
+            if (d == 0) dst[c * (DP + 2) + DP] = M, dst[c * (DP + 2) + DP + 1] = count ? l : -1.0f;
+        }
+    });
+}
+
+// Joins the shares of a unit.
+template <class E, int DP>
+__global__ __launch_bounds__(256) void merge_kernel(Selected k) {
+    typedef typename E::T T;
+    const AttnBlocksArgs &a = k.s.a;
+    const uint32_t kh = blockIdx.x % a.Hkv, tile = blockIdx.x / a.Hkv % k.tiles, tok = blockIdx.x / a.Hkv / k.tiles;
+    RowAt at;
+    if (!row_of(a.pb, nullptr, tok, &at)) return;
+    const uint32_t G = a.H / a.Hkv, rows = G - tile * kUnit < kUnit ? G - tile * kUnit : kUnit;
+    constexpr uint32_t kStride = kUnit * (DP + 2);
+    const float *src = k.part + uint64_t(blockIdx.x) * k.shares * kStride;
+    const uint32_t lane = threadIdx.x & 63u;
+    bool any = false;
+    for (uint32_t w = lane; w < k.shares; w += 64) any |= !(src[w * kStride + DP + 1] < 0.0f);
+    const bool none = __ballot(any) == 0;
+    for (uint32_t c = pk_uni(threadIdx.x >> 6); c < rows; c += 4)
+        join_row<E, DP>(src + c * (DP + 2), kStride, k.shares, a.D, none,
+                        static_cast<T *>(a.out) + (uint64_t(tok) * a.H + kh * G + tile * kUnit + c) * a.D);
+}
+
+bool matrix_applies(const AttnSelectedArgs &s) {
+    const AttnBlocksArgs &a = s.a;
+    const uint32_t es = a.dtype == 8 ? 4 : 2;
+    const auto at16 = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+    return a.D <= 256 && a.D % 16 == 0 && a.block >= 16 && (a.block & (a.block - 1)) == 0 && at16(a.q) &&
+           uint64_t(a.q_stride) * es % 16 == 0 && at16(a.kq) && at16(a.vq);
+}
+uint32_t padded(uint32_t D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
+uint32_t tiles_of(const AttnBlocksArgs &a) { return (a.H / a.Hkv + kUnit - 1) / kUnit; }
+uint64_t units_of(const AttnBlocksArgs &a) { return uint64_t(a.pb.tokens) * a.Hkv * tiles_of(a); }
+// Entries a workgroup: the whole list (kMaxList of them at most), but where the units leave
+// CUs idle and the list is four rounds of eight wavefronts, shares for as many workgroups as
+// there are CUs, of four 32-key steps at least. One row of 8 kv heads over 2048 and 16384 keys
+// whole and in shares: 19 and 117 us against 11 and 17; 4 rows over 8192, 67 against 20; 16
+// over 2048, 24 against 21; 8 rows over 256, 6.0 against 8.2. Every share has an entry.
+uint32_t entries_of(const AttnSelectedArgs &s) {
+    const uint64_t units = units_of(s.a), steps = uint64_t(s.top) * s.a.block / kStep;
+    uint64_t shares = (s.top + kMaxList - 1) / kMaxList;
+    if (steps >= 32 && units < 256) shares = std::max(shares, std::min(256 / units, steps / 4));
+    shares = std::min<uint64_t>(shares, s.top);
+    return uint32_t((s.top + shares - 1) / shares);
+}
+uint32_t shares_of(const AttnSelectedArgs &s) { return (s.top + entries_of(s) - 1) / entries_of(s); }
+// Eight wavefronts a workgroup, four where there are two of them a CU and more (512 and 1024
+// units over 2048 keys each: 54 and 105 us with eight, 49 and 93 with four) and past 128 dims,
+// whose registers hold two steps.
+bool four_waves(const AttnSelectedArgs &s) { return s.a.D > 128 || units_of(s.a) >= 512; }
+
+template <class E, int DP>
+void launch_few(const Selected &k, hipStream_t stream) {
+    const dim3 grid(uint32_t(units_of(k.s.a)), k.shares);
+    constexpr int kMost = DP > 128 ? 4 : 8;
+    if (four_waves(k.s)) few_kernel<E, DP, 4><<<grid, 256, 0, stream>>>(k);
+    else few_kernel<E, DP, kMost><<<grid, 64 * kMost, 0, stream>>>(k);
+    if (k.shares > 1) merge_kernel<E, DP><<<grid.x, 256, 0, stream>>>(k);
+}
+template <class E>
+void launch_few(const Selected &k, hipStream_t stream) {
+    if (k.s.a.D <= 64) launch_few<E, 64>(k, stream);
+    else if (k.s.a.D <= 128) launch_few<E, 128>(k, stream);
+    else launch_few<E, 256>(k, stream);
+}
+
+// -------------------------------------------------------------- general form ----
+// One wavefront a token and head, any head_dim, block and alignment.
 struct BlockSrc {
     const int8_t *kp, *vp;
     const float *ks, *vs;
@@ -61,14 +221,27 @@ void launch(const AttnSelectedArgs &s, float mul, hipStream_t stream) {
 
 }  // namespace
 
-size_t attn_selected_scratch_bytes(const AttnSelectedArgs &) { return 0; }
+size_t attn_selected_scratch_bytes(const AttnSelectedArgs &s) {
+    if (!matrix_applies(s) || shares_of(s) == 1) return 0;
+    return size_t(units_of(s.a)) * shares_of(s) * kUnit * (padded(s.a.D) + 2) * 4;
+}
 
 uint64_t attn_selected_threads(const AttnSelectedArgs &s) {
+    if (matrix_applies(s)) return units_of(s.a) * shares_of(s) * (four_waves(s) ? 256 : 512);
     return (uint64_t(s.a.pb.tokens) * s.a.H + 3) / 4 * 256;
 }
 
-hipError_t launch_attn_selected(const AttnSelectedArgs &s, void *, hipStream_t stream) {
+hipError_t launch_attn_selected(const AttnSelectedArgs &s, void *scratch, hipStream_t stream) {
     const float mul = kLog2e / s.a.score_scale;
+    if (matrix_applies(s)) {
+        Selected k;
+        k.s = s, k.mul = mul, k.shift = uint32_t(__builtin_ctz(s.a.block)), k.tiles = tiles_of(s.a);
+        k.shares = shares_of(s), k.per = entries_of(s), k.part = static_cast<float *>(scratch);
+        if (s.a.dtype == 7) launch_few<Bf16>(k, stream);
+        else if (s.a.dtype == 6) launch_few<F16>(k, stream);
+        else launch_few<F32>(k, stream);
+        return hipGetLastError();
+    }
     if (s.a.dtype == 7) launch<Bf16>(s, mul, stream);
     else if (s.a.dtype == 6) launch<F16>(s, mul, stream);
     else launch<F32>(s, mul, stream);

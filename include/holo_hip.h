@@ -650,7 +650,7 @@ typedef struct holo_kv_block_select_call {
  * over, a block listed twice counts twice. Scores, softmax, roundings and the result as
  * in 128; a row that sees no key is zeros, and what a row does not see, blocks that its
  * list does not name among it, does not reach its result. kv_heads 0 means heads; head_dim
- * <= 1024; bucket_rows * head_dim <= 2^30; top <= 2^20; tokens * heads * (top / 4 + 1) <
+ * <= 1024; bucket_rows * head_dim <= 2^30; top <= 2^20; tokens * heads * (top / 512 + 1) <
  * 2^24 in any form. Long lists and few rows take scratch. */
 typedef struct holo_attention_i8_selected_call {
     holo_buffer_ref q;
