@@ -629,8 +629,8 @@ typedef struct holo_kv_block_bounds_call {
  * ceil(bucket_rows / block_rows), 2, head_dim]; k_scales f32 [batch * kv_heads,
  * ceil(bucket_rows / block_rows)]; lens u32 [batch], device-resident. kv_heads 0 means
  * heads; head_dim <= 1024, heads / kv_heads * head_dim <= 2^17, at most 2^20 blocks a
- * plane, kv_heads times those at most 2^28, top <= 2^20; (tokens + 16 batch) * kv_heads *
- * (blocks / 64 + 1) < 2^24 in any form. Takes scratch. */
+ * plane, kv_heads times those at most 2^28, top <= 2^20; in any form tokens * kv_heads <
+ * 2^24 and (tokens / 16 + batch) * kv_heads * (blocks / 256 + 1) < 2^24. Takes scratch. */
 typedef struct holo_kv_block_select_call {
     holo_buffer_ref q;
     holo_buffer_ref bounds;
