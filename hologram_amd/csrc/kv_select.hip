@@ -13,43 +13,127 @@ constexpr uint32_t kThreads = 256;
 // One workgroup a touched block and head, found as KvBlockAppend finds them: sequence s
 // owns the places [floor(starts[s] / block) + 2 s, floor(starts[s + 1] / block) + 2 (s +
 // 1)).
-__global__ __launch_bounds__(kThreads) void bounds_kernel(KvBoundsArgs a) {
-    __shared__ int lo_of[kPackedMaxDim], hi_of[kPackedMaxDim];
-    const uint32_t kh = blockIdx.x % a.Hkv, place = blockIdx.x / a.Hkv, tid = threadIdx.x;
+struct Touched {
+    const int8_t *src;       // its rows
+    int8_t *dst;
+    uint32_t rows;
+};
+__device__ __forceinline__ bool touched_block(const KvBoundsArgs &a, Touched *o) {
+    const uint32_t kh = blockIdx.x % a.Hkv, place = blockIdx.x / a.Hkv;
     if (blockIdx.x == 0) check_starts(a.pb);
-    const uint32_t b = last_at_most(a.pb.batch, place, [&](uint32_t s) {
-        return uint64_t(start_of(a.pb, s) / a.block) + 2ull * s;
-    });
-    const uint32_t r0 = start_of(a.pb, b), r1 = start_of(a.pb, b + 1);
-    if (r1 <= r0) return;
-    const uint64_t at = uint64_t(r0 / a.block) + 2ull * b;
-    if (place < at) return;
-    const uint64_t pos = a.pos[b], end = pos + (r1 - r0) < a.bucket ? pos + (r1 - r0) : a.bucket;
-    const uint64_t j = uint64_t(uint32_t(pos) / a.block) + (place - at), first = j * a.block;
-    if (pos >= end || first >= end) return;
-    const uint32_t rows = uint32_t(first + a.block < end ? a.block : end - first);
-    const uint64_t plane = uint64_t(b) * a.Hkv + kh, nb = (uint64_t(a.bucket) + a.block - 1) / a.block;
-    const int8_t *src = a.cache + (plane * a.bucket + first) * a.D;
-    int8_t *dst = a.bounds + (plane * nb + j) * 2 * a.D;
+    const auto place_at = [&](uint32_t v, uint32_t s) { return uint64_t(v / a.block) + 2ull * s; };
+    const RowAt at = sequence_at(a.pb, a.pos, place, place_at);
+    const uint64_t begin = place_at(at.lo, at.b);
+    if (at.hi <= at.lo || place < begin) return false;
+    const uint64_t pos = at.of, past = pos + (at.hi - at.lo), end = past < a.bucket ? past : a.bucket;
+    const uint64_t j = uint64_t(at.of / a.block) + (place - begin), first = j * a.block;
+    if (pos >= end || first >= end) return false;
+    const uint64_t plane = uint64_t(at.b) * a.Hkv + kh, nb = (uint64_t(a.bucket) + a.block - 1) / a.block;
+    o->rows = uint32_t(first + a.block < end ? a.block : end - first);
+    o->src = a.cache + (plane * a.bucket + first) * a.D;
+    o->dst = a.bounds + (plane * nb + j) * 2 * a.D;
+    return true;
+}
+
+// General form: an element a thread.
+__global__ __launch_bounds__(kThreads) void bounds_any_kernel(KvBoundsArgs a) {
+    __shared__ int lo_of[kPackedMaxDim], hi_of[kPackedMaxDim];
+    const uint32_t tid = threadIdx.x;
+    Touched t;
+    if (!touched_block(a, &t)) return;
     for (uint32_t d = tid; d < a.D; d += kThreads) lo_of[d] = 127, hi_of[d] = -128;
     __syncthreads();
-    for (uint32_t i = tid; i < rows * a.D; i += kThreads) {
-        const int v = src[i];
+    for (uint32_t i = tid; i < t.rows * a.D; i += kThreads) {
+        const int v = t.src[i];
         atomicMin(&lo_of[i % a.D], v);
         atomicMax(&hi_of[i % a.D], v);
     }
     __syncthreads();
-    for (uint32_t d = tid; d < a.D; d += kThreads) dst[d] = int8_t(lo_of[d]), dst[a.D + d] = int8_t(hi_of[d]);
+    for (uint32_t d = tid; d < a.D; d += kThreads) t.dst[d] = int8_t(lo_of[d]), t.dst[a.D + d] = int8_t(hi_of[d]);
+}
+
+// Wide form: sixteen bytes a thread and row, so many rows at once as 256 threads hold. A
+// byte's order is that of the 16-bit number whose upper half it is: two minima an
+// instruction. The threads' bounds then meet in LDS, P threads a word of the result.
+constexpr uint32_t kBoundsDim = 256;
+typedef short i16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t bytes_min(uint32_t x, uint32_t y) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(i16x2, x), __builtin_bit_cast(i16x2, y)));
+}
+__device__ __forceinline__ uint32_t bytes_max(uint32_t x, uint32_t y) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(i16x2, x), __builtin_bit_cast(i16x2, y)));
+}
+// Of four bytes the even and the odd ones as upper halves, and back.
+__device__ __forceinline__ uint32_t even_of(uint32_t w) { return (w << 8) & 0xff00ff00u; }
+__device__ __forceinline__ uint32_t odd_of(uint32_t w) { return w & 0xff00ff00u; }
+__device__ __forceinline__ uint32_t joined(uint32_t even, uint32_t odd) { return (even >> 8 & 0x00ff00ffu) | (odd & 0xff00ff00u); }
+
+template <int P>
+__global__ __launch_bounds__(kThreads) void bounds_kernel(KvBoundsArgs a) {
+    __shared__ __align__(16) uint32_t part[2][kThreads][4];      // smallest and largest, by thread
+    const uint32_t tid = threadIdx.x, per = a.D / 16, groups = kThreads / per, c = tid % per, g = tid / per;
+    Touched t;
+    if (!touched_block(a, &t)) return;
+    uint32_t lo[2][4], hi[2][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) lo[0][i] = lo[1][i] = 0x7f007f00u, hi[0][i] = hi[1][i] = 0x80008000u;
+    if (g < groups) {
+        const uint4 *row = reinterpret_cast<const uint4 *>(t.src) + c;
+        for (uint32_t r = g; r < t.rows; r += 4 * groups) {
+            uint4 v[4];
+#pragma unroll
+            for (uint32_t q = 0; q < 4; ++q)      // (a row past the block: the first one again)
+                v[q] = row[uint64_t(r + q * groups < t.rows ? r + q * groups : r) * per];
+#pragma unroll
+            for (uint32_t q = 0; q < 4; ++q) {
+                const uint32_t w[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t e = even_of(w[i]), o = odd_of(w[i]);
+                    lo[0][i] = bytes_min(lo[0][i], e), lo[1][i] = bytes_min(lo[1][i], o);
+                    hi[0][i] = bytes_max(hi[0][i], e), hi[1][i] = bytes_max(hi[1][i], o);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) part[0][tid][i] = joined(lo[0][i], lo[1][i]), part[1][tid][i] = joined(hi[0][i], hi[1][i]);
+    }
+    __syncthreads();
+    const uint32_t o = tid / P, p = tid % P, words = a.D / 4;
+    if (o >= 2 * words) return;
+    const bool large = o >= words;
+    const uint32_t word = large ? o - words : o, *from = &part[large][word / 4][word % 4];
+    uint32_t e = large ? 0x80008000u : 0x7f007f00u, d = e;
+    const uint32_t used = groups < t.rows ? groups : t.rows;
+    for (uint32_t i = p; i < used; i += P) {
+        const uint32_t w = from[i * per * 4];
+        e = large ? bytes_max(e, even_of(w)) : bytes_min(e, even_of(w));
+        d = large ? bytes_max(d, odd_of(w)) : bytes_min(d, odd_of(w));
+    }
+#pragma unroll
+    for (int x = P / 2; x >= 1; x >>= 1) {
+        const uint32_t e2 = __shfl_xor(e, x, 64), d2 = __shfl_xor(d, x, 64);
+        e = large ? bytes_max(e, e2) : bytes_min(e, e2);
+        d = large ? bytes_max(d, d2) : bytes_min(d, d2);
+    }
+    if (p == 0) reinterpret_cast<uint32_t *>(t.dst)[o] = joined(e, d);
 }
 
 uint32_t bounds_places(const KvBoundsArgs &a) { return (a.pb.tokens / a.block + 2 * a.pb.batch) * a.Hkv; }
 
 // ------------------------------------------------------------------ select ----
-// Two launches. The first leaves a row's sums over dims and heads of the larger of Q lo
-// and Q hi, whole numbers: with P[d] the sum over the kv head's heads of Q's positive
-// parts and N[d] of its negative ones, that is P . hi + N . lo (a negative scale: P . lo +
-// N . hi), one product for all heads. The second takes a row's scores, sum times scale,
-// exact in f64, and picks.
+// A row's sums over dims and heads of the larger of Q lo and Q hi are whole numbers: with
+// P[d] the sum over the kv head's heads of Q's positive parts and N[d] of its negative
+// ones, P . hi + N . lo (a negative scale: P . lo + N . hi), one product for all heads. The
+// pick takes the scores, sum times scale, exact in f64. Up to 640 blocks both are one
+// launch, the sums in LDS (whole_kernel); past that two, whose first reads the bounds with
+// as many workgroups as there are blocks to read (tile_sums_kernel, pick_kernel).
+// Bound by latency, the bytes are few: 32 rows over 2048 to 65536 keys in blocks of 32, 8 kv
+// heads of 128 dims, 40 MB of bounds, 21 us, 14 of them the sums (a workgroup's chain of search,
+// rows, bounds and store; 2.8 TB/s) and 7 the pick (a barrier a turn); 8 rows over up to 2000
+// keys 5.4 us; 2459 rows of four chunks over up to 30000 keys in blocks of 64, 37 us, a third
+// of the cycles in vector instructions of the pick, half of them waits. The general sums, and
+// a pick by eight bits at a time in LDS: 55, 9.4 and 437 us.
 struct Select {
     KvSelectArgs a;
     int32_t *sums;       // [row1 - row0][Hkv][nb]
@@ -201,13 +285,48 @@ __global__ __launch_bounds__(kThreads) void pick_any_kernel(Select k) {
     });
 }
 
-// The pick of at most 64 kWaves kHold blocks: kWaves wavefronts a row and kv head, a key
-// kHold a lane in registers. The border is found by halving the range of the keys' upper
-// words until `want` keys are at or above it (some twelve counts of ballots for scores that
-// lie evenly; 64 at most, which leaves equal keys).
-template <int kWaves, int kHold, class Sum>
-__device__ __forceinline__ void pick_row(const KvSelectArgs &a, uint32_t seen, Sum sum, const float *ks, int32_t *out,
-                                         uint32_t (*shared)[kWaves]) {
+// The largest over a wavefront, in every lane.
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    auto row = [&](auto ctrl) {
+        const uint32_t o = uint32_t(__builtin_amdgcn_update_dpp(0, int(v), decltype(ctrl)::value, 0xf, 0xf, true));
+        v = o > v ? o : v;
+    };
+    row(std::integral_constant<int, 0xb1>{});     // lane ^ 1
+    row(std::integral_constant<int, 0x4e>{});     // lane ^ 2
+    row(std::integral_constant<int, 0x141>{});    // 7 - lane of eight
+    row(std::integral_constant<int, 0x140>{});    // 15 - lane of sixteen
+    const auto x = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = x[0] > x[1] ? x[0] : x[1];
+    const auto y = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return y[0] > y[1] ? y[0] : y[1];
+}
+
+// Lanes before this one whose bit is set.
+__device__ __forceinline__ uint32_t before(uint64_t m) {
+    return __builtin_amdgcn_mbcnt_hi(uint32_t(m >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(m), 0u));
+}
+
+// A number in the scores' order, equal for some that are not: where the sums are below 2^24
+// (kSmall), the product in f32, one rounding, which keeps the order; else score_key's upper
+// word.
+template <bool kSmall>
+__device__ __forceinline__ uint32_t rough_key(int32_t sum, float scale) {
+    if constexpr (!kSmall) return uint32_t(score_key(sum, scale) >> 32);
+    float v = float(sum) * scale;
+    if (v != v) v = INFINITY;
+    const uint32_t u = __float_as_uint(v + 0.0f);
+    return u ^ (uint32_t(int32_t(u) >> 31) | 0x80000000u);
+}
+
+// The pick of at most 64 kWaves kHold blocks: kWaves wavefronts a row and kv head, kHold
+// rough keys a lane in registers. The border is found by halving their range until `want` of
+// them are at or above it, some ten counts of ballots for scores that lie evenly. Where that
+// leaves equal rough keys at the border, those are halved by their exact ones; what is
+// equal then goes by its order.
+// sum(j) and scale(j) may be asked for any j below 64 kWaves kHold.
+template <int kWaves, int kHold, bool kSmall, class Sum, class Scale>
+__device__ __forceinline__ void pick_row(const KvSelectArgs &a, uint32_t seen, Sum sum, Scale scale, int32_t *out,
+                                         uint64_t *shared) {
     const uint32_t lane = threadIdx.x & 63u, wave = kWaves == 1 ? 0u : pk_uni(threadIdx.x >> 6), tid = 64 * wave + lane;
     constexpr uint32_t kAll = 64 * kWaves;
     if (seen <= a.top) {
@@ -218,95 +337,145 @@ __device__ __forceinline__ void pick_row(const KvSelectArgs &a, uint32_t seen, S
     for (uint32_t i = tid; i < a.first; i += kAll) out[i] = int32_t(i);
     for (uint32_t i = tid; i < a.last; i += kAll) out[a.top - a.last + i] = int32_t(end + i);
     if (want == 0) return;
-    uint64_t key[kHold];
-    uint32_t low = 0xffffffffu, high = 0;
+    uint32_t key[kHold], high = 0, low = 0;      // (low: the complement of the smallest)
 #pragma unroll
     for (int q = 0; q < kHold; ++q) {
-        const uint32_t i = tid + q * kAll;
-        key[q] = 0;
-        if (i < n) {
-            key[q] = score_key(sum(a.first + i), ks[a.first + i]);
-            const uint32_t u = uint32_t(key[q] >> 32);
-            low = u < low ? u : low, high = u > high ? u : high;
-        }
+        const uint32_t j = tid + q * kAll;
+        const bool in = j - a.first < n;
+        const uint32_t k = rough_key<kSmall>(sum(j), scale(j));
+        key[q] = in ? k : 0u;                                    // (below every key)
+        high = key[q] > high ? key[q] : high;
+        const uint32_t down = in ? ~k : 0u;
+        low = down > low ? down : low;
     }
-    // what the wavefronts hold alike: a turn's numbers in one of two rows, so that one
+    // what the wavefronts hold, joined: a turn's numbers in one of two rows, so that one
     // barrier a turn is enough
     uint32_t turn = 0;
-    auto others = [&](uint32_t mine, auto join) {
+    auto others = [&](uint64_t mine, auto join) __attribute__((always_inline)) {
         if constexpr (kWaves == 1) return mine;
-        uint32_t *row = shared[turn];
+        uint64_t *row = shared + turn * kWaves;
         turn ^= 1;
         if (lane == 0) row[wave] = mine;
         __syncthreads();
-        uint32_t v = row[0];
+        uint64_t v = row[0];
 #pragma unroll
         for (int w = 1; w < kWaves; ++w) v = join(v, row[w]);
-        return pk_uni(v);
+        return uint64_t(pk_uni(uint32_t(v))) | uint64_t(pk_uni(uint32_t(v >> 32))) << 32;
     };
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) {
-        const uint32_t l = __shfl_xor(low, o, 64), h = __shfl_xor(high, o, 64);
-        low = l < low ? l : low, high = h > high ? h : high;
-    }
-    low = others(pk_uni(low), [](uint32_t x, uint32_t y) { return x < y ? x : y; });
-    high = others(pk_uni(high), [](uint32_t x, uint32_t y) { return x > y ? x : y; });
-    auto count = [&](uint64_t border) {
-        uint32_t c = 0;
-#pragma unroll
-        for (int q = 0; q < kHold; ++q) c += uint32_t(__popcll(__ballot(key[q] >= border)));
-        return others(c, [](uint32_t x, uint32_t y) { return x + y; });
+    const uint64_t ends = others(uint64_t(pk_uni(wave_max(low))) << 32 | pk_uni(wave_max(high)), [](uint64_t x, uint64_t y) {
+        const uint32_t xl = uint32_t(x), yl = uint32_t(y), xh = uint32_t(x >> 32), yh = uint32_t(y >> 32);
+        return uint64_t(xh > yh ? xh : yh) << 32 | (xl > yl ? xl : yl);
+    });
+    // The border of the `want` largest of `all`: at lo and above are `want` or more, at hi and
+    // above fewer. Several wavefronts take three borders a turn: half the turns, each a barrier.
+    constexpr int kBorders = kWaves == 1 ? 1 : 3;
+    struct Border {
+        uint64_t at;
+        uint32_t from, above;      // keys at it and above, keys above it
     };
-    // at lo and above are `want` or more, at hi and above fewer
-    uint64_t lo = uint64_t(low) << 32, hi = (uint64_t(high) + 1) << 32;
-    uint32_t at_lo = n, at_hi = 0;
-    while (at_lo != want && hi - lo > 1) {
-        const uint64_t mid = lo + (hi - lo) / 2;
-        const uint32_t c = count(mid);
-        if (c >= want) lo = mid, at_lo = c;
-        else hi = mid, at_hi = c;
-    }
-    // those above the border, and of those at it the first (all, but for equal keys)
-    const bool exact = at_lo == want;
-    const uint32_t left = exact ? 0u : want - at_hi;
-    const uint64_t sure = exact ? lo : hi;
-    uint32_t above = 0, ties = 0;
+    auto halve = [&](auto lo, auto hi, uint32_t all, uint32_t want, auto at_least) __attribute__((always_inline)) {
+        uint32_t at_lo = all, at_hi = 0;
+        while (at_lo != want && hi - lo > 1) {
+            const auto half = (hi - lo) / 2;
+            if constexpr (kBorders == 1) {
+                const auto mid = lo + half;
+                uint32_t c = 0;
 #pragma unroll
-    for (int q = 0; q < kHold; ++q) {
-        const bool more = key[q] >= sure, tie = !exact && key[q] == lo;
-        const uint64_t m = __ballot(more), t = __ballot(tie), before = (1ull << lane) - 1;
-        uint32_t ab = above, tb = ties;
+                for (int q = 0; q < kHold; ++q) c += uint32_t(__popcll(__ballot(at_least(q, mid))));
+                const bool up = c >= want;
+                lo = up ? mid : lo, at_lo = up ? c : at_lo;
+                hi = up ? hi : mid, at_hi = up ? at_hi : c;
+            } else {
+                const auto part = (hi - lo) / 4, m0 = lo + part, m1 = lo + half, m2 = m1 + part;
+                uint32_t c[3] = {0, 0, 0};
+#pragma unroll
+                for (int q = 0; q < kHold; ++q) {
+                    c[0] += uint32_t(__popcll(__ballot(at_least(q, m0))));
+                    c[1] += uint32_t(__popcll(__ballot(at_least(q, m1))));
+                    c[2] += uint32_t(__popcll(__ballot(at_least(q, m2))));
+                }
+                const uint64_t sum = others(c[0] | uint64_t(c[1]) << 20 | uint64_t(c[2]) << 40,
+                                            [](uint64_t x, uint64_t y) { return x + y; });
+                const uint32_t c0 = uint32_t(sum) & 0xfffffu, c1 = uint32_t(sum >> 20) & 0xfffffu, c2 = uint32_t(sum >> 40);
+                // (a count of `want` is met by the highest border that has it)
+                const bool u0 = c0 >= want, u1 = c1 >= want, u2 = c2 >= want;
+                hi = u2 ? hi : u1 ? m2 : u0 ? m1 : m0, at_hi = u2 ? at_hi : u1 ? c2 : u0 ? c1 : c0;
+                lo = u2 ? m2 : u1 ? m1 : u0 ? m0 : lo, at_lo = u2 ? c2 : u1 ? c1 : u0 ? c0 : at_lo;
+            }
+        }
+        return Border{lo, at_lo, at_hi};
+    };
+    const uint32_t least = ~uint32_t(ends >> 32), past = uint32_t(ends) + 1;
+    const Border rough = halve(least, past, n, want, [&](int q, uint32_t mid) { return key[q] >= mid; });
+    const uint32_t lo = uint32_t(rough.at), at_lo = rough.from, at_hi = rough.above;
+    // Lanes that hold a bit of `m`, in the blocks' order: how many before this one of key q
+    uint32_t seen_before = 0;
+    auto place = [&](uint64_t m) __attribute__((always_inline)) {
+        uint32_t at = seen_before;
         if constexpr (kWaves == 1) {
-            above += uint32_t(__popcll(m)), ties += uint32_t(__popcll(t));
+            seen_before += uint32_t(__popcll(m));
         } else {
-            const uint32_t packed = uint32_t(__popcll(m)) | uint32_t(__popcll(t)) << 16;
-            uint32_t *row = shared[turn];
+            uint64_t *row = shared + turn * kWaves;
             turn ^= 1;
-            if (lane == 0) row[wave] = packed;
+            if (lane == 0) row[wave] = uint64_t(__popcll(m));
             __syncthreads();
 #pragma unroll
             for (uint32_t w = 0; w < kWaves; ++w) {
-                ab += w < wave ? row[w] & 0xffffu : 0u, tb += w < wave ? row[w] >> 16 : 0u;
-                above += row[w] & 0xffffu, ties += row[w] >> 16;
+                at += w < wave ? uint32_t(row[w]) : 0u;
+                seen_before += uint32_t(row[w]);
             }
         }
-        ab += uint32_t(__popcll(m & before)), tb += uint32_t(__popcll(t & before));
-        if (more || (tie && tb < left)) out[a.first + ab + (tb < left ? tb : left)] = int32_t(a.first + tid + q * kAll);
+        return at + before(m);
+    };
+    int32_t *to = out + a.first;
+    if (at_lo == want) {
+#pragma unroll
+        for (int q = 0; q < kHold; ++q) {
+            const bool chosen = key[q] >= lo;
+            const uint32_t at = place(__ballot(chosen));
+            if (chosen) to[at] = int32_t(tid + q * kAll);
+        }
+        return;
+    }
+    uint64_t exact[kHold];
+    const uint32_t need = want - at_hi;
+#pragma unroll
+    for (int q = 0; q < kHold; ++q) {
+        const uint32_t j = tid + q * kAll;
+        exact[q] = key[q] == lo ? score_key(sum(j), scale(j)) : 0;
+    }
+    const Border fine = halve(uint64_t(1), ~uint64_t(0), at_lo - at_hi, need, [&](int q, uint64_t mid) { return exact[q] >= mid; });
+    // of the equal ones at the last border the first `left`
+    const uint64_t sure = fine.from == need ? fine.at : fine.at + 1;
+    const uint32_t left = fine.from == need ? 0u : need - fine.above;
+    uint32_t chosen = 0;      // a bit a held key
+#pragma unroll
+    for (int q = 0; q < kHold; ++q) {
+        const bool more = key[q] > lo || (key[q] == lo && exact[q] >= sure), tie = key[q] == lo && exact[q] == fine.at && !more;
+        const uint32_t at = place(__ballot(tie));
+        chosen |= uint32_t(more || (tie && at < left)) << q;
+    }
+    seen_before = 0;
+#pragma unroll
+    for (int q = 0; q < kHold; ++q) {
+        const bool in = chosen >> q & 1;
+        const uint32_t at = place(__ballot(in));
+        if (in) to[at] = int32_t(tid + q * kAll);
     }
 }
 
-template <int kWaves, int kHold>
+template <int kHold, bool kSmall>
 __global__ __launch_bounds__(256) void pick_kernel(Select k) {
-    __shared__ uint32_t shared[2][kWaves];
+    __shared__ uint64_t shared[8];
     const KvSelectArgs &a = k.a;
-    const uint32_t unit = kWaves == 1 ? blockIdx.x * 4 + pk_uni(threadIdx.x >> 6) : blockIdx.x;
-    const uint32_t tok = k.row0 + unit / a.Hkv, kh = unit % a.Hkv;
+    const uint32_t tok = k.row0 + blockIdx.x / a.Hkv, kh = blockIdx.x % a.Hkv;
     RowAt at;
-    if (tok >= k.row1 || !row_of(a.pb, a.lens, tok, &at)) return;
+    if (!row_of(a.pb, a.lens, tok, &at)) return;
     const int32_t *sums = k.sums + (uint64_t(tok - k.row0) * a.Hkv + kh) * k.nb;
-    pick_row<kWaves, kHold>(a, blocks_seen(a, at.of, at.hi - at.lo, tok - at.lo), [&](uint32_t j) { return sums[j]; },
-                            a.ks + (uint64_t(at.b) * a.Hkv + kh) * k.nb, a.out + (uint64_t(tok) * a.Hkv + kh) * a.top,
-                            shared);
+    const float *ks = a.ks + (uint64_t(at.b) * a.Hkv + kh) * k.nb;
+    const auto in = [&](uint32_t j) { return j < k.nb ? j : k.nb - 1; };
+    pick_row<4, kHold, kSmall>(a, blocks_seen(a, at.of, at.hi - at.lo, tok - at.lo), [&](uint32_t j) { return sums[in(j)]; },
+                                    [&](uint32_t j) { return ks[in(j)]; }, a.out + (uint64_t(tok) * a.Hkv + kh) * a.top, shared);
 }
 
 // ------------------------------------------------- the sums in matrix form ----
@@ -330,20 +499,31 @@ __device__ __forceinline__ void split_rows(const KvSelectArgs &a, uint32_t lo, u
     constexpr int VD = DP / 16;
     const uint32_t tid = threadIdx.x, row = tid >> 4, d0 = VD * (tid & 15u), G = a.H / a.Hkv;
     const bool live = row < m && d0 < a.D;
+    if (row >= kTile) return;
     const T *q = static_cast<const T *>(a.q) + uint64_t(lo + t0 + (live ? row : 0u)) * a.q_stride + uint64_t(kh) * G * a.D + d0;
     struct Dims {
         T x[VD];
     };
-    uint32_t top = 0;
-    if (live)
-        for (uint32_t h = 0; h < G; ++h) {
-            const Dims v = *reinterpret_cast<const Dims *>(__builtin_assume_aligned(q + h * a.D, sizeof(Dims) < 16 ? sizeof(Dims) : 16));
+    constexpr uint32_t kHeld = 4;      // heads in registers between the two, asked for at once
+    auto head = [&](uint32_t h) {
+        return *reinterpret_cast<const Dims *>(__builtin_assume_aligned(q + h * a.D, sizeof(Dims) < 16 ? sizeof(Dims) : 16));
+    };
+    Dims held[kHeld] = {};
 #pragma unroll
-            for (int e = 0; e < VD; ++e) {
-                const uint32_t u = __float_as_uint(E::widen(v.x[e])) & 0x7fffffffu;
-                if (u < 0x7f800000u && u > top) top = u;
-            }
+    for (uint32_t h = 0; h < kHeld; ++h)
+        if (live && h < G) held[h] = head(h);
+    uint32_t top = 0;
+    auto see = [&](const Dims &v) {
+#pragma unroll
+        for (int e = 0; e < VD; ++e) {
+            const uint32_t u = __float_as_uint(E::widen(v.x[e])) & 0x7fffffffu;
+            if (u < 0x7f800000u && u > top) top = u;
         }
+    };
+#pragma unroll
+    for (uint32_t h = 0; h < kHeld; ++h) see(held[h]);
+    if (live)
+        for (uint32_t h = kHeld; h < G; ++h) see(head(h));
 #pragma unroll
     for (int o = 8; o >= 1; o >>= 1) {
         const uint32_t u = __shfl_xor(top, o, 64);
@@ -351,15 +531,17 @@ __device__ __forceinline__ void split_rows(const KvSelectArgs &a, uint32_t lo, u
     }
     const float inv = top ? 1.0f / block_scale(top) : 0.0f;
     int p[VD] = {}, n[VD] = {};
-    if (live)
-        for (uint32_t h = 0; h < G; ++h) {
-            const Dims v = *reinterpret_cast<const Dims *>(__builtin_assume_aligned(q + h * a.D, sizeof(Dims) < 16 ? sizeof(Dims) : 16));
+    auto add = [&](const Dims &v) {
 #pragma unroll
-            for (int e = 0; e < VD; ++e) {
-                const int x = q8(E::widen(v.x[e]), inv);
-                p[e] += x > 0 ? x : 0, n[e] += x < 0 ? x : 0;
-            }
+        for (int e = 0; e < VD; ++e) {
+            const int x = q8(E::widen(v.x[e]), inv);
+            p[e] += x > 0 ? x : 0, n[e] += x < 0 ? x : 0;
         }
+    };
+#pragma unroll
+    for (uint32_t h = 0; h < kHeld; ++h) add(held[h]);
+    if (live)
+        for (uint32_t h = kHeld; h < G; ++h) add(head(h));
 #pragma unroll
     for (int w = 0; w < VD / 4; ++w) {
         uint32_t out[4] = {0, 0, 0, 0};
@@ -375,64 +557,78 @@ __device__ __forceinline__ void split_rows(const KvSelectArgs &a, uint32_t lo, u
     }
 }
 
-// The sums of blocks [j0, j1) for the rows in `parts`, by four wavefronts, sixteen blocks a
-// step: put(row, block, four blocks' sums).
-template <int DP, class Put>
-__device__ __forceinline__ void tile_sums(const KvSelectArgs &a, uint64_t plane, uint32_t nb, uint32_t j0, uint32_t j1,
-                                          const QParts<DP> &parts, Put put) {
-    constexpr int NKS = DP / 64;
-    const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, g = lane >> 4, wave = pk_uni(threadIdx.x >> 6);
-    const auto src = range(a.bounds + plane * nb * 2 * a.D, nb * 2 * a.D);
-    const float *ks = a.ks + plane * nb;
+// The sums of blocks [j0, j1) of a plane for the rows in `parts`, by W wavefronts, sixteen
+// blocks a step. start() asks for a wavefront's first two steps, run() calls put(row, block,
+// four blocks' sums).
+template <int DP, int W>
+struct TileSums {
+    static constexpr int NKS = DP / 64, kDepth = 2;
+    static constexpr uint32_t kNext = W * kTile;
     struct Bytes {
         i32x4 lo[NKS], hi[NKS];
         float scale;
     };
-    auto load = [&](uint32_t jt, Bytes &x) __attribute__((always_inline)) {
-        const uint32_t j = jt + r, at = j < j1 ? j * 2 * a.D + 16 * g : kOob;
+    __amdgpu_buffer_rsrc_t src;
+    const float *ks;
+    uint32_t D, j0, j1, jt;
+    Bytes ring[kDepth];
+
+    __device__ __forceinline__ void load(uint32_t from, Bytes &x) const {
+        const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, g = lane >> 4;
+        const uint32_t j = from + r, at = j < j1 ? j * 2 * D + 16 * g : kOob;
 #pragma unroll
         for (int s = 0; s < NKS; ++s) {
-            const uint32_t o = 64 * s + 16 * g < a.D ? at + 64 * s : kOob;
+            const uint32_t o = 64 * s + 16 * g < D ? at + 64 * s : kOob;
             x.lo[s] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(src, o, 0, 0));
-            x.hi[s] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(src, o + a.D, 0, 0));
+            x.hi[s] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(src, o + D, 0, 0));
         }
         x.scale = ks[j < j1 ? j : j0];
-    };
-    i32x4 part[4][NKS];
+    }
+    __device__ __forceinline__ void start(const KvSelectArgs &a, uint64_t plane, uint32_t nb, uint32_t first, uint32_t end) {
+        src = range(a.bounds + plane * nb * 2 * a.D, nb * 2 * a.D);
+        ks = a.ks + plane * nb, D = a.D, j0 = first, j1 = end, jt = j0 + kTile * pk_uni(threadIdx.x >> 6);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < kDepth; ++i)
+            if (jt + i * kNext < j1) load(jt + i * kNext, ring[i]);
+    }
+    template <class Put>
+    __device__ __forceinline__ void run(const QParts<DP> &parts, Put put) {
+        const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, g = lane >> 4;
+        i32x4 part[4][NKS];
 #pragma unroll
-        for (int s = 0; s < NKS; ++s) part[i][s] = *reinterpret_cast<const i32x4 *>(&parts.b[i][r][64 * s + 16 * g]);
-    auto step = [&](uint32_t jt, Bytes &x) __attribute__((always_inline)) {
-        if (__any(x.scale < 0.0f)) {
-            const bool turn = x.scale < 0.0f;
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int s = 0; s < NKS; ++s) part[i][s] = *reinterpret_cast<const i32x4 *>(&parts.b[i][r][64 * s + 16 * g]);
+        auto step = [&](uint32_t from, Bytes &x) __attribute__((always_inline)) {
+            if (__any(x.scale < 0.0f)) {
+                const bool turn = x.scale < 0.0f;
+#pragma unroll
+                for (int s = 0; s < NKS; ++s) {
+                    const i32x4 lo = x.lo[s], hi = x.hi[s];
+                    x.lo[s] = turn ? hi : lo, x.hi[s] = turn ? lo : hi;
+                }
+            }
+            i32x4 up = {0, 0, 0, 0}, down = {0, 0, 0, 0};
 #pragma unroll
             for (int s = 0; s < NKS; ++s) {
-                const i32x4 lo = x.lo[s], hi = x.hi[s];
-                x.lo[s] = turn ? hi : lo, x.hi[s] = turn ? lo : hi;
+                up = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.hi[s], part[0][s], up, 0, 0, 0);
+                down = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.hi[s], part[1][s], down, 0, 0, 0);
+                up = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.lo[s], part[2][s], up, 0, 0, 0);
+                down = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.lo[s], part[3][s], down, 0, 0, 0);
+            }
+            put(r, from + 4 * g, up * 256 + down);
+        };
+        while (jt < j1) {
+#pragma unroll
+            for (int i = 0; i < kDepth; ++i) {
+                if (jt >= j1) break;
+                step(jt, ring[i]);
+                if (jt + kDepth * kNext < j1) load(jt + kDepth * kNext, ring[i]);
+                jt += kNext;
             }
         }
-        i32x4 up = {0, 0, 0, 0}, down = {0, 0, 0, 0};
-#pragma unroll
-        for (int s = 0; s < NKS; ++s) {
-            up = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.hi[s], part[0][s], up, 0, 0, 0);
-            down = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.hi[s], part[1][s], down, 0, 0, 0);
-            up = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.lo[s], part[2][s], up, 0, 0, 0);
-            down = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.lo[s], part[3][s], down, 0, 0, 0);
-        }
-        put(r, jt + 4 * g, up * 256 + down);
-    };
-    Bytes ring[2];
-    uint32_t jt = j0 + kTile * wave;
-    if (jt < j1) load(jt, ring[0]);
-    for (; jt < j1; jt += 8 * kTile) {
-        load(jt + 4 * kTile, ring[1]);
-        step(jt, ring[0]);
-        if (jt + 4 * kTile >= j1) break;
-        load(jt + 8 * kTile, ring[0]);
-        step(jt + 4 * kTile, ring[1]);
     }
-}
+};
 
 // The sums alone, kRange blocks a workgroup: grid places * Hkv, ranges.
 constexpr uint32_t kRange = 256;
@@ -442,14 +638,17 @@ __global__ __launch_bounds__(256) void tile_sums_kernel(Select k) {
     const KvSelectArgs &a = k.a;
     if (blockIdx.x == 0 && blockIdx.y == 0) check_starts(a.pb);
     Place at;
-    if (!place_of(a.pb, 1, kTile, blockIdx.x / a.Hkv, &at)) return;
+    uint32_t len;
+    if (!place_of(a.pb, 1, kTile, blockIdx.x / a.Hkv, &at, a.lens, &len)) return;
     const uint32_t kh = blockIdx.x % a.Hkv, n = at.hi - at.lo, t0 = at.unit * kTile, m = n - t0 < kTile ? n - t0 : kTile;
-    const uint32_t first = at.lo + t0, seen = blocks_seen(a, a.lens[at.b], n, t0 + m - 1), j0 = blockIdx.y * kRange;
+    const uint32_t first = at.lo + t0, seen = blocks_seen(a, len, n, t0 + m - 1), j0 = blockIdx.y * kRange;
     if (first + m <= k.row0 || first >= k.row1 || seen <= a.top || j0 >= seen - a.last) return;
     const uint32_t end = seen - a.last, j1 = end - j0 < kRange ? end : j0 + kRange;
+    TileSums<DP, 4> tiles;
+    tiles.start(a, uint64_t(at.b) * a.Hkv + kh, k.nb, j0, j1);
     split_rows<E, DP>(a, at.lo, t0, m, kh, parts);
     __syncthreads();
-    tile_sums<DP>(a, uint64_t(at.b) * a.Hkv + kh, k.nb, j0, j1, parts, [&](uint32_t r, uint32_t j, i32x4 v) {
+    tiles.run(parts, [&](uint32_t r, uint32_t j, i32x4 v) {
         if (r >= m || first + r < k.row0 || first + r >= k.row1) return;
         int32_t *to = k.sums + (uint64_t(first + r - k.row0) * a.Hkv + kh) * k.nb + j;
 #pragma unroll
@@ -458,31 +657,37 @@ __global__ __launch_bounds__(256) void tile_sums_kernel(Select k) {
     });
 }
 
-// Sums and pick in one launch, the sums of sixteen rows in LDS: for up to kWhole blocks.
-constexpr uint32_t kWhole = 640;
-template <class E, int DP, int kHold>
-__global__ __launch_bounds__(256) void whole_kernel(Select k) {
+// Sums and pick in one launch, the sums of kRows rows in LDS, for at most kMost blocks.
+constexpr uint32_t kRows = 16;
+constexpr int kWaves = 8;
+template <class E, int DP, int kMost, bool kSmall>
+__global__ __launch_bounds__(64 * kWaves) void whole_kernel(Select k) {
     __shared__ QParts<DP> parts;
-    extern __shared__ __align__(16) int32_t sums[];       // [kTile][pitch]
+    __shared__ __align__(16) int32_t sums[kRows][kMost + 4];
+    __shared__ float scale_of[kMost];
     const KvSelectArgs &a = k.a;
     if (blockIdx.x == 0) check_starts(a.pb);
     Place at;
-    if (!place_of(a.pb, 1, kTile, blockIdx.x / a.Hkv, &at)) return;
-    const uint32_t kh = blockIdx.x % a.Hkv, n = at.hi - at.lo, t0 = at.unit * kTile, m = n - t0 < kTile ? n - t0 : kTile;
-    const uint32_t len = a.lens[at.b], seen = blocks_seen(a, len, n, t0 + m - 1), pitch = k.nb + 4 + (4 - k.nb % 4) % 4;
+    uint32_t len;
+    if (!place_of(a.pb, 1, kRows, blockIdx.x / a.Hkv, &at, a.lens, &len)) return;
+    const uint32_t kh = blockIdx.x % a.Hkv, n = at.hi - at.lo, t0 = at.unit * kRows, m = n - t0 < kRows ? n - t0 : kRows;
+    const uint32_t seen = blocks_seen(a, len, n, t0 + m - 1);
     const uint64_t plane = uint64_t(at.b) * a.Hkv + kh;
     if (seen > a.top) {
+        const uint32_t j1 = seen - a.last;
+        TileSums<DP, kWaves> tiles;
+        tiles.start(a, plane, k.nb, 0, j1);
+        for (uint32_t j = threadIdx.x; j < j1; j += 64 * kWaves) scale_of[j] = a.ks[plane * k.nb + j];
         split_rows<E, DP>(a, at.lo, t0, m, kh, parts);
         __syncthreads();
-        const uint32_t j1 = seen - a.last;
-        tile_sums<DP>(a, plane, k.nb, 0, j1, parts, [&](uint32_t r, uint32_t j, i32x4 v) {
-            if (j < j1) *reinterpret_cast<i32x4 *>(sums + r * pitch + j) = v;
+        tiles.run(parts, [&](uint32_t r, uint32_t j, i32x4 v) {
+            if (r < m && j < j1) *reinterpret_cast<i32x4 *>(&sums[r][j]) = v;
         });
         __syncthreads();
     }
-    for (uint32_t t = pk_uni(threadIdx.x >> 6); t < m; t += 4)
-        pick_row<1, kHold>(a, blocks_seen(a, len, n, t0 + t), [&](uint32_t j) { return sums[t * pitch + j]; },
-                           a.ks + plane * k.nb, a.out + (uint64_t(at.lo + t0 + t) * a.Hkv + kh) * a.top, nullptr);
+    for (uint32_t t = pk_uni(threadIdx.x >> 6); t < m; t += kWaves)
+        pick_row<1, kMost / 64, kSmall>(a, blocks_seen(a, len, n, t0 + t), [&](uint32_t j) { return sums[t][j]; },
+                                        [&](uint32_t j) { return scale_of[j]; }, a.out + (uint64_t(at.lo + t0 + t) * a.Hkv + kh) * a.top, nullptr);
 }
 
 uint32_t blocks_of(const KvSelectArgs &a) { return uint32_t((uint64_t(a.bucket) + a.block - 1) / a.block); }
@@ -499,19 +704,27 @@ bool matrix_applies(const KvSelectArgs &a) {
     return a.D <= 256 && a.D % 16 == 0 && a.H / a.Hkv <= 128 && reinterpret_cast<uintptr_t>(a.bounds) % 16 == 0 &&
            reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && uint64_t(a.q_stride) * es % 16 == 0;
 }
-uint32_t places_of(const KvSelectArgs &a) { return a.pb.tokens / kTile + a.pb.batch; }
-bool whole(const KvSelectArgs &a) { return matrix_applies(a) && blocks_of(a) <= kWhole; }
+bool whole(const KvSelectArgs &a) { return matrix_applies(a) && blocks_of(a) <= 640; }
+uint32_t places_of(const KvSelectArgs &a) { return a.pb.tokens / (whole(a) ? kRows : kTile) + a.pb.batch; }
+bool small_sums(const KvSelectArgs &a) { return uint64_t(a.H / a.Hkv) * a.D * 127 * 128 < (1u << 24); }
 
+template <class E, int DP, bool kSmall>
+void launch_whole(const Select &k, hipStream_t stream) {
+    const uint32_t grid = places_of(k.a) * k.a.Hkv;
+    if (k.nb <= 256) whole_kernel<E, DP, 256, kSmall><<<grid, 64 * kWaves, 0, stream>>>(k);
+    else if (k.nb <= 512) whole_kernel<E, DP, 512, kSmall><<<grid, 64 * kWaves, 0, stream>>>(k);
+    else whole_kernel<E, DP, 640, kSmall><<<grid, 64 * kWaves, 0, stream>>>(k);
+}
 template <class E, int DP>
 void launch_tiles(const Select &k, hipStream_t stream) {
-    const uint32_t grid = places_of(k.a) * k.a.Hkv;
     if (!whole(k.a)) {
-        if (k.nb > k.a.top) tile_sums_kernel<E, DP><<<dim3(grid, (k.nb + kRange - 1) / kRange), 256, 0, stream>>>(k);
-        return;
+        const dim3 grid(places_of(k.a) * k.a.Hkv, (k.nb + kRange - 1) / kRange);
+        if (k.nb > k.a.top) tile_sums_kernel<E, DP><<<grid, 256, 0, stream>>>(k);
+    } else if (small_sums(k.a)) {
+        launch_whole<E, DP, true>(k, stream);
+    } else {
+        launch_whole<E, DP, false>(k, stream);
     }
-    const uint32_t pitch = k.nb + 4 + (4 - k.nb % 4) % 4, bytes = kTile * pitch * 4;
-    if (k.nb <= 256) whole_kernel<E, DP, 4><<<grid, 256, bytes, stream>>>(k);
-    else whole_kernel<E, DP, kWhole / 64><<<grid, 256, bytes, stream>>>(k);
 }
 template <class E>
 void launch_sums(const Select &k, hipStream_t stream) {
@@ -527,12 +740,12 @@ void launch_sums(const Select &k, hipStream_t stream) {
     }
 }
 
+template <bool kSmall>
 void launch_pick(const Select &k, hipStream_t stream) {
     const uint32_t units = (k.row1 - k.row0) * k.a.Hkv;
-    if (k.nb <= 2048 && units >= 2048) pick_kernel<1, 32><<<(units + 3) / 4, 256, 0, stream>>>(k);
-    else if (k.nb <= 1024) pick_kernel<4, 4><<<units, 256, 0, stream>>>(k);
-    else if (k.nb <= 2048) pick_kernel<4, 8><<<units, 256, 0, stream>>>(k);
-    else if (k.nb <= 4096) pick_kernel<4, 16><<<units, 256, 0, stream>>>(k);
+    if (k.nb <= 1024) pick_kernel<4, kSmall><<<units, 256, 0, stream>>>(k);
+    else if (k.nb <= 2048) pick_kernel<8, kSmall><<<units, 256, 0, stream>>>(k);
+    else if (k.nb <= 4096) pick_kernel<16, kSmall><<<units, 256, 0, stream>>>(k);
     else pick_any_kernel<<<units, kThreads, 0, stream>>>(k);
 }
 
@@ -541,7 +754,13 @@ void launch_pick(const Select &k, hipStream_t stream) {
 uint64_t kv_bounds_threads(const KvBoundsArgs &a) { return uint64_t(bounds_places(a)) * kThreads; }
 
 hipError_t launch_kv_bounds(const KvBoundsArgs &a, hipStream_t stream) {
-    bounds_kernel<<<bounds_places(a), kThreads, 0, stream>>>(a);
+    const uint32_t grid = bounds_places(a);
+    if (a.D > kBoundsDim || a.D % 16 != 0 || reinterpret_cast<uintptr_t>(a.cache) % 16 != 0 ||
+        reinterpret_cast<uintptr_t>(a.bounds) % 4 != 0)
+        bounds_any_kernel<<<grid, kThreads, 0, stream>>>(a);
+    else if (a.D <= 64) bounds_kernel<8><<<grid, kThreads, 0, stream>>>(a);
+    else if (a.D <= 128) bounds_kernel<4><<<grid, kThreads, 0, stream>>>(a);
+    else bounds_kernel<2><<<grid, kThreads, 0, stream>>>(a);
     return hipGetLastError();
 }
 
@@ -551,7 +770,7 @@ size_t kv_select_scratch_bytes(const KvSelectArgs &a) {
 
 uint64_t kv_select_threads(const KvSelectArgs &a) {
     const uint64_t units = uint64_t(rows_a_pass(a)) * a.Hkv, tiles = uint64_t(places_of(a)) * a.Hkv;
-    if (whole(a)) return tiles * 256;
+    if (whole(a)) return tiles * 64 * kWaves;
     const uint64_t sums = (matrix_applies(a) ? tiles : units) * ((blocks_of(a) + kRange - 1) / kRange);
     return (sums > units ? sums : units) * kThreads;
 }
@@ -565,7 +784,7 @@ hipError_t launch_kv_select(const KvSelectArgs &a, void *scratch, hipStream_t st
         if (a.dtype == 7) launch_sums<Bf16>(k, stream);
         else if (a.dtype == 6) launch_sums<F16>(k, stream);
         else launch_sums<F32>(k, stream);
-        if (!whole(a)) launch_pick(k, stream);
+        if (!whole(a)) small_sums(a) ? launch_pick<true>(k, stream) : launch_pick<false>(k, stream);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }

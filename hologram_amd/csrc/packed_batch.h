@@ -42,18 +42,21 @@ __device__ __forceinline__ uint32_t last_at_most(uint32_t n, uint64_t t, F at) {
 // `unit`, or one more, so that neither a prefix sum nor the lengths are needed on the
 // host. (tokens * m < 2^30.) Its first and one-past-last row and the place's number
 // in it; false for a place that no unit of the sequence takes. As last_at_most, with
-// the bounds taken from the probes of its last step.
+// the bounds taken from the probes of its last step; *of, where asked for, is the
+// sequence's element of `per` (u32 [batch]), loaded beside the offsets.
 struct Place {
     uint32_t b, lo, hi, unit;
 };
-__device__ __forceinline__ bool place_of(const PackedBatch &pb, uint32_t m, uint32_t unit, uint32_t t, Place *o) {
+__device__ __forceinline__ bool place_of(const PackedBatch &pb, uint32_t m, uint32_t unit, uint32_t t, Place *o,
+                                         const uint32_t *per = nullptr, uint32_t *of = nullptr) {
     const uint32_t lane = threadIdx.x & 63u;
-    uint32_t lo = 0, n = pb.batch, v;
+    uint32_t lo = 0, n = pb.batch, v, x = 0;
     int at;
     for (;;) {
         const uint32_t step = (n + 63) / 64;
         const uint64_t s = lo + uint64_t(lane) * step;
         v = start_of(pb, s < pb.batch ? uint32_t(s) : pb.batch);
+        if (of) x = per[s < pb.batch ? uint32_t(s) : pb.batch - 1];
         const uint64_t hit = __ballot(lane * uint64_t(step) < n && v * m / unit + s <= t);
         at = hit ? 63 - __builtin_clzll(hit) : 0;
         lo = pk_uni(lo + at * step);
@@ -63,36 +66,44 @@ __device__ __forceinline__ bool place_of(const PackedBatch &pb, uint32_t m, uint
     o->b = lo;
     o->lo = __builtin_amdgcn_readlane(v, at);
     o->hi = at < 63 ? __builtin_amdgcn_readlane(v, at + 1) : pk_uni(start_of(pb, lo + 1));
+    if (of) *of = __builtin_amdgcn_readlane(x, at);
     const uint32_t first = o->lo * m / unit + lo;
     o->unit = t - first;
     return o->hi > o->lo && t >= first && o->unit * unit < (o->hi - o->lo) * m;
 }
 
-// The sequence that holds row `t`: its number, its first and one-past-last row and its
-// element of `per` (u32 [batch], or null), loaded beside the offsets; false for a row
-// outside every sequence. As place_of.
+// The largest sequence s with at(its first row, s) <= t (0 if there is none), for `at` that
+// does not decrease: its number, its first and one-past-last row and its element of `per`
+// (u32 [batch], or null), loaded beside the offsets. As place_of.
 struct RowAt {
     uint32_t b, lo, hi, of;
 };
-__device__ __forceinline__ bool row_of(const PackedBatch &pb, const uint32_t *per, uint32_t t, RowAt *o) {
+template <class At>
+__device__ __forceinline__ RowAt sequence_at(const PackedBatch &pb, const uint32_t *per, uint64_t t, At at) {
     const uint32_t lane = threadIdx.x & 63u;
     uint32_t lo = 0, n = pb.batch, v, x;
-    int at;
+    int found;
     for (;;) {
         const uint32_t step = (n + 63) / 64;
         const uint64_t s = lo + uint64_t(lane) * step;
         v = start_of(pb, s < pb.batch ? uint32_t(s) : pb.batch);
         x = per ? per[s < pb.batch ? uint32_t(s) : pb.batch - 1] : 0u;
-        const uint64_t hit = __ballot(lane * uint64_t(step) < n && v <= t);
-        at = hit ? 63 - __builtin_clzll(hit) : 0;
-        lo = pk_uni(lo + at * step);
+        const uint64_t hit = __ballot(lane * uint64_t(step) < n && at(v, uint32_t(s)) <= t);
+        found = hit ? 63 - __builtin_clzll(hit) : 0;
+        lo = pk_uni(lo + found * step);
         if (step == 1) break;
         n = pk_uni(pb.batch - lo < step ? pb.batch - lo : step);
     }
-    o->b = lo;
-    o->lo = __builtin_amdgcn_readlane(v, at);
-    o->hi = at < 63 ? __builtin_amdgcn_readlane(v, at + 1) : pk_uni(start_of(pb, lo + 1));
-    o->of = __builtin_amdgcn_readlane(x, at);
+    RowAt o;
+    o.b = lo;
+    o.lo = __builtin_amdgcn_readlane(v, found);
+    o.hi = found < 63 ? __builtin_amdgcn_readlane(v, found + 1) : pk_uni(start_of(pb, lo + 1));
+    o.of = __builtin_amdgcn_readlane(x, found);
+    return o;
+}
+// The sequence that holds row `t`; false for a row outside every sequence.
+__device__ __forceinline__ bool row_of(const PackedBatch &pb, const uint32_t *per, uint32_t t, RowAt *o) {
+    *o = sequence_at(pb, per, t, [](uint32_t v, uint32_t) { return uint64_t(v); });
     return t >= o->lo && t < o->hi;
 }
 
