@@ -58,7 +58,7 @@ __device__ __forceinline__ void few_segment(const Blocks &k, const Place &at, ui
     const float *ks = a.ks + plane * nb, *vs = a.vs + plane * nb;
     auto load = [&](uint32_t blk, KvStep<DP> &x) __attribute__((always_inline)) {
         const uint32_t so = blk < end ? blk * a.D : kOob;   // past the share: nothing is read
-        kv.load({so, so + 16 * a.D}, x);
+        kv.template load<true>({so, so + 16 * a.D}, x);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const uint32_t i = (blk + 16 * h) >> k.shift, c = i < nb ? i : nb - 1;

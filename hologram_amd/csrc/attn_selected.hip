@@ -13,7 +13,14 @@ namespace {
 // A unit is a token, a kv head and sixteen of its heads: the columns of the matrix
 // instructions (i8_rows.h). Its workgroup reads the list with the blocks' scales into LDS,
 // drops the tail that names nothing, and its wavefronts take the 32-key steps of the
-// blocks in turn.
+// blocks in turn. Where the units are many and have at most eight heads, the columns are two
+// groups of eight, each over every other 16 keys (group_step): half the scores a lane.
+// Bound by the bytes where each row has its own: 32 rows over 2048 keys of 8 kv heads of
+// 128 dims, 134 MB, 28 us or 4.8 TB/s; 128 rows 89 us, 6.0 TB/s. By the L2s' reads where rows
+// share them: 712 rows of two chunks over 2048 keys each, 3 GB out of the caches, 271 us, 11
+// TB/s (one group, whose registers leave two wavefronts a SIMD: 303). By latency where they
+// are few: 8 rows over 256 keys 6.0 us, 26 f32 rows of drafts over 1280 keys 15. A wavefront a
+// row and head (below): 1560 us, 11.5 ms, 131 us, 754 us.
 constexpr uint32_t kMaxList = 512;            // entries a workgroup takes
 constexpr uint32_t kNone = 0x80000000u;       // past every key
 
@@ -31,8 +38,10 @@ struct Entry {
     float ks, vs;
 };
 
-template <class E, int DP, int W>
-__global__ __launch_bounds__(64 * W) void few_kernel(Selected k) {
+template <class E, int DP, int W, int C, bool kOnce>
+__global__ __launch_bounds__(64 * W, DP > 128 ? 1 : C == 2 ? 3 : 2) void few_kernel(Selected k) {
+    constexpr int S = C > 2 ? C / 2 : 1;       // loads of two 16-key steps a turn
+    constexpr uint32_t kHeads = kUnit / C;
     typedef typename E::T T;
     __shared__ FewLds<E, DP, W> lds;
     __shared__ Entry list[kMaxList];
@@ -57,46 +66,60 @@ __global__ __launch_bounds__(64 * W) void few_kernel(Selected k) {
         if (ok) atomicMax(&last, i + 1);
     }
     const uint32_t r = tid & 15u, h0 = kh * G + tile * kUnit, rows = G - tile * kUnit < kUnit ? G - tile * kUnit : kUnit;
-    const bool live = r < rows;
+    const bool live = r % kHeads < rows;
     RowQ<E, DP> q;
-    q.load(static_cast<const T *>(a.q) + uint64_t(tok) * a.q_stride + uint64_t(h0 + (live ? r : 0u)) * a.D, live, a.D, k.mul);
+    q.load(static_cast<const T *>(a.q) + uint64_t(tok) * a.q_stride + uint64_t(h0 + (live ? r % kHeads : 0u)) * a.D, live, a.D, k.mul);
     __syncthreads();
-    const uint32_t count = pk_uni(last), deep = k.shift - 4;              // 2^deep halves a block
-    const uint32_t halves = count << deep, steps = (halves + 1) / 2;
+    const uint32_t count = pk_uni(last), deep = k.shift - 4;              // 2^deep 16-key steps a block
+    const uint32_t halves = count << deep, turns = (halves + 2 * S - 1) / (2 * S);
     const KvPlane<DP> kv(a.kq + plane * a.bucket * a.D, a.vq + plane * a.bucket * a.D, a.bucket, a.D);
-    struct Keys {
-        uint32_t key[2];
+    struct Turn {
+        KvStep<DP> x[S];
+        uint32_t key[2];      // the steps' first keys (C == 1), or the column's step's
+        float ks, vs;
     };
-    auto load = [&](uint32_t step, KvStep<DP> &x, Keys &o) __attribute__((always_inline)) {
-        uint32_t so[2];
+    // A 16-key step of the list: its entry, and its first key (kNone past the list)
+    auto half_at = [&](uint32_t half, Entry *e) __attribute__((always_inline)) {
+        *e = list[half < halves ? half >> deep : 0u];
+        return half < halves && e->key != kNone ? e->key + 16 * (half & ((1u << deep) - 1)) : kNone;
+    };
+    auto load = [&](uint32_t turn, Turn &o) __attribute__((always_inline)) {
+        Entry e;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t half = 2 * step + h, i = half < halves ? half >> deep : 0u;
-            const Entry e = list[i];
-            const bool in = half < halves && e.key != kNone;
-            o.key[h] = pk_uni(in ? e.key + 16 * (half & ((1u << deep) - 1)) : kNone);
-            so[h] = o.key[h] == kNone ? kOob : o.key[h] * a.D;
-            x.ks[h] = e.ks, x.vs[h] = e.vs;
+        for (int t = 0; t < S; ++t) {
+            uint32_t so[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t key = pk_uni(half_at(2 * (S * turn + t) + h, &e));
+                so[h] = key == kNone ? kOob : key * a.D;
+                if constexpr (C == 1) o.key[h] = key, o.x[t].ks[h] = e.ks, o.x[t].vs[h] = e.vs;
+            }
+            kv.template load<kOnce>(so, o.x[t]);
         }
-        kv.load(so, x);
+        if constexpr (C > 1) {
+            o.key[0] = half_at(2 * S * turn + r / kHeads, &e);
+            o.ks = e.ks, o.vs = e.vs;
+        }
     };
     State<DP> st;
     st.clear();
-    auto take = [&](const KvStep<DP> &x, const Keys &o) __attribute__((always_inline)) {
-        few_step<E, DP>(st, x, q, o.key, o.key[0] + 16 > sees || o.key[1] + 16 > sees, sees, sees);
+    auto take = [&](const Turn &o) __attribute__((always_inline)) {
+        if constexpr (C == 1)
+            few_step<E, DP>(st, o.x[0], q, o.key, o.key[0] + 16 > sees || o.key[1] + 16 > sees, sees, sees);
+        else
+            group_step<E, DP, C>(st, o.x, q, o.key[0], o.ks, o.vs, sees);
     };
-    KvStep<DP> ring[2];
-    Keys key[2];
-    if (wave < steps) load(wave, ring[0], key[0]);
-    for (uint32_t i = wave; i < steps; i += 2 * W) {
-        if (i + W < steps) load(i + W, ring[1], key[1]);
-        take(ring[0], key[0]);
-        if (i + W >= steps) break;
-        if (i + 2 * W < steps) load(i + 2 * W, ring[0], key[0]);
-        take(ring[1], key[1]);
+    Turn ring[2];
+    if (wave < turns) load(wave, ring[0]);
+    for (uint32_t i = wave; i < turns; i += 2 * W) {
+        if (i + W < turns) load(i + W, ring[1]);
+        take(ring[0]);
+        if (i + W >= turns) break;
+        if (i + 2 * W < turns) load(i + 2 * W, ring[0]);
+        take(ring[1]);
     }
     float *dst = k.part + (uint64_t(blockIdx.x) * k.shares + share) * (kUnit * (DP + 2));
-    join_waves<E, DP, W>(st, rows, a.D, lds, [&](uint32_t c, uint32_t d, float o, float M, float l) {
+    join_waves<E, DP, W, C>(st, rows, a.D, lds, [&](uint32_t c, uint32_t d, float o, float M, float l) {
         if (k.shares == 1) {
             static_cast<T *>(a.out)[(uint64_t(tok) * a.H + h0 + c) * a.D + d] = E::narrow(count ? o / l : 0.0f);
         } else {
@@ -154,12 +177,26 @@ uint32_t shares_of(const AttnSelectedArgs &s) { return (s.top + entries_of(s) - 
 // whose registers hold two steps.
 bool four_waves(const AttnSelectedArgs &s) { return s.a.D > 128 || units_of(s.a) >= 512; }
 
+// One row a sequence reads its blocks once; of several, the next may read them again from
+// the caches (712 rows of two chunks: 359 us past the caches, 303 through them; 64 rows of as
+// many sequences 48.6 and 51.6).
+bool reads_once(const AttnSelectedArgs &s) { return s.a.pb.tokens <= s.a.pb.batch; }
+
 template <class E, int DP>
 void launch_few(const Selected &k, hipStream_t stream) {
     const dim3 grid(uint32_t(units_of(k.s.a)), k.shares);
-    constexpr int kMost = DP > 128 ? 4 : 8;
-    if (four_waves(k.s)) few_kernel<E, DP, 4><<<grid, 256, 0, stream>>>(k);
-    else few_kernel<E, DP, kMost><<<grid, 64 * kMost, 0, stream>>>(k);
+    constexpr uint32_t kMost = DP > 128 ? 4 : 8, kGroups = DP > 128 ? 1 : 2;
+    const bool once = reads_once(k.s);
+    if (four_waves(k.s) && k.s.a.H / k.s.a.Hkv <= kUnit / kGroups) {
+        if (once) few_kernel<E, DP, 4, kGroups, true><<<grid, 256, 0, stream>>>(k);
+        else few_kernel<E, DP, 4, kGroups, false><<<grid, 256, 0, stream>>>(k);
+    } else if (four_waves(k.s)) {
+        if (once) few_kernel<E, DP, 4, 1, true><<<grid, 256, 0, stream>>>(k);
+        else few_kernel<E, DP, 4, 1, false><<<grid, 256, 0, stream>>>(k);
+    } else {
+        if (once) few_kernel<E, DP, kMost, 1, true><<<grid, 64 * kMost, 0, stream>>>(k);
+        else few_kernel<E, DP, kMost, 1, false><<<grid, 64 * kMost, 0, stream>>>(k);
+    }
     if (k.shares > 1) merge_kernel<E, DP><<<grid.x, 256, 0, stream>>>(k);
 }
 template <class E>

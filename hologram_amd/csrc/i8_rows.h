@@ -123,23 +123,24 @@ struct KvPlane {
         voff = NDB * r < D ? 4 * g * D + NDB * r : kOob;
     }
     // The steps at bytes at[0] and at[1] of the plane (kOob: nothing is read, zeros).
-    // Non-temporal: the cache is read once.
+    // kOnce: non-temporal, for a cache that is read once.
+    template <bool kOnce>
     __device__ __forceinline__ void load(const uint32_t (&at)[2], KvStep<DP> &x) const {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int s = 0; s < NKS; ++s)
-                x.k[h][s] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, koff[s] + at[h], 0, 2));
+                x.k[h][s] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, koff[s] + at[h], 0, kOnce ? 2 : 0));
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const uint32_t o = voff + (at[j >> 2] + (j & 3) * D);
             if constexpr (VW == 1) {
-                x.v[j][0] = __builtin_amdgcn_raw_buffer_load_b32(rv, o, 0, 2);
+                x.v[j][0] = __builtin_amdgcn_raw_buffer_load_b32(rv, o, 0, kOnce ? 2 : 0);
             } else if constexpr (VW == 2) {
-                const auto w = __builtin_amdgcn_raw_buffer_load_b64(rv, o, 0, 2);
+                const auto w = __builtin_amdgcn_raw_buffer_load_b64(rv, o, 0, kOnce ? 2 : 0);
                 x.v[j][0] = w[0], x.v[j][1] = w[1];
             } else {
-                const auto w = __builtin_amdgcn_raw_buffer_load_b128(rv, o, 0, 2);
+                const auto w = __builtin_amdgcn_raw_buffer_load_b128(rv, o, 0, kOnce ? 2 : 0);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) x.v[j][i] = w[i];
             }
@@ -302,9 +303,96 @@ __device__ __forceinline__ void few_step(State<DP> &st, const KvStep<DP> &x, con
     }
 }
 
-// The wavefronts' states joined: 2^(m_w - M) of each, their units of 2^(ve - 7) made one.
-// put(row, dim, O, maximum, sum) of `rows` rows; the workgroup's LDS is free again after it.
-template <class E, int DP, int W, class Put>
+// few_step for rows that are few: C column groups of 16 / C rows, each over a 16-key step of
+// its own (C of them, in C / 2 loads), so that a lane's scores are four and not four times
+// C. Column r is row r % (16 / C) over step r / (16 / C): the products are made for all
+// columns and those of a column's step kept, and its weights enter the products with V as
+// zeros but for its step's keys. `key`, `ks` and `vs` are of the column's step.
+template <class E, int DP, int C>
+__device__ __forceinline__ void group_step(State<DP> &st, const KvStep<DP> (&x)[C / 2], const RowQ<E, DP> &q, uint32_t key,
+                                           float ks, float vs, uint32_t lim) {
+    constexpr int NKS = DP / 64, VW = DP / 64;
+    constexpr bool kF32 = std::is_same_v<E, F32>;
+    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, group = (lane & 15u) / (16 / C);
+    constexpr float kLag = 8.0f;
+    i32x4 a[3];
+#pragma unroll
+    for (int h = 0; h < C; ++h) {
+        i32x4 b[3] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+        for (int c = 0; c < NKS; ++c) {
+            const i32x4 kf = __builtin_bit_cast(i32x4, x[h / 2].k[h % 2][c]);
+#pragma unroll
+            for (int p = 0; p < 3; ++p) b[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf, q.part[p][c], b[p], 0, 0, 0);
+        }
+#pragma unroll
+        for (int p = 0; p < 3; ++p)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a[p][i] = h == 0 || group == uint32_t(h) ? b[p][i] : a[p][i];
+    }
+    float s[4];
+    const float c = ks * q.mul;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = fmaf(float(a[0][i]), 65536.0f, float(a[1][i] * 256 + a[2][i])) * c;
+    if (__any(key + 16 > lim)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] = key + 4 * g + i < lim ? s[i] : -INFINITY;
+        vs = key < lim ? vs : 0.0f;
+    }
+    const float mt = column_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
+    const float av = fabsf(vs);
+    int ve = kVeMin;
+    if (av > 0.0f && av <= 3.4028235e38f) (void)frexpf(av, &ve);   // av < 2^ve
+    ve = st.ve > ve ? st.ve : ve;
+    if (__any(mt > st.m + kLag || ve > st.ve)) {
+        const float mn = mt > st.m + kLag ? mt : st.m;
+        const float al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(st.m - mn);
+        st.l *= al;
+        const float sh = ldexpf(al, st.ve - ve);
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d) st.o[d] *= sh;
+        st.m = mn, st.ve = ve;
+    }
+    const float ref = st.m == -INFINITY ? 0.0f : st.m, f = weight_factor(vs, ve);
+    typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+    f16x4 hi, lo;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float p = __builtin_amdgcn_exp2f(s[i] - ref);
+        st.l += p;
+        const float w = kF32 ? rounded(p * f) : p * f;
+        hi[i] = _Float16(w);
+        if constexpr (kF32) lo[i] = _Float16(left_over(w, float(hi[i])));
+    }
+    auto of_step = [&](f16x4 w, int t) __attribute__((always_inline)) {
+        const uint2 v = __builtin_bit_cast(uint2, w);
+        const bool first = group == uint32_t(2 * t), second = group == uint32_t(2 * t + 1);
+        return __builtin_bit_cast(f16x8, u32x4{first ? v.x : 0u, first ? v.y : 0u, second ? v.x : 0u, second ? v.y : 0u});
+    };
+#pragma unroll
+    for (int t = 0; t < C / 2; ++t) {
+        const f16x8 wh = of_step(hi, t);
+        f16x8 wl;
+        if constexpr (kF32) wl = of_step(lo, t);
+#pragma unroll
+        for (int n = 0; n < VW; ++n) {
+            uint32_t words[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) words[j] = x[t].v[j][n] ^ 0x80808080u;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const f16x8 v = key_column(words, e);
+                st.o[4 * n + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, wh, st.o[4 * n + e], 0, 0, 0);
+                if constexpr (kF32) st.o[4 * n + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, wl, st.o[4 * n + e], 0, 0, 0);
+            }
+        }
+    }
+}
+
+// The wavefronts' states joined: 2^(m_w - M) of each, their units of 2^(ve - 7) made one; of C
+// column groups too. put(row, dim, O, maximum, sum) of `rows` rows; the workgroup's LDS is
+// free again after it.
+template <class E, int DP, int W, int C = 1, class Put>
 __device__ __forceinline__ void join_waves(State<DP> &st, uint32_t rows, uint32_t D, FewLds<E, DP, W> &lds, Put put) {
     constexpr int NDB = DP / 16;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, r = lane & 15u, g = lane >> 4, wave = pk_uni(tid >> 6);
@@ -318,17 +406,22 @@ __device__ __forceinline__ void join_waves(State<DP> &st, uint32_t rows, uint32_
     __syncthreads();
     for (uint32_t i = tid; i < rows * D; i += 64 * W) {
         const uint32_t c = i / D, d = i - c * D;
-        float M = lds.m[0][c];
+        float M = -INFINITY;
 #pragma unroll
-        for (int w = 1; w < W; ++w) M = fmaxf(M, lds.m[w][c]);
+        for (int w = 0; w < W; ++w)
+#pragma unroll
+            for (int n = 0; n < C; ++n) M = fmaxf(M, lds.m[w][c + 16 / C * n]);
         const float ref = M == -INFINITY ? 0.0f : M;
         float o = 0.0f, l = 0.0f;
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const float e = __builtin_amdgcn_exp2f(lds.m[w][c] - ref);
-            l += lds.l[w][c] * e;
-            o += ldexpf(lds.o[w][c][d], lds.ve[w][c] - 7) * e;
-        }
+        for (int w = 0; w < W; ++w)
+#pragma unroll
+            for (int n = 0; n < C; ++n) {
+                const uint32_t r = c + 16 / C * n;
+                const float e = __builtin_amdgcn_exp2f(lds.m[w][r] - ref);
+                l += lds.l[w][r] * e;
+                o += ldexpf(lds.o[w][r][d], lds.ve[w][r] - 7) * e;
+            }
         put(c, d, o, M, l);
     }
     __syncthreads();

@@ -313,3 +313,90 @@ def test_captured_on_a_stream_of_its_own(torch_cuda):
             assert np.array_equal(got, w)
     be.close()
     eager.close()
+
+
+# ------------------------------------------------- many rows of few heads ----
+MANY = [  # sequences' rows, lens, H, Hkv, D, bucket, block, top
+    ([130, 1, 0, 60], [700, 33, 9, 60], 16, 4, 64, 704, 16, 7),      # steps that end inside a turn
+    ([180], [900], 3, 3, 128, 1000, 32, 9),                          # one head a kv head, a bucket off the blocks
+    ([70, 70, 70], [300, 3, 800], 12, 4, 96, 800, 64, 5),            # three heads a kv head, rows that see nothing
+    ([1] * 300, [700 - 2 * i for i in range(300)], 4, 2, 128, 704, 128, 3),   # one token each
+    ([90, 50], [500, 520], 16, 4, 80, 520, 16, 1),                   # one step a row
+    ([300], [640], 10, 2, 64, 640, 16, 21),                          # five heads: not of them
+    ([130, 20], [900, 640], 8, 4, 256, 900, 16, 5),                  # nor 256 dims
+]
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("rows,lens,H,Hkv,D,bucket,block,top", MANY)
+def test_many_rows_of_few_heads(torch_cuda, backend, rows, lens, H, Hkv, D, bucket, block, top, dtype):
+    rng = np.random.default_rng(sum(rows) + D)
+    for scales, kind in (("powers", "choice"), ("any", "anything")):
+        c = selected_case(rng, rows, lens, H, Hkv, D, bucket, block, top, dtype, scales, 0, kind)
+        check_selected(run_selected(torch_cuda, backend, c), c)
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("D,block", [(64, 16), (128, 32)])
+def test_many_rows_what_a_row_does_not_see_stays_out(torch_cuda, backend, dtype, D, block):
+    """As above for many rows of few heads: the steps of one turn lie in different columns, and a
+    scale that is NaN or infinite reaches none but the rows that see its block."""
+    rng = np.random.default_rng(D)
+    n, nb, top = 150, 24, 7
+    c = selected_case(rng, [n, n], [nb * block - 3, nb * block - 2 * block], 8, 2, D, nb * block, block, top, dtype)
+    odd = 2 * rng.permutation(nb // 2 - 2)[:top] + 1
+    c["lists"][:] = odd[None, None, :]
+    c["lists"][:, :, 3] = nb - 1
+    clean = run_selected(torch_cuda, backend, c)
+    check_selected(clean, c)
+    for s in ("ks", "vs"):
+        c[s] = c[s].copy()
+        c[s][:, :, 0:nb - 1:2] = np.nan if s == "ks" else np.inf
+        c[s][1, :, nb - 1] = np.nan
+    assert np.array_equal(run_selected(torch_cuda, backend, c), clean)
+    for s in ("ks", "vs"):
+        old = c[s][0, 1, odd[1]]
+        c[s][0, 1, odd[1]] = np.nan
+        got = run_selected(torch_cuda, backend, c)
+        c[s][0, 1, odd[1]] = old
+        sees = np.array([int(c["lens"][0]) - (n - 1 - t) > odd[1] * block for t in range(n)])
+        assert np.array_equal(got[:, :4], clean[:, :4]) and np.array_equal(got[n:], clean[n:])
+        assert np.isnan(decode(got[:n][sees][:, 4:], dtype)).all()
+        assert np.array_equal(got[:n][~sees], clean[:n][~sees])
+
+
+def test_many_rows_large_and_small_block_scales(torch_cuda, backend):
+    rng = np.random.default_rng(9)
+    c = selected_case(rng, [150, 150], [4000, 390], 8, 2, 64, 4000, 16, 25, DTYPE_F32)
+    c["vs"] = (2.0 ** rng.integers(-30, 31, c["vs"].shape)).astype(np.float32)
+    c["vs"][:, :, 3] = 0.0
+    c["vs"][:, :, ::5] *= -1.0
+    check_selected(run_selected(torch_cuda, backend, c), c)
+
+
+@pytest.mark.parametrize("n", [3, 300])
+def test_a_row_of_scores_that_are_infinite(torch_cuda, backend, n):
+    """K scales of -infinity give scores of either infinity, which make the row NaN as the formula
+    does; a query that is not finite makes its own head's row NaN and no other."""
+    rng = np.random.default_rng(n)
+    c = selected_case(rng, [n], [600], 8, 2, 64, 640, 16, 5, DTYPE_BF16)
+    c["lists"][:] = np.array([3, 9, 20, 21, 36])
+    clean = run_selected(torch_cuda, backend, c)
+    q = decode(c["q"], DTYPE_BF16).reshape(n, -1).copy()
+    q[1, 64 + 5], q[2, 5 * 64] = np.nan, np.inf                # head 1 of row 1, head 5 of row 2
+    c["q"] = encode(q, DTYPE_BF16).reshape(n, -1)
+    got = run_selected(torch_cuda, backend, c)
+    keep = np.ones((n, 8), bool)
+    keep[1, 1] = keep[2, 5] = False
+    assert np.array_equal(got[keep], clean[keep]) and np.isnan(decode(got[~keep], DTYPE_BF16)).all()
+    c["ks"][0, 1, 20] = -np.inf
+    got = run_selected(torch_cuda, backend, c)
+    assert np.array_equal(got[:, :4][keep[:, :4]], clean[:, :4][keep[:, :4]])
+    # a score of +infinity, or 0 times infinity, among those that the row sees: weights that are NaN
+    q = decode(c["q"], DTYPE_BF16).reshape(n, 8, 64)
+    with np.errstate(invalid="ignore"):
+        dots = q[:, 4:] @ c["k"][0, 1, 320:336].astype(np.float64).T              # [n, 4, 16]
+    sees = (320 + np.arange(16) < 600 - (n - 1 - np.arange(n))[:, None])[:, None]   # [n, 1, 16]
+    nan = (sees & ~(dots > 0)).any(axis=2) | ~keep[:, 4:]
+    assert np.array_equal(np.isnan(decode(got[:, 4:], DTYPE_BF16)).reshape(n, 4, 64).all(axis=2), nan)
+    assert np.array_equal(np.isnan(decode(got[:, 4:], DTYPE_BF16)).reshape(n, 4, 64).any(axis=2), nan)
