@@ -125,6 +125,9 @@ SELECT_SHAPES = [  # rows, lens, H, Hkv, D, bucket, block, top, first, last, pad
     ([1, 2], [600, 640], 4, 2, 64, 640, 64, 10, 1, 1, 0),                      # every block fits the list
     ([1, 1], [600, 640], 4, 2, 64, 640, 64, 12, 1, 1, 0),                      # the list is longer
     ([17, 16], [333, 3000], 12, 4, 128, 3001, 16, 16, 1, 1, 0),
+    ([9, 1], [700, 650], 4, 2, 64, 704, 16, 6, 1, 1, 1),                       # the tiles' sizes, rows off 16 bytes
+    ([3], [900], 256, 1, 64, 900, 16, 9, 1, 1, 0),                             # more heads than two int8 parts hold
+    ([2, 1], [2500, 2000], 16, 1, 128, 2500, 4, 20, 1, 1, 0),                  # sums past 2^24
 ]
 
 
@@ -167,6 +170,25 @@ def test_select_equal_scores_go_by_their_order(torch_cuda, backend, rows, bucket
             c["ks"][:, :, ::11], c["ks"][:, :, 1::13] = np.nan, np.inf
             c["ks"][:, :, 2::17] = -np.inf
         check_select(run_select(torch_cuda, backend, c), c)
+
+
+@pytest.mark.parametrize("H", [2, 64])
+@pytest.mark.parametrize("D", [64, 72])
+@pytest.mark.parametrize("rows,bucket", [([1, 1], 1200), ([20, 33], 1200), ([1, 1], 8000), ([1, 1], 20000)])
+def test_select_scores_next_to_one_another(torch_cuda, backend, rows, bucket, D, H):
+    """Scales from the least subnormal to the largest number, scores that differ in their last bit
+    or past f32's: the exact order decides, not a rounded one's."""
+    rng = np.random.default_rng(bucket + D + H)
+    c = select_case(rng, rows, [bucket - 5, bucket], H, 2, D, bucket, 4, 37, DTYPE_BF16)
+    c["ks"] = np.ldexp(rng.uniform(0.5, 1.0, c["ks"].shape), rng.integers(-148, 129, c["ks"].shape)).astype(np.float32)
+    c["ks"][:, :, ::4] *= -1.0
+    check_select(run_select(torch_cuda, backend, c), c)
+    c["bounds"][:] = c["bounds"][:, :, :1]          # one block's bounds under scales a step apart
+    c["ks"] = (1.0 + rng.integers(0, 40, c["ks"].shape) * 2.0 ** -23).astype(np.float32)
+    check_select(run_select(torch_cuda, backend, c), c)
+    c["ks"][:] = np.float32(3.3e38)                 # all past f32's largest
+    c["bounds"] = select_case(rng, rows, [0, 0], H, 2, D, bucket, 4, 37, DTYPE_BF16)["bounds"]
+    check_select(run_select(torch_cuda, backend, c), c)
 
 
 @pytest.mark.parametrize("dtype", ALL)
