@@ -82,7 +82,7 @@ __global__ __launch_bounds__(256) void rows_kernel(QkNormRotaryArgs a) {
 // rotated part, then two after another of the rest. A workgroup takes T tokens: their
 // angles' cos and sin once, in LDS, for all heads; while those are taken the first rows
 // are on their way, and each pass's under the one before. Bound by the bytes, each read
-// and written once: 30720 rows of 32 + 8 heads of 128 bf16, both normed, 629 MB in 110 us,
+// and written once: 30,720 rows of 32 + 8 heads of 128 bf16, both normed, 629 MB in 110 us,
 // 5.7 TB/s (a copy of as much: 117 us); 8576 rows of f16, half of each head turned, 176 MB
 // in 33 us, 5.3 (34). The general form: 775 and 179 us. The stores go past the caches:
 // 115 and 37 us where they did not. One token each of 32 sequences: 4.1 us, a workgroup's
@@ -240,7 +240,7 @@ bool wide_applies(const QkNormRotaryArgs &a) {
 
 // Tokens a workgroup: more take the angles' part of its time once, fewer leave less of the
 // GPU idle at the end, some 6000 workgroups are enough (8576 rows with 1, 2 and 4: 37, 38
-// and 40 us; 30720: 148, 121 and 115).
+// and 40 us; 30,720: 148, 121 and 115).
 uint32_t tokens_of(const QkNormRotaryArgs &a) { return a.pb.tokens >= 24576 ? 4 : a.pb.tokens >= 12288 ? 2 : 1; }
 // Workgroups that share a token's passes: one a pass while that leaves CUs free (32 rows:
 // 4.1 us, 4.7 with one for all).

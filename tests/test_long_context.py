@@ -133,7 +133,7 @@ def test_sizes_that_would_wrap_are_refused():
         validate(KernelCall.KvBlockBounds(replace(BOUNDS, bucket_rows=1 << 23, block_rows=1 << 22, head_dim=1024)),
                  [1 << 50] * 4)
     with pytest.raises(UnsupportedOp, match="launch"):
-        validate(KernelCall.KvBlockSelect(replace(SELECT, tokens=1 << 24, heads=2, kv_heads=2)), [1 << 50] * 6)
+        validate(KernelCall.KvBlockSelect(replace(SELECT, tokens=1 << 24, heads=2, kv_heads=2, head_dim=24)), [1 << 50] * 6)
     with pytest.raises(UnsupportedOp, match="launch"):
         validate(KernelCall.AttentionI8Selected(replace(SELECTED, tokens=1 << 26, heads=2)), [1 << 60] * 9)
     with pytest.raises(UnsupportedOp, match="launch"):
