@@ -57,7 +57,8 @@ __global__ __launch_bounds__(kThreads) void bounds_any_kernel(KvBoundsArgs a) {
 // instruction. The threads' bounds then meet in LDS, P threads a word of the result.
 // Bound by a workgroup's chain (search, rows, LDS, store): behind one row of 32 sequences,
 // 8 heads of 128 dims, 4.0 us; behind 16 prompts of 100 to 8000 rows in blocks of 64, 28 MB,
-// 14.5 (the general form: 6.5 and 28).
+// 13.2 (the general form: 6.5 and 28; four rows a turn, two of them the first again in blocks
+// of 64, 14.5).
 constexpr uint32_t kBoundsDim = 256;
 typedef short i16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t bytes_min(uint32_t x, uint32_t y) {
@@ -82,13 +83,13 @@ __global__ __launch_bounds__(kThreads) void bounds_kernel(KvBoundsArgs a) {
     for (int i = 0; i < 4; ++i) lo[0][i] = lo[1][i] = 0x7f007f00u, hi[0][i] = hi[1][i] = 0x80008000u;
     if (g < groups) {
         const uint4 *row = reinterpret_cast<const uint4 *>(t.src) + c;
-        for (uint32_t r = g; r < t.rows; r += 4 * groups) {
-            uint4 v[4];
+        for (uint32_t r = g; r < t.rows; r += 2 * groups) {
+            uint4 v[2];
 #pragma unroll
-            for (uint32_t q = 0; q < 4; ++q)      // (a row past the block: the first one again)
+            for (uint32_t q = 0; q < 2; ++q)      // (a row past the block: the first one again)
                 v[q] = row[uint64_t(r + q * groups < t.rows ? r + q * groups : r) * per];
 #pragma unroll
-            for (uint32_t q = 0; q < 4; ++q) {
+            for (uint32_t q = 0; q < 2; ++q) {
                 const uint32_t w[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {

@@ -236,17 +236,20 @@ def test_steps_of_a_long_context(torch_cuda, backend, dtype, interleaved):
     s.session.close()
 
 
-def test_captured_on_a_stream_of_its_own(torch_cuda):
+@pytest.mark.parametrize("bucket,top", [(2048, 40), (20480, 100)])
+def test_captured_on_a_stream_of_its_own(torch_cuda, bucket, top):
     """The four calls in one graph on another stream than torch's: every replay, over other inputs and
-    lengths, is the eager result, bit for bit."""
+    lengths, is the eager result, bit for bit; with lists and attention of one launch each, and of
+    two that share the backend's scratch."""
     torch = torch_cuda
     from hologram_amd import (KvBlockBoundsCall, KvBlockSelectCall, QkNormRotaryCall)
     rng = np.random.default_rng(11)
-    H, Hkv, D, bucket, block, top, tokens, dtype = 8, 2, 64, 2048, 16, 40, 12, DTYPE_BF16
+    H, Hkv, D, block, tokens, dtype = 8, 2, 64, 16, 12, DTYPE_BF16
+    far = bucket - 2048
     nb = bucket // block
     cases = []
-    for rows, lens in (([1, 1, 1], [2000, 40, 900]), ([4, 4, 4], [2000, 2048, 5]), ([12, 0, 0], [1500, 0, 0]),
-                       ([0, 1, 11], [0, 1, 2000])):
+    for rows, lens in (([1, 1, 1], [far + 2000, 40, 900]), ([4, 4, 4], [2000, bucket, 5]), ([12, 0, 0], [far + 1500, 0, 0]),
+                       ([0, 1, 11], [0, 1, far + 2000])):
         c = blocks_case(rng, rows, lens, H, Hkv, D, bucket, block, dtype)
         c["x"] = encode(rng.standard_normal((tokens, (H + Hkv) * D)), dtype).reshape(tokens, -1)
         c["pos"] = np.maximum(np.array(lens, np.int64) - rows, 0).astype(np.uint32)
