@@ -70,7 +70,10 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : C == 2 ? 3 : 2) void few_ker
     RowQ<E, DP> q;
     q.load(static_cast<const T *>(a.q) + uint64_t(tok) * a.q_stride + uint64_t(h0 + (live ? r % kHeads : 0u)) * a.D, live, a.D, k.mul);
     __syncthreads();
-    const uint32_t count = pk_uni(last), deep = k.shift - 4;              // 2^deep 16-key steps a block
+    // 2^deep 16-key steps a block, of one longer than what the row sees those that hold it (so
+    // the steps of a list are at most 2^31)
+    const uint32_t reach = sees <= 16 ? 4u : 32u - uint32_t(__builtin_clz(sees - 1));
+    const uint32_t count = pk_uni(last), deep = (k.shift < reach ? k.shift : reach) - 4;
     const uint32_t halves = count << deep, turns = (halves + 2 * S - 1) / (2 * S);
     const KvPlane<DP> kv(a.kq + plane * a.bucket * a.D, a.vq + plane * a.bucket * a.D, a.bucket, a.D);
     struct Turn {

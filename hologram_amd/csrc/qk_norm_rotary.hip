@@ -2,6 +2,8 @@
 // position (QkNormRotary, 130).
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "holo_kernels.h"
 #include "packed_tile.h"
 
@@ -246,8 +248,8 @@ uint32_t tokens_of(const QkNormRotaryArgs &a) { return a.pb.tokens >= 24576 ? 4 
 // 4.1 us, 4.7 with one for all).
 uint32_t shares_of(const QkNormRotaryArgs &a) {
     const uint32_t rows = a.D <= 64 ? 64 : a.D <= 128 ? 32 : 16;
-    const uint64_t passes = (a.H + rows - 1) / rows + (a.Hkv + rows - 1) / rows;
-    return passes * a.pb.tokens <= 1024 ? uint32_t(passes) : 1;
+    const uint32_t passes = (a.H + rows - 1) / rows + (a.Hkv + rows - 1) / rows;
+    return a.pb.tokens > 1024 ? 1 : std::min(passes, 1024 / a.pb.tokens);
 }
 
 template <class E>

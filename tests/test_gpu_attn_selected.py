@@ -72,6 +72,9 @@ SHAPES = [  # rows, lens, H, Hkv, D, bucket, block, top, pad
     ([1, 2], [9000, 8000], 34, 2, 64, 9024, 64, 130, 0),                  # three times 16 heads' tiles
     ([1], [64], 1, 1, 1024, 64, 16, 4, 0),
     ([2], [5000], 2, 1, 16, 5000, 256, 20, 0),
+    ([1, 2], [60, 33], 4, 2, 64, 70, 1 << 31, 40, 0),                     # one block, longer than any cache
+    ([3], [900], 2, 1, 128, 1000, 1 << 16, 3, 0),
+    ([2, 1], [5, 4100], 2, 1, 64, 12288, 4096, 3, 0),                     # a block of which few rows are seen
 ]
 
 
@@ -327,6 +330,7 @@ MANY = [  # sequences' rows, lens, H, Hkv, D, bucket, block, top
     ([90, 50], [500, 520], 16, 4, 80, 520, 16, 1),                   # one step a row
     ([300], [640], 10, 2, 64, 640, 16, 21),                          # five heads: not of them
     ([130, 20], [900, 640], 8, 4, 256, 900, 16, 5),                  # nor 256 dims
+    ([200], [120], 8, 4, 64, 128, 1 << 20, 4),                       # one block, listed several times
 ]
 
 

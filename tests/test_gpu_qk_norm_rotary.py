@@ -80,6 +80,7 @@ SHAPES = [  # rows, pos, H, Hkv, D, rot, pad
     ([5, 6], [1, 2], 3, 1, 64, 6, 0),                       # pairs that are no whole 16 bytes
     ([5, 6], [1, 2], 3, 1, 64, 64, 1),                      # the wide form's sizes, rows off 16 bytes
     ([2], [1], 100, 4, 128, 128, 0),                        # several passes a token
+    ([2], [1], 33000, 33000, 16, 16, 0),                    # more passes than workgroups share
     ([4, 4], [8, 9], 2, 2, 37, 20, 1),                      # nothing aligned, an odd head
     ([6], [50], 2, 1, 1024, 1024, 0),
     ([6], [50], 1, 1, 1000, 500, 0),
