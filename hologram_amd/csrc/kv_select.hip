@@ -213,10 +213,10 @@ __device__ __forceinline__ uint64_t score_key(int32_t sum, float scale) {
     return u >> 63 ? ~u : u | (1ull << 63);
 }
 
-// The pick of any number of blocks: a workgroup a row and kv head. The `want` largest keys of n are those above
-// a border that is found eight bits at a time from the top by counting, which ends as
-// soon as what shares the border's bits is wanted whole; keys that are equal to the last
-// bit go by their order.
+// The pick of any number of blocks: a workgroup a row and kv head. The `want` largest keys
+// of n are those above a border that is found eight bits at a time from the top by counting,
+// which ends as soon as what shares the border's bits is wanted whole; keys that are equal to
+// the last bit go by their order.
 __global__ __launch_bounds__(kThreads) void pick_any_kernel(Select k) {
     constexpr uint32_t kWaves = kThreads / 64;
     __shared__ uint32_t bins[256], waves[kWaves], picked[3], above_of[kWaves], ties_of[kWaves];

@@ -1,6 +1,7 @@
 // packed_batch.h — what the packed-batch kernels (attn_packed.hip, attn_blocks.hip,
-// attn_selected.hip, kv_blocks.hip, kv_select.hip, qk_norm_rotary.hip) share: finding a workgroup's sequence among the device-resident
-// offsets, widening and narrowing, and the attention of one row at a time.
+// attn_selected.hip, kv_blocks.hip, kv_select.hip, qk_norm_rotary.hip) share: finding a
+// workgroup's sequence among the device-resident offsets, widening and narrowing, and the
+// attention of one row at a time.
 #pragma once
 
 #include <hip/hip_runtime.h>
