@@ -129,7 +129,7 @@ uint32_t bounds_places(const KvBoundsArgs &a) { return (a.pb.tokens / a.block + 
 // A row's sums over dims and heads of the larger of Q lo and Q hi are whole numbers: with
 // P[d] the sum over the kv head's heads of Q's positive parts and N[d] of its negative
 // ones, P . hi + N . lo (a negative scale: P . lo + N . hi), one product for all heads. The
-// pick takes the scores, sum times scale, exact in f64. Up to 640 blocks both are one
+// pick takes the scores, sum times scale, exactly. Up to 640 blocks both are one
 // launch, the sums in LDS (whole_kernel); past that two, whose first reads the bounds with
 // as many workgroups as there are blocks to read (tile_sums_kernel, pick_kernel).
 // Bound by latency, the bytes are few: 32 rows over 2048 to 65536 keys in blocks of 32, 8 kv
@@ -205,18 +205,39 @@ __global__ __launch_bounds__(kThreads) void sums_kernel(Select k) {
     k.sums[(uint64_t(tok - k.row0) * a.Hkv + kh) * k.nb + j] = sum;
 }
 
-// A score as a number in its order: NaN as infinity, -0 as 0. Never 0.
+// A score as a number in its order, exact: NaN as infinity, -0 as 0. Never 0. Sums of kBits bits:
+// up to 29 of them times the scale's 24 are f64's 53; past that (a group of more than 2^15
+// elements) the number is made of whole ones, 9 bits of exponent (1 to 308) and the 54 behind the
+// leading one of the product's 55. That took 5% longer where f64 is enough (one row over 20000
+// blocks: 127 and 120 us; 32 over 6000: 130 and 123).
+template <int kBits>
 __device__ __forceinline__ uint64_t score_key(int32_t sum, float scale) {
-    double v = double(sum) * double(scale);
-    if (v != v) v = INFINITY;
-    const uint64_t u = uint64_t(__double_as_longlong(v + 0.0));
-    return u >> 63 ? ~u : u | (1ull << 63);
+    if constexpr (kBits <= 29) {
+        double v = double(sum) * double(scale);
+        if (v != v) v = INFINITY;
+        const uint64_t u = uint64_t(__double_as_longlong(v + 0.0));
+        return u >> 63 ? ~u : u | (1ull << 63);
+    }
+    const uint32_t u = __float_as_uint(scale), e = u >> 23 & 255u, fraction = u & 0x7fffffu;
+    bool down = (sum < 0) != (u >> 31 != 0);
+    uint64_t size;
+    if (e == 255u) {
+        size = 511ull << 54;
+        down = down && fraction == 0 && sum != 0;      // (0 times infinity is NaN too)
+    } else {
+        const uint64_t m = uint64_t(uint32_t(sum < 0 ? -sum : sum)) * (e ? fraction | 1u << 23 : fraction);
+        const uint32_t lead = m ? uint32_t(__builtin_clzll(m)) : 63u;
+        size = m ? uint64_t(63u - lead + (e ? e : 1u)) << 54 | (m << lead << 1) >> 10 : 0ull;
+        down = down && m != 0;
+    }
+    return down ? (1ull << 63) - 1 - size : 1ull << 63 | size;
 }
 
 // The pick of any number of blocks: a workgroup a row and kv head. The `want` largest keys
 // of n are those above a border that is found eight bits at a time from the top by counting,
 // which ends as soon as what shares the border's bits is wanted whole; keys that are equal to
 // the last bit go by their order.
+template <int kBits>
 __global__ __launch_bounds__(kThreads) void pick_any_kernel(Select k) {
     constexpr uint32_t kWaves = kThreads / 64;
     __shared__ uint32_t bins[256], waves[kWaves], picked[3], above_of[kWaves], ties_of[kWaves];
@@ -240,7 +261,7 @@ __global__ __launch_bounds__(kThreads) void pick_any_kernel(Select k) {
     auto each = [&](auto f) {
         for (uint32_t i0 = 0; i0 < n; i0 += kThreads) {
             const uint32_t i = i0 + tid;
-            f(i < n, i < n ? score_key(sums[i], ks[i]) : 0);
+            f(i < n, i < n ? score_key<kBits>(sums[i], ks[i]) : 0);
         }
     };
     uint64_t border = 0, mask = 0;
@@ -310,12 +331,11 @@ __device__ __forceinline__ uint32_t before(uint64_t m) {
     return __builtin_amdgcn_mbcnt_hi(uint32_t(m >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(m), 0u));
 }
 
-// A number in the scores' order, equal for some that are not: where the sums are below 2^24
-// (kSmall), the product in f32, one rounding, which keeps the order; else score_key's upper
-// word.
-template <bool kSmall>
+// A number in the scores' order, equal for some that are not: for sums of 24 bits the product
+// in f32, one rounding, which keeps the order; else score_key's upper word.
+template <int kBits>
 __device__ __forceinline__ uint32_t rough_key(int32_t sum, float scale) {
-    if constexpr (!kSmall) return uint32_t(score_key(sum, scale) >> 32);
+    if constexpr (kBits > 24) return uint32_t(score_key<kBits>(sum, scale) >> 32);
     float v = float(sum) * scale;
     if (v != v) v = INFINITY;
     const uint32_t u = __float_as_uint(v + 0.0f);
@@ -328,7 +348,7 @@ __device__ __forceinline__ uint32_t rough_key(int32_t sum, float scale) {
 // leaves equal rough keys at the border, those are halved by their exact ones; what is
 // equal then goes by its order.
 // sum(j) and scale(j) may be asked for any j below 64 kWaves kHold.
-template <int kWaves, int kHold, bool kSmall, class Sum, class Scale>
+template <int kWaves, int kHold, int kBits, class Sum, class Scale>
 __device__ __forceinline__ void pick_row(const KvSelectArgs &a, uint32_t seen, Sum sum, Scale scale, int32_t *out,
                                          uint64_t *shared) {
     const uint32_t lane = threadIdx.x & 63u, wave = kWaves == 1 ? 0u : pk_uni(threadIdx.x >> 6), tid = 64 * wave + lane;
@@ -346,7 +366,7 @@ __device__ __forceinline__ void pick_row(const KvSelectArgs &a, uint32_t seen, S
     for (int q = 0; q < kHold; ++q) {
         const uint32_t j = tid + q * kAll;
         const bool in = j - a.first < n;
-        const uint32_t k = rough_key<kSmall>(sum(j), scale(j));
+        const uint32_t k = rough_key<kBits>(sum(j), scale(j));
         key[q] = in ? k : 0u;                                    // (below every key)
         high = key[q] > high ? key[q] : high;
         const uint32_t down = in ? ~k : 0u;
@@ -446,7 +466,7 @@ __device__ __forceinline__ void pick_row(const KvSelectArgs &a, uint32_t seen, S
 #pragma unroll
     for (int q = 0; q < kHold; ++q) {
         const uint32_t j = tid + q * kAll;
-        exact[q] = key[q] == lo ? score_key(sum(j), scale(j)) : 0;
+        exact[q] = key[q] == lo ? score_key<kBits>(sum(j), scale(j)) : 0;
     }
     const Border fine = halve(uint64_t(1), ~uint64_t(0), at_lo - at_hi, need, [&](int q, uint64_t mid) { return exact[q] >= mid; });
     // of the equal ones at the last border the first `left`
@@ -468,7 +488,7 @@ __device__ __forceinline__ void pick_row(const KvSelectArgs &a, uint32_t seen, S
     }
 }
 
-template <int kHold, bool kSmall>
+template <int kHold, int kBits>
 __global__ __launch_bounds__(256) void pick_kernel(Select k) {
     __shared__ uint64_t shared[8];
     const KvSelectArgs &a = k.a;
@@ -478,7 +498,7 @@ __global__ __launch_bounds__(256) void pick_kernel(Select k) {
     const int32_t *sums = k.sums + (uint64_t(tok - k.row0) * a.Hkv + kh) * k.nb;
     const float *ks = a.ks + (uint64_t(at.b) * a.Hkv + kh) * k.nb;
     const auto in = [&](uint32_t j) { return j < k.nb ? j : k.nb - 1; };
-    pick_row<4, kHold, kSmall>(a, blocks_seen(a, at.of, at.hi - at.lo, tok - at.lo), [&](uint32_t j) { return sums[in(j)]; },
+    pick_row<4, kHold, kBits>(a, blocks_seen(a, at.of, at.hi - at.lo, tok - at.lo), [&](uint32_t j) { return sums[in(j)]; },
                                     [&](uint32_t j) { return ks[in(j)]; }, a.out + (uint64_t(tok) * a.Hkv + kh) * a.top, shared);
 }
 
@@ -665,7 +685,7 @@ __global__ __launch_bounds__(256) void tile_sums_kernel(Select k) {
 // Sums and pick in one launch, the sums of kRows rows in LDS, for at most kMost blocks.
 constexpr uint32_t kRows = 16;
 constexpr int kWaves = 8;
-template <class E, int DP, int kMost, bool kSmall>
+template <class E, int DP, int kMost, int kBits>
 __global__ __launch_bounds__(64 * kWaves) void whole_kernel(Select k) {
     __shared__ QParts<DP> parts;
     __shared__ __align__(16) int32_t sums[kRows][kMost + 4];
@@ -691,7 +711,7 @@ __global__ __launch_bounds__(64 * kWaves) void whole_kernel(Select k) {
         __syncthreads();
     }
     for (uint32_t t = pk_uni(threadIdx.x >> 6); t < m; t += kWaves)
-        pick_row<1, kMost / 64, kSmall>(a, blocks_seen(a, len, n, t0 + t), [&](uint32_t j) { return sums[t][j]; },
+        pick_row<1, kMost / 64, kBits>(a, blocks_seen(a, len, n, t0 + t), [&](uint32_t j) { return sums[t][j]; },
                                         [&](uint32_t j) { return scale_of[j]; }, a.out + (uint64_t(at.lo + t0 + t) * a.Hkv + kh) * a.top, nullptr);
 }
 
@@ -713,24 +733,29 @@ bool matrix_applies(const KvSelectArgs &a) {
 // of up to 512 blocks 11 us and two launches 15, 2459 rows of chunks 37 and 95.
 bool whole(const KvSelectArgs &a) { return matrix_applies(a) && blocks_of(a) <= 640; }
 uint32_t places_of(const KvSelectArgs &a) { return a.pb.tokens / (whole(a) ? kRows : kTile) + a.pb.batch; }
-bool small_sums(const KvSelectArgs &a) { return uint64_t(a.H / a.Hkv) * a.D * 127 * 128 < (1u << 24); }
+// Bits of the sums, of at most 127 * 128 an element: 24, 29 or 31 (the matrix form's groups of up
+// to 128 heads of 256 dims: 24 or 29).
+int sum_bits(const KvSelectArgs &a) {
+    const uint64_t most = uint64_t(a.H / a.Hkv) * a.D * 127 * 128;
+    return most < (1u << 24) ? 24 : most < (1u << 29) ? 29 : 31;
+}
 
-template <class E, int DP, bool kSmall>
+template <class E, int DP, int kBits>
 void launch_whole(const Select &k, hipStream_t stream) {
     const uint32_t grid = places_of(k.a) * k.a.Hkv;
-    if (k.nb <= 256) whole_kernel<E, DP, 256, kSmall><<<grid, 64 * kWaves, 0, stream>>>(k);
-    else if (k.nb <= 512) whole_kernel<E, DP, 512, kSmall><<<grid, 64 * kWaves, 0, stream>>>(k);
-    else whole_kernel<E, DP, 640, kSmall><<<grid, 64 * kWaves, 0, stream>>>(k);
+    if (k.nb <= 256) whole_kernel<E, DP, 256, kBits><<<grid, 64 * kWaves, 0, stream>>>(k);
+    else if (k.nb <= 512) whole_kernel<E, DP, 512, kBits><<<grid, 64 * kWaves, 0, stream>>>(k);
+    else whole_kernel<E, DP, 640, kBits><<<grid, 64 * kWaves, 0, stream>>>(k);
 }
 template <class E, int DP>
 void launch_tiles(const Select &k, hipStream_t stream) {
     if (!whole(k.a)) {
         const dim3 grid(places_of(k.a) * k.a.Hkv, (k.nb + kRange - 1) / kRange);
         if (k.nb > k.a.top) tile_sums_kernel<E, DP><<<grid, 256, 0, stream>>>(k);
-    } else if (small_sums(k.a)) {
-        launch_whole<E, DP, true>(k, stream);
+    } else if (sum_bits(k.a) == 24) {
+        launch_whole<E, DP, 24>(k, stream);
     } else {
-        launch_whole<E, DP, false>(k, stream);
+        launch_whole<E, DP, 29>(k, stream);
     }
 }
 template <class E>
@@ -747,13 +772,13 @@ void launch_sums(const Select &k, hipStream_t stream) {
     }
 }
 
-template <bool kSmall>
+template <int kBits>
 void launch_pick(const Select &k, hipStream_t stream) {
     const uint32_t units = (k.row1 - k.row0) * k.a.Hkv;
-    if (k.nb <= 1024) pick_kernel<4, kSmall><<<units, 256, 0, stream>>>(k);
-    else if (k.nb <= 2048) pick_kernel<8, kSmall><<<units, 256, 0, stream>>>(k);
-    else if (k.nb <= 4096) pick_kernel<16, kSmall><<<units, 256, 0, stream>>>(k);
-    else pick_any_kernel<<<units, kThreads, 0, stream>>>(k);
+    if (k.nb <= 1024) pick_kernel<4, kBits><<<units, 256, 0, stream>>>(k);
+    else if (k.nb <= 2048) pick_kernel<8, kBits><<<units, 256, 0, stream>>>(k);
+    else if (k.nb <= 4096) pick_kernel<16, kBits><<<units, 256, 0, stream>>>(k);
+    else pick_any_kernel<kBits><<<units, kThreads, 0, stream>>>(k);
 }
 
 }  // namespace
@@ -791,7 +816,12 @@ hipError_t launch_kv_select(const KvSelectArgs &a, void *scratch, hipStream_t st
         if (a.dtype == 7) launch_sums<Bf16>(k, stream);
         else if (a.dtype == 6) launch_sums<F16>(k, stream);
         else launch_sums<F32>(k, stream);
-        if (!whole(a)) small_sums(a) ? launch_pick<true>(k, stream) : launch_pick<false>(k, stream);
+        if (!whole(a)) {
+            const int bits = sum_bits(a);
+            if (bits == 24) launch_pick<24>(k, stream);
+            else if (bits == 29) launch_pick<29>(k, stream);
+            else launch_pick<31>(k, stream);
+        }
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }

@@ -1,5 +1,7 @@
 """KvBlockBounds (131) and KvBlockSelect (132) on the device: both are whole numbers, so they equal
 the 64-bit restatement."""
+import math
+
 import numpy as np
 import pytest
 
@@ -256,3 +258,46 @@ def test_bad_offsets_are_reported(torch_cuda, backend, starts):
         with pytest.raises(SlotOutOfRange):
             run_select(torch_cuda, backend, c)
         backend.synchronize()
+
+
+def nearly_equal_pair(rng, sums, scale_sign):
+    """Blocks a < b and mantissas (24 bits) whose products with their sums differ, b's score the larger,
+    by less than f64 tells apart; whole numbers throughout."""
+    while True:
+        a, b = sorted(rng.choice(np.arange(1, len(sums) - 1), 2, replace=False).tolist())
+        sa, sb = int(sums[a]), int(sums[b])
+        if math.gcd(sa, sb) != 1:
+            continue
+        for d in (1, 2, 3):
+            d *= -scale_sign                 # sa ma - sb mb = d
+            ma = d * pow(sa, -1, sb) % sb
+            mb = (sa * ma - d) // sb
+            if all(1 << 23 <= m < 1 << 24 for m in (ma, mb)) and float(sa * ma) == float(sb * mb):
+                return a, b, ma, mb
+
+
+@pytest.mark.parametrize("nb", [90, 4200])
+@pytest.mark.parametrize("H,D", [(2048, 64), (1820, 72)])
+def test_select_scores_past_53_bits(torch_cuda, backend, H, D, nb):
+    """Groups of 2^17 elements, whose sums have 31 bits and whose scores 55: two of them that f64
+    would round to the same number are not equal, and the later block, whose score is the larger,
+    is the one. (Scores of either sign; all others far below.)"""
+    rng = np.random.default_rng(H + nb)
+    B, block = 12, 4
+    q = rng.integers(100, 128, (H, D))
+    q[0, 0] = 127
+    lo = rng.integers(100, 128, (nb, D))
+    sums = lo @ q.sum(axis=0)
+    assert sums.min() > 1 << 30 and sums.max() < 1 << 31
+    ks, want = np.zeros((B, 1, nb), np.float32), np.zeros((B, 1, 3), np.int32)
+    for s in range(B):
+        sign = 1 if s % 2 else -1
+        ks[s] = sign * 2.0 ** (-60 if sign > 0 else 60)
+        a, b, ma, mb = nearly_equal_pair(rng, sums, sign)
+        ks[s, 0, a], ks[s, 0, b] = (sign * m * 2.0 ** -30 for m in (ma, mb))
+        want[s, 0] = 0, b, nb - 1
+    c = dict(rows=[1] * B, lens=np.full(B, nb * block, np.uint32), H=H, Hkv=1, D=D, bucket=nb * block, block=block,
+             top=3, first=1, last=1, dtype=DTYPE_BF16, pad=0, gap=0, starts=starts_of([1] * B), ks=ks)
+    c["q"] = encode(np.broadcast_to(q.reshape(-1), (B, H * D)).astype(np.float64), DTYPE_BF16).reshape(B, -1)
+    c["bounds"] = np.broadcast_to(lo[None, None, :, None], (B, 1, nb, 2, D)).astype(np.int8)
+    assert np.array_equal(run_select(torch_cuda, backend, c), want)
