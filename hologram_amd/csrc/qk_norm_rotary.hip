@@ -14,8 +14,8 @@ namespace {
 // with n = rint(2 x / pi), x - n pi / 2 in two steps of one rounding each keeps 2^-50 of
 // a radian for every |x| < 2^50, where f32 would lose the angle itself from some
 // thousand positions on; what is left, at most pi / 4, is f32's.
-__device__ __forceinline__ void turn(uint32_t pos, float freq, float *c, float *s) {
-    const double x = double(pos) * double(freq), low = fma(double(pos), double(freq), -x);
+__device__ __forceinline__ void turn(double pos, float freq, float *c, float *s) {
+    const double x = pos * double(freq), low = fma(pos, double(freq), -x);
     const double n = rint(x * 0.63661977236758134308);
     double r = fma(-n, 1.57079632679489655800, x);
     r = fma(-n, 6.12323399573676603587e-17, r) + low;
@@ -26,11 +26,12 @@ __device__ __forceinline__ void turn(uint32_t pos, float freq, float *c, float *
     *s = quarter & 1 ? (quarter == 1 ? cs : -cs) : (quarter == 0 ? sn : -sn);
 }
 
-// The position of token `tok` in its sequence; false outside every sequence.
-__device__ __forceinline__ bool position(const QkNormRotaryArgs &a, uint32_t tok, uint32_t *pos) {
+// The position of token `tok` in its sequence (33 bits, pos[b] + t); false outside every
+// sequence.
+__device__ __forceinline__ bool position(const QkNormRotaryArgs &a, uint32_t tok, double *pos) {
     RowAt at;
     if (!row_of(a.pb, a.pos, tok, &at)) return false;
-    *pos = at.of + (tok - at.lo);
+    *pos = double(at.of) + double(tok - at.lo);
     return true;
 }
 
@@ -42,7 +43,8 @@ __global__ __launch_bounds__(256) void rows_kernel(QkNormRotaryArgs a) {
     const uint32_t lane = threadIdx.x & 63u, all = a.H + a.Hkv;
     const uint64_t item = uint64_t(blockIdx.x) * 4 + pk_uni(threadIdx.x >> 6);
     const uint32_t tok = uint32_t(item / all);
-    uint32_t h = uint32_t(item - uint64_t(tok) * all), pos;
+    uint32_t h = uint32_t(item - uint64_t(tok) * all);
+    double pos;
     if (tok >= a.pb.tokens || !position(a, tok, &pos)) return;
     const int which = h >= a.H;
     h -= which ? a.H : 0;
@@ -109,7 +111,7 @@ __global__ __launch_bounds__(256) void wide_kernel(QkNormRotaryArgs a, uint32_t 
     typedef typename E::T V;
     constexpr uint32_t kRows = 256 / L;         // rows a pass
     __shared__ __align__(16) float cos_of[4][kWideDim / 2], sin_of[4][kWideDim / 2];
-    __shared__ uint32_t pos_of[4];
+    __shared__ double pos_of[4];
     __shared__ bool in_of[4];
     const uint32_t tid = threadIdx.x, l = tid % L, tok0 = blockIdx.x * T, half = a.rot / 2, turned = a.rot / 8;
     const uint32_t toks = a.pb.tokens - tok0 < T ? a.pb.tokens - tok0 : T;
@@ -140,7 +142,7 @@ __global__ __launch_bounds__(256) void wide_kernel(QkNormRotaryArgs a, uint32_t 
     load(p0, ring[0]);
     const uint32_t wave = pk_uni(tid >> 6);
     if (wave < toks) {
-        uint32_t pos = 0;
+        double pos = 0.0;
         const bool in = position(a, tok0 + wave, &pos);
         if ((tid & 63u) == 0) pos_of[wave] = pos, in_of[wave] = in;
     }

@@ -187,3 +187,12 @@ def test_bad_offsets_are_reported(torch_cuda, backend, starts, D):
     with pytest.raises(SlotOutOfRange):
         run_rotary(torch_cuda, backend, c)
     backend.synchronize()
+
+
+@pytest.mark.parametrize("interleaved", [0, 1])
+@pytest.mark.parametrize("D", [128, 36])
+def test_positions_past_32_bits(torch_cuda, backend, D, interleaved):
+    """A position is pos[b] + t, also where the sum passes 32 bits."""
+    rng = np.random.default_rng(D)
+    c = rotary_case(rng, [5, 40, 3], [0xFFFFFFFE, 0xFFFFFFFF, 0xFFFFFFF0], 2, 1, D, D, DTYPE_F32, 0, interleaved)
+    check_rotary(run_rotary(torch_cuda, backend, c), c)
