@@ -233,6 +233,18 @@ __device__ __forceinline__ uint64_t score_key(int32_t sum, float scale) {
     return down ? (1ull << 63) - 1 - size : 1ull << 63 | size;
 }
 
+// The lists where the plane's blocks all fit: no sums, no pick. A workgroup a row and kv head.
+__global__ __launch_bounds__(kThreads) void every_block_kernel(Select k) {
+    const KvSelectArgs &a = k.a;
+    if (blockIdx.x == 0) check_starts(a.pb);
+    const uint32_t tok = k.row0 + blockIdx.x / a.Hkv, kh = blockIdx.x % a.Hkv;
+    RowAt at;
+    if (!row_of(a.pb, a.lens, tok, &at)) return;
+    const uint32_t seen = blocks_seen(a, at.of, at.hi - at.lo, tok - at.lo);
+    int32_t *out = a.out + (uint64_t(tok) * a.Hkv + kh) * a.top;
+    for (uint32_t i = threadIdx.x; i < a.top; i += kThreads) out[i] = i < seen ? int32_t(i) : -1;
+}
+
 // The pick of any number of blocks: a workgroup a row and kv head. The `want` largest keys
 // of n are those above a border that is found eight bits at a time from the top by counting,
 // which ends as soon as what shares the border's bits is wanted whole; keys that are equal to
@@ -751,7 +763,7 @@ template <class E, int DP>
 void launch_tiles(const Select &k, hipStream_t stream) {
     if (!whole(k.a)) {
         const dim3 grid(places_of(k.a) * k.a.Hkv, (k.nb + kRange - 1) / kRange);
-        if (k.nb > k.a.top) tile_sums_kernel<E, DP><<<grid, 256, 0, stream>>>(k);
+        tile_sums_kernel<E, DP><<<grid, 256, 0, stream>>>(k);
     } else if (sum_bits(k.a) == 24) {
         launch_whole<E, DP, 24>(k, stream);
     } else {
@@ -762,7 +774,7 @@ template <class E>
 void launch_sums(const Select &k, hipStream_t stream) {
     if (!matrix_applies(k.a)) {
         const dim3 grid((k.row1 - k.row0) * k.a.Hkv, (k.nb + kThreads - 1) / kThreads);
-        if (k.nb > k.a.top) sums_kernel<E><<<grid, kThreads, 0, stream>>>(k);
+        sums_kernel<E><<<grid, kThreads, 0, stream>>>(k);
     } else if (k.a.D <= 64) {
         launch_tiles<E, 64>(k, stream);
     } else if (k.a.D <= 128) {
@@ -813,14 +825,18 @@ hipError_t launch_kv_select(const KvSelectArgs &a, void *scratch, hipStream_t st
     const uint32_t step = whole(a) ? a.pb.tokens : rows_a_pass(a);
     for (uint32_t r = 0; r < a.pb.tokens; r += step) {
         k.row0 = r, k.row1 = a.pb.tokens - r < step ? a.pb.tokens : r + step;
-        if (a.dtype == 7) launch_sums<Bf16>(k, stream);
-        else if (a.dtype == 6) launch_sums<F16>(k, stream);
-        else launch_sums<F32>(k, stream);
-        if (!whole(a)) {
-            const int bits = sum_bits(a);
-            if (bits == 24) launch_pick<24>(k, stream);
-            else if (bits == 29) launch_pick<29>(k, stream);
-            else launch_pick<31>(k, stream);
+        if (!whole(a) && k.nb <= a.top) {
+            every_block_kernel<<<(k.row1 - k.row0) * a.Hkv, kThreads, 0, stream>>>(k);
+        } else {
+            if (a.dtype == 7) launch_sums<Bf16>(k, stream);
+            else if (a.dtype == 6) launch_sums<F16>(k, stream);
+            else launch_sums<F32>(k, stream);
+            if (!whole(a)) {
+                const int bits = sum_bits(a);
+                if (bits == 24) launch_pick<24>(k, stream);
+                else if (bits == 29) launch_pick<29>(k, stream);
+                else launch_pick<31>(k, stream);
+            }
         }
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;

@@ -301,3 +301,20 @@ def test_select_scores_past_53_bits(torch_cuda, backend, H, D, nb):
     c["q"] = encode(np.broadcast_to(q.reshape(-1), (B, H * D)).astype(np.float64), DTYPE_BF16).reshape(B, -1)
     c["bounds"] = np.broadcast_to(lo[None, None, :, None], (B, 1, nb, 2, D)).astype(np.int8)
     assert np.array_equal(run_select(torch_cuda, backend, c), want)
+
+
+@pytest.mark.parametrize("D,bucket,block,top", [
+    (72, 320, 16, 20),                       # the general form, as many entries as blocks
+    (72, 320, 16, 33),
+    (64, 1300, 2, 650),                      # two launches
+    (64, 9000, 2, 4600),                     # and more blocks than a workgroup holds
+])
+@pytest.mark.parametrize("starts", [[0, 9, 4, 20], [0, 5, 9, 21], [2**32 - 1, 0, 3, 20], [20, 0, 20, 0]])
+def test_bad_offsets_are_reported_where_every_block_fits_the_list(torch_cuda, backend, starts, D, bucket, block, top):
+    rng = np.random.default_rng(0)
+    c = select_case(rng, [9, 5, 6], [300, 200, 100], 4, 2, D, bucket, block, top, DTYPE_BF16)
+    check_select(run_select(torch_cuda, backend, c), c)
+    c["starts"] = np.array(starts, np.uint32)
+    with pytest.raises(SlotOutOfRange):
+        run_select(torch_cuda, backend, c)
+    backend.synchronize()
