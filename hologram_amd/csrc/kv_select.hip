@@ -744,6 +744,8 @@ bool matrix_applies(const KvSelectArgs &a) {
 // One launch while a row's sums and their scales fit three workgroups into a CU's LDS: 32 rows
 // of up to 512 blocks 11 us and two launches 15, 2459 rows of chunks 37 and 95.
 bool whole(const KvSelectArgs &a) { return matrix_applies(a) && blocks_of(a) <= 640; }
+// A list of every block takes neither sums nor their scratch.
+bool every_block(const KvSelectArgs &a) { return !whole(a) && blocks_of(a) <= a.top; }
 uint32_t places_of(const KvSelectArgs &a) { return a.pb.tokens / (whole(a) ? kRows : kTile) + a.pb.batch; }
 // Bits of the sums, of at most 127 * 128 an element: 24, 29 or 31 (the matrix form's groups of up
 // to 128 heads of 256 dims: 24 or 29).
@@ -809,7 +811,7 @@ hipError_t launch_kv_bounds(const KvBoundsArgs &a, hipStream_t stream) {
 }
 
 size_t kv_select_scratch_bytes(const KvSelectArgs &a) {
-    return whole(a) ? 0 : size_t(rows_a_pass(a)) * a.Hkv * blocks_of(a) * 4;
+    return whole(a) || every_block(a) ? 0 : size_t(rows_a_pass(a)) * a.Hkv * blocks_of(a) * 4;
 }
 
 uint64_t kv_select_threads(const KvSelectArgs &a) {
@@ -825,7 +827,7 @@ hipError_t launch_kv_select(const KvSelectArgs &a, void *scratch, hipStream_t st
     const uint32_t step = whole(a) ? a.pb.tokens : rows_a_pass(a);
     for (uint32_t r = 0; r < a.pb.tokens; r += step) {
         k.row0 = r, k.row1 = a.pb.tokens - r < step ? a.pb.tokens : r + step;
-        if (!whole(a) && k.nb <= a.top) {
+        if (every_block(a)) {
             every_block_kernel<<<(k.row1 - k.row0) * a.Hkv, kThreads, 0, stream>>>(k);
         } else {
             if (a.dtype == 7) launch_sums<Bf16>(k, stream);

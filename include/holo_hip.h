@@ -630,7 +630,9 @@ typedef struct holo_kv_block_bounds_call {
  * ceil(bucket_rows / block_rows)]; lens u32 [batch], device-resident. kv_heads 0 means
  * heads; head_dim <= 1024, heads / kv_heads * head_dim <= 2^17, at most 2^20 blocks a
  * plane, kv_heads times those at most 2^28, top <= 2^20; in any form tokens * kv_heads <
- * 2^24 and (tokens / 16 + batch) * kv_heads * (blocks / 256 + 1) < 2^24. Takes scratch. */
+ * 2^24 and (tokens / 16 + batch) * kv_heads * (blocks / 256 + 1) < 2^24. Where a plane has
+ * more than `top` blocks it may take scratch, at most 256 MiB or one row's kv_heads *
+ * blocks * 4 bytes. */
 typedef struct holo_kv_block_select_call {
     holo_buffer_ref q;
     holo_buffer_ref bounds;

@@ -5,9 +5,9 @@ import math
 import numpy as np
 import pytest
 
-from conftest import from_dev
+from conftest import from_dev, to_dev
 from hologram_amd import (DTYPE_BF16, DTYPE_F16, DTYPE_F32, DTYPE_I8, BufferRef, DequantizeCall,
-                          KernelCall, KvBlockBoundsCall, KvBlockSelectCall, SlotOutOfRange)
+                          DeviceWorkspace, HipBackend, KernelCall, KvBlockBoundsCall, KvBlockSelectCall, SlotOutOfRange)
 from long_context_reference import block_bounds, select_blocks
 from packed_reference import ALL, decode, encode
 from test_gpu_packed_batch import dispatch, starts_of
@@ -318,3 +318,35 @@ def test_bad_offsets_are_reported_where_every_block_fits_the_list(torch_cuda, ba
     with pytest.raises(SlotOutOfRange):
         run_select(torch_cuda, backend, c)
     backend.synchronize()
+
+
+@pytest.mark.parametrize("D,top", [(64, 700), (72, 640)])
+def test_a_list_of_every_block_is_captured_without_an_eager_run(torch_cuda, D, top):
+    """It takes no scratch: nothing has to be dispatched before the capture. Each replay over other
+    lengths is the restatement's."""
+    torch = torch_cuda
+    rng = np.random.default_rng(D)
+    cases = [select_case(rng, [5, 0, 15], lens, 4, 2, D, 1280, 2, top, DTYPE_BF16)
+             for lens in ([1280, 7, 15], [6, 0, 1279], [1, 1, 900])]
+    stream = torch.cuda.Stream()
+    be = HipBackend(0, stream.cuda_stream)
+    ts = [to_dev(torch, cases[0][n]) for n in ("q", "bounds", "ks", "starts", "lens")]
+    out = torch.empty((20, 2, top), dtype=torch.int32, device="cuda")
+    ws = DeviceWorkspace()
+    for s, t in enumerate([*ts, out]):
+        ws.bind(s, t)
+    call = KernelCall.KvBlockSelect(KvBlockSelectCall(*[BufferRef(s) for s in range(6)], 20, 3, 4, 2, 1280, 2, D, 0,
+                                                      top, 1, 1, DTYPE_BF16))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        be.dispatch(call, ws)
+    for turn in (1, 2, 0, 2):
+        for n, t in zip(("q", "bounds", "ks", "starts", "lens"), ts):
+            t.copy_(to_dev(torch, cases[turn][n]))
+        out.fill_(-7)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        check_select(out.cpu().numpy(), cases[turn])
+    be.close()
