@@ -1758,6 +1758,8 @@ int do_qk_norm_rotary(holo_backend *be, const SlotTable &st, const holo_qk_norm_
     const bool has_k = c.k.slot != HOLO_SLOT_ABSENT;
     const uint32_t hkv = !has_k ? 0 : c.kv_heads == 0 ? c.heads : c.kv_heads;
     HOLO_TRY(packed_shape(op, c.tokens, c.batch, c.heads, has_k ? hkv : 1, c.head_dim, c.dtype));
+    if (!has_k && c.k_output.slot != HOLO_SLOT_ABSENT)   // (a session would count it as written)
+        return fail(HOLO_ERR_UNSUPPORTED_OP, "qk_norm_rotary: k_output without k");
     if (c.rotary_dim > c.head_dim)
         return fail(HOLO_ERR_SHAPE_MISMATCH, "qk_norm_rotary: rotary_dim above head_dim");
     if (c.rotary_dim % 2 != 0) return fail(HOLO_ERR_UNSUPPORTED_OP, "qk_norm_rotary: rotary_dim must be even");

@@ -572,10 +572,10 @@ typedef struct holo_logits_process_call {
  * f32(magnitude_bits), 0: 1. Angles are taken in f64 and reduced there, so they keep
  * f32's precision at every position while |p * freq| < 2^50; everything else is f32,
  * rounded to nearest once. rotary_dim 0: no rotation, freqs may be absent. k may be
- * absent (with k_output, k_gamma): q alone. q_stride and k_stride are the elements
- * from one token to the next (0: tight); the outputs are tight, and neither overlaps
- * an input or the other. kv_heads 0 means heads; head_dim <= 1024. tokens * (heads +
- * kv_heads) < 2^26 in any form. */
+ * absent, k_output with it (one without the other is refused): q alone. q_stride and
+ * k_stride are the elements from one token to the next (0: tight); the outputs are
+ * tight, and neither overlaps an input or the other. kv_heads 0 means heads; head_dim
+ * <= 1024. tokens * (heads + kv_heads) < 2^26 in any form. */
 typedef struct holo_qk_norm_rotary_call {
     holo_buffer_ref q;
     holo_buffer_ref k;

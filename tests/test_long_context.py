@@ -200,3 +200,18 @@ def test_a_graph_of_them_loads_and_its_caches_move_in_place():
     assert moved == 3
     labels = s.output_labels(["blake3:%064x" % i for i in range(9)])
     assert len(set(labels)) == len(labels) == 9
+
+
+def test_an_output_for_k_without_k_is_refused():
+    """The call would not write it, but a session would label it as written."""
+    for change in (dict(k=NO_BUFFER), dict(k=NO_BUFFER, k_gamma=NO_BUFFER), dict(k=NO_BUFFER, norms=0, rotary_dim=0)):
+        with pytest.raises(UnsupportedOp, match="k_output"):
+            validate(KernelCall.QkNormRotary(replace(ROTARY, **change)), ROTARY_SIZES)
+    w = HoloWriter()
+    w.inputs = [PortDescriptor("q", 0, 640, DTYPE_BF16, [640]), PortDescriptor("starts", 1, 2, DTYPE_I32, [2])]
+    w.outputs = [PortDescriptor("q'", 2, 640, DTYPE_BF16, [640]), PortDescriptor("k'", 3, 640, DTYPE_BF16, [640])]
+    alone = QkNormRotaryCall(R(0, 0, 1280), NO_BUFFER, NO_BUFFER, NO_BUFFER, R(1, 0, 8), NO_BUFFER, NO_BUFFER,
+                             R(2, 0, 1280), R(3, 0, 1280), 10, 1, 1, 0, 64, 0)
+    w.kernel_calls, w.exec_plan = [KernelCall.QkNormRotary(alone)], [[0]]
+    with pytest.raises(UnsupportedOp, match="k_output"):
+        HipSession(None, w.finish())
