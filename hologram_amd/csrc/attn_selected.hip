@@ -21,7 +21,8 @@ namespace {
 // TB/s (one group, whose registers leave two wavefronts a SIMD: 303). By latency where they
 // are few: 8 rows over 256 keys 6.0 us, 26 f32 rows of drafts over 1280 keys 15. A wavefront a
 // row and head (below): 1560 us, 11.5 ms, 131 us, 754 us.
-constexpr uint32_t kMaxList = 512;            // entries a workgroup takes
+constexpr uint32_t kMaxList = 512;            // entries a workgroup takes at once
+constexpr uint32_t kMostParts = 8192;         // shares' results in scratch: 135 MB at 256 dims, 68 at 128
 constexpr uint32_t kNone = 0x80000000u;       // past every key
 
 struct Selected {
@@ -38,7 +39,8 @@ struct Entry {
     float ks, vs;
 };
 
-template <class E, int DP, int W, int C, bool kOnce>
+// kRounds: a share's entries kMaxList at a time.
+template <class E, int DP, int W, int C, bool kOnce, bool kRounds>
 __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : C == 2 ? 3 : 2) void few_kernel(Selected k) {
     constexpr int S = C > 2 ? C / 2 : 1;       // loads of two 16-key steps a turn
     constexpr uint32_t kHeads = kUnit / C;
@@ -54,27 +56,30 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : C == 2 ? 3 : 2) void few_ker
     if (!row_of(a.pb, a.lens, tok, &at)) return;
     const uint32_t sees = visible_keys(at.of, at.hi - at.lo, tok - at.lo, a.bucket), G = a.H / a.Hkv;
     const uint64_t plane = uint64_t(at.b) * a.Hkv + kh, nb = (uint64_t(a.bucket) + a.block - 1) >> k.shift;
-    const uint32_t e0 = share * k.per, n = k.s.top - e0 < k.per ? k.s.top - e0 : k.per;
+    const uint32_t e0 = share * k.per, mine = k.s.top - e0 < k.per ? k.s.top - e0 : k.per;
     const int32_t *ids = k.s.blocks + (uint64_t(tok) * a.Hkv + kh) * k.s.top + e0;
-    if (tid == 0) last = 0;
-    __syncthreads();
-    for (uint32_t i = tid; i < n; i += 64 * W) {
-        const int32_t id = ids[i];
-        const bool ok = id >= 0 && uint64_t(id) << k.shift < sees;
-        const uint64_t j = plane * nb + (ok ? uint32_t(id) : 0u);
-        list[i] = Entry{ok ? uint32_t(id) << k.shift : kNone, a.ks[j], a.vs[j]};
-        if (ok) atomicMax(&last, i + 1);
-    }
+    auto read_list = [&](uint32_t from) __attribute__((always_inline)) {
+        if (tid == 0) last = 0;
+        __syncthreads();
+        const uint32_t n = mine - from < kMaxList ? mine - from : kMaxList;
+        for (uint32_t i = tid; i < n; i += 64 * W) {
+            const int32_t id = ids[from + i];
+            const bool ok = id >= 0 && uint64_t(id) << k.shift < sees;
+            const uint64_t j = plane * nb + (ok ? uint32_t(id) : 0u);
+            list[i] = Entry{ok ? uint32_t(id) << k.shift : kNone, a.ks[j], a.vs[j]};
+            if (ok) atomicMax(&last, i + 1);
+        }
+    };
+    read_list(0);
     const uint32_t r = tid & 15u, h0 = kh * G + tile * kUnit, rows = G - tile * kUnit < kUnit ? G - tile * kUnit : kUnit;
     const bool live = r % kHeads < rows;
     RowQ<E, DP> q;
     q.load(static_cast<const T *>(a.q) + uint64_t(tok) * a.q_stride + uint64_t(h0 + (live ? r % kHeads : 0u)) * a.D, live, a.D, k.mul);
-    __syncthreads();
     // 2^deep 16-key steps a block, of one longer than what the row sees those that hold it (so
     // the steps of a list are at most 2^31)
     const uint32_t reach = sees <= 16 ? 4u : 32u - uint32_t(__builtin_clz(sees - 1));
-    const uint32_t count = pk_uni(last), deep = (k.shift < reach ? k.shift : reach) - 4;
-    const uint32_t halves = count << deep, turns = (halves + 2 * S - 1) / (2 * S);
+    const uint32_t deep = (k.shift < reach ? k.shift : reach) - 4;
+    uint32_t halves;
     const KvPlane<DP> kv(a.kq + plane * a.bucket * a.D, a.vq + plane * a.bucket * a.D, a.bucket, a.D);
     struct Turn {
         KvStep<DP> x[S];
@@ -112,22 +117,33 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : C == 2 ? 3 : 2) void few_ker
         else
             group_step<E, DP, C>(st, o.x, q, o.key[0], o.ks, o.vs, sees);
     };
-    Turn ring[2];
-    if (wave < turns) load(wave, ring[0]);
-    for (uint32_t i = wave; i < turns; i += 2 * W) {
-        if (i + W < turns) load(i + W, ring[1]);
-        take(ring[0]);
-        if (i + W >= turns) break;
-        if (i + 2 * W < turns) load(i + 2 * W, ring[0]);
-        take(ring[1]);
+    bool any = false;
+    for (uint32_t from = 0;;) {
+        __syncthreads();
+        const uint32_t count = pk_uni(last);
+        any |= count != 0;
+        halves = count << deep;
+        const uint32_t turns = (halves + 2 * S - 1) / (2 * S);
+        Turn ring[2];
+        if (wave < turns) load(wave, ring[0]);
+        for (uint32_t i = wave; i < turns; i += 2 * W) {
+            if (i + W < turns) load(i + W, ring[1]);
+            take(ring[0]);
+            if (i + W >= turns) break;
+            if (i + 2 * W < turns) load(i + 2 * W, ring[0]);
+            take(ring[1]);
+        }
+        if (!kRounds || (from += kMaxList) >= mine) break;
+        __syncthreads();      // (no wavefront reads the list that follows before all are done with this one)
+        read_list(from);
     }
     float *dst = k.part + (uint64_t(blockIdx.x) * k.shares + share) * (kUnit * (DP + 2));
     join_waves<E, DP, W, C>(st, rows, a.D, lds, [&](uint32_t c, uint32_t d, float o, float M, float l) {
         if (k.shares == 1) {
-            static_cast<T *>(a.out)[(uint64_t(tok) * a.H + h0 + c) * a.D + d] = E::narrow(count ? o / l : 0.0f);
+            static_cast<T *>(a.out)[(uint64_t(tok) * a.H + h0 + c) * a.D + d] = E::narrow(any ? o / l : 0.0f);
         } else {
             dst[c * (DP + 2) + d] = o;
-            if (d == 0) dst[c * (DP + 2) + DP] = M, dst[c * (DP + 2) + DP + 1] = count ? l : -1.0f;
+            if (d == 0) dst[c * (DP + 2) + DP] = M, dst[c * (DP + 2) + DP + 1] = any ? l : -1.0f;
         }
     });
 }
@@ -162,14 +178,17 @@ bool matrix_applies(const AttnSelectedArgs &s) {
 uint32_t padded(uint32_t D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 uint32_t tiles_of(const AttnBlocksArgs &a) { return (a.H / a.Hkv + kUnit - 1) / kUnit; }
 uint64_t units_of(const AttnBlocksArgs &a) { return uint64_t(a.pb.tokens) * a.Hkv * tiles_of(a); }
-// Entries a workgroup: the whole list (kMaxList of them at most), but where the units leave
-// CUs idle and the list is four rounds of eight wavefronts, shares for as many workgroups as
-// there are CUs, of four 32-key steps at least. One row of 8 kv heads over 2048 and 16384 keys
-// whole and in shares: 19 and 117 us against 11 and 17; 4 rows over 8192, 67 against 20; 16
-// over 2048, 24 against 21; 8 rows over 256, 6.0 against 8.2. Every share has an entry.
+// Entries a workgroup: at most kMaxList while that makes no more than kMostParts shares in all,
+// else more, kMaxList at a time, and past kMostParts / 2 units all of them (4096 rows of 8 kv
+// heads with 600 blocks of 16 keys: 6.37 ms, two shares each and 545 MB of scratch 6.50; 600
+// with 1024: 3.03, 3.05). But where the units leave CUs idle and the list is four rounds of
+// eight wavefronts, shares for as many workgroups as there are CUs, of four 32-key steps at
+// least. One row of 8 kv heads over 2048 and 16384 keys whole and in shares: 19 and 117 us
+// against 11 and 17; 4 rows over 8192, 67 against 20; 16 over 2048, 24 against 21; 8 rows over
+// 256, 6.0 against 8.2. Every share has an entry.
 uint32_t entries_of(const AttnSelectedArgs &s) {
     const uint64_t units = units_of(s.a), steps = uint64_t(s.top) * s.a.block / kStep;
-    uint64_t shares = (s.top + kMaxList - 1) / kMaxList;
+    uint64_t shares = std::min<uint64_t>((s.top + kMaxList - 1) / kMaxList, std::max<uint64_t>(kMostParts / units, 1));
     if (steps >= 32 && units < 256) shares = std::max(shares, std::min(256 / units, steps / 4));
     shares = std::min<uint64_t>(shares, s.top);
     return uint32_t((s.top + shares - 1) / shares);
@@ -185,21 +204,21 @@ bool four_waves(const AttnSelectedArgs &s) { return s.a.D > 128 || units_of(s.a)
 // many sequences 48.6 and 51.6).
 bool reads_once(const AttnSelectedArgs &s) { return s.a.pb.tokens <= s.a.pb.batch; }
 
+template <class E, int DP, int W, int C, bool kRounds>
+void launch_form(const Selected &k, dim3 grid, hipStream_t stream) {
+    if (reads_once(k.s)) few_kernel<E, DP, W, C, true, kRounds><<<grid, 64 * W, 0, stream>>>(k);
+    else few_kernel<E, DP, W, C, false, kRounds><<<grid, 64 * W, 0, stream>>>(k);
+}
 template <class E, int DP>
 void launch_few(const Selected &k, hipStream_t stream) {
     const dim3 grid(uint32_t(units_of(k.s.a)), k.shares);
     constexpr uint32_t kMost = DP > 128 ? 4 : 8, kGroups = DP > 128 ? 1 : 2;
-    const bool once = reads_once(k.s);
-    if (four_waves(k.s) && k.s.a.H / k.s.a.Hkv <= kUnit / kGroups) {
-        if (once) few_kernel<E, DP, 4, kGroups, true><<<grid, 256, 0, stream>>>(k);
-        else few_kernel<E, DP, 4, kGroups, false><<<grid, 256, 0, stream>>>(k);
-    } else if (four_waves(k.s)) {
-        if (once) few_kernel<E, DP, 4, 1, true><<<grid, 256, 0, stream>>>(k);
-        else few_kernel<E, DP, 4, 1, false><<<grid, 256, 0, stream>>>(k);
-    } else {
-        if (once) few_kernel<E, DP, kMost, 1, true><<<grid, 64 * kMost, 0, stream>>>(k);
-        else few_kernel<E, DP, kMost, 1, false><<<grid, 64 * kMost, 0, stream>>>(k);
-    }
+    const bool rounds = k.per > kMaxList, groups = k.s.a.H / k.s.a.Hkv <= kUnit / kGroups;
+    if (rounds && groups) launch_form<E, DP, 4, kGroups, true>(k, grid, stream);
+    else if (rounds) launch_form<E, DP, 4, 1, true>(k, grid, stream);
+    else if (four_waves(k.s) && groups) launch_form<E, DP, 4, kGroups, false>(k, grid, stream);
+    else if (four_waves(k.s)) launch_form<E, DP, 4, 1, false>(k, grid, stream);
+    else launch_form<E, DP, kMost, 1, false>(k, grid, stream);
     if (k.shares > 1) merge_kernel<E, DP><<<grid.x, 256, 0, stream>>>(k);
 }
 template <class E>

@@ -652,8 +652,8 @@ typedef struct holo_kv_block_select_call {
  * over, a block listed twice counts twice. Scores, softmax, roundings and the result as
  * in 128; a row that sees no key is zeros, and what a row does not see, blocks that its
  * list does not name among it, does not reach its result. kv_heads 0 means heads; head_dim
- * <= 1024; bucket_rows * head_dim <= 2^30; top <= 2^20; tokens * heads * (top / 512 + 1) <
- * 2^24 in any form. Long lists and few rows take scratch. */
+ * <= 1024; bucket_rows * head_dim <= 2^30; top <= 2^20; tokens * heads < 2^24 in any form.
+ * Long lists and few rows may take scratch, at most 136 MB. */
 typedef struct holo_attention_i8_selected_call {
     holo_buffer_ref q;
     holo_buffer_ref k_cache;

@@ -407,3 +407,63 @@ def test_a_row_of_scores_that_are_infinite(torch_cuda, backend, n):
     nan = (sees & ~(dots > 0)).any(axis=2) | ~keep[:, 4:]
     assert np.array_equal(np.isnan(decode(got[:, 4:], DTYPE_BF16)).reshape(n, 4, 64).all(axis=2), nan)
     assert np.array_equal(np.isnan(decode(got[:, 4:], DTYPE_BF16)).reshape(n, 4, 64).any(axis=2), nan)
+
+
+# ------------------------------------------------- lists past one workgroup's ----
+def long_lists(rng, tokens, kv, top, nb, filled):
+    """Lists of `top` entries of which `filled` name blocks, among them the places about each 512th;
+    the others are out of range."""
+    lists = rng.choice([-1, nb, nb + 5, -2**31, 2**31 - 1], (tokens, kv, top)).astype(np.int64)
+    edges = [i for c in range(0, top + 1, 512) for i in (c - 1, c, c + 1) if 0 <= i < top]
+    for _ in range(filled):
+        at = rng.integers(0, top, (tokens, kv))
+        at = np.where(rng.random((tokens, kv)) < 0.6, rng.choice(edges, (tokens, kv)), at)
+        np.put_along_axis(lists, at[..., None], rng.integers(0, nb, (tokens, kv, 1)), axis=2)
+    lists[::5] = -1                          # rows whose list names nothing
+    lists[1::5, :, :min(top, 512)] = -1      # and whose first 512 do not
+    return lists.astype(np.int32)
+
+
+@pytest.mark.parametrize("dtype", [DTYPE_BF16, DTYPE_F32])
+@pytest.mark.parametrize("rows,lens,H,Hkv,D,bucket,block,top", [
+    ([4100, 0, 60], [4000, 3, 700], 8, 2, 64, 4096, 16, 513),        # one share: two rounds of a list
+    ([2100], [2200], 16, 4, 128, 2208, 32, 1300),                    # three rounds
+    ([8200], [9000], 17, 1, 64, 9008, 16, 600),                      # more heads than 16
+    ([3000], [3000], 1, 1, 128, 3008, 16, 1600),                     # two shares of two rounds each
+    ([700], [700], 4, 1, 256, 704, 16, 1100),                        # a share a round
+    ([2], [700], 4, 2, 64, 704, 16, 30000),                          # few rows, more shares than rounds
+])
+def test_lists_of_several_rounds(torch_cuda, backend, rows, lens, H, Hkv, D, bucket, block, top, dtype):
+    rng = np.random.default_rng(top)
+    c = selected_case(rng, rows, lens, H, Hkv, D, bucket, block, 1, dtype)
+    c["top"], nb = top, -(-bucket // block)
+    c["lists"] = long_lists(rng, sum(rows), Hkv, top, nb - 2, 5)
+    c["ks"], c["vs"] = c["ks"].copy(), c["vs"].copy()
+    c["ks"][:, :, nb - 2:], c["vs"][:, :, nb - 2:] = np.nan, np.inf          # blocks that nothing names
+    c["lists"][c["lists"] == nb - 2] = -1
+    check_selected(run_selected(torch_cuda, backend, c), c)
+
+
+def test_long_lists_of_many_rows_take_little_scratch(torch_cuda):
+    """16384 rows with lists of 513 entries: what the backend allocates stays below the 136 MB that
+    the header states, and the result is the formula's."""
+    torch = torch_cuda
+    rng = np.random.default_rng(1)
+    c = selected_case(rng, [16384], [16400], 1, 1, 256, 16400, 16, 1, DTYPE_BF16)
+    c["top"], c["lists"] = 513, long_lists(rng, 16384, 1, 513, 1025, 3)
+    be = HipBackend(0, torch.cuda.current_stream().cuda_stream)
+    before = []
+
+    class Watched:
+        def dispatch(self, call, ws):
+            torch.cuda.synchronize()
+            before.append(torch.cuda.mem_get_info()[0])
+            be.dispatch(call, ws)
+
+        def synchronize(self):
+            be.synchronize()
+            before.append(torch.cuda.mem_get_info()[0])
+    got = run_selected(torch, Watched(), c)
+    assert before[0] - before[1] < 140 << 20, (before[0] - before[1]) >> 20
+    check_selected(got, c)
+    be.close()
