@@ -1123,23 +1123,31 @@ def _flat_form(ctype):
     nested structures of to_c() took 3-5 us of a dispatch's 6, longer than a
     small kernel runs (six BufferRefs: 4.5 us, packed 1.6). What pack takes and
     to_c() does not (an integer type other than int), or the other way round (a
-    value past its field, which to_c() wraps), gives None."""
+    value past its field, which to_c() wraps), gives None. Beside the bytes:
+    whether they are read from ints of BufferRefs and payloads of _FLAT alone, all
+    of them frozen, in one look at the types (a call that is dispatched once pays
+    for it)."""
     fmt, exprs, end = "<" + _CODE[dict(_ffi.KernelCallC._fields_)["tag"]], ["t"], 4
+    held = {}
     for path, t, at in _leaves("p", ctype, _ffi.KernelCallC.u.offset):
         fmt += f"{at - end}x" + _CODE[t]
-        exprs.append(f"int({path})" if path.endswith(("b_packed", "bq_omajor")) else path)
+        converted = path.endswith(("b_packed", "bq_omajor"))
+        exprs.append(f"int({path})" if converted else path)
+        parts = path.split(".")
+        held.update(dict.fromkeys(".".join(parts[:n]) for n in range(2, len(parts) + converted)))
         end = at + ctypes.sizeof(t)
     layout = struct.Struct(fmt + f"{ctypes.sizeof(_ffi.KernelCallC) - end}x")
     values = eval(f"lambda t, p: ({', '.join(exprs)})")  # noqa: S307 (names of this module's fields)
+    types = eval(f"lambda p: ({''.join(f'type({x}), ' for x in held)})")  # noqa: S307
 
     def form(tag, payload):
         v = values(tag, payload)
         if not _INTS.issuperset(map(type, v)):
-            return None
+            return None, False
         try:
-            return layout.pack(*v)
+            return layout.pack(*v), _FROZEN.issuperset(types(payload))
         except struct.error:
-            return None
+            return None, False
     return form
 
 
@@ -1170,6 +1178,7 @@ _FLAT = {cls: _flat_form(ctype) for cls, ctype in (
     (KvBlockSelectCall, _ffi.KvBlockSelectCallC),
     (AttentionI8SelectedCall, _ffi.AttentionI8SelectedCallC),
     (MatMulDequantCall, _ffi.MatMulDequantCallC))}
+_FROZEN = _INTS.union((BufferRef,), _FLAT)
 
 
 def dispatch_form(call: "KernelCall"):
@@ -1179,28 +1188,13 @@ def dispatch_form(call: "KernelCall"):
     kept = call.__dict__.get("_packed")
     if kept is not None:
         return kept
-    payload = call.payload
-    form = _FLAT.get(type(payload))
-    packed = form and form(call.tag, payload)
+    form = _FLAT.get(type(call.payload))
+    packed, frozen = form(call.tag, call.payload) if form else (None, False)
     if not packed:
         return ctypes.byref(call.to_c())
-    if type(call) is KernelCall and _all_frozen(payload):
+    if frozen and type(call) is KernelCall:
         object.__setattr__(call, "_packed", packed)
     return packed
-
-
-def _all_frozen(payload) -> bool:
-    """Whether what a payload of _FLAT holds is numbers, BufferRefs and payloads of _FLAT."""
-    for v in payload.__dict__.values():
-        t = type(v)
-        if t in _INTS:
-            continue
-        if t is BufferRef:
-            if not _INTS.issuperset(map(type, v.__dict__.values())):
-                return False
-        elif t not in _FLAT or not _all_frozen(v):
-            return False
-    return True
 
 
 def _attn_c(p: DecodeAttentionI8Call) -> _ffi.DecodeAttentionI8CallC:
