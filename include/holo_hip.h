@@ -619,11 +619,12 @@ typedef struct holo_kv_block_bounds_call {
  * the others those of the largest score, the lower block of equal ones. In ascending
  * order, -1 behind them. output i32 [tokens, kv_heads, top].
  * A block's score is k_scale * sum over the kv head's heads h and dims d of the larger
- * (k_scale < 0: the smaller) of Q[h][d] * lo[d] and Q[h][d] * hi[d], with lo and hi its
- * bounds (131) and Q = rne(q / 2^e), 2^e the least power of two, e >= -126, with max|q|
- * <= 127 * 2^e over the group's finite elements (those that are not count as 0). Whole
- * numbers times an f32: scores are compared exactly. One that is NaN ranks as positive
- * infinity. keep_last >= 1, keep_first + keep_last <= top: the block that holds a row's
+ * (k_scale < 0: the smaller) of Q[h][d] * lo[d] and Q[h][d] * hi[d], with lo <= hi its
+ * bounds as 131 leaves them (of any others, hi for a positive Q and lo for a negative
+ * one, k_scale < 0 the other way round) and Q = rne(q / 2^e), 2^e the least power of
+ * two, e >= -126, with max|q| <= 127 * 2^e over the group's finite elements (those that
+ * are not count as 0). Whole numbers times an f32: scores are compared exactly. One that
+ * is NaN ranks as positive infinity. keep_last >= 1, keep_first + keep_last <= top: the block that holds a row's
  * last key may hold later rows, so its bounds and scale are never looked at.
  * q of bf16, f16 or f32 (q_stride as in 128); bounds int8 [batch * kv_heads,
  * ceil(bucket_rows / block_rows), 2, head_dim]; k_scales f32 [batch * kv_heads,

@@ -8,7 +8,7 @@ import pytest
 from conftest import from_dev, to_dev
 from hologram_amd import (DTYPE_BF16, DTYPE_F16, DTYPE_F32, DTYPE_I8, BufferRef, DequantizeCall,
                           DeviceWorkspace, HipBackend, KernelCall, KvBlockBoundsCall, KvBlockSelectCall, SlotOutOfRange)
-from long_context_reference import block_bounds, select_blocks
+from long_context_reference import block_bounds, eight_bits, select_blocks
 from packed_reference import ALL, decode, encode
 from test_gpu_packed_batch import dispatch, starts_of
 
@@ -350,3 +350,26 @@ def test_a_list_of_every_block_is_captured_without_an_eager_run(torch_cuda, D, t
         torch.cuda.synchronize()
         check_select(out.cpu().numpy(), cases[turn])
     be.close()
+
+
+@pytest.mark.parametrize("D", [64, 72])
+def test_select_bounds_that_are_not_in_order(torch_cuda, backend, D):
+    """Where lo is above hi, a block that nothing has bounded yet, hi still goes with the positive
+    elements of Q and lo with the negative ones, the other way round under a negative scale."""
+    rng = np.random.default_rng(D)
+    c = select_case(rng, [30], [1000], 4, 2, D, 1000, 8, 9, DTYPE_F32)
+    c["bounds"] = rng.integers(-128, 128, c["bounds"].shape, dtype=np.int8)
+    c["ks"][:, :, ::3] *= -1.0
+    got = run_select(torch_cuda, backend, c)
+    q = decode(c["q"], DTYPE_F32).reshape(30, 2, 2, D)
+    lo, hi = c["bounds"][0].astype(np.int64).transpose(2, 0, 1, 3)               # [kv, nb, D]
+    for t in range(30):
+        seen = -(-(1000 - 29 + t) // 8)
+        j = np.arange(1, seen - 1)
+        for h in range(2):
+            x = eight_bits(q[t, h]).astype(np.int64)
+            up, down = np.maximum(x, 0).sum(axis=0), np.minimum(x, 0).sum(axis=0)
+            s = c["ks"][0, h, j].astype(np.float64)
+            score = s * np.where(s < 0, lo[h, j] @ up + hi[h, j] @ down, hi[h, j] @ up + lo[h, j] @ down)
+            best = j[np.argsort(-score, kind="stable")[:7]]
+            assert got[t, h].tolist() == sorted([0, *best.tolist(), seen - 1])
