@@ -39,10 +39,9 @@ struct Entry {
     float ks, vs;
 };
 
-// kRounds: a share's entries kMaxList at a time.
+// C column groups (1 or 2). kRounds: a share's entries kMaxList at a time.
 template <class E, int DP, int W, int C, bool kOnce, bool kRounds>
 __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : C == 2 ? 3 : 2) void few_kernel(Selected k) {
-    constexpr int S = C > 2 ? C / 2 : 1;       // loads of two 16-key steps a turn
     constexpr uint32_t kHeads = kUnit / C;
     typedef typename E::T T;
     __shared__ FewLds<E, DP, W> lds;
@@ -82,9 +81,9 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : C == 2 ? 3 : 2) void few_ker
     uint32_t halves;
     const KvPlane<DP> kv(a.kq + plane * a.bucket * a.D, a.vq + plane * a.bucket * a.D, a.bucket, a.D);
     struct Turn {
-        KvStep<DP> x[S];
-        uint32_t key[2];      // the steps' first keys (C == 1), or the column's step's
-        float ks, vs;
+        KvStep<DP> x;         // two 16-key steps
+        uint32_t key[2];      // their first keys (C == 1), or the column's step's
+        float ks, vs;         // (C == 2) the column's step's
     };
     // A 16-key step of the list: its entry, and its first key (kNone past the list)
     auto half_at = [&](uint32_t half, Entry *e) __attribute__((always_inline)) {
@@ -93,19 +92,16 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : C == 2 ? 3 : 2) void few_ker
     };
     auto load = [&](uint32_t turn, Turn &o) __attribute__((always_inline)) {
         Entry e;
+        uint32_t so[2];
 #pragma unroll
-        for (int t = 0; t < S; ++t) {
-            uint32_t so[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint32_t key = pk_uni(half_at(2 * (S * turn + t) + h, &e));
-                so[h] = key == kNone ? kOob : key * a.D;
-                if constexpr (C == 1) o.key[h] = key, o.x[t].ks[h] = e.ks, o.x[t].vs[h] = e.vs;
-            }
-            kv.template load<kOnce>(so, o.x[t]);
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t key = pk_uni(half_at(2 * turn + h, &e));
+            so[h] = key == kNone ? kOob : key * a.D;
+            if constexpr (C == 1) o.key[h] = key, o.x.ks[h] = e.ks, o.x.vs[h] = e.vs;
         }
-        if constexpr (C > 1) {
-            o.key[0] = half_at(2 * S * turn + r / kHeads, &e);
+        kv.template load<kOnce>(so, o.x);
+        if constexpr (C == 2) {
+            o.key[0] = half_at(2 * turn + r / kHeads, &e);
             o.ks = e.ks, o.vs = e.vs;
         }
     };
@@ -113,9 +109,9 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : C == 2 ? 3 : 2) void few_ker
     st.clear();
     auto take = [&](const Turn &o) __attribute__((always_inline)) {
         if constexpr (C == 1)
-            few_step<E, DP>(st, o.x[0], q, o.key, o.key[0] + 16 > sees || o.key[1] + 16 > sees, sees, sees);
+            few_step<E, DP>(st, o.x, q, o.key, o.key[0] + 16 > sees || o.key[1] + 16 > sees, sees, sees);
         else
-            group_step<E, DP, C>(st, o.x, q, o.key[0], o.ks, o.vs, sees);
+            group_step<E, DP>(st, o.x, q, o.key[0], o.ks, o.vs, sees);
     };
     bool any = false;
     for (uint32_t from = 0;;) {
@@ -123,7 +119,7 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : C == 2 ? 3 : 2) void few_ker
         const uint32_t count = pk_uni(last);
         any |= count != 0;
         halves = count << deep;
-        const uint32_t turns = (halves + 2 * S - 1) / (2 * S);
+        const uint32_t turns = (halves + 1) / 2;
         Turn ring[2];
         if (wave < turns) load(wave, ring[0]);
         for (uint32_t i = wave; i < turns; i += 2 * W) {
@@ -212,13 +208,18 @@ void launch_form(const Selected &k, dim3 grid, hipStream_t stream) {
 template <class E, int DP>
 void launch_few(const Selected &k, hipStream_t stream) {
     const dim3 grid(uint32_t(units_of(k.s.a)), k.shares);
-    constexpr uint32_t kMost = DP > 128 ? 4 : 8, kGroups = DP > 128 ? 1 : 2;
-    const bool rounds = k.per > kMaxList, groups = k.s.a.H / k.s.a.Hkv <= kUnit / kGroups;
-    if (rounds && groups) launch_form<E, DP, 4, kGroups, true>(k, grid, stream);
-    else if (rounds) launch_form<E, DP, 4, 1, true>(k, grid, stream);
-    else if (four_waves(k.s) && groups) launch_form<E, DP, 4, kGroups, false>(k, grid, stream);
-    else if (four_waves(k.s)) launch_form<E, DP, 4, 1, false>(k, grid, stream);
-    else launch_form<E, DP, kMost, 1, false>(k, grid, stream);
+    const bool rounds = k.per > kMaxList;
+    if constexpr (DP > 128) {
+        if (rounds) launch_form<E, DP, 4, 1, true>(k, grid, stream);
+        else launch_form<E, DP, 4, 1, false>(k, grid, stream);
+    } else {
+        const bool groups = k.s.a.H / k.s.a.Hkv <= kUnit / 2;
+        if (rounds && groups) launch_form<E, DP, 4, 2, true>(k, grid, stream);
+        else if (rounds) launch_form<E, DP, 4, 1, true>(k, grid, stream);
+        else if (four_waves(k.s) && groups) launch_form<E, DP, 4, 2, false>(k, grid, stream);
+        else if (four_waves(k.s)) launch_form<E, DP, 4, 1, false>(k, grid, stream);
+        else launch_form<E, DP, 8, 1, false>(k, grid, stream);
+    }
     if (k.shares > 1) merge_kernel<E, DP><<<grid.x, 256, 0, stream>>>(k);
 }
 template <class E>

@@ -303,32 +303,33 @@ __device__ __forceinline__ void few_step(State<DP> &st, const KvStep<DP> &x, con
     }
 }
 
-// few_step for rows that are few: C column groups of 16 / C rows, each over a 16-key step of
-// its own (C of them, in C / 2 loads), so that a lane's scores are four and not four times
-// C. Column r is row r % (16 / C) over step r / (16 / C): the products are made for all
-// columns and those of a column's step kept, and its weights enter the products with V as
-// zeros but for its step's keys. `key`, `ks` and `vs` are of the column's step.
-template <class E, int DP, int C>
-__device__ __forceinline__ void group_step(State<DP> &st, const KvStep<DP> (&x)[C / 2], const RowQ<E, DP> &q, uint32_t key,
+// few_step for at most eight rows: two column groups of eight, each over a 16-key step of its
+// own, so that a lane's scores are four and not eight. Column r is row r % 8 over step r / 8: the
+// products are made for all columns and those of a column's step kept, and its weights enter the
+// products with V as zeros but for its step's keys. `key`, `ks` and `vs` are of the column's
+// step.
+template <class E, int DP>
+__device__ __forceinline__ void group_step(State<DP> &st, const KvStep<DP> &x, const RowQ<E, DP> &q, uint32_t key,
                                            float ks, float vs, uint32_t lim) {
     constexpr int NKS = DP / 64, VW = DP / 64;
     constexpr bool kF32 = std::is_same_v<E, F32>;
-    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, group = (lane & 15u) / (16 / C);
+    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4;
+    const bool second = (lane & 15u) >= 8;
     constexpr float kLag = 8.0f;
     i32x4 a[3];
 #pragma unroll
-    for (int h = 0; h < C; ++h) {
+    for (int h = 0; h < 2; ++h) {
         i32x4 b[3] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
         for (int c = 0; c < NKS; ++c) {
-            const i32x4 kf = __builtin_bit_cast(i32x4, x[h / 2].k[h % 2][c]);
+            const i32x4 kf = __builtin_bit_cast(i32x4, x.k[h][c]);
 #pragma unroll
             for (int p = 0; p < 3; ++p) b[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf, q.part[p][c], b[p], 0, 0, 0);
         }
 #pragma unroll
         for (int p = 0; p < 3; ++p)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) a[p][i] = h == 0 || group == uint32_t(h) ? b[p][i] : a[p][i];
+            for (int i = 0; i < 4; ++i) a[p][i] = h == 0 || second ? b[p][i] : a[p][i];
     }
     float s[4];
     const float c = ks * q.mul;
@@ -364,27 +365,23 @@ __device__ __forceinline__ void group_step(State<DP> &st, const KvStep<DP> (&x)[
         hi[i] = _Float16(w);
         if constexpr (kF32) lo[i] = _Float16(left_over(w, float(hi[i])));
     }
-    auto of_step = [&](f16x4 w, int t) __attribute__((always_inline)) {
+    auto of_step = [&](f16x4 w) __attribute__((always_inline)) {
         const uint2 v = __builtin_bit_cast(uint2, w);
-        const bool first = group == uint32_t(2 * t), second = group == uint32_t(2 * t + 1);
-        return __builtin_bit_cast(f16x8, u32x4{first ? v.x : 0u, first ? v.y : 0u, second ? v.x : 0u, second ? v.y : 0u});
+        return __builtin_bit_cast(f16x8, u32x4{second ? 0u : v.x, second ? 0u : v.y, second ? v.x : 0u, second ? v.y : 0u});
     };
+    const f16x8 wh = of_step(hi);
+    f16x8 wl;
+    if constexpr (kF32) wl = of_step(lo);
 #pragma unroll
-    for (int t = 0; t < C / 2; ++t) {
-        const f16x8 wh = of_step(hi, t);
-        f16x8 wl;
-        if constexpr (kF32) wl = of_step(lo, t);
+    for (int n = 0; n < VW; ++n) {
+        uint32_t words[8];
 #pragma unroll
-        for (int n = 0; n < VW; ++n) {
-            uint32_t words[8];
+        for (int j = 0; j < 8; ++j) words[j] = x.v[j][n] ^ 0x80808080u;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) words[j] = x[t].v[j][n] ^ 0x80808080u;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const f16x8 v = key_column(words, e);
-                st.o[4 * n + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, wh, st.o[4 * n + e], 0, 0, 0);
-                if constexpr (kF32) st.o[4 * n + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, wl, st.o[4 * n + e], 0, 0, 0);
-            }
+        for (int e = 0; e < 4; ++e) {
+            const f16x8 v = key_column(words, e);
+            st.o[4 * n + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, wh, st.o[4 * n + e], 0, 0, 0);
+            if constexpr (kF32) st.o[4 * n + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, wl, st.o[4 * n + e], 0, 0, 0);
         }
     }
 }
