@@ -16,11 +16,12 @@ namespace {
 // blocks in turn. Where the units are many and have at most eight heads, the columns are two
 // groups of eight, each over every other 16 keys (group_step): half the scores a lane.
 // Bound by the bytes where each row has its own: 32 rows over 2048 keys of 8 kv heads of
-// 128 dims, 134 MB, 28 us or 4.8 TB/s; 128 rows 89 us, 6.0 TB/s. By the L2s' reads where rows
-// share them: 712 rows of two chunks over 2048 keys each, 3 GB out of the caches, 271 us, 11
-// TB/s (one group, whose registers leave two wavefronts a SIMD: 303). By latency where they
-// are few: 8 rows over 256 keys 6.0 us, 26 f32 rows of drafts over 1280 keys 15. A wavefront a
-// row and head (below): 1560 us, 11.5 ms, 131 us, 754 us.
+// 128 dims, 134 MB, 28 us or 4.8 TB/s; 128 rows 89 us, 6.0 TB/s. By vector instructions where
+// rows share them: 712 rows of two chunks over 2048 keys each, 270 us, 108 M of them, two thirds
+// of the SIMDs' cycles (a third turn V's bytes into f16; the 3 GB out of the L2s are 11 TB/s, less
+// than a third of what those hold; one group, whose registers leave two wavefronts a SIMD: 303).
+// By latency where they are few: 8 rows over 256 keys 6.0 us, 26 f32 rows of drafts over 1280
+// keys 15. A wavefront a row and head (below): 1560 us, 11.5 ms, 131 us, 754 us.
 constexpr uint32_t kMaxList = 512;            // entries a workgroup takes at once
 constexpr uint32_t kMostParts = 8192;         // shares' results in scratch: 135 MB at 256 dims, 68 at 128
 constexpr uint32_t kNone = 0x80000000u;       // past every key

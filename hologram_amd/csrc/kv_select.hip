@@ -135,7 +135,7 @@ uint32_t bounds_places(const KvBoundsArgs &a) { return (a.pb.tokens / a.block + 
 // Bound by latency, the bytes are few: 32 rows over 2048 to 65536 keys in blocks of 32, 8 kv
 // heads of 128 dims, 40 MB of bounds, 21 us, 14 of them the sums (a workgroup's chain of search,
 // rows, bounds and store; 2.8 TB/s) and 7 the pick (a barrier a turn); 8 rows over up to 2000
-// keys 5.4 us; 2459 rows of four chunks over up to 30000 keys in blocks of 64, 37 us, a third
+// keys 5.4 us; 2459 rows of four chunks over up to 30000 keys in blocks of 64, 35 us, a third
 // of the cycles in vector instructions of the pick, half of them waits. The general sums, and
 // a pick by eight bits at a time in LDS: 55, 9.4 and 437 us.
 struct Select {
@@ -741,8 +741,9 @@ bool matrix_applies(const KvSelectArgs &a) {
     return a.D <= 256 && a.D % 16 == 0 && a.H / a.Hkv <= 128 && reinterpret_cast<uintptr_t>(a.bounds) % 16 == 0 &&
            reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && uint64_t(a.q_stride) * es % 16 == 0;
 }
-// One launch while a row's sums and their scales fit three workgroups into a CU's LDS: 32 rows
-// of up to 512 blocks 11 us and two launches 15, 2459 rows of chunks 37 and 95.
+// One launch while sixteen rows' sums and their scales fit three workgroups into a CU's LDS (two
+// past 128 dims): 32 rows of up to 512 blocks 11 us and two launches 15, 2459 rows of chunks 35
+// and 95.
 bool whole(const KvSelectArgs &a) { return matrix_applies(a) && blocks_of(a) <= 640; }
 // A list of every block takes neither sums nor their scratch.
 bool every_block(const KvSelectArgs &a) { return !whole(a) && blocks_of(a) <= a.top; }
