@@ -637,7 +637,8 @@ class LogitsProcessCall:
 @dataclass(frozen=True)
 class QkNormRotaryCall:
     """New (discriminant 130): q and k normed by the head and rotated by position
-    (include/holo_hip.h); NO_BUFFER for k, a gamma or freqs that a call does not use."""
+    (include/holo_hip.h); NO_BUFFER for k with k_output, a gamma, pos or freqs that a call does
+    not use."""
     q: BufferRef
     k: BufferRef
     q_gamma: BufferRef

@@ -575,7 +575,7 @@ typedef struct holo_logits_process_call {
  * absent, k_output with it (one without the other is refused): q alone. q_stride and
  * k_stride are the elements from one token to the next (0: tight); the outputs are
  * tight, and neither overlaps an input or the other. kv_heads 0 means heads; head_dim
- * <= 1024. tokens * (heads + kv_heads) < 2^26 in any form. */
+ * <= 1024. tokens * (heads + kv_heads) <= 2^26 - 4 in any form. */
 typedef struct holo_qk_norm_rotary_call {
     holo_buffer_ref q;
     holo_buffer_ref k;
@@ -631,7 +631,7 @@ typedef struct holo_kv_block_bounds_call {
  * ceil(bucket_rows / block_rows)]; lens u32 [batch], device-resident. kv_heads 0 means
  * heads; head_dim <= 1024, heads / kv_heads * head_dim <= 2^17, at most 2^20 blocks a
  * plane, kv_heads times those at most 2^28, top <= 2^20; in any form tokens * kv_heads <
- * 2^24 and (tokens / 16 + batch) * kv_heads * (blocks / 256 + 1) < 2^24. Where a plane has
+ * 2^24 and (tokens / 16 + batch) * kv_heads * (blocks / 256 + 1) < 2^23. Where a plane has
  * more than `top` blocks it may take scratch, at most 256 MiB or one row's kv_heads *
  * blocks * 4 bytes. */
 typedef struct holo_kv_block_select_call {

@@ -215,3 +215,23 @@ def test_an_output_for_k_without_k_is_refused():
     w.kernel_calls, w.exec_plan = [KernelCall.QkNormRotary(alone)], [[0]]
     with pytest.raises(UnsupportedOp, match="k_output"):
         HipSession(None, w.finish())
+
+
+@pytest.mark.parametrize("head_dim,rot", [(2, 2), (16, 16), (128, 32)])
+def test_the_largest_launches_that_the_header_names_are_taken(head_dim, rot):
+    """Right below each call's bound, in whatever form the sizes take."""
+    huge = [1 << 60] * 9
+    alone = replace(ROTARY, k=NO_BUFFER, k_output=NO_BUFFER, heads=1, kv_heads=0, head_dim=head_dim, rotary_dim=rot)
+    validate(KernelCall.QkNormRotary(replace(alone, tokens=(1 << 26) - 4)), huge)
+    with pytest.raises(UnsupportedOp, match="launch"):
+        validate(KernelCall.QkNormRotary(replace(alone, tokens=1 << 26)), huge)
+    for bucket in (100, 640 * 32, 641 * 32):
+        most = ((1 << 23) - 1) // (-(-bucket // 32) // 256 + 1)
+        for tokens, batch in ((16, most - 1), (16 * (most - 3), 2)):
+            c = replace(SELECT, tokens=min(tokens, (1 << 24) - 1), batch=batch, heads=1, kv_heads=1, head_dim=head_dim,
+                        bucket_rows=bucket)
+            validate(KernelCall.KvBlockSelect(c), huge)
+    for block in (32, 33):
+        c = replace(SELECTED, tokens=(1 << 24) - 1, batch=2, heads=1, kv_heads=1, head_dim=head_dim, block_rows=block,
+                    top=1 << 20)
+        validate(KernelCall.AttentionI8Selected(c), huge)
